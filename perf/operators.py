@@ -8,9 +8,9 @@ which the block's largest magnitude does not pass 448, the largest e4m3 value.
            weights.
   norm     residual add and root-mean-square norm, the norm's output in 8 bits (add_rms_norm_fp8);
            the residual's delta is fp16, or fp32 partial sums of a split projection.
-  project  a projection of 8-bit rows by an 8-bit weight (gemm_fp8): fp32 partial sums of K splits,
-           fp16, or SwiGLU of a stacked [gate | up] weight in fp16 or in 8 bits. Up to 128 rows the
-           input may also be fp16 rows, rounded to 8 bits on the way in.
+  project  a projection of 8-bit rows by an 8-bit weight (gemm_fp8): fp32 partial sums of K splits (a
+           decode step's rows, up to 128), fp16, or SwiGLU of a stacked [gate | up] weight in fp16 or in
+           8 bits. Up to 128 rows the input may also be fp16 rows, rounded to 8 bits on the way in.
   qkv      the q|k|v projection with RoPE, K and V written to their slots of the paged pool
            (qkv_rope_append_fp8).
 
@@ -74,10 +74,12 @@ def draw(rng):
         return {"kind": kind, "m": _log(rng, 1, 2048), "k": _log(rng, 256, HIDDEN, 16)}
     out = rng.choice(("partials", "half", "swiglu", "swiglu_fp8"))
     case = {"kind": kind, "m": _log(rng, 1, 2048), "out": out}
+    if out == "partials":  # a decode step's rows
+        case["m"] = min(case["m"], _log(rng, 1, 128))
     case["n"] = _log(rng, 128, 2 * MLP if out.startswith("swiglu") else QKV, 32 if out == "swiglu_fp8" else 8)
     case["k"] = _log(rng, 128, HIDDEN if out.startswith("swiglu") else MLP, 16)
     case["splits"] = rng.choice((1, 2, 3, 4)) if out == "partials" and case["k"] >= 1024 else 1
-    case["half_x"] = case["m"] <= 128 and rng.random() < 0.5
+    case["half_x"] = case["m"] <= 128 and out != "swiglu_fp8" and rng.random() < 0.5
     return case
 
 
