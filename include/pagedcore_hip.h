@@ -348,6 +348,81 @@ int pc_qkv_rope_append(void* query_out, void* key_out, void* value_out, const vo
 int pc_prefill_attention(void* out, const void* query, const void* key, const void* value, int32_t tokens,
                          void* stream);
 
+/*
+ * 8-bit rows: the operands of the projections below. A row of `width` columns is
+ *   values [rows][width] e4m3 (the finite form: largest value 448, no infinity), 16-byte aligned, and
+ *   scales [rows][pc_fp8_scale_stride(width)] bytes, 4-byte aligned: byte b holds the biased exponent
+ *          s in [1, 254] of the power of two 2^(s - 127) that multiplies columns 128 b .. 128 b + 127
+ *          (the last block may be shorter); the bytes past the blocks are neither used nor written.
+ * Rounding a row: s is the smallest with which the block's largest finite magnitude is at most
+ * 448 * 2^(s - 127) (1 for a block of zeros); value = e4m3(x * 2^(127 - s)), to nearest even.
+ * An infinity or NaN becomes a NaN, and leaves the scale of its block alone.
+ * None of this is in the reference, whose weights and activations are fp16; the entry points stand
+ * where those below are cited.
+ */
+#define PC_FP8_BLOCK 128
+
+/* Bytes between the scales of two rows: ceil(width / 128) rounded up to a multiple of 4; 0 for a width outside
+ * [1, 2^22]. */
+int32_t pc_fp8_scale_stride(int32_t width);
+
+/*
+ * Rounds fp16 rows (x [rows][width], row stride x_stride elements, a multiple of 8) to 8 bits; width a
+ * multiple of 16 up to 2^22. x 16-byte aligned.
+ */
+int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride, int64_t rows, int32_t width, void* stream);
+
+/*
+ * Residual add fused with RMSNorm, its output in 8 bits: pc_add_rms_norm (reference
+ * src/pagedcore/dense.py:17-21, decoder.py:191-192) for the 8-bit projections.
+ *   h = fp16(hidden + delta), or hidden where delta is null
+ *   hidden_out = h (may be `hidden` itself; may be null where delta is null)
+ *   values, scales = (h * rsqrt(mean(h^2) + eps) * weight, in fp32) rounded to 8 bits
+ * The _parts form takes delta as fp32 partial sums [splits][rows][width], added in split order and
+ * rounded to fp16 once, splits in [1, 64]. width a multiple of 16 up to 8192; no output may
+ * overlap another buffer but for hidden_out and hidden; all 16-byte aligned.
+ */
+int pc_add_rms_norm_fp8(void* values, void* scales, void* hidden_out, const void* hidden, const void* delta,
+                        const void* weight, int64_t rows, int32_t width, float eps, void* stream);
+int pc_add_rms_norm_parts_fp8(void* values, void* scales, void* hidden_out, const void* hidden, const float* delta_parts,
+                              int32_t splits, const void* weight, int64_t rows, int32_t width, float eps, void* stream);
+
+/*
+ * Projection of 8-bit rows by an 8-bit weight: Y[i][j] = sum_l x[i][l] * w[j][l] over what the values stand for,
+ * added in fp32. pc_gemm_m128 and pc_gemm_rows (reference src/pagedcore/dense.py:91-104) with half the weight.
+ *
+ *   x  [m][k] 8-bit rows; or, for m up to PC_FP8_STREAM_ROWS and x_scales null, fp16 rows, rounded to 8 bits
+ *      in the kernel as pc_quantize_fp8 rounds them
+ *   w  [n][k] 8-bit rows (a weight as stored, rounded by pc_quantize_fp8)
+ *   out, by epilogue:
+ *     PC_GEMM_PARTIALS    [splits][m][n] fp32, m up to PC_FP8_STREAM_ROWS: split s sums the blocks (of 128
+ *                         columns, B in all) [s B / splits, (s + 1) B / splits), splits up to min(B, 64)
+ *     PC_GEMM_HALF        [m][n] fp16
+ *     PC_GEMM_SWIGLU      [m][n / 2] fp16, w the stacked [gate | up] weight: fp16(silu(Yg) * Yu), silu and the
+ *                         product in fp32, one rounding
+ *     PC_GEMM_SWIGLU_FP8  the same rounded to 8 bits: out [m][n / 2] values, out_scales their scales (null for the
+ *                         other epilogues); 8-bit x
+ * splits is 1 but for PC_GEMM_PARTIALS. m in [1, 65536]; k a multiple of 16 up to 2^22; n a multiple of 4 (of 8 for
+ * PC_GEMM_SWIGLU, of 32 for PC_GEMM_SWIGLU_FP8); m * k, n * k and splits * m * n up to 2^31; x, w and out 16-byte
+ * aligned; out must not overlap an input. PC_GEMM_PARTIALS adds exact products in fp32. The
+ * other forms may add them, above PC_FP8_STREAM_ROWS rows, on the 8-bit matrix instruction, which adds eight at a time
+ * aligned to the largest: 1.5e-5 of the result's norm on normal data, beside fp16's rounding.
+ */
+#define PC_GEMM_SWIGLU_FP8 4
+#define PC_FP8_STREAM_ROWS 128
+int pc_gemm_fp8(void* out, void* out_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
+                int32_t m, int32_t n, int32_t k, int32_t splits, int32_t epilogue, void* stream);
+
+/*
+ * The q|k|v projection of 8-bit rows (or fp16 ones, as above) with pc_rope_kv_append as its epilogue:
+ * pc_qkv_rope_append with w [2560][k] in 8 bits, k a multiple of 16 up to 2^18. The projections are
+ * PC_GEMM_HALF's, bit for bit; the other arguments and what is done with them are those of pc_qkv_rope_append.
+ */
+int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, const void* x, const void* x_scales,
+                           const void* w, const void* w_scales, int32_t m, int32_t k, const int64_t* positions,
+                           const void* rope_table, int32_t rope_positions, void* pool, int64_t num_blocks, int32_t layer,
+                           const int64_t* slot_mapping, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 LIBRARY_NAME = "libpagedcore_hip.so"
 
 _lock = threading.Lock()
@@ -141,6 +141,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pc_gemm_m128.argtypes = [_p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]
     lib.pc_gemm_rows.restype = ctypes.c_int
     lib.pc_gemm_rows.argtypes = [_p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]
+    lib.pc_fp8_scale_stride.restype = _i32
+    lib.pc_fp8_scale_stride.argtypes = [_i32]
+    lib.pc_quantize_fp8.restype = ctypes.c_int
+    lib.pc_quantize_fp8.argtypes = [_p, _p, _p, _i64, _i64, _i32, _p]
+    lib.pc_add_rms_norm_fp8.restype = ctypes.c_int
+    lib.pc_add_rms_norm_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _i64, _i32, ctypes.c_float, _p]
+    lib.pc_add_rms_norm_parts_fp8.restype = ctypes.c_int
+    lib.pc_add_rms_norm_parts_fp8.argtypes = [_p, _p, _p, _p, _p, _i32, _p, _i64, _i32, ctypes.c_float, _p]
+    lib.pc_gemm_fp8.restype = ctypes.c_int
+    lib.pc_gemm_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]
+    lib.pc_qkv_rope_append_fp8.restype = ctypes.c_int
+    lib.pc_qkv_rope_append_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _i32, _p, _i64, _i32, _p, _p]
 
 
 def load() -> ctypes.CDLL:
@@ -606,3 +618,186 @@ def prefill_attention(out: Tensor, query: Tensor, key: Tensor, value: Tensor) ->
         out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), tokens, _stream(query.device)
     )
     _check(lib, "pc_prefill_attention", status)
+
+
+# 8-bit rows (include/pagedcore_hip.h): e4m3 values with a power of two per row and block of 128 columns.
+FP8_BLOCK = 128
+FP8_STREAM_ROWS = 128  # rows up to which a projection takes fp16 x and gives partial sums
+GEMM_SWIGLU_FP8 = 4
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def fp8_scale_stride(width: int) -> int:
+    """Scales of a row of `width` columns: one per 128 columns, padded to a multiple of 4."""
+    return (width + 4 * FP8_BLOCK - 1) // (4 * FP8_BLOCK) * 4
+
+
+def empty_fp8(rows: int, width: int, device: torch.device) -> Tuple[Tensor, Tensor]:
+    """Uninitialised 8-bit rows: values float8_e4m3fn [rows, width] and scales float8_e8m0fnu
+    [rows, fp8_scale_stride(width)]."""
+    return (
+        torch.empty((rows, width), dtype=_E4M3, device=device),
+        torch.empty((rows, fp8_scale_stride(width)), dtype=_E8M0, device=device),
+    )
+
+
+def _check_fp8(name: str, values: Tensor, scales: Tensor, shape: Tuple[int, int], device: torch.device) -> None:
+    """8-bit rows of `shape` as the kernels take them."""
+    if values.dtype != _E4M3 or values.shape != shape or not values.is_contiguous() or values.device != device:
+        raise HipExtensionError(f"{name} must be contiguous float8_e4m3fn {list(shape)} on {device}")
+    expected = (shape[0], fp8_scale_stride(shape[1]))
+    if scales is None or scales.dtype != _E8M0 or scales.shape != expected or not scales.is_contiguous() or scales.device != device:
+        raise HipExtensionError(f"the scales of {name} must be contiguous float8_e8m0fnu {list(expected)} on {device}")
+
+
+def _check_half(name: str, tensor: Tensor, shape: Tuple[int, ...], device: torch.device) -> None:
+    if tensor.dtype != torch.float16 or tensor.shape != shape or not tensor.is_contiguous() or tensor.device != device:
+        raise HipExtensionError(f"{name} must be contiguous float16 {list(shape)} on {device}")
+
+
+def _gpu_of(tensor: Tensor) -> torch.device:
+    """The tensor's device, which has to be the current one: the launch goes to its current stream."""
+    device = tensor.device
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise HipExtensionError(f"the tensors are on {device}, which is not the current GPU")
+    return device
+
+
+def quantize_fp8(values: Tensor, scales: Tensor, x: Tensor) -> None:
+    """Round fp16 rows to 8 bits: x float16 [rows, width] with unit column stride and a row stride that is a
+    multiple of 8, width a multiple of 16; values and scales as empty_fp8 gives them. A block's scale
+    is the smallest power of two with which its largest finite magnitude does not pass 448;
+    infinities and NaN become NaN."""
+    device = _gpu_of(x)
+    if x.dim() != 2 or x.dtype != torch.float16 or (x.stride(1) != 1 and x.numel()):
+        raise HipExtensionError("x must be float16 [rows, width] with unit column stride")
+    rows, width = x.shape
+    _check_fp8("values", values, scales, (rows, width), device)
+    lib = load()
+    stride = x.stride(0) if rows > 1 else width
+    status = lib.pc_quantize_fp8(values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows, width, _stream(device))
+    if status:
+        _check(lib, "pc_quantize_fp8", status)
+
+
+def add_rms_norm_fp8(
+    values: Tensor, scales: Tensor, hidden_out: Optional[Tensor], hidden: Tensor, delta: Optional[Tensor], weight: Tensor,
+    eps: float = 1e-5,
+) -> None:
+    """hidden_out = hidden + delta (float16; the same tensor as `hidden` to add in place, or None without
+    a delta); values, scales = RMSNorm(hidden_out) * weight in 8 bits, rounded once from fp32. delta: None,
+    float16 [rows, width], or float32 split-K partial sums [splits, rows, width] (rounded to float16 once)."""
+    device = _gpu_of(hidden)
+    if hidden.dim() != 2:
+        raise HipExtensionError("hidden must be float16 [rows, width]")
+    rows, width = shape = tuple(hidden.shape)
+    _check_half("hidden", hidden, shape, device)
+    _check_half("weight", weight, (width,), device)
+    _check_fp8("values", values, scales, shape, device)
+    if hidden_out is not None:
+        _check_half("hidden_out", hidden_out, shape, device)
+    lib = load()
+    if delta is not None and delta.dim() == 3:
+        if delta.dtype != torch.float32 or delta.shape[1:] != shape or not delta.is_contiguous() or delta.device != device:
+            raise HipExtensionError(f"partial sums must be contiguous float32 [splits, {rows}, {width}] on {device}")
+        status = lib.pc_add_rms_norm_parts_fp8(
+            values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), delta.data_ptr(), delta.shape[0],
+            weight.data_ptr(), rows, width, eps, _stream(device),
+        )
+    else:
+        if delta is not None:
+            _check_half("delta", delta, shape, device)
+        status = lib.pc_add_rms_norm_fp8(
+            values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), _ptr(delta), weight.data_ptr(), rows,
+            width, eps, _stream(device),
+        )
+    if status:
+        _check(lib, "pc_add_rms_norm_fp8", status)
+
+
+def _check_fp8_product(x: Tensor, x_scales: Optional[Tensor], w: Tensor, w_scales: Tensor) -> torch.device:
+    device = _gpu_of(x)
+    if x.dim() != 2 or w.dim() != 2:
+        raise HipExtensionError("x and w must be [m, k] and [n, k]")
+    m, k = x.shape
+    if x_scales is None:
+        _check_half("x without scales", x, (m, k), device)
+    else:
+        _check_fp8("x", x, x_scales, (m, k), device)
+    _check_fp8("w", w, w_scales, (w.shape[0], k), device)
+    return device
+
+
+def gemm_fp8(
+    out: Tensor, x: Tensor, x_scales: Optional[Tensor], w: Tensor, w_scales: Tensor, *, out_scales: Optional[Tensor] = None,
+    splits: int = 1, epilogue: int = GEMM_PARTIALS,
+) -> None:
+    """Projection x @ w.T of 8-bit rows by an 8-bit weight (pc_gemm_fp8): x [m, k] and w [n, k] as quantize_fp8
+    leaves them, or x float16 with x_scales None for up to FP8_STREAM_ROWS rows. out: float32
+    [splits, m, n] (GEMM_PARTIALS, up to FP8_STREAM_ROWS rows), float16 [m, n] (GEMM_HALF) or [m, n // 2]
+    (GEMM_SWIGLU, w the stacked [gate | up] weight), or 8-bit rows [m, n // 2] with out_scales
+    (GEMM_SWIGLU_FP8)."""
+    device = _check_fp8_product(x, x_scales, w, w_scales)
+    (m, k), n = x.shape, w.shape[0]
+    if epilogue == GEMM_SWIGLU_FP8:
+        _check_fp8("out", out, out_scales, (m, n // 2), device)
+    elif epilogue == GEMM_PARTIALS:
+        if out.dtype != torch.float32 or out.shape != (splits, m, n) or not out.is_contiguous() or out.device != device:
+            raise HipExtensionError(f"out must be contiguous float32 [{splits}, {m}, {n}] on {device}")
+    elif epilogue == GEMM_HALF or epilogue == GEMM_SWIGLU:
+        _check_half("out", out, (m, n if epilogue == GEMM_HALF else n // 2), device)
+    else:
+        raise HipExtensionError(f"unknown GEMM epilogue {epilogue}")
+    lib = load()
+    status = lib.pc_gemm_fp8(
+        out.data_ptr(), _ptr(out_scales), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), m, n, k, splits,
+        epilogue, _stream(device),
+    )
+    if status:
+        _check(lib, "pc_gemm_fp8", status)
+
+
+def qkv_rope_append_fp8(
+    query_out: Tensor,
+    x: Tensor,
+    x_scales: Optional[Tensor],
+    w: Tensor,
+    w_scales: Tensor,
+    positions: Tensor,
+    rope_table: Tensor,
+    *,
+    key_out: Optional[Tensor] = None,
+    value_out: Optional[Tensor] = None,
+    pool: Optional[Tensor] = None,
+    layer: int = 0,
+    slot_mapping: Optional[Tensor] = None,
+) -> None:
+    """qkv_rope_append of 8-bit rows (or float16 ones, as gemm_fp8 takes them) by the stacked q | k | v weight
+    [2560, k] in 8 bits, in one launch (pc_qkv_rope_append_fp8)."""
+    device = _check_fp8_product(x, x_scales, w, w_scales)
+    m, k = x.shape
+    if w.shape[0] != 2560:
+        raise HipExtensionError("w must be [2560, k]")
+    if query_out.numel() != m * 2048 or query_out.dtype != torch.float16 or not query_out.is_contiguous() or query_out.device != device:
+        raise HipExtensionError(f"query_out must be contiguous float16 [{m}, 32, 64] on {device}")
+    for name, rows in (("key_out", key_out), ("value_out", value_out)):
+        if rows is not None:
+            _check_half(name, rows, (m, 4, 64), device)
+    for name, rows in (("positions", positions), ("slot_mapping", slot_mapping)):
+        if rows is not None and (rows.dtype != torch.int64 or rows.shape != (m,) or not rows.is_contiguous() or rows.device != device):
+            raise HipExtensionError(f"{name} must be contiguous int64 [{m}] on {device}")
+    if rope_table.dim() != 3:
+        raise HipExtensionError("rope_table must be float16 [positions, 2, 32]")
+    _check_half("rope_table", rope_table, (rope_table.shape[0], 2, 32), device)
+    if pool is not None:
+        if pool.dim() != 6:
+            raise HipExtensionError("pool must be float16 [22, 2, blocks, 16, 4, 64]")
+        _check_half("pool", pool, (22, 2, pool.shape[2], 16, 4, 64), device)
+    lib = load()
+    status = lib.pc_qkv_rope_append_fp8(
+        query_out.data_ptr(), _ptr(key_out), _ptr(value_out), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(),
+        m, k, positions.data_ptr(), rope_table.data_ptr(), rope_table.shape[0], _ptr(pool),
+        pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping), _stream(device),
+    )
+    if status:
+        _check(lib, "pc_qkv_rope_append_fp8", status)

@@ -1,0 +1,131 @@
+// Entry points of the 8-bit projections: the checks of their arguments, and which kernel takes a call.
+
+#include "fp8_gemm.h"
+
+namespace {
+
+using namespace fp8_gemm;
+using pc_internal::aligned;
+using pc_internal::set_error;
+
+constexpr int kMaxRows = 1 << 16;
+constexpr int kMaxK = 1 << 22;     // tile-relative byte offsets fit 32 bits
+constexpr int kMaxQkvK = 1 << 18;  // 2560 rows of W within 32-bit offsets
+constexpr int kStreamRows = PC_FP8_STREAM_ROWS;
+
+// The checks that both entry points share; PC_OK, or an error.
+int check(const Args& a, int64_t max_k) {
+  if (!a.x || !a.w || !a.w_scales) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (a.m < 1 || a.m > kMaxRows) return set_error(PC_ERR_ARGUMENT, "m = %d outside [1, %d]", a.m, kMaxRows);
+  if (a.k < 16 || a.k % 16 != 0 || a.k > max_k) {
+    return set_error(PC_ERR_ARGUMENT, "k = %d must be a multiple of 16 in [16, %lld]", a.k, static_cast<long long>(max_k));
+  }
+  if (static_cast<int64_t>(a.m) * a.k > (int64_t{1} << 31) || static_cast<int64_t>(a.n) * a.k > (int64_t{1} << 31)) {
+    return set_error(PC_ERR_ARGUMENT, "GEMM of %d x %d x %d too large", a.m, a.n, a.k);
+  }
+  if (!a.x_scales && a.m > kStreamRows) {
+    return set_error(PC_ERR_ARGUMENT, "fp16 x takes up to %d rows: quantize %d rows first", kStreamRows, a.m);
+  }
+  if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.x_scales, 4) || !aligned(a.w_scales, 4)) {
+    return set_error(PC_ERR_ARGUMENT, "x and w must be 16-byte aligned, scales 4-byte aligned");
+  }
+  return PC_OK;
+}
+
+// Decode rows stream the weight; more rows take tiles.
+bool streams(const Args& a) { return a.m <= kStreamRows; }
+
+}  // namespace
+
+extern "C" {
+
+int pc_gemm_fp8(void* out, void* out_scales, const void* x, const void* x_scales, const void* w, const void* w_scales,
+                int32_t m, int32_t n, int32_t k, int32_t splits, int32_t epilogue, void* stream) {
+  Args a{};
+  a.x = x;
+  a.x_scales = static_cast<const uint8_t*>(x_scales);
+  a.w = static_cast<const uint8_t*>(w);
+  a.w_scales = static_cast<const uint8_t*>(w_scales);
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.splits = splits;
+  a.out = out;
+  a.out_scales = static_cast<uint8_t*>(out_scales);
+  if (!out) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (n < 1) return set_error(PC_ERR_ARGUMENT, "n must be positive");
+  if (int rc = check(a, kMaxK)) return rc;
+  if (!aligned(out, 16) || !aligned(out_scales, 4)) {
+    return set_error(PC_ERR_ARGUMENT, "out must be 16-byte aligned, scales 4-byte aligned");
+  }
+  if (epilogue != PC_GEMM_PARTIALS && epilogue != PC_GEMM_HALF && epilogue != PC_GEMM_SWIGLU && epilogue != PC_GEMM_SWIGLU_FP8) {
+    return set_error(PC_ERR_ARGUMENT, "unknown epilogue %d", epilogue);
+  }
+  const Form form = static_cast<Form>(epilogue);
+  const int columns = form == kSwiGLUFp8 ? 32 : form == kSwiGLU ? 8 : 4;
+  if (n % columns != 0) return set_error(PC_ERR_ARGUMENT, "n = %d must be a multiple of %d", n, columns);
+  if ((out_scales != nullptr) != (form == kSwiGLUFp8)) {
+    return set_error(PC_ERR_ARGUMENT, "out_scales belong to PC_GEMM_SWIGLU_FP8, and only to it");
+  }
+  if (form == kPartials) {
+    const int blocks = (k + PC_FP8_BLOCK - 1) / PC_FP8_BLOCK;
+    if (splits < 1 || splits > 64 || splits > blocks) {
+      return set_error(PC_ERR_ARGUMENT, "splits %d outside [1, 64] or more than k's %d blocks", splits, blocks);
+    }
+    if (m > kStreamRows) return set_error(PC_ERR_ARGUMENT, "fp32 partial sums take up to %d rows, not %d", kStreamRows, m);
+    if (static_cast<int64_t>(splits) * m * n > (int64_t{1} << 31)) {
+      return set_error(PC_ERR_ARGUMENT, "GEMM of %d x %d x %d with %d splits too large", m, n, k, splits);
+    }
+  } else if (splits != 1) {
+    return set_error(PC_ERR_ARGUMENT, "only partial sums take splits");
+  }
+  if (form == kSwiGLUFp8 && !x_scales) return set_error(PC_ERR_ARGUMENT, "PC_GEMM_SWIGLU_FP8 takes 8-bit x");
+  (void)hipGetLastError();
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return form != kSwiGLUFp8 && streams(a) ? launch_stream(a, form, s) : launch_tiles(a, form, s);
+}
+
+int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, const void* x, const void* x_scales,
+                           const void* w, const void* w_scales, int32_t m, int32_t k, const int64_t* positions,
+                           const void* rope_table, int32_t rope_positions, void* pool, int64_t num_blocks, int32_t layer,
+                           const int64_t* slot_mapping, void* stream) {
+  using namespace rope_device;
+  Args a{};
+  a.x = x;
+  a.x_scales = static_cast<const uint8_t*>(x_scales);
+  a.w = static_cast<const uint8_t*>(w);
+  a.w_scales = static_cast<const uint8_t*>(w_scales);
+  a.m = m;
+  a.n = kQkvElems;
+  a.k = k;
+  a.splits = 1;
+  if (!query_out || !positions || !rope_table) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (int rc = check(a, kMaxQkvK)) return rc;
+  if (rope_positions < 1) return set_error(PC_ERR_ARGUMENT, "rope_positions must be positive");
+  if ((pool == nullptr) != (slot_mapping == nullptr)) {
+    return set_error(PC_ERR_ARGUMENT, "pool and slot_mapping must both be given or both be null");
+  }
+  if (pool != nullptr) {
+    if (num_blocks < 1 || num_blocks > INT32_MAX) {
+      return set_error(PC_ERR_ARGUMENT, "num_blocks %lld out of range", static_cast<long long>(num_blocks));
+    }
+    if (layer < 0 || layer >= kLayers) return set_error(PC_ERR_ARGUMENT, "layer %d outside [0, 22)", layer);
+  }
+  if (!aligned(query_out, 16) || !aligned(key_out, 16) || !aligned(value_out, 16) || !aligned(rope_table, 16) || !aligned(pool, 16)) {
+    return set_error(PC_ERR_ARGUMENT, "buffers must be 16-byte aligned");
+  }
+  a.positions = positions;
+  a.slots = slot_mapping;
+  a.rope.table = static_cast<const _Float16*>(rope_table);
+  a.rope.table_positions = rope_positions;
+  a.rope.query = static_cast<_Float16*>(query_out);
+  a.rope.kind_elems = pool ? num_blocks * kSlots * kRowElems : 0;
+  a.rope.layer_pool = pool ? static_cast<_Float16*>(pool) + static_cast<int64_t>(layer) * 2 * a.rope.kind_elems : nullptr;
+  a.rope.key = static_cast<_Float16*>(key_out);
+  a.rope.value = static_cast<_Float16*>(value_out);
+  (void)hipGetLastError();
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return streams(a) ? launch_stream(a, kRope, s) : launch_tiles(a, kRope, s);
+}
+
+}  // extern "C"

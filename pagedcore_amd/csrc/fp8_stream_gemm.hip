@@ -1,0 +1,336 @@
+// 8-bit projection of a decode step's rows: Y = X W^T with W e4m3 [n][k] and X e4m3 or fp16 [m][k],
+// both with a power of two per row and block of 128 columns (fp8_device.h). It takes the place of
+// torch.nn.functional.linear on fp16 weights (reference src/pagedcore/dense.py:91-104 via
+// src/pagedcore/decoder.py:156-199).
+//
+//   Y[i][j] = sum over blocks b of 2^(sx[i][b] + sw[j][b]) * (sum over l in b of x[i][l] w[j][l])
+//
+// The weight is the stream: n k bytes from HBM, half of what the fp16 form reads. One workgroup
+// computes 16 MT rows of X times 16 NT rows of W; its waves take the 128-column blocks v, v + WAVES, ...
+// of the split's K range, so every byte of the tile is fetched by exactly one wave, through a ring
+// of D slots of its own (LDS DMA, whole 128-byte lines), with no barrier in the loop. The waves' sums
+// are added in wave order at the end.
+//
+// The products run on the fp16 matrix instruction, the operands widened from e4m3 in registers
+// (exact). The 8-bit instruction would add eight products at a time aligned to the largest and drop what lies
+// below about 2^-14 of it (measured: 1.5e-5 of the result's norm; fp32 sums of fp16 products: 5e-8), and
+// its rate is not needed here: the conversions (16 per 16 rows and block) and the narrower matrix
+// instruction hide behind the weight's stream at a decode step's rows. An fp16 X is rounded
+// to 8 bits in the same registers, with the values and scales of pc_quantize_fp8, so that a decode step
+// needs no launch for it.
+
+#include "fp8_gemm.h"
+
+namespace fp8_gemm {
+namespace {
+
+using namespace fp8_device;
+using namespace rope_device;
+using gemm_device::float4_t;
+using gemm_device::half4_t;
+using gemm_device::half8_t;
+using gemm_device::lds_offset;
+using gemm_device::lds_ptr;
+using gemm_device::raise_lds_limit;
+using gemm_device::wait_vm;
+using pc_internal::check_launch;
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+
+// The words of a 16-byte LDS chunk.
+__device__ __forceinline__ uint4_t lds_words(uint32_t addr) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) uint4_t*>(static_cast<uintptr_t>(addr));
+}
+__device__ __forceinline__ uint32_t lds_word(uint32_t addr) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(static_cast<uintptr_t>(addr));
+}
+
+// Eight e4m3 as fp16, exactly.
+__device__ __forceinline__ half8_t widen(uint32_t a, uint32_t b) {
+  const half2_t p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+  const half2_t q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+  const half2_t r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+  const half2_t s = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+  return half8_t{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+
+// Eight fp16 divided by a power of two, rounded to e4m3, as fp16.
+__device__ __forceinline__ half8_t round_fp8(half8_t v, float inverse) {
+  const uint32_t a = pack4(static_cast<float>(v[0]) * inverse, static_cast<float>(v[1]) * inverse,
+                           static_cast<float>(v[2]) * inverse, static_cast<float>(v[3]) * inverse);
+  const uint32_t b = pack4(static_cast<float>(v[4]) * inverse, static_cast<float>(v[5]) * inverse,
+                           static_cast<float>(v[6]) * inverse, static_cast<float>(v[7]) * inverse);
+  return widen(a, b);
+}
+
+template <int MT, int NT, int WAVES, int D, bool HALFX>
+struct Shape {
+  static constexpr int XB = MT * (HALFX ? 4096 : 2048);  // X part of a unit: 16 MT rows of 128 columns
+  static constexpr int WB = NT * 2048;
+  static constexpr int SB = HALFX ? 256 : 512;           // scale words: W's rows, then X's
+  static constexpr int UB = XB + WB + SB;
+  static constexpr int PER = (XB + WB) / 1024 + SB / 256;  // DMA instructions per unit
+  static constexpr int RING = WAVES * D * UB;
+  static constexpr int SUMS = WAVES * MT * NT * 1024;
+  static constexpr int LDS = RING > SUMS ? RING : SUMS;
+  static_assert(LDS <= 160 * 1024, "ring and accumulator exchange fit the CU's LDS");
+  static_assert((D - 1) * PER < 64 && D >= 2 && D <= 4, "vmcnt counts the later units");
+  static_assert(NT <= 4 && MT <= 4, "one scale word per lane");
+};
+
+template <int MT, int NT, int WAVES, int D, bool HALFX, Form E>
+__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tiles, int mtiles) {
+  using S = Shape<MT, NT, WAVES, D, HALFX>;
+  constexpr int kRowsX = 16 * MT;
+  constexpr int kCols = paired(E) ? 8 * NT : 16 * NT;  // output columns per tile (pairs of them)
+  constexpr int kXSize = HALFX ? 2 : 1;                // bytes per element of X
+  constexpr int kXBytes = S::XB, kWBytes = S::WB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int r16 = lane & 15, g = lane >> 4;
+  // Workgroups of one W tile (one per X tile) are 8 apart, on one XCD: W comes from HBM once.
+  int id = blockIdx.x, mtile = 0;
+  if (mtiles > 1) {
+    const int q = id >> 3;
+    mtile = q % mtiles;
+    id = (q / mtiles) * 8 + (id & 7);
+  }
+  const int tile = id % tiles, split = id / tiles;
+  if (split >= a.splits) return;  // the grid is rounded up to 8 tiles
+  const int m = a.m, n = a.n, k = a.k;
+  const int limit = paired(E) ? n / 2 : n;
+  const int blocks = (k + kBlock - 1) / kBlock;
+  const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / a.splits);
+  const int end = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / a.splits);
+  const int mine = (end - first - wave + WAVES - 1) / WAVES;
+
+  // Row r of the tile's W part, relative to its first; rows past the matrix repeat its last row.
+  const int last = limit - 1 - kCols * tile;
+  auto w_row = [&](int r) {
+    if constexpr (E == kSwiGLU) return r < kCols ? min(r, last) : limit + min(r - kCols, last);
+    else if constexpr (E == kRope) return pair_row(kCols * tile) + (r < kCols ? r : kHalfDim + r - kCols);
+    else return min(r, last);
+  };
+  const int last_x = m - 1 - kRowsX * mtile;
+  const char* const xbase = static_cast<const char*>(a.x) + static_cast<int64_t>(kRowsX) * mtile * k * kXSize;
+  const uint8_t* const wbase = a.w + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * k);
+  const int stride = scale_stride(k);
+  const uint8_t* const xscales = HALFX ? nullptr : a.x_scales + static_cast<int64_t>(kRowsX) * mtile * stride;
+  const uint8_t* const wscales = a.w_scales + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * stride);
+  const uint32_t ws_off = w_row(min(lane, 16 * NT - 1)) * stride;
+  const uint32_t xs_off = min(min(lane, kRowsX - 1), last_x) * stride;
+
+  // DMA of 1 KiB: eight rows of 128 bytes (lane L takes row L / 8 and the chunk stored at position
+  // L % 8: chunk c of row r at c ^ (r & 7)), or four fp16 rows of 256 (position c ^ (r & 15)). Chunks
+  // past the columns, in the last block alone, fetch chunk 0 of their row in place.
+  char* const ring = smem + wave * D * S::UB;
+  auto issue = [&](char* slot, int t) {
+    const int b = first + wave + WAVES * t;
+    const int left = k - kBlock * b;  // columns of this block and later ones
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      const int c = 16 * ((lane & 7) ^ (lane >> 3));
+      const uint32_t off = static_cast<uint32_t>(w_row(r)) * static_cast<uint32_t>(k) + (c < left ? c : 0);
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wbase + static_cast<int64_t>(kBlock) * b + off),
+                                       lds_ptr(slot + kXBytes + i * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kXBytes / 1024; ++i) {
+      const int r = HALFX ? 4 * i + (lane >> 4) : 8 * i + (lane >> 3);
+      const int c = HALFX ? 16 * ((lane & 15) ^ (r & 15)) : 16 * ((lane & 7) ^ (lane >> 3));
+      const uint32_t off = static_cast<uint32_t>(min(r, last_x)) * static_cast<uint32_t>(k * kXSize) + (c < left * kXSize ? c : 0);
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xbase + static_cast<int64_t>(kBlock * kXSize) * b + off),
+                                       lds_ptr(slot + i * 1024), 16, 0, 0);
+    }
+    const int word = b & ~3;
+    __builtin_amdgcn_global_load_lds(static_cast<const void*>(wscales + ws_off + word), lds_ptr(slot + kXBytes + kWBytes), 4, 0, 0);
+    if constexpr (!HALFX) {
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xscales + xs_off + word), lds_ptr(slot + kXBytes + kWBytes + 256), 4, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  };
+
+  float4_t acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+  const uint32_t ring0 = lds_offset(ring);
+  // The block t of this wave in slot d. Lane (r16, g) holds columns 16 g .. + 15 and 64 + 16 g .. + 15 of
+  // row r16 of each 16 rows, as four fragments of eight.
+  auto unit = [&](int d, int t) {
+    const int b = first + wave + WAVES * t;
+    const int left = k - kBlock * b;
+    const int shift = 8 * (b & 3);
+    const uint32_t base = ring0 + d * S::UB;
+    half8_t xf[MT][4];
+    float sx[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if constexpr (HALFX) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const int c = 8 * (f >> 1) + 2 * g + (f & 1);
+          const uint4_t words = lds_words(base + j * 4096 + r16 * 256 + ((c ^ r16) * 16));
+          xf[j][f] = 8 * c < left ? __builtin_bit_cast(half8_t, words) : half8_t{};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_magnitude(static_cast<float>(xf[j][f][e])));
+        }
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
+        largest = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
+        largest = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+        const int scale = scale_of(largest);
+        sx[j] = power_of(scale);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) xf[j][f] = round_fp8(xf[j][f], inverse_of(scale));
+      } else {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int c = 4 * p + g;
+          uint4_t words = lds_words(base + j * 2048 + r16 * 128 + ((c ^ (r16 & 7)) * 16));
+          if (16 * c >= left) words = uint4_t{0, 0, 0, 0};
+          xf[j][2 * p] = widen(words[0], words[1]);
+          xf[j][2 * p + 1] = widen(words[2], words[3]);
+        }
+        const uint32_t word = lds_word(base + S::XB + S::WB + 256 + (16 * j + r16) * 4);
+        sx[j] = power_of((word >> shift) & 255);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      half8_t wf[4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint4_t words = lds_words(base + S::XB + i * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
+        wf[2 * p] = widen(words[0], words[1]);
+        wf[2 * p + 1] = widen(words[2], words[3]);
+      }
+      const uint4_t words = lds_words(base + S::XB + S::WB + (16 * i + 4 * g) * 4);
+      float sw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sw[e] = power_of((words[e] >> shift) & 255);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < 4; ++f) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[f], xf[j][f], sum, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[e] * sx[j], sw[e], acc[i][j][e]);
+      }
+    }
+  };
+
+#pragma unroll
+  for (int t = 0; t < D; ++t) {
+    if (t < mine) issue(ring + t * S::UB, t);
+  }
+  // Unit t in slot t % D: its DMA has landed once at most the later units' are outstanding.
+  for (int t = 0; t < mine; ++t) {
+    const int later = min(D - 1, mine - 1 - t);
+    if (D > 3 && later == 3) wait_vm<(D > 3 ? 3 : 1) * S::PER>();
+    else if (D > 2 && later == 2) wait_vm<(D > 2 ? 2 : 1) * S::PER>();
+    else if (later == 1) wait_vm<S::PER>();
+    else wait_vm<0>();
+    const int d = t % D;
+    unit(d, t);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done before the slot is refilled
+    if (t + D < mine) issue(ring + d * S::UB, t + D);
+  }
+
+  // Sums to LDS (over the rings, once every wave is done with its own), then added in wave order:
+  // acc[i][j] of lane (r16, g) holds X row 16 j + r16, W rows 16 i + 4 g .. + 3.
+  __syncthreads();
+  float4_t* sums = reinterpret_cast<float4_t*>(smem);
+  constexpr int T = MT * NT, Q = kCols / 4;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[(wave * T + i * MT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < Q * kRowsX; e += 64 * WAVES) {
+    const int q = e % Q, r = e / Q;
+    const int row = kRowsX * mtile + r, col = kCols * tile + 4 * q;
+    auto total = [&](int quad) {
+      const float4_t* p = sums + ((quad >> 2) * MT + (r >> 4)) * 64 + 16 * (quad & 3) + (r & 15);
+      float4_t v = p[0];
+#pragma unroll
+      for (int u = 1; u < WAVES; ++u) v += p[u * T * 64];
+      return v;
+    };
+    if (row >= m || col >= limit) continue;
+    const float4_t v = total(q);
+    if constexpr (E == kPartials) {
+      float* y = static_cast<float*>(a.out) + (static_cast<int64_t>(split) * m + row) * n + col;
+      *reinterpret_cast<float4_t*>(y) = v;
+    } else {
+      half4_t o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(v[i]);
+      if constexpr (E == kHalf) {
+        *reinterpret_cast<half4_t*>(static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * n + col) = o;
+      } else {
+        const float4_t u = total(Q + q);
+        if constexpr (E == kSwiGLU) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(v[i] / (1.0f + expf(-v[i])) * u[i]);
+          *reinterpret_cast<half4_t*>(static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * limit + col) = o;
+        } else {
+          half4_t high;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) high[i] = static_cast<_Float16>(u[i]);
+          const RopeRow rope = rope_row(a.rope, a.positions[row], (a.slots ? a.slots : a.positions)[row], a.slots != nullptr);
+          const _Float16* table = rope.table + col % kHalfDim;
+          store_pairs(a.rope, rope, row, col, o, high, *reinterpret_cast<const half4_t*>(table),
+                      *reinterpret_cast<const half4_t*>(table + kHalfDim));
+        }
+      }
+    }
+  }
+}
+
+template <int MT, int NT, int WAVES, int D, bool HALFX, Form E>
+int launch(const Args& a, hipStream_t s) {
+  using S = Shape<MT, NT, WAVES, D, HALFX>;
+  constexpr int cols = paired(E) ? 8 * NT : 16 * NT;
+  static_assert(E != kRope || kHalfDim % cols == 0, "a tile's pairs lie in one head");
+  auto kernel = fp8_stream_kernel<MT, NT, WAVES, D, HALFX, E>;
+  static std::atomic<uint64_t> raised{0};
+  if (int rc = raise_lds_limit(reinterpret_cast<const void*>(kernel), S::LDS, raised)) return rc;
+  const int tiles = ((paired(E) ? a.n / 2 : a.n) + cols - 1) / cols;
+  const int mtiles = (a.m + 16 * MT - 1) / (16 * MT);
+  int64_t grid = static_cast<int64_t>(tiles) * a.splits;
+  if (mtiles > 1) grid = (grid + 7) / 8 * 8 * mtiles;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), S::LDS, s, a, tiles, mtiles);
+  return check_launch("fp8_stream_gemm");
+}
+
+template <bool HALFX, Form E>
+int launch_rows(const Args& a, hipStream_t s) {
+  return a.m <= 16 ? launch<1, 2, 4, 3, HALFX, E>(a, s) : launch<2, 2, 4, 2, HALFX, E>(a, s);
+}
+
+template <Form E>
+int launch_form(const Args& a, hipStream_t s) {
+  return a.x_scales ? launch_rows<false, E>(a, s) : launch_rows<true, E>(a, s);
+}
+
+}  // namespace
+
+int launch_stream(const Args& a, Form form, hipStream_t s) {
+  switch (form) {
+    case kPartials: return launch_form<kPartials>(a, s);
+    case kHalf: return launch_form<kHalf>(a, s);
+    case kSwiGLU: return launch_form<kSwiGLU>(a, s);
+    default: return launch_form<kRope>(a, s);
+  }
+}
+
+}  // namespace fp8_gemm
