@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_fp8_kernel(const _Float
     const bool mine = column(c) < width;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = mine ? h[c][i] * norm * static_cast<float>(wt[c][i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) y[i] = mine ? h[c][i] * static_cast<float>(wt[c][i]) * norm : 0.0f;  // the first product is exact
     int scale;
     const uint2_t packed = round8(y, scale);
     if (!mine) continue;

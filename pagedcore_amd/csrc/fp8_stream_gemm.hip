@@ -56,13 +56,21 @@ __device__ __forceinline__ half8_t widen(uint32_t a, uint32_t b) {
   return half8_t{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
-// Eight fp16 divided by a power of two, rounded to e4m3, as fp16.
-__device__ __forceinline__ half8_t round_fp8(half8_t v, float inverse) {
-  const uint32_t a = pack4(static_cast<float>(v[0]) * inverse, static_cast<float>(v[1]) * inverse,
-                           static_cast<float>(v[2]) * inverse, static_cast<float>(v[3]) * inverse);
-  const uint32_t b = pack4(static_cast<float>(v[4]) * inverse, static_cast<float>(v[5]) * inverse,
-                           static_cast<float>(v[6]) * inverse, static_cast<float>(v[7]) * inverse);
-  return widen(a, b);
+// Eight fp16 divided by `scale`, a power of two, rounded to e4m3, as fp16 (the conversion divides by its
+// scale operand exactly before it rounds, and turns infinities and NaN into NaN).
+__device__ __forceinline__ half8_t round_fp8(half8_t v, float scale) {
+  short2_t a{}, b{};
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, half2_t{v[0], v[1]}, scale, false);
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, half2_t{v[2], v[3]}, scale, true);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, half2_t{v[4], v[5]}, scale, false);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, half2_t{v[6], v[7]}, scale, true);
+  return widen(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+
+// The larger of two pairs of fp16 magnitudes, as bits (so that infinities and NaN come out on top).
+__device__ __forceinline__ uint32_t max_magnitudes(uint32_t a, uint32_t b) {
+  typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
 }
 
 template <int MT, int NT, int WAVES, int D, bool HALFX>
@@ -80,8 +88,19 @@ struct Shape {
   static_assert(NT <= 4 && MT <= 4, "one scale word per lane");
 };
 
+// The arguments that only the end of the kernel reads; those before it are preloaded into SGPRs at wave
+// launch (no kernel-argument round trip before the first DMA).
+struct Rest {
+  void* out;
+  const int64_t* positions;
+  const int64_t* slots;
+  RopeOut rope;
+};
+
 template <int MT, int NT, int WAVES, int D, bool HALFX, Form E>
-__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tiles, int mtiles) {
+__global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, const uint8_t* w, const uint8_t* x_scales,
+                                                                const uint8_t* w_scales, int m, int n, int k, int splits,
+                                                                int tiles, int mtiles, Rest rest) {
   using S = Shape<MT, NT, WAVES, D, HALFX>;
   constexpr int kRowsX = 16 * MT;
   constexpr int kCols = paired(E) ? 8 * NT : 16 * NT;  // output columns per tile (pairs of them)
@@ -99,58 +118,70 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tile
     id = (q / mtiles) * 8 + (id & 7);
   }
   const int tile = id % tiles, split = id / tiles;
-  if (split >= a.splits) return;  // the grid is rounded up to 8 tiles
-  const int m = a.m, n = a.n, k = a.k;
+  if (split >= splits) return;  // the grid is rounded up to 8 tiles
   const int limit = paired(E) ? n / 2 : n;
   const int blocks = (k + kBlock - 1) / kBlock;
-  const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / a.splits);
-  const int end = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / a.splits);
+  const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
+  const int end = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / splits);
   const int mine = (end - first - wave + WAVES - 1) / WAVES;
 
   // Row r of the tile's W part, relative to its first; rows past the matrix repeat its last row.
-  const int last = limit - 1 - kCols * tile;
+  const int last = limit - 1 - kCols * tile, last_x = m - 1 - kRowsX * mtile;
   auto w_row = [&](int r) {
     if constexpr (E == kSwiGLU) return r < kCols ? min(r, last) : limit + min(r - kCols, last);
     else if constexpr (E == kRope) return pair_row(kCols * tile) + (r < kCols ? r : kHalfDim + r - kCols);
     else return min(r, last);
   };
-  const int last_x = m - 1 - kRowsX * mtile;
-  const char* const xbase = static_cast<const char*>(a.x) + static_cast<int64_t>(kRowsX) * mtile * k * kXSize;
-  const uint8_t* const wbase = a.w + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * k);
-  const int stride = scale_stride(k);
-  const uint8_t* const xscales = HALFX ? nullptr : a.x_scales + static_cast<int64_t>(kRowsX) * mtile * stride;
-  const uint8_t* const wscales = a.w_scales + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * stride);
-  const uint32_t ws_off = w_row(min(lane, 16 * NT - 1)) * stride;
-  const uint32_t xs_off = min(min(lane, kRowsX - 1), last_x) * stride;
-
   // DMA of 1 KiB: eight rows of 128 bytes (lane L takes row L / 8 and the chunk stored at position
-  // L % 8: chunk c of row r at c ^ (r & 7)), or four fp16 rows of 256 (position c ^ (r & 15)). Chunks
-  // past the columns, in the last block alone, fetch chunk 0 of their row in place.
+  // L % 8: chunk c of row r at c ^ (r & 7)), or four fp16 rows of 256 (position c ^ (r & 15)).
+  const int row8 = lane >> 3;
+  const int chunk = 16 * ((lane & 7) ^ row8);
+  uint32_t xoff[kXBytes / 1024], woff[2 * NT];
+  int xchunk[kXBytes / 1024];
+#pragma unroll
+  for (int i = 0; i < 2 * NT; ++i) woff[i] = static_cast<uint32_t>(w_row(8 * i + row8)) * static_cast<uint32_t>(k);
+#pragma unroll
+  for (int i = 0; i < kXBytes / 1024; ++i) {
+    const int r = HALFX ? 4 * i + (lane >> 4) : 8 * i + row8;
+    xoff[i] = static_cast<uint32_t>(min(r, last_x)) * static_cast<uint32_t>(k * kXSize);
+    xchunk[i] = HALFX ? 16 * ((lane & 15) ^ (r & 15)) : chunk;
+  }
+  const char* const xbase = static_cast<const char*>(x) + static_cast<int64_t>(kRowsX) * mtile * k * kXSize;
+  const uint8_t* const wbase = w + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * k);
+  const int stride = scale_stride(k);
+  const uint8_t* const xscale = HALFX ? nullptr : x_scales + (static_cast<int64_t>(kRowsX) * mtile + min(min(lane, kRowsX - 1), last_x)) * stride;
+  const uint8_t* const wscale = w_scales + ((E == kRope ? 0 : static_cast<int64_t>(kCols) * tile) + w_row(min(lane, 16 * NT - 1))) * stride;
+  // RoPE: thread e ends with quad e % Q of row e / Q of the tile (one each at most). Its position
+  // and slot are loaded before the stream's first unit and the table values behind it, so that
+  // the stream hides both round trips (loads return in order: an older one in flight only
+  // makes the waits below longer).
+  constexpr int T = MT * NT, Q = kCols / 4;  // Q: groups of four output columns
+  static_assert(E != kRope || (kHalfDim % kCols == 0 && Q * kRowsX <= 64 * WAVES), "one quad of one head per thread");
+  int64_t position = 0, slot_of = 0;
+  if constexpr (E == kRope) {
+    const int row = min(kRowsX * mtile + static_cast<int>(threadIdx.x) / Q, m - 1);
+    position = rest.positions[row];
+    slot_of = (rest.slots != nullptr ? rest.slots : rest.positions)[row];
+  }
   char* const ring = smem + wave * D * S::UB;
   auto issue = [&](char* slot, int t) {
     const int b = first + wave + WAVES * t;
     const int left = k - kBlock * b;  // columns of this block and later ones
+    const uint8_t* const wblock = wbase + static_cast<int64_t>(kBlock) * b;
+    const char* const xblock = xbase + static_cast<int64_t>(kBlock * kXSize) * b;
+    // Chunks past the columns, in the last block alone, fetch chunk 0 of their row in place.
+    const int wc = chunk < left ? chunk : 0;
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      const int r = 8 * i + (lane >> 3);
-      const int c = 16 * ((lane & 7) ^ (lane >> 3));
-      const uint32_t off = static_cast<uint32_t>(w_row(r)) * static_cast<uint32_t>(k) + (c < left ? c : 0);
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wbase + static_cast<int64_t>(kBlock) * b + off),
-                                       lds_ptr(slot + kXBytes + i * 1024), 16, 0, 0);
-    }
+    for (int i = 0; i < 2 * NT; ++i)
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wblock + (woff[i] + wc)), lds_ptr(slot + kXBytes + i * 1024), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kXBytes / 1024; ++i) {
-      const int r = HALFX ? 4 * i + (lane >> 4) : 8 * i + (lane >> 3);
-      const int c = HALFX ? 16 * ((lane & 15) ^ (r & 15)) : 16 * ((lane & 7) ^ (lane >> 3));
-      const uint32_t off = static_cast<uint32_t>(min(r, last_x)) * static_cast<uint32_t>(k * kXSize) + (c < left * kXSize ? c : 0);
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xbase + static_cast<int64_t>(kBlock * kXSize) * b + off),
+    for (int i = 0; i < kXBytes / 1024; ++i)
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xblock + (xoff[i] + (xchunk[i] < left * kXSize ? xchunk[i] : 0))),
                                        lds_ptr(slot + i * 1024), 16, 0, 0);
-    }
-    const int word = b & ~3;
-    __builtin_amdgcn_global_load_lds(static_cast<const void*>(wscales + ws_off + word), lds_ptr(slot + kXBytes + kWBytes), 4, 0, 0);
+    __builtin_amdgcn_global_load_lds(static_cast<const void*>(wscale + (b & ~3)), lds_ptr(slot + kXBytes + kWBytes), 4, 0, 0);
     if constexpr (!HALFX) {
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xscales + xs_off + word), lds_ptr(slot + kXBytes + kWBytes + 256), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xscale + (b & ~3)), lds_ptr(slot + kXBytes + kWBytes + 256), 4, 0, 0);
     }
     asm volatile("" ::: "memory");
   };
@@ -174,23 +205,39 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tile
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       if constexpr (HALFX) {
-        float largest = 0.0f;
+        uint32_t most = 0;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           const int c = 8 * (f >> 1) + 2 * g + (f & 1);
-          const uint4_t words = lds_words(base + j * 4096 + r16 * 256 + ((c ^ r16) * 16));
-          xf[j][f] = 8 * c < left ? __builtin_bit_cast(half8_t, words) : half8_t{};
+          uint4_t words = lds_words(base + j * 4096 + r16 * 256 + ((c ^ r16) * 16));
+          if (8 * c >= left) words = uint4_t{0, 0, 0, 0};
+          xf[j][f] = __builtin_bit_cast(half8_t, words);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_magnitude(static_cast<float>(xf[j][f][e])));
+          for (int e = 0; e < 4; ++e) most = max_magnitudes(most, words[e] & 0x7fff7fffu);
         }
-        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
-        largest = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
-        largest = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-        const int scale = scale_of(largest);
-        sx[j] = power_of(scale);
+        most = max(most & 0xffffu, most >> 16);
+        const auto p = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+        most = max(p[0], p[1]);
+        const auto q = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+        most = max(q[0], q[1]);
+        float largest = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(most)));
+        if (most >= 0x7c00u) {  // an infinity or NaN in the block: the largest of the others
+          largest = 0.0f;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) xf[j][f] = round_fp8(xf[j][f], inverse_of(scale));
+          for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_magnitude(static_cast<float>(xf[j][f][e])));
+        }
+        // every lane takes part in the exchange; where nothing was infinite it changes nothing
+        if (__builtin_amdgcn_ballot_w64(most >= 0x7c00u)) {
+          const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
+          largest = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+          const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
+          largest = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
+        }
+        sx[j] = power_of(scale_of(largest));
+#pragma unroll
+        for (int f = 0; f < 4; ++f) xf[j][f] = round_fp8(xf[j][f], sx[j]);
       } else {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -232,6 +279,14 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tile
   for (int t = 0; t < D; ++t) {
     if (t < mine) issue(ring + t * S::UB, t);
   }
+  [[maybe_unused]] RopeRow rope{};
+  [[maybe_unused]] half4_t cs{}, sn{};
+  if constexpr (E == kRope) {
+    rope = rope_row(rest.rope, position, slot_of, rest.slots != nullptr);
+    const _Float16* table = rope.table + (kCols * tile + 4 * (static_cast<int>(threadIdx.x) % Q)) % kHalfDim;
+    cs = *reinterpret_cast<const half4_t*>(table);
+    sn = *reinterpret_cast<const half4_t*>(table + kHalfDim);
+  }
   // Unit t in slot t % D: its DMA has landed once at most the later units' are outstanding.
   for (int t = 0; t < mine; ++t) {
     const int later = min(D - 1, mine - 1 - t);
@@ -249,7 +304,6 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tile
   // acc[i][j] of lane (r16, g) holds X row 16 j + r16, W rows 16 i + 4 g .. + 3.
   __syncthreads();
   float4_t* sums = reinterpret_cast<float4_t*>(smem);
-  constexpr int T = MT * NT, Q = kCols / 4;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -268,28 +322,25 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(Args a, int tile
     if (row >= m || col >= limit) continue;
     const float4_t v = total(q);
     if constexpr (E == kPartials) {
-      float* y = static_cast<float*>(a.out) + (static_cast<int64_t>(split) * m + row) * n + col;
+      float* y = static_cast<float*>(rest.out) + (static_cast<int64_t>(split) * m + row) * n + col;
       *reinterpret_cast<float4_t*>(y) = v;
     } else {
       half4_t o;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(v[i]);
       if constexpr (E == kHalf) {
-        *reinterpret_cast<half4_t*>(static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * n + col) = o;
+        *reinterpret_cast<half4_t*>(static_cast<_Float16*>(rest.out) + static_cast<int64_t>(row) * n + col) = o;
       } else {
         const float4_t u = total(Q + q);
         if constexpr (E == kSwiGLU) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(v[i] / (1.0f + expf(-v[i])) * u[i]);
-          *reinterpret_cast<half4_t*>(static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * limit + col) = o;
+          *reinterpret_cast<half4_t*>(static_cast<_Float16*>(rest.out) + static_cast<int64_t>(row) * limit + col) = o;
         } else {
           half4_t high;
 #pragma unroll
           for (int i = 0; i < 4; ++i) high[i] = static_cast<_Float16>(u[i]);
-          const RopeRow rope = rope_row(a.rope, a.positions[row], (a.slots ? a.slots : a.positions)[row], a.slots != nullptr);
-          const _Float16* table = rope.table + col % kHalfDim;
-          store_pairs(a.rope, rope, row, col, o, high, *reinterpret_cast<const half4_t*>(table),
-                      *reinterpret_cast<const half4_t*>(table + kHalfDim));
+          store_pairs(rest.rope, rope, row, col, o, high, cs, sn);
         }
       }
     }
@@ -300,7 +351,6 @@ template <int MT, int NT, int WAVES, int D, bool HALFX, Form E>
 int launch(const Args& a, hipStream_t s) {
   using S = Shape<MT, NT, WAVES, D, HALFX>;
   constexpr int cols = paired(E) ? 8 * NT : 16 * NT;
-  static_assert(E != kRope || kHalfDim % cols == 0, "a tile's pairs lie in one head");
   auto kernel = fp8_stream_kernel<MT, NT, WAVES, D, HALFX, E>;
   static std::atomic<uint64_t> raised{0};
   if (int rc = raise_lds_limit(reinterpret_cast<const void*>(kernel), S::LDS, raised)) return rc;
@@ -308,7 +358,8 @@ int launch(const Args& a, hipStream_t s) {
   const int mtiles = (a.m + 16 * MT - 1) / (16 * MT);
   int64_t grid = static_cast<int64_t>(tiles) * a.splits;
   if (mtiles > 1) grid = (grid + 7) / 8 * 8 * mtiles;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), S::LDS, s, a, tiles, mtiles);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), S::LDS, s, a.x, a.w, a.x_scales,
+                     a.w_scales, a.m, a.n, a.k, a.splits, tiles, mtiles, Rest{a.out, a.positions, a.slots, a.rope});
   return check_launch("fp8_stream_gemm");
 }
 
