@@ -37,6 +37,8 @@ using pc_internal::check_launch;
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef int int8v_t __attribute__((ext_vector_type(8)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 // The words of a 16-byte LDS chunk.
@@ -56,15 +58,15 @@ __device__ __forceinline__ half8_t widen(uint32_t a, uint32_t b) {
   return half8_t{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
-// Eight fp16 divided by `scale`, a power of two, rounded to e4m3, as fp16 (the conversion divides by its
-// scale operand exactly before it rounds, and turns infinities and NaN into NaN).
-__device__ __forceinline__ half8_t round_fp8(half8_t v, float scale) {
+// Eight fp16 divided by `scale`, a power of two, rounded to e4m3 (the conversion divides by its scale
+// operand exactly before it rounds, and turns infinities and NaN into NaN).
+__device__ __forceinline__ uint2_t round_fp8(half8_t v, float scale) {
   short2_t a{}, b{};
   a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, half2_t{v[0], v[1]}, scale, false);
   a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, half2_t{v[2], v[3]}, scale, true);
   b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, half2_t{v[4], v[5]}, scale, false);
   b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, half2_t{v[6], v[7]}, scale, true);
-  return widen(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+  return uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
 // The larger of two pairs of fp16 magnitudes, as bits (so that infinities and NaN come out on top).
@@ -92,24 +94,27 @@ struct Shape {
 // launch (no kernel-argument round trip before the first DMA).
 struct Rest {
   void* out;
-  const int64_t* positions;
   const int64_t* slots;
   RopeOut rope;
 };
 
 template <int MT, int NT, int WAVES, int D, bool HALFX, Form E>
 __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, const uint8_t* w, const uint8_t* x_scales,
-                                                                const uint8_t* w_scales, int m, int n, int k, int splits,
-                                                                int tiles, int mtiles, Rest rest) {
+                                                                const uint8_t* w_scales, int m, int n, int k,
+                                                                int splits_mtiles, const int64_t* positions, Rest rest) {
   using S = Shape<MT, NT, WAVES, D, HALFX>;
   constexpr int kRowsX = 16 * MT;
   constexpr int kCols = paired(E) ? 8 * NT : 16 * NT;  // output columns per tile (pairs of them)
+  constexpr bool kExact = E == kPartials;
   constexpr int kXSize = HALFX ? 2 : 1;                // bytes per element of X
   constexpr int kXBytes = S::XB, kWBytes = S::WB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r16 = lane & 15, g = lane >> 4;
+  const int limit = paired(E) ? n / 2 : n;
+  const int tiles = (limit + kCols - 1) / kCols;
+  const int splits = splits_mtiles >> 16, mtiles = splits_mtiles & 65535;
   // Workgroups of one W tile (one per X tile) are 8 apart, on one XCD: W comes from HBM once.
   int id = blockIdx.x, mtile = 0;
   if (mtiles > 1) {
@@ -119,7 +124,6 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   }
   const int tile = id % tiles, split = id / tiles;
   if (split >= splits) return;  // the grid is rounded up to 8 tiles
-  const int limit = paired(E) ? n / 2 : n;
   const int blocks = (k + kBlock - 1) / kBlock;
   const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
   const int end = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / splits);
@@ -160,8 +164,8 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   int64_t position = 0, slot_of = 0;
   if constexpr (E == kRope) {
     const int row = min(kRowsX * mtile + static_cast<int>(threadIdx.x) / Q, m - 1);
-    position = rest.positions[row];
-    slot_of = (rest.slots != nullptr ? rest.slots : rest.positions)[row];
+    position = positions[row];
+    slot_of = (rest.slots != nullptr ? rest.slots : positions)[row];
   }
   char* const ring = smem + wave * D * S::UB;
   auto issue = [&](char* slot, int t) {
@@ -193,84 +197,115 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
     for (int j = 0; j < MT; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
   const uint32_t ring0 = lds_offset(ring);
+  // 32 fp16 of a row's block in this lane, 128 in the four lanes of the row: rounded, and the scale.
+  auto round_row = [&](uint32_t base, int left, uint4_t (&eight)[2], int& scale) {
+    half8_t v[4];
+    uint32_t most = 0;
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const int c = 8 * (f >> 1) + 2 * g + (f & 1);
+      uint4_t words = lds_words(base + r16 * 256 + ((c ^ r16) * 16));
+      if (8 * c >= left) words = uint4_t{0, 0, 0, 0};
+      v[f] = __builtin_bit_cast(half8_t, words);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = max_magnitudes(most, words[e] & 0x7fff7fffu);
+    }
+    auto widest = [](uint32_t bits) {  // over the row's lanes; non-negative floats and fp16 compare as their bits do
+      const auto p = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+      const uint32_t half = max(p[0], p[1]);
+      const auto q = __builtin_amdgcn_permlane16_swap(half, half, false, false);
+      return max(q[0], q[1]);
+    };
+    most = widest(max(most & 0xffffu, most >> 16));
+    float largest = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(most)));
+    if (__builtin_amdgcn_ballot_w64(most >= 0x7c00u)) {  // an infinity or NaN in some row: the largest of the others
+      float finite = 0.0f;
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) finite = fmaxf(finite, finite_magnitude(static_cast<float>(v[f][e])));
+      largest = __uint_as_float(widest(__float_as_uint(finite)));
+    }
+    scale = scale_of(largest);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint2_t a = round_fp8(v[2 * p], power_of(scale)), b = round_fp8(v[2 * p + 1], power_of(scale));
+      eight[p] = uint4_t{a[0], a[1], b[0], b[1]};
+    }
+  };
   // The block t of this wave in slot d. Lane (r16, g) holds columns 16 g .. + 15 and 64 + 16 g .. + 15 of
-  // row r16 of each 16 rows, as four fragments of eight.
+  // row r16 of each 16 rows.
   auto unit = [&](int d, int t) {
     const int b = first + wave + WAVES * t;
     const int left = k - kBlock * b;
     const int shift = 8 * (b & 3);
     const uint32_t base = ring0 + d * S::UB;
-    half8_t xf[MT][4];
-    float sx[MT];
+    uint4_t x8[MT][2];
+    int xs[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       if constexpr (HALFX) {
-        uint32_t most = 0;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const int c = 8 * (f >> 1) + 2 * g + (f & 1);
-          uint4_t words = lds_words(base + j * 4096 + r16 * 256 + ((c ^ r16) * 16));
-          if (8 * c >= left) words = uint4_t{0, 0, 0, 0};
-          xf[j][f] = __builtin_bit_cast(half8_t, words);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) most = max_magnitudes(most, words[e] & 0x7fff7fffu);
-        }
-        most = max(most & 0xffffu, most >> 16);
-        const auto p = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-        most = max(p[0], p[1]);
-        const auto q = __builtin_amdgcn_permlane16_swap(most, most, false, false);
-        most = max(q[0], q[1]);
-        float largest = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(most)));
-        if (most >= 0x7c00u) {  // an infinity or NaN in the block: the largest of the others
-          largest = 0.0f;
-#pragma unroll
-          for (int f = 0; f < 4; ++f)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_magnitude(static_cast<float>(xf[j][f][e])));
-        }
-        // every lane takes part in the exchange; where nothing was infinite it changes nothing
-        if (__builtin_amdgcn_ballot_w64(most >= 0x7c00u)) {
-          const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
-          largest = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
-          const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
-          largest = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
-        }
-        sx[j] = power_of(scale_of(largest));
-#pragma unroll
-        for (int f = 0; f < 4; ++f) xf[j][f] = round_fp8(xf[j][f], sx[j]);
+        round_row(base + j * 4096, left, x8[j], xs[j]);
       } else {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int c = 4 * p + g;
-          uint4_t words = lds_words(base + j * 2048 + r16 * 128 + ((c ^ (r16 & 7)) * 16));
-          if (16 * c >= left) words = uint4_t{0, 0, 0, 0};
-          xf[j][2 * p] = widen(words[0], words[1]);
-          xf[j][2 * p + 1] = widen(words[2], words[3]);
+          x8[j][p] = lds_words(base + j * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
         }
-        const uint32_t word = lds_word(base + S::XB + S::WB + 256 + (16 * j + r16) * 4);
-        sx[j] = power_of((word >> shift) & 255);
+        if (left < kBlock) {  // columns past the matrix
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            if (16 * (4 * p + g) >= left) x8[j][p] = uint4_t{0, 0, 0, 0};
+        }
+        xs[j] = (lds_word(base + S::XB + S::WB + 256 + (16 * j + r16) * 4) >> shift) & 255;
       }
     }
+    if constexpr (kExact) {
+      half8_t xf[MT][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      half8_t wf[4];
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint4_t words = lds_words(base + S::XB + i * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
-        wf[2 * p] = widen(words[0], words[1]);
-        wf[2 * p + 1] = widen(words[2], words[3]);
+        for (int f = 0; f < 4; ++f) xf[j][f] = widen(x8[j][f >> 1][2 * (f & 1)], x8[j][f >> 1][2 * (f & 1) + 1]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        half8_t wf[4];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint4_t words = lds_words(base + S::XB + i * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
+          wf[2 * p] = widen(words[0], words[1]);
+          wf[2 * p + 1] = widen(words[2], words[3]);
+        }
+        const uint4_t words = lds_words(base + S::XB + S::WB + (16 * i + 4 * g) * 4);
+        float4_t sum[MT];
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+            sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[f], xf[j][f], f ? sum[j] : float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float sw = power_of((words[e] >> shift) & 255);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[i][j][e] = fmaf(sum[j][e] * power_of(xs[j]), sw, acc[i][j][e]);
+        }
       }
-      const uint4_t words = lds_words(base + S::XB + S::WB + (16 * i + 4 * g) * 4);
-      float sw[4];
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sw[e] = power_of((words[e] >> shift) & 255);
+      for (int i = 0; i < NT; ++i) {
+        int8v_t wf;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < 2; ++p) {
+          const uint4_t words = lds_words(base + S::XB + i * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
 #pragma unroll
-        for (int f = 0; f < 4; ++f) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[f], xf[j][f], sum, 0, 0, 0);
+          for (int e = 0; e < 4; ++e) wf[4 * p + e] = static_cast<int>(words[e]);
+        }
+        const int ws = (lds_word(base + S::XB + S::WB + (16 * i + r16) * 4) >> shift) & 255;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[e] * sx[j], sw[e], acc[i][j][e]);
+        for (int j = 0; j < MT; ++j) {
+          int8v_t xf;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) xf[e] = static_cast<int>(x8[j][e >> 2][e & 3]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[i][j], 0, 0, 0, ws, 0, xs[j]);
+        }
       }
     }
   };
@@ -359,7 +394,7 @@ int launch(const Args& a, hipStream_t s) {
   int64_t grid = static_cast<int64_t>(tiles) * a.splits;
   if (mtiles > 1) grid = (grid + 7) / 8 * 8 * mtiles;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), S::LDS, s, a.x, a.w, a.x_scales,
-                     a.w_scales, a.m, a.n, a.k, a.splits, tiles, mtiles, Rest{a.out, a.positions, a.slots, a.rope});
+                     a.w_scales, a.m, a.n, a.k, a.splits * 65536 + mtiles, a.positions, Rest{a.out, a.slots, a.rope});
   return check_launch("fp8_stream_gemm");
 }
 

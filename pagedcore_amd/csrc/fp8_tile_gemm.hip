@@ -60,8 +60,19 @@ struct Shape {
   static_assert(LDS <= 160 * 1024, "ring fits the CU's LDS");
 };
 
+// The arguments that only the end of the kernel reads.
+struct Rest {
+  void* out;
+  uint8_t* out_scales;
+  const int64_t* positions;
+  const int64_t* slots;
+  RopeOut rope;
+};
+
 template <int BM, int BN, int WM, int WN, int ST, Form E>
-__global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntiles, int mtiles) {
+__global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, const uint8_t* w, const uint8_t* x_scales,
+                                                                const uint8_t* w_scales, int m, int n, int k, int ntiles,
+                                                                int mtiles, Rest rest) {
   using S = Shape<BM, BN, WM, WN, ST>;
   constexpr int TM = S::TM, TN = S::TN, MT = S::MT, NT = S::NT;
   constexpr int kWaves = S::WAVES, kXBytes = S::XB, kWBytes = S::WB;
@@ -72,7 +83,6 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   const int wm = wave % WM, wn = wave / WM;
-  const int m = a.m, n = a.n, k = a.k;
 
   // XCD j takes the j-th eighth of the tiles (the hardware deals workgroups to XCDs in turn):
   // groups of kTileGroup X tiles, W tiles, and X tiles fastest.
@@ -99,11 +109,11 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
       return min(r, last);
     }
   };
-  const char* const xbase = static_cast<const char*>(a.x) + static_cast<int64_t>(BM) * mtile * k;
-  const uint8_t* const wbase = a.w + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * k);
+  const char* const xbase = static_cast<const char*>(x) + static_cast<int64_t>(BM) * mtile * k;
+  const uint8_t* const wbase = w + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * k);
   const int stride = scale_stride(k);
-  const uint8_t* const xscales = a.x_scales + static_cast<int64_t>(BM) * mtile * stride;
-  const uint8_t* const wscales = a.w_scales + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * stride);
+  const uint8_t* const xscales = x_scales + static_cast<int64_t>(BM) * mtile * stride;
+  const uint8_t* const wscales = w_scales + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * stride);
 
   // DMA of 1 KiB: rows 8 i .. 8 i + 7, lane L takes row 8 i + L / 8 and the chunk stored at position L % 8
   // (chunk c of row r at c ^ (r & 7)). Chunks past the columns, in the last block alone, fetch chunk
@@ -154,58 +164,89 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
     if (t < steps) issue(smem + t * S::STAGE, t);
   }
 
-  const uint32_t lds0 = lds_offset(smem);
   // Lane (r32, h) holds 32 of a half block's 64 columns: chunks 4 s + 2 h and 4 s + 2 h + 1 of half s.
-  auto fragment = [&](uint32_t base, int row, int s) {
-    const int c = 4 * s + 2 * h;
-    const int4v_t p = lds_chunk(base + row * 128 + ((c ^ (row & 7)) * 16));
-    const int4v_t q = lds_chunk(base + row * 128 + (((c + 1) ^ (row & 7)) * 16));
+  const uint32_t lds0 = lds_offset(smem);
+  uint32_t at[2][2];  // of half s, chunk 4 s + 2 h + c, in row r32 of a group of rows
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) at[s][c] = lds0 + r32 * 128 + (((4 * s + 2 * h + c) ^ (r32 & 7)) * 16);
+  struct Half {
+    int8v_t x[MT], w[NT];
+  };
+  auto fragment = [&](uint32_t row_base, int s) {
+    const int4v_t p = lds_chunk(at[s][0] + row_base), q = lds_chunk(at[s][1] + row_base);
     return int8v_t{p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
   };
-  for (int t = 0; t < steps; ++t) {
-    // Stage t has landed for every wave: at most the later stages issued are outstanding in this one,
-    // and the barrier holds until the others say the same.
-    const int later = min(ST - 2, steps - 1 - t);
-    if (t == 0) {  // nothing refilled yet: up to ST - 1 later stages
-      const int ahead = min(ST - 1, steps - 1);
-      if (ST > 3 && ahead == 3) wait_vm<(ST > 3 ? 3 : 1) * S::PER>();
-      else if (ST > 2 && ahead == 2) wait_vm<(ST > 2 ? 2 : 1) * S::PER>();
-      else if (ahead == 1) wait_vm<S::PER>();
-      else wait_vm<0>();
-    } else if (ST > 3 && later == 2) wait_vm<(ST > 3 ? 2 : 1) * S::PER>();
-    else if (ST > 2 && later == 1) wait_vm<S::PER>();
-    else wait_vm<0>();
-    stage_barrier();
-    // Every wave has read stage t - 1: refill it.
-    if (t > 0 && t - 1 + ST < steps) issue(smem + ((t - 1) % ST) * S::STAGE, t - 1 + ST);
-    const uint32_t xs = lds0 + (t % ST) * S::STAGE, ws = xs + S::XB, ss = ws + S::WB + (t & 3);
-    int sx[MT], sw[NT];
+  auto read = [&](Half& f, uint32_t slot, int s, int t) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sx[j] = lds_byte(ss + (wm * TM + 32 * j + r32) * 4);
+    for (int i = 0; i < NT; ++i) f.w[i] = fragment(slot + S::XB + (wn * TN + 32 * i) * 128, s);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) sw[i] = lds_byte(ss + (BM + wn * TN + 32 * i + r32) * 4);
-    const int left = k - kBlock * t;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      int8v_t xf[MT], wf[NT];
+    for (int j = 0; j < MT; ++j) f.x[j] = fragment(slot + (wm * TM + 32 * j) * 128, s);
+    const int left = k - kBlock * t - 16 * (4 * s + 2 * h);  // columns from this lane's first
+    if (k - kBlock * t < kBlock) {                           // columns past the matrix: whole chunks of 16
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        xf[j] = fragment(xs, wm * TM + 32 * j + r32, s);
-        if (left < kBlock) {  // columns past the matrix: 16-column chunks, whole ones
-          const int c = 4 * s + 2 * h;
-          if (16 * c >= left) xf[j] = int8v_t{};
-          else if (16 * (c + 1) >= left) xf[j] = int8v_t{xf[j][0], xf[j][1], xf[j][2], xf[j][3], 0, 0, 0, 0};
-        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f.x[j][e] = left > 16 * (e >> 2) ? f.x[j][e] : 0;
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) wf[i] = fragment(ws, wn * TN + 32 * i + r32, s);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], xf[j], acc[i][j], 0, 0, 0, sw[i], 0, sx[j]);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done before the barrier that lets the slot be refilled
+  };
+  struct Scales {
+    int x[MT], w[NT];
+  };
+  auto read_scales = [&](Scales& f, uint32_t slot, int t) {
+    const uint32_t base = lds0 + slot + S::XB + S::WB + (t & 3) + 4 * r32;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) f.w[i] = lds_byte(base + (BM + wn * TN + 32 * i) * 4);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) f.x[j] = lds_byte(base + (wm * TM + 32 * j) * 4);
+  };
+  auto multiply = [&](const Half& f, const Scales& scales) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.w[i], f.x[j], acc[i][j], 0, 0, 0, scales.w[i], 0, scales.x[j]);
+  };
+  // A stage has landed for every wave: at most `later` stages issued after it are outstanding in
+  // this one, and the barrier holds until the others say the same.
+  auto landed = [&](int later) {
+    if (ST > 3 && later == 3) wait_vm<(ST > 3 ? 3 : 1) * S::PER>();
+    else if (ST > 2 && later == 2) wait_vm<(ST > 2 ? 2 : 1) * S::PER>();
+    else if (later == 1) wait_vm<S::PER>();
+    else wait_vm<0>();
+    stage_barrier();
+  };
+  // The second half's operands are read before the first half's products, and the next stage's first
+  // half before the second half's, so that LDS latency and the barrier hide behind matrix work.
+  Half one, two;
+  Scales now, next;
+  landed(min(ST - 1, steps - 1));
+  read(one, 0, 0, 0);
+  read_scales(now, 0, 0);
+  int slot = 0;
+#pragma nounroll
+  for (int t = 0; t < steps; ++t) {
+    read(two, slot * S::STAGE, 1, t);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(one, now);
+    __builtin_amdgcn_sched_barrier(0);
+    // This wave has read all of stage t; once every wave has (the barrier below), its slot is
+    // refilled with stage t + ST.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int following = slot + 1 == ST ? 0 : slot + 1;
+    if (t + 1 < steps) {
+      landed(min(ST - 2, steps - 2 - t));
+      if (t + ST < steps) issue(smem + slot * S::STAGE, t + ST);
+      read(one, following * S::STAGE, 0, t + 1);
+      read_scales(next, following * S::STAGE, t + 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(two, now);
+    __builtin_amdgcn_sched_barrier(0);
+    now = next;
+    slot = following;
   }
 
   // acc[i][j] of lane (r32, h), element 4 q + e: X row wm TM + 32 j + r32, W row wn TN + 32 i + 8 q + 4 h + e
@@ -244,7 +285,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
       const int scale = scale_of(most);
       const float inverse = inverse_of(scale);
       if (row >= m) continue;
-      if (wn == 0 && h == 0) a.out_scales[static_cast<int64_t>(row) * scale_stride(limit) + tile] = static_cast<uint8_t>(scale);
+      if (wn == 0 && h == 0) rest.out_scales[static_cast<int64_t>(row) * scale_stride(limit) + tile] = static_cast<uint8_t>(scale);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -252,7 +293,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
           const int col = col0 + 32 * i + 8 * q;
           const uint32_t packed = pack4(acc[i][j][4 * q] * inverse, acc[i][j][4 * q + 1] * inverse,
                                         acc[i][j][4 * q + 2] * inverse, acc[i][j][4 * q + 3] * inverse);
-          if (col < limit) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + static_cast<int64_t>(row) * limit + col) = packed;
+          if (col < limit) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(rest.out) + static_cast<int64_t>(row) * limit + col) = packed;
         }
       }
     }
@@ -262,7 +303,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
       const int row = BM * mtile + wm * TM + 32 * j + r32;
       if (row >= m) continue;
       [[maybe_unused]] RopeRow rope{};
-      if constexpr (E == kRope) rope = rope_row(a.rope, a.positions[row], (a.slots ? a.slots : a.positions)[row], a.slots != nullptr);
+      if constexpr (E == kRope) rope = rope_row(rest.rope, rest.positions[row], (rest.slots ? rest.slots : rest.positions)[row], rest.slots != nullptr);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -285,10 +326,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Args a, int ntil
 #pragma unroll
             for (int e = 0; e < 4; ++e) high[e] = static_cast<_Float16>(acc[i + P][j][4 * q + e]);
             const _Float16* table = rope.table + col % kHalfDim;
-            store_pairs(a.rope, rope, row, col, o, high, *reinterpret_cast<const half4_t*>(table),
+            store_pairs(rest.rope, rope, row, col, o, high, *reinterpret_cast<const half4_t*>(table),
                         *reinterpret_cast<const half4_t*>(table + kHalfDim));
           } else {
-            *reinterpret_cast<half4_t*>(static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * limit + col) = o;
+            *reinterpret_cast<half4_t*>(static_cast<_Float16*>(rest.out) + static_cast<int64_t>(row) * limit + col) = o;
           }
         }
       }
@@ -306,7 +347,8 @@ int launch(const Args& a, hipStream_t s) {
   const int ntiles = ((paired(E) ? a.n / 2 : a.n) + cols - 1) / cols, mtiles = (a.m + BM - 1) / BM;
   const int64_t total = static_cast<int64_t>(ntiles) * mtiles;
   const int64_t grid = (total + kXCDs - 1) / kXCDs * kXCDs;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WM * WN), S::LDS, s, a, ntiles, mtiles);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * WM * WN), S::LDS, s, a.x, a.w, a.x_scales, a.w_scales,
+                     a.m, a.n, a.k, ntiles, mtiles, Rest{a.out, a.out_scales, a.positions, a.slots, a.rope});
   return check_launch("fp8_tile_gemm");
 }
 
