@@ -6,8 +6,8 @@
 //   Y[i][j] = sum over blocks b of 2^(sx[i][b] + sw[j][b]) * (sum over l in b of x[i][l] w[j][l])
 //
 // The weight is the stream: n k bytes from HBM, half of what the fp16 form reads. One workgroup
-// computes 16 MT rows of X times 16 NT rows of W; its waves take the 128-column blocks v, v + WAVES, ...
-// of the split's K range, so every byte of the tile is fetched by exactly one wave, through a ring
+// computes 16 MT rows of X times 16 NT rows of W; its waves take runs of the split's blocks of 128 columns,
+// so every byte of the tile is fetched by exactly one wave, through a ring
 // of D slots of its own (LDS DMA, whole 128-byte lines), with no barrier in the loop. The waves' sums
 // are added in wave order at the end.
 //
@@ -79,10 +79,11 @@ template <int MT, int NT, int WAVES, int D, bool HALFX>
 struct Shape {
   static constexpr int XB = MT * (HALFX ? 4096 : 2048);  // X part of a unit: 16 MT rows of 128 columns
   static constexpr int WB = NT * 2048;
-  static constexpr int SB = HALFX ? 256 : 512;           // scale words: W's rows, then X's
-  static constexpr int UB = XB + WB + SB;
-  static constexpr int PER = (XB + WB) / 1024 + SB / 256;  // DMA instructions per unit
-  static constexpr int RING = WAVES * D * UB;
+  static constexpr int UB = XB + WB;
+  static constexpr int PER = UB / 1024;                  // DMA instructions per unit
+  static constexpr int SB = HALFX ? 256 : 512;           // four blocks' scales: W's rows, then X's
+  static constexpr int WAVE = D * UB + 2 * SB;
+  static constexpr int RING = WAVES * WAVE;
   static constexpr int SUMS = WAVES * MT * NT * 1024;
   static constexpr int LDS = RING > SUMS ? RING : SUMS;
   static_assert(LDS <= 160 * 1024, "ring and accumulator exchange fit the CU's LDS");
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   constexpr int kCols = paired(E) ? 8 * NT : 16 * NT;  // output columns per tile (pairs of them)
   constexpr bool kExact = E == kPartials;
   constexpr int kXSize = HALFX ? 2 : 1;                // bytes per element of X
-  constexpr int kXBytes = S::XB, kWBytes = S::WB;
+  constexpr int kXBytes = S::XB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -127,7 +128,9 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   const int blocks = (k + kBlock - 1) / kBlock;
   const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
   const int end = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / splits);
-  const int mine = (end - first - wave + WAVES - 1) / WAVES;
+  // This wave's blocks: a run of them, so that four in a row share the words of their scales.
+  const int begin = first + wave * (end - first) / WAVES;
+  const int mine = first + (wave + 1) * (end - first) / WAVES - begin;
 
   // Row r of the tile's W part, relative to its first; rows past the matrix repeat its last row.
   const int last = limit - 1 - kCols * tile, last_x = m - 1 - kRowsX * mtile;
@@ -167,15 +170,26 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
     position = positions[row];
     slot_of = (rest.slots != nullptr ? rest.slots : positions)[row];
   }
-  char* const ring = smem + wave * D * S::UB;
+  char* const ring = smem + wave * S::WAVE;
+  char* const scale_ring = ring + D * S::UB;
+  constexpr int kScaleBytes = S::SB;
   auto issue = [&](char* slot, int t) {
-    const int b = first + wave + WAVES * t;
+    const int b = begin + t;
     const int left = k - kBlock * b;  // columns of this block and later ones
     const uint8_t* const wblock = wbase + static_cast<int64_t>(kBlock) * b;
     const char* const xblock = xbase + static_cast<int64_t>(kBlock * kXSize) * b;
     // Chunks past the columns, in the last block alone, fetch chunk 0 of their row in place.
     const int wc = chunk < left ? chunk : 0;
     asm volatile("" ::: "memory");
+    // The scales of blocks b & ~3 .. + 3, with the first of them that this wave takes (ahead of its data: the
+    // waits count the data's instructions, and two more in flight only make one of them longer).
+    if (t == 0 || (b & 3) == 0) {
+      char* const words = scale_ring + ((b >> 2) & 1) * kScaleBytes;
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wscale + (b & ~3)), lds_ptr(words), 4, 0, 0);
+      if constexpr (!HALFX) {
+        __builtin_amdgcn_global_load_lds(static_cast<const void*>(xscale + (b & ~3)), lds_ptr(words + 256), 4, 0, 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2 * NT; ++i)
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(wblock + (woff[i] + wc)), lds_ptr(slot + kXBytes + i * 1024), 16, 0, 0);
@@ -183,10 +197,6 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
     for (int i = 0; i < kXBytes / 1024; ++i)
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(xblock + (xoff[i] + (xchunk[i] < left * kXSize ? xchunk[i] : 0))),
                                        lds_ptr(slot + i * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds(static_cast<const void*>(wscale + (b & ~3)), lds_ptr(slot + kXBytes + kWBytes), 4, 0, 0);
-    if constexpr (!HALFX) {
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xscale + (b & ~3)), lds_ptr(slot + kXBytes + kWBytes + 256), 4, 0, 0);
-    }
     asm volatile("" ::: "memory");
   };
 
@@ -236,8 +246,9 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   // The block t of this wave in slot d. Lane (r16, g) holds columns 16 g .. + 15 and 64 + 16 g .. + 15 of
   // row r16 of each 16 rows.
   auto unit = [&](int d, int t) {
-    const int b = first + wave + WAVES * t;
+    const int b = begin + t;
     const int left = k - kBlock * b;
+    const uint32_t scales = ring0 + D * S::UB + ((b >> 2) & 1) * S::SB;
     const int shift = 8 * (b & 3);
     const uint32_t base = ring0 + d * S::UB;
     uint4_t x8[MT][2];
@@ -256,7 +267,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
           for (int p = 0; p < 2; ++p)
             if (16 * (4 * p + g) >= left) x8[j][p] = uint4_t{0, 0, 0, 0};
         }
-        xs[j] = (lds_word(base + S::XB + S::WB + 256 + (16 * j + r16) * 4) >> shift) & 255;
+        xs[j] = (lds_word(scales + 256 + (16 * j + r16) * 4) >> shift) & 255;
       }
     }
     if constexpr (kExact) {
@@ -274,7 +285,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
           wf[2 * p] = widen(words[0], words[1]);
           wf[2 * p + 1] = widen(words[2], words[3]);
         }
-        const uint4_t words = lds_words(base + S::XB + S::WB + (16 * i + 4 * g) * 4);
+        const uint4_t words = lds_words(scales + (16 * i + 4 * g) * 4);
         float4_t sum[MT];
 #pragma unroll
         for (int f = 0; f < 4; ++f)
@@ -298,7 +309,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
 #pragma unroll
           for (int e = 0; e < 4; ++e) wf[4 * p + e] = static_cast<int>(words[e]);
         }
-        const int ws = (lds_word(base + S::XB + S::WB + (16 * i + r16) * 4) >> shift) & 255;
+        const int ws = (lds_word(scales + (16 * i + r16) * 4) >> shift) & 255;
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
           int8v_t xf;

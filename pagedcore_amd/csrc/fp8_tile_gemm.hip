@@ -48,14 +48,14 @@ struct Shape {
   static constexpr int WAVES = WM * WN;
   static constexpr int TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;
   static constexpr int XB = BM * 128, WB = BN * 128;
-  static constexpr int GROUPS = (BM + BN) / 64;                // of 64 rows, one scale DMA each
+  static constexpr int STAGE = XB + WB;
+  static constexpr int GROUPS = (BM + BN) / 16;                // of 16 rows, one DMA of 16 blocks' scales each
   static constexpr int SI = (GROUPS + WAVES - 1) / WAVES;
-  static constexpr int STAGE = XB + WB + GROUPS * 256;
+  static constexpr int SB = GROUPS * 256;                      // 16 blocks' scales, twice
   static constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;  // DMA instructions per wave and stage
-  static constexpr int PER = XI + WI + SI;
-  static constexpr int LDS = ST * STAGE;
+  static constexpr int PER = XI + WI;
+  static constexpr int LDS = ST * STAGE + 2 * SB;
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && TM % 32 == 0 && TN % 32 == 0, "waves share the tile evenly");
-  static_assert(BM % 64 == 0 && BN % 64 == 0, "whole groups of scales");
   static_assert((ST - 1) * PER < 64 && ST >= 2 && ST <= 4, "vmcnt counts the later stages");
   static_assert(LDS <= 160 * 1024, "ring fits the CU's LDS");
 };
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
                                                                 int mtiles, Rest rest) {
   using S = Shape<BM, BN, WM, WN, ST>;
   constexpr int TM = S::TM, TN = S::TN, MT = S::MT, NT = S::NT;
-  constexpr int kWaves = S::WAVES, kXBytes = S::XB, kWBytes = S::WB;
+  constexpr int kWaves = S::WAVES, kXBytes = S::XB;
   constexpr int kCols = paired(E) ? BN / 2 : BN;  // output columns (or pairs) per tile
   static_assert(!paired(E) || NT % 2 == 0, "a wave holds both rows of its pairs");
   static_assert(E != kSwiGLUFp8 || kCols == kBlock, "a tile holds the columns of one scale");
@@ -125,19 +125,30 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   for (int i = 0; i < S::XI; ++i) xoff[i] = static_cast<uint32_t>(min(8 * (i * S::WAVES + wave) + row8, last_x)) * static_cast<uint32_t>(k);
 #pragma unroll
   for (int i = 0; i < S::WI; ++i) woff[i] = static_cast<uint32_t>(w_row(8 * (i * S::WAVES + wave) + row8)) * static_cast<uint32_t>(k);
-  // Scales: four blocks' of 64 rows per instruction, X's rows and then W's. Waves beyond the groups repeat the last.
+  // Scales: 16 bytes (16 blocks) of 16 rows per instruction, a word per lane, X's rows and then W's. Waves
+  // beyond the groups repeat the last. A row's words past its scales repeat its first.
   const uint8_t* sbase[S::SI];
   int sgroup[S::SI];
 #pragma unroll
   for (int i = 0; i < S::SI; ++i) {
     sgroup[i] = min(i * S::WAVES + wave, S::GROUPS - 1);
-    const int r = 64 * sgroup[i];
-    sbase[i] = r < BM ? xscales + static_cast<int64_t>(min(r + lane, last_x)) * stride
-                      : wscales + static_cast<int64_t>(w_row(r - BM + lane)) * stride;
+    const int r = 16 * sgroup[i] + (lane >> 2);
+    sbase[i] = r < BM ? xscales + static_cast<int64_t>(min(r, last_x)) * stride : wscales + static_cast<int64_t>(w_row(r - BM)) * stride;
   }
+  char* const scale_ring = smem + ST * S::STAGE;
+  constexpr int kScaleBytes = S::SB;
   auto issue = [&](char* stage, int b) {
     const int off = chunk < k - kBlock * b ? chunk : 0;
     asm volatile("" ::: "memory");
+    // The scales of 16 blocks with the first of them, ahead of its data (the waits count the data's
+    // instructions: a few more in flight only make one wait in 16 stages longer).
+    if ((b & 15) == 0) {
+      const int word = b + 4 * (lane & 3) < stride ? b + 4 * (lane & 3) : 0;
+#pragma unroll
+      for (int i = 0; i < S::SI; ++i)
+        __builtin_amdgcn_global_load_lds(static_cast<const void*>(sbase[i] + word),
+                                         lds_ptr(scale_ring + ((b >> 4) & 1) * kScaleBytes + sgroup[i] * 256), 4, 0, 0);
+    }
 #pragma unroll
     for (int i = 0; i < S::WI; ++i)
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(wbase + static_cast<int64_t>(kBlock) * b + woff[i] + off),
@@ -146,10 +157,6 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     for (int i = 0; i < S::XI; ++i)
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(xbase + static_cast<int64_t>(kBlock) * b + xoff[i] + off),
                                        lds_ptr(stage + (i * kWaves + wave) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < S::SI; ++i)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(sbase[i] + (b & ~3)),
-                                       lds_ptr(stage + kXBytes + kWBytes + sgroup[i] * 256), 4, 0, 0);
     asm volatile("" ::: "memory");
   };
 
@@ -195,12 +202,12 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   struct Scales {
     int x[MT], w[NT];
   };
-  auto read_scales = [&](Scales& f, uint32_t slot, int t) {
-    const uint32_t base = lds0 + slot + S::XB + S::WB + (t & 3) + 4 * r32;
+  auto read_scales = [&](Scales& f, int t) {
+    const uint32_t base = lds0 + ST * S::STAGE + ((t >> 4) & 1) * S::SB + (t & 15) + 16 * r32;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) f.w[i] = lds_byte(base + (BM + wn * TN + 32 * i) * 4);
+    for (int i = 0; i < NT; ++i) f.w[i] = lds_byte(base + (BM + wn * TN + 32 * i) * 16);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) f.x[j] = lds_byte(base + (wm * TM + 32 * j) * 4);
+    for (int j = 0; j < MT; ++j) f.x[j] = lds_byte(base + (wm * TM + 32 * j) * 16);
   };
   auto multiply = [&](const Half& f, const Scales& scales) {
 #pragma unroll
@@ -224,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   Scales now, next;
   landed(min(ST - 1, steps - 1));
   read(one, 0, 0, 0);
-  read_scales(now, 0, 0);
+  read_scales(now, 0);
   int slot = 0;
 #pragma nounroll
   for (int t = 0; t < steps; ++t) {
@@ -240,7 +247,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
       landed(min(ST - 2, steps - 2 - t));
       if (t + ST < steps) issue(smem + slot * S::STAGE, t + ST);
       read(one, following * S::STAGE, 0, t + 1);
-      read_scales(next, following * S::STAGE, t + 1);
+      read_scales(next, t + 1);
     }
     __builtin_amdgcn_sched_barrier(0);
     multiply(two, now);
