@@ -69,6 +69,9 @@ __device__ __forceinline__ uint2_t round_fp8(half8_t v, float scale) {
   return uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
+// What X holds past its columns.
+__device__ const uint4 zeros[1] = {};
+
 // The larger of two pairs of fp16 magnitudes, as bits (so that infinities and NaN come out on top).
 __device__ __forceinline__ uint32_t max_magnitudes(uint32_t a, uint32_t b) {
   typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
     const int left = k - kBlock * b;  // columns of this block and later ones
     const uint8_t* const wblock = wbase + static_cast<int64_t>(kBlock) * b;
     const char* const xblock = xbase + static_cast<int64_t>(kBlock * kXSize) * b;
-    // Chunks past the columns, in the last block alone, fetch chunk 0 of their row in place.
+    // Chunks past the columns, in the last block alone: X's are zeros, W's chunk 0 of their row in place.
     const int wc = chunk < left ? chunk : 0;
     asm volatile("" ::: "memory");
     // The scales of blocks b & ~3 .. + 3, with the first of them that this wave takes (ahead of its data: the
@@ -194,9 +197,10 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
     for (int i = 0; i < 2 * NT; ++i)
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(wblock + (woff[i] + wc)), lds_ptr(slot + kXBytes + i * 1024), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kXBytes / 1024; ++i)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xblock + (xoff[i] + (xchunk[i] < left * kXSize ? xchunk[i] : 0))),
-                                       lds_ptr(slot + i * 1024), 16, 0, 0);
+    for (int i = 0; i < kXBytes / 1024; ++i) {
+      const char* const src = xchunk[i] < left * kXSize ? xblock + (xoff[i] + xchunk[i]) : reinterpret_cast<const char*>(zeros);
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(src), lds_ptr(slot + i * 1024), 16, 0, 0);
+    }
     asm volatile("" ::: "memory");
   };
 
@@ -208,14 +212,13 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
 
   const uint32_t ring0 = lds_offset(ring);
   // 32 fp16 of a row's block in this lane, 128 in the four lanes of the row: rounded, and the scale.
-  auto round_row = [&](uint32_t base, int left, uint4_t (&eight)[2], int& scale) {
+  auto round_row = [&](uint32_t base, uint4_t (&eight)[2], int& scale) {
     half8_t v[4];
     uint32_t most = 0;
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
       const int c = 8 * (f >> 1) + 2 * g + (f & 1);
-      uint4_t words = lds_words(base + r16 * 256 + ((c ^ r16) * 16));
-      if (8 * c >= left) words = uint4_t{0, 0, 0, 0};
+      const uint4_t words = lds_words(base + r16 * 256 + ((c ^ r16) * 16));
       v[f] = __builtin_bit_cast(half8_t, words);
 #pragma unroll
       for (int e = 0; e < 4; ++e) most = max_magnitudes(most, words[e] & 0x7fff7fffu);
@@ -247,7 +250,6 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
   // row r16 of each 16 rows.
   auto unit = [&](int d, int t) {
     const int b = begin + t;
-    const int left = k - kBlock * b;
     const uint32_t scales = ring0 + D * S::UB + ((b >> 2) & 1) * S::SB;
     const int shift = 8 * (b & 3);
     const uint32_t base = ring0 + d * S::UB;
@@ -256,16 +258,11 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       if constexpr (HALFX) {
-        round_row(base + j * 4096, left, x8[j], xs[j]);
+        round_row(base + j * 4096, x8[j], xs[j]);
       } else {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           x8[j][p] = lds_words(base + j * 2048 + r16 * 128 + (((4 * p + g) ^ (r16 & 7)) * 16));
-        }
-        if (left < kBlock) {  // columns past the matrix
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-            if (16 * (4 * p + g) >= left) x8[j][p] = uint4_t{0, 0, 0, 0};
         }
         xs[j] = (lds_word(scales + 256 + (16 * j + r16) * 4) >> shift) & 255;
       }

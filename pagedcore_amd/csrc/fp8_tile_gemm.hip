@@ -16,6 +16,8 @@
 
 #include "fp8_gemm.h"
 
+#include <type_traits>
+
 namespace fp8_gemm {
 namespace {
 
@@ -42,6 +44,12 @@ __device__ __forceinline__ int4v_t lds_chunk(uint32_t addr) {
 __device__ __forceinline__ int lds_byte(uint32_t addr) {
   return *reinterpret_cast<const __attribute__((address_space(3))) uint8_t*>(static_cast<uintptr_t>(addr));
 }
+
+// What X holds past its columns.
+__device__ const uint4 zeros[1] = {};
+
+// Where chunk 0 of row r of a part is stored, of 8.
+__device__ __forceinline__ int place(int r) { return (r & 7) ^ ((r >> 4) & 1); }
 
 template <int BM, int BN, int WM, int WN, int ST>
 struct Shape {
@@ -115,16 +123,25 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   const uint8_t* const xscales = x_scales + static_cast<int64_t>(BM) * mtile * stride;
   const uint8_t* const wscales = w_scales + (E == kRope ? 0 : static_cast<int64_t>(kCols) * tile * stride);
 
-  // DMA of 1 KiB: rows 8 i .. 8 i + 7, lane L takes row 8 i + L / 8 and the chunk stored at position L % 8
-  // (chunk c of row r at c ^ (r & 7)). Chunks past the columns, in the last block alone, fetch chunk
-  // 0 of their row in place.
+  // DMA of 1 KiB: rows 8 i .. 8 i + 7 of a part, lane L takes row r = 8 i + L / 8 and the chunk stored at
+  // position L % 8: chunk c of row r at c ^ place(r), so that the 16 lanes that an operand read serves at
+  // once find 16 banks of 16 bytes (rows 0-3, 12-15, 20-23 and 24-27 of 32, or the other 16). Chunks past the
+  // columns, in the last block alone: X's are zeros, W's chunk 0 of their row in place.
   const int row8 = lane >> 3;
-  const int chunk = 16 * ((lane & 7) ^ row8);
   uint32_t xoff[S::XI], woff[S::WI];
+  int xchunk[S::XI], wchunk[S::WI];
 #pragma unroll
-  for (int i = 0; i < S::XI; ++i) xoff[i] = static_cast<uint32_t>(min(8 * (i * S::WAVES + wave) + row8, last_x)) * static_cast<uint32_t>(k);
+  for (int i = 0; i < S::XI; ++i) {
+    const int r = 8 * (i * S::WAVES + wave) + row8;
+    xchunk[i] = 16 * ((lane & 7) ^ place(r));
+    xoff[i] = static_cast<uint32_t>(min(r, last_x)) * static_cast<uint32_t>(k);
+  }
 #pragma unroll
-  for (int i = 0; i < S::WI; ++i) woff[i] = static_cast<uint32_t>(w_row(8 * (i * S::WAVES + wave) + row8)) * static_cast<uint32_t>(k);
+  for (int i = 0; i < S::WI; ++i) {
+    const int r = 8 * (i * S::WAVES + wave) + row8;
+    wchunk[i] = 16 * ((lane & 7) ^ place(r));
+    woff[i] = static_cast<uint32_t>(w_row(r)) * static_cast<uint32_t>(k);
+  }
   // Scales: 16 bytes (16 blocks) of 16 rows per instruction, a word per lane, X's rows and then W's. Waves
   // beyond the groups repeat the last. A row's words past its scales repeat its first.
   const uint8_t* sbase[S::SI];
@@ -138,7 +155,9 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   char* const scale_ring = smem + ST * S::STAGE;
   constexpr int kScaleBytes = S::SB;
   auto issue = [&](char* stage, int b) {
-    const int off = chunk < k - kBlock * b ? chunk : 0;
+    const int left = k - kBlock * b;
+    const uint8_t* const wblock = wbase + static_cast<int64_t>(kBlock) * b;
+    const char* const xblock = xbase + static_cast<int64_t>(kBlock) * b;
     asm volatile("" ::: "memory");
     // The scales of 16 blocks with the first of them, ahead of its data (the waits count the data's
     // instructions: a few more in flight only make one wait in 16 stages longer).
@@ -151,12 +170,13 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     }
 #pragma unroll
     for (int i = 0; i < S::WI; ++i)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wbase + static_cast<int64_t>(kBlock) * b + woff[i] + off),
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(wblock + (woff[i] + (wchunk[i] < left ? wchunk[i] : 0))),
                                        lds_ptr(stage + kXBytes + (i * kWaves + wave) * 1024), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < S::XI; ++i)
-      __builtin_amdgcn_global_load_lds(static_cast<const void*>(xbase + static_cast<int64_t>(kBlock) * b + xoff[i] + off),
-                                       lds_ptr(stage + (i * kWaves + wave) * 1024), 16, 0, 0);
+    for (int i = 0; i < S::XI; ++i) {
+      const char* const src = xchunk[i] < left ? xblock + (xoff[i] + xchunk[i]) : reinterpret_cast<const char*>(zeros);
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(src), lds_ptr(stage + (i * kWaves + wave) * 1024), 16, 0, 0);
+    }
     asm volatile("" ::: "memory");
   };
 
@@ -177,7 +197,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) at[s][c] = lds0 + r32 * 128 + (((4 * s + 2 * h + c) ^ (r32 & 7)) * 16);
+    for (int c = 0; c < 2; ++c) at[s][c] = lds0 + r32 * 128 + (((4 * s + 2 * h + c) ^ place(r32)) * 16);
   struct Half {
     int8v_t x[MT], w[NT];
   };
@@ -185,19 +205,11 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     const int4v_t p = lds_chunk(at[s][0] + row_base), q = lds_chunk(at[s][1] + row_base);
     return int8v_t{p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
   };
-  auto read = [&](Half& f, uint32_t slot, int s, int t) {
+  auto read = [&](Half& f, uint32_t slot, int s) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) f.w[i] = fragment(slot + S::XB + (wn * TN + 32 * i) * 128, s);
 #pragma unroll
     for (int j = 0; j < MT; ++j) f.x[j] = fragment(slot + (wm * TM + 32 * j) * 128, s);
-    const int left = k - kBlock * t - 16 * (4 * s + 2 * h);  // columns from this lane's first
-    if (k - kBlock * t < kBlock) {                           // columns past the matrix: whole chunks of 16
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f.x[j][e] = left > 16 * (e >> 2) ? f.x[j][e] : 0;
-      }
-    }
   };
   struct Scales {
     int x[MT], w[NT];
@@ -215,6 +227,11 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
 #pragma unroll
       for (int j = 0; j < MT; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.w[i], f.x[j], acc[i][j], 0, 0, 0, scales.w[i], 0, scales.x[j]);
+    // Nothing but this keeps the compiler from moving the products behind the barrier that follows.
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) asm volatile("" : "+v"(acc[i][j]));
   };
   // A stage has landed for every wave: at most `later` stages issued after it are outstanding in
   // this one, and the barrier holds until the others say the same.
@@ -226,35 +243,43 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     stage_barrier();
   };
   // The second half's operands are read before the first half's products, and the next stage's first
-  // half before the second half's, so that LDS latency and the barrier hide behind matrix work.
+  // half before the second half's, so that LDS latency and the barrier hide behind matrix work. A slot is
+  // refilled with stage t + ST once every wave has read all of stage t (the barrier).
   Half one, two;
   Scales now, next;
   landed(min(ST - 1, steps - 1));
-  read(one, 0, 0, 0);
+  read(one, 0, 0);
   read_scales(now, 0);
   int slot = 0;
-#pragma nounroll
-  for (int t = 0; t < steps; ++t) {
-    read(two, slot * S::STAGE, 1, t);
+  auto step = [&](int t, auto refill) {
+    read(two, slot * S::STAGE, 1);
     __builtin_amdgcn_sched_barrier(0);
     multiply(one, now);
     __builtin_amdgcn_sched_barrier(0);
-    // This wave has read all of stage t; once every wave has (the barrier below), its slot is
-    // refilled with stage t + ST.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int following = slot + 1 == ST ? 0 : slot + 1;
-    if (t + 1 < steps) {
+    if constexpr (decltype(refill)::value) {
+      landed(ST - 2);
+      issue(smem + slot * S::STAGE, t + ST);
+    } else {
       landed(min(ST - 2, steps - 2 - t));
-      if (t + ST < steps) issue(smem + slot * S::STAGE, t + ST);
-      read(one, following * S::STAGE, 0, t + 1);
-      read_scales(next, t + 1);
     }
+    read(one, following * S::STAGE, 0);
+    read_scales(next, t + 1);
     __builtin_amdgcn_sched_barrier(0);
     multiply(two, now);
     __builtin_amdgcn_sched_barrier(0);
     now = next;
     slot = following;
-  }
+  };
+  int t = 0;
+#pragma nounroll
+  for (; t + ST < steps; ++t) step(t, std::true_type{});
+#pragma nounroll
+  for (; t + 1 < steps; ++t) step(t, std::false_type{});
+  read(two, slot * S::STAGE, 1);
+  multiply(one, now);
+  multiply(two, now);
 
   // acc[i][j] of lane (r32, h), element 4 q + e: X row wm TM + 32 j + r32, W row wn TN + 32 i + 8 q + 4 h + e
   // of the tile.
