@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_stream_kernel(const void* x, c
         const float4_t u = total(Q + q);
         if constexpr (E == kSwiGLU) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(v[i] / (1.0f + expf(-v[i])) * u[i]);
+          for (int i = 0; i < 4; ++i) o[i] = static_cast<_Float16>(silu_mul(v[i], u[i]));
           *reinterpret_cast<half4_t*>(static_cast<_Float16*>(rest.out) + static_cast<int64_t>(row) * limit + col) = o;
         } else {
           half4_t high;

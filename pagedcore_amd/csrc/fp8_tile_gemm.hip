@@ -258,14 +258,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int following = slot + 1 == ST ? 0 : slot + 1;
-    if constexpr (decltype(refill)::value) {
-      landed(ST - 2);
-      issue(smem + slot * S::STAGE, t + ST);
-    } else {
-      landed(min(ST - 2, steps - 2 - t));
-    }
+    landed(decltype(refill)::value ? ST - 2 : min(ST - 2, steps - 2 - t));
     read(one, following * S::STAGE, 0);
     read_scales(next, t + 1);
+    if constexpr (decltype(refill)::value) issue(smem + slot * S::STAGE, t + ST);
     __builtin_amdgcn_sched_barrier(0);
     multiply(two, now);
     __builtin_amdgcn_sched_barrier(0);
@@ -297,8 +293,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
       for (int i = 0; i < P; ++i) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float gate = acc[i][j][e];
-          acc[i][j][e] = gate / (1.0f + expf(-gate)) * acc[i + P][j][e];
+          acc[i][j][e] = silu_mul(acc[i][j][e], acc[i + P][j][e]);
           most = fmaxf(most, finite_magnitude(acc[i][j][e]));
         }
       }
@@ -345,10 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
           half4_t o;
           if constexpr (E == kSwiGLU) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float gate = acc[i][j][4 * q + e];
-              o[e] = static_cast<_Float16>(gate / (1.0f + expf(-gate)) * acc[i + P][j][4 * q + e]);
-            }
+            for (int e = 0; e < 4; ++e) o[e] = static_cast<_Float16>(silu_mul(acc[i][j][4 * q + e], acc[i + P][j][4 * q + e]));
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = static_cast<_Float16>(acc[i][j][4 * q + e]);
