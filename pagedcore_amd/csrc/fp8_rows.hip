@@ -43,25 +43,35 @@ __device__ __forceinline__ uint2_t round8(const float (&y)[8], int& scale) {
                  pack4(y[4] * inverse, y[5] * inverse, y[6] * inverse, y[7] * inverse)};
 }
 
-// One block of 128 columns per 16 lanes. What bounds it: HBM (2 bytes read, 1 written per element).
+// One block of 128 columns per 16 lanes and turn, kTurns turns with every load before the first use. What bounds
+// it: HBM (2 bytes read, 1 written per element).
+constexpr int kTurns = 2;
 __global__ __launch_bounds__(kThreads) void quantize_fp8_kernel(uint8_t* values, uint8_t* scales, const _Float16* x,
-                                                                int64_t x_stride, int64_t blocks, int32_t row_blocks,
+                                                                int64_t x_stride, uint32_t blocks, uint32_t row_blocks,
                                                                 int32_t width) {
-  const int64_t block = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + threadIdx.x / 16;
-  if (block >= blocks) return;
-  const int64_t row = block / row_blocks;
-  const int in_row = static_cast<int>(block - row * row_blocks);
-  const int column = in_row * kBlock + 8 * (threadIdx.x % 16);
-  float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (column < width) {
-    const half8_t v = *reinterpret_cast<const half8_t*>(x + row * x_stride + column);
+  half8_t v[kTurns];
+  uint32_t row[kTurns], in_row[kTurns];
+  const uint32_t first = blockIdx.x * (kTurns * kThreads / 16) + threadIdx.x / 16;
+  auto column = [&](int i) { return static_cast<int>(in_row[i] * kBlock + 8 * (threadIdx.x % 16)); };
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(v[i]);
+  for (int i = 0; i < kTurns; ++i) {
+    const uint32_t block = min(first + i * (kThreads / 16), blocks - 1);  // past the end: the last again, not stored
+    row[i] = block / row_blocks;
+    in_row[i] = block - row[i] * row_blocks;
+    v[i] = half8_t{};
+    if (column(i) < width) v[i] = *reinterpret_cast<const half8_t*>(x + row[i] * x_stride + column(i));
   }
-  int scale;
-  const uint2_t packed = round8(y, scale);
-  if (column < width) *reinterpret_cast<uint2_t*>(values + row * width + column) = packed;
-  if (threadIdx.x % 16 == 0) scales[row * scale_stride(width) + in_row] = static_cast<uint8_t>(scale);
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(v[i][e]);
+    int scale;
+    const uint2_t packed = round8(y, scale);
+    if (first + i * (kThreads / 16) >= blocks) return;
+    if (column(i) < width) *reinterpret_cast<uint2_t*>(values + static_cast<int64_t>(row[i]) * width + column(i)) = packed;
+    if (threadIdx.x % 16 == 0) scales[static_cast<int64_t>(row[i]) * scale_stride(width) + in_row[i]] = static_cast<uint8_t>(scale);
+  }
 }
 
 template <int CTRL>
@@ -79,59 +89,75 @@ __device__ __forceinline__ float wave_sum(float x) {
   return add_dpp<0x121>(x);
 }
 
-constexpr int kNoDelta = -1, kHalfDelta = 0;  // else: that many fp32 partial sums (kAnySplits: `splits`)
-constexpr int kAnySplits = 64;
+constexpr int kNoDelta = -1, kHalfDelta = 0;  // else: that many fp32 partial sums
+constexpr int kAnySplits = 64;                // a count without its own instance (`splits`)
 
 // One workgroup per row, eight columns per thread and chunk. The sum of the residual stream is an
 // fp16 row (the next layer's residual), rounded as the fp16 form rounds it; the mean of squares and the
 // norm are fp32. What bounds it: at decode sizes one round trip of memory (every load is issued
-// before the first wait), at prompt sizes HBM.
-template <int CHUNKS, int DELTA>
+// before the first wait; the split counts of a decode step have instances of their own for that), at
+// prompt sizes HBM. FULL: every thread has all its chunks (no branch around the loads).
+template <int CHUNKS, bool FULL, int DELTA>
 __global__ __launch_bounds__(kThreads) void add_rms_norm_fp8_kernel(const _Float16* hidden, const void* delta,
                                                                     int64_t parts_stride, const _Float16* weight,
-                                                                    _Float16* hidden_out, uint8_t* values, uint8_t* scales,
-                                                                    int32_t splits, int32_t width, float eps) {
+                                                                    _Float16* hidden_out, uint8_t* values, int32_t splits,
+                                                                    int32_t width, uint8_t* scales, float eps) {
+  constexpr int kParts = DELTA > 0 && DELTA < kAnySplits ? DELTA : 1;
   __shared__ float wave_sums[kThreads / 64];
   const int64_t base = static_cast<int64_t>(blockIdx.x) * width;
   const int tid = threadIdx.x;
   auto column = [&](int c) { return 8 * (tid + c * kThreads); };
-  float h[CHUNKS][8];
-  half8_t wt[CHUNKS];
+  auto mine = [&](int c) { return FULL || column(c) < width; };
+  half8_t sum[CHUNKS], wt[CHUNKS], d[CHUNKS];
+  float4_t lo[CHUNKS][kParts], hi[CHUNKS][kParts];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    sum[c] = wt[c] = half8_t{};
+    if (!mine(c)) continue;
+    const int64_t at = base + column(c);
+    if constexpr (DELTA == kHalfDelta) d[c] = *reinterpret_cast<const half8_t*>(static_cast<const _Float16*>(delta) + at);
+    if constexpr (DELTA > 0) {
+#pragma unroll
+      for (int s = 0; s < kParts; ++s) {
+        lo[c][s] = *reinterpret_cast<const float4_t*>(static_cast<const float*>(delta) + at + s * parts_stride);
+        hi[c][s] = *reinterpret_cast<const float4_t*>(static_cast<const float*>(delta) + at + s * parts_stride + 4);
+      }
+    }
+    sum[c] = *reinterpret_cast<const half8_t*>(hidden + at);
+    wt[c] = *reinterpret_cast<const half8_t*>(weight + column(c));
+  }
   float squares = 0.0f;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[c][i] = 0.0f;
-    if (column(c) >= width) continue;
+    if (!mine(c)) continue;
     const int64_t at = base + column(c);
-    half8_t sum = *reinterpret_cast<const half8_t*>(hidden + at);
-    wt[c] = *reinterpret_cast<const half8_t*>(weight + column(c));
-    if constexpr (DELTA != kNoDelta) {
-      half8_t d;
-      if constexpr (DELTA == kHalfDelta) {
-        d = *reinterpret_cast<const half8_t*>(static_cast<const _Float16*>(delta) + at);
-      } else {
-        const float* parts = static_cast<const float*>(delta) + at;
-        float4_t lo = *reinterpret_cast<const float4_t*>(parts), hi = *reinterpret_cast<const float4_t*>(parts + 4);
-        for (int s = 1; s < (DELTA == kAnySplits ? splits : DELTA); ++s) {
-          lo += *reinterpret_cast<const float4_t*>(parts + s * parts_stride);
-          hi += *reinterpret_cast<const float4_t*>(parts + s * parts_stride + 4);
-        }
+    if constexpr (DELTA > 0) {  // added in split order
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          d[i] = static_cast<_Float16>(lo[i]);
-          d[i + 4] = static_cast<_Float16>(hi[i]);
+      for (int s = 1; s < kParts; ++s) {
+        lo[c][0] += lo[c][s];
+        hi[c][0] += hi[c][s];
+      }
+      if constexpr (DELTA == kAnySplits) {
+        const float* parts = static_cast<const float*>(delta) + at;
+#pragma unroll 4
+        for (int s = 1; s < splits; ++s) {
+          lo[c][0] += *reinterpret_cast<const float4_t*>(parts + s * parts_stride);
+          hi[c][0] += *reinterpret_cast<const float4_t*>(parts + s * parts_stride + 4);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] = static_cast<_Float16>(static_cast<float>(sum[i]) + static_cast<float>(d[i]));
+      for (int i = 0; i < 4; ++i) {
+        d[c][i] = static_cast<_Float16>(lo[c][0][i]);
+        d[c][i + 4] = static_cast<_Float16>(hi[c][0][i]);
+      }
     }
-    if (hidden_out != nullptr) *reinterpret_cast<half8_t*>(hidden_out + at) = sum;
+    if constexpr (DELTA != kNoDelta) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[c][i] = static_cast<float>(sum[i]);
-      squares += h[c][i] * h[c][i];
+      for (int i = 0; i < 8; ++i) sum[c][i] = static_cast<_Float16>(static_cast<float>(sum[c][i]) + static_cast<float>(d[c][i]));
     }
+    if (DELTA != kNoDelta || hidden_out != nullptr) *reinterpret_cast<half8_t*>(hidden_out + at) = sum[c];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) squares += static_cast<float>(sum[c][i]) * static_cast<float>(sum[c][i]);
   }
   squares = wave_sum(squares);
   if ((tid & 63) == 0) wave_sums[tid >> 6] = squares;
@@ -142,13 +168,18 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_fp8_kernel(const _Float
   const float norm = 1.0f / sqrtf(total / static_cast<float>(width) + eps);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const bool mine = column(c) < width;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = mine ? h[c][i] * static_cast<float>(wt[c][i]) * norm : 0.0f;  // the first product is exact
+    for (int i = 0; i < 8; ++i) {  // the first product is exact in fp32
+      y[i] = static_cast<float>(sum[c][i]) * static_cast<float>(wt[c][i]) * norm;
+    }
+    if (!FULL && !mine(c)) {  // a NaN norm times a column past the row is not the block's
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = 0.0f;
+    }
     int scale;
     const uint2_t packed = round8(y, scale);
-    if (!mine) continue;
+    if (!mine(c)) continue;
     *reinterpret_cast<uint2_t*>(values + base + column(c)) = packed;
     if (tid % 16 == 0) {
       scales[static_cast<int64_t>(blockIdx.x) * scale_stride(width) + column(c) / kBlock] = static_cast<uint8_t>(scale);
@@ -175,21 +206,28 @@ int add_rms_norm_fp8(void* values, void* scales, void* hidden_out, const void* h
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows)), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
                        static_cast<const _Float16*>(hidden), parts ? static_cast<const void*>(parts) : delta, rows * width,
-                       static_cast<const _Float16*>(weight), static_cast<_Float16*>(hidden_out),
-                       static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales), splits, width, eps);
+                       static_cast<const _Float16*>(weight), static_cast<_Float16*>(hidden_out), static_cast<uint8_t*>(values),
+                       splits, width, static_cast<uint8_t*>(scales), eps);
   };
   auto with_delta = [&](auto instance) {
     constexpr int D = decltype(instance)::value;
+    const bool full = width % (8 * kThreads) == 0;
     switch ((width / 8 - 1) / kThreads) {
-      case 0: return launch(add_rms_norm_fp8_kernel<1, D>);
-      case 1: return launch(add_rms_norm_fp8_kernel<2, D>);
-      case 2: return launch(add_rms_norm_fp8_kernel<3, D>);
-      default: return launch(add_rms_norm_fp8_kernel<4, D>);
+      case 0: return full ? launch(add_rms_norm_fp8_kernel<1, true, D>) : launch(add_rms_norm_fp8_kernel<1, false, D>);
+      case 1: return launch(add_rms_norm_fp8_kernel<2, false, D>);
+      case 2: return launch(add_rms_norm_fp8_kernel<3, false, D>);
+      default: return launch(add_rms_norm_fp8_kernel<4, false, D>);
     }
   };
-  if (parts) with_delta(std::integral_constant<int, kAnySplits>{});
+  // Two to eight parts at once where a thread has one chunk of them (the registers of more do not repay).
+  const bool one_chunk = width <= 8 * kThreads;
+  if (!parts && !delta) with_delta(std::integral_constant<int, kNoDelta>{});
   else if (delta) with_delta(std::integral_constant<int, kHalfDelta>{});
-  else with_delta(std::integral_constant<int, kNoDelta>{});
+  else if (splits == 1) with_delta(std::integral_constant<int, 1>{});
+  else if (splits == 2) with_delta(std::integral_constant<int, 2>{});
+  else if (splits == 4 && one_chunk) with_delta(std::integral_constant<int, 4>{});
+  else if (splits == 8 && one_chunk) with_delta(std::integral_constant<int, 8>{});
+  else with_delta(std::integral_constant<int, kAnySplits>{});
   return check_launch("add_rms_norm_fp8");
 }
 
@@ -213,12 +251,13 @@ int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride,
     return set_error(PC_ERR_ARGUMENT, "values and x must be 16-byte aligned, scales 4-byte aligned");
   }
   const int32_t row_blocks = (width + kBlock - 1) / kBlock;
-  if (rows > (int64_t{INT32_MAX} * (kThreads / 16)) / row_blocks) return set_error(PC_ERR_ARGUMENT, "quantize_fp8 too large");
-  const int64_t blocks = rows * row_blocks;
+  constexpr int kPerGroup = kTurns * kThreads / 16;
+  if (rows > (INT32_MAX - kPerGroup) / row_blocks) return set_error(PC_ERR_ARGUMENT, "quantize_fp8 too large");
+  const uint32_t blocks = static_cast<uint32_t>(rows * row_blocks);
   (void)hipGetLastError();
-  hipLaunchKernelGGL(quantize_fp8_kernel, dim3(static_cast<uint32_t>((blocks + kThreads / 16 - 1) / (kThreads / 16))),
-                     dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<uint8_t*>(values),
-                     static_cast<uint8_t*>(scales), static_cast<const _Float16*>(x), x_stride, blocks, row_blocks, width);
+  hipLaunchKernelGGL(quantize_fp8_kernel, dim3((blocks + kPerGroup - 1) / kPerGroup), dim3(kThreads), 0,
+                     static_cast<hipStream_t>(stream), static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales),
+                     static_cast<const _Float16*>(x), x_stride, blocks, static_cast<uint32_t>(row_blocks), width);
   return check_launch("quantize_fp8");
 }
 
