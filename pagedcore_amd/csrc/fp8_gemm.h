@@ -34,8 +34,29 @@ struct Args {
   rope_device::RopeOut rope;
 };
 
-int launch_stream(const Args& a, Form form, hipStream_t s);  // not kSwiGLUFp8
-int launch_tiles(const Args& a, Form form, hipStream_t s);   // not kPartials, e4m3 x
+// A kernel instance that can take a call, and the estimate of its time (us).
+struct Choice {
+  int index;
+  float time;
+};
+
+// An estimate's constants: a launch, a round of workgroups on the CUs, a block of 128 columns of one round (the
+// slowest wave's), 10^6 bytes of weight.
+struct Cost {
+  float launch, round, block, weight;
+};
+inline float estimate(const Cost& c, int64_t workgroups, int blocks, const Args& a) {
+  const float rounds = static_cast<float>((workgroups + 255) / 256);
+  return c.launch + rounds * (c.round + c.block * blocks) + c.weight * 1e-6f * static_cast<float>(a.n) * static_cast<float>(a.k);
+}
+
+// A q|k|v product, as fp16 or rotated: both take the same instance, so that they have the same bits.
+inline bool qkv_product(const Args& a, Form form) { return form == kRope || (form == kHalf && a.n == rope_device::kQkvElems); }
+
+Choice choose_stream(const Args& a, Form form);  // not kSwiGLUFp8
+Choice choose_tile(const Args& a, Form form);    // not kPartials, e4m3 x
+int launch_stream(const Args& a, Form form, int index, hipStream_t s);
+int launch_tile(const Args& a, Form form, int index, hipStream_t s);
 
 }  // namespace fp8_gemm
 

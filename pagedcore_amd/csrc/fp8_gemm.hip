@@ -11,7 +11,7 @@ using pc_internal::set_error;
 constexpr int kMaxRows = 1 << 16;
 constexpr int kMaxK = 1 << 22;     // tile-relative byte offsets fit 32 bits
 constexpr int kMaxQkvK = 1 << 18;  // 2560 rows of W within 32-bit offsets
-constexpr int kStreamRows = PC_FP8_STREAM_ROWS;
+constexpr int kStreamRows = PC_FP8_STREAM_ROWS;  // of fp16 x and of fp32 partial sums
 
 // The checks that both entry points share; PC_OK, or an error.
 int check(const Args& a, int64_t max_k) {
@@ -32,8 +32,14 @@ int check(const Args& a, int64_t max_k) {
   return PC_OK;
 }
 
-// Decode rows stream the weight; more rows take tiles.
-bool streams(const Args& a) { return a.m <= kStreamRows; }
+// The kernel with the shorter estimate: fp32 partial sums and fp16 x are the streams' alone, 8-bit outputs the
+// tiles'.
+int launch(const Args& a, Form form, hipStream_t s) {
+  (void)hipGetLastError();
+  const Choice stream = form == kSwiGLUFp8 ? Choice{-1, INFINITY} : choose_stream(a, form);
+  const Choice tile = form == kPartials || !a.x_scales ? Choice{-1, INFINITY} : choose_tile(a, form);
+  return stream.time <= tile.time ? launch_stream(a, form, stream.index, s) : launch_tile(a, form, tile.index, s);
+}
 
 }  // namespace
 
@@ -80,9 +86,7 @@ int pc_gemm_fp8(void* out, void* out_scales, const void* x, const void* x_scales
     return set_error(PC_ERR_ARGUMENT, "only partial sums take splits");
   }
   if (form == kSwiGLUFp8 && !x_scales) return set_error(PC_ERR_ARGUMENT, "PC_GEMM_SWIGLU_FP8 takes 8-bit x");
-  (void)hipGetLastError();
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  return form != kSwiGLUFp8 && streams(a) ? launch_stream(a, form, s) : launch_tiles(a, form, s);
+  return launch(a, form, static_cast<hipStream_t>(stream));
 }
 
 int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, const void* x, const void* x_scales,
@@ -123,9 +127,7 @@ int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, cons
   a.rope.layer_pool = pool ? static_cast<_Float16*>(pool) + static_cast<int64_t>(layer) * 2 * a.rope.kind_elems : nullptr;
   a.rope.key = static_cast<_Float16*>(key_out);
   a.rope.value = static_cast<_Float16*>(value_out);
-  (void)hipGetLastError();
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  return streams(a) ? launch_stream(a, kRope, s) : launch_tiles(a, kRope, s);
+  return launch(a, kRope, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -406,24 +406,107 @@ int launch(const Args& a, hipStream_t s) {
   return check_launch("fp8_stream_gemm");
 }
 
-template <bool HALFX, Form E>
-int launch_rows(const Args& a, hipStream_t s) {
-  return a.m <= 16 ? launch<1, 2, 4, 3, HALFX, E>(a, s) : launch<2, 2, 4, 2, HALFX, E>(a, s);
+// The instances, in the four cases of what X is and what the products run on. The constants are fitted to
+// the times of every instance at 8000 calls (m 1 to 2048, n 256 to 11264, k 256 to 5632, 1 to 8 splits, every form,
+// weights from HBM): the instance taken, of these and the tiles, is 1 % off the fastest of all on average, more
+// than 20 % off at 1 % of the calls (1.8 times at worst, where a second round has few workgroups).
+struct Instance {
+  int mt, nt, waves;
+  Cost cost;
+};
+constexpr Instance kEight[] = {  // e4m3 X on the 8-bit instruction
+    {1, 1, 4, {2.15f, 0.16f, 0.22f, 0.09f}}, {1, 2, 4, {2.22f, 0.0f, 0.32f, 0.13f}},  {2, 2, 4, {2.04f, 0.31f, 0.41f, 0.13f}},
+    {3, 2, 4, {0.93f, 1.55f, 0.55f, 0.13f}}, {4, 2, 4, {0.91f, 1.71f, 0.64f, 0.14f}}, {4, 3, 4, {0.87f, 2.21f, 0.77f, 0.13f}},
+    {4, 4, 4, {0.96f, 2.26f, 0.93f, 0.14f}},
+};
+constexpr Instance kEightExact[] = {  // e4m3 X widened: fp32 partial sums
+    {1, 2, 4, {2.16f, 0.12f, 0.47f, 0.09f}}, {2, 2, 4, {2.02f, 0.39f, 0.63f, 0.11f}}, {4, 4, 4, {0.9f, 2.5f, 1.66f, 0.2f}},
+};
+constexpr Instance kHalfX[] = {  // fp16 X rounded, on the 8-bit instruction
+    {1, 1, 4, {2.19f, 0.18f, 0.5f, 0.02f}},  {1, 2, 4, {2.22f, 0.06f, 0.56f, 0.09f}}, {1, 2, 8, {0.85f, 1.33f, 0.92f, 0.13f}},
+    {2, 3, 4, {0.93f, 1.79f, 1.13f, 0.13f}}, {2, 4, 4, {0.84f, 1.84f, 1.28f, 0.14f}},
+};
+constexpr Instance kHalfXExact[] = {
+    {1, 1, 4, {1.95f, 0.36f, 0.55f, 0.04f}}, {1, 2, 4, {2.11f, 0.27f, 0.67f, 0.08f}}, {1, 2, 8, {1.04f, 1.3f, 1.17f, 0.11f}},
+    {2, 3, 4, {0.97f, 1.77f, 1.46f, 0.16f}}, {2, 4, 4, {0.9f, 1.83f, 1.72f, 0.18f}},  {4, 4, 3, {1.08f, 2.52f, 2.74f, 0.19f}},
+};
+
+// Whether an instance can end with the rotation, as the kernel asserts, and adds in the order of the others that can.
+constexpr bool rotates(const Instance& i) {
+  return i.waves == 4 && kHalfDim % (8 * i.nt) == 0 && 2 * i.nt * 16 * i.mt <= 64 * i.waves;
 }
 
+template <int N>
+Choice fastest(const Args& a, Form form, const Instance (&instances)[N]) {
+  Choice best{-1, INFINITY};
+  for (int i = 0; i < N; ++i) {
+    const Instance& t = instances[i];
+    if (i > 0 && 16 * (t.mt - 1) >= a.m) continue;  // a second X tile without rows
+    if (qkv_product(a, form) && !rotates(t)) continue;
+    const int cols = paired(form) ? 8 * t.nt : 16 * t.nt, width = paired(form) ? a.n / 2 : a.n;
+    const int blocks = (a.k + kBlock - 1) / kBlock;
+    const int64_t workgroups =
+        static_cast<int64_t>((width + cols - 1) / cols) * a.splits * ((a.m + 16 * t.mt - 1) / (16 * t.mt));
+    const float time = estimate(t.cost, workgroups, ((blocks + a.splits - 1) / a.splits + t.waves - 1) / t.waves, a);
+    if (time < best.time) best = Choice{i, time};
+  }
+  return best;
+}
+
+// Rings of two units, three where one 16 x 16 tile leaves the LDS for them.
 template <Form E>
-int launch_form(const Args& a, hipStream_t s) {
-  return a.x_scales ? launch_rows<false, E>(a, s) : launch_rows<true, E>(a, s);
+int launch_index(const Args& a, int index, hipStream_t s) {
+  if constexpr (E == kPartials) {
+    if (a.x_scales) {
+      switch (index) {
+        case 0: return launch<1, 2, 4, 2, false, E>(a, s);
+        case 1: return launch<2, 2, 4, 2, false, E>(a, s);
+        default: return launch<4, 4, 4, 2, false, E>(a, s);
+      }
+    }
+    switch (index) {
+      case 0: return launch<1, 1, 4, 3, true, E>(a, s);
+      case 1: return launch<1, 2, 4, 2, true, E>(a, s);
+      case 2: return launch<1, 2, 8, 2, true, E>(a, s);
+      case 3: return launch<2, 3, 4, 2, true, E>(a, s);
+      case 4: return launch<2, 4, 4, 2, true, E>(a, s);
+      default: return launch<4, 4, 3, 2, true, E>(a, s);
+    }
+  } else {
+    if (a.x_scales) {
+      switch (index) {
+        case 0: return launch<1, 1, 4, 3, false, E>(a, s);
+        case 1: return launch<1, 2, 4, 2, false, E>(a, s);
+        case 2: return launch<2, 2, 4, 2, false, E>(a, s);
+        case 3: return launch<3, 2, 4, 2, false, E>(a, s);
+        case 4: return launch<4, 2, 4, 2, false, E>(a, s);
+      }
+      if constexpr (E != kRope) return index == 5 ? launch<4, 3, 4, 2, false, E>(a, s) : launch<4, 4, 4, 2, false, E>(a, s);
+    } else {
+      switch (index) {
+        case 0: return launch<1, 1, 4, 3, true, E>(a, s);
+        case 1: return launch<1, 2, 4, 2, true, E>(a, s);
+        case 4: return launch<2, 4, 4, 2, true, E>(a, s);
+      }
+      if constexpr (E != kRope) return index == 2 ? launch<1, 2, 8, 2, true, E>(a, s) : launch<2, 3, 4, 2, true, E>(a, s);
+    }
+    return pc_internal::set_error(PC_ERR_ARGUMENT, "no kernel instance %d", index);
+  }
 }
 
 }  // namespace
 
-int launch_stream(const Args& a, Form form, hipStream_t s) {
+Choice choose_stream(const Args& a, Form form) {
+  if (form == kPartials) return a.x_scales ? fastest(a, form, kEightExact) : fastest(a, form, kHalfXExact);
+  return a.x_scales ? fastest(a, form, kEight) : fastest(a, form, kHalfX);
+}
+
+int launch_stream(const Args& a, Form form, int index, hipStream_t s) {
   switch (form) {
-    case kPartials: return launch_form<kPartials>(a, s);
-    case kHalf: return launch_form<kHalf>(a, s);
-    case kSwiGLU: return launch_form<kSwiGLU>(a, s);
-    default: return launch_form<kRope>(a, s);
+    case kPartials: return launch_index<kPartials>(a, index, s);
+    case kHalf: return launch_index<kHalf>(a, index, s);
+    case kSwiGLU: return launch_index<kSwiGLU>(a, index, s);
+    default: return launch_index<kRope>(a, index, s);
   }
 }
 

@@ -376,14 +376,64 @@ int launch(const Args& a, hipStream_t s) {
   return check_launch("fp8_tile_gemm");
 }
 
+// The instances and their constants (fitted as those of fp8_stream_gemm.hip). Eight waves of 32 x 64 outputs beat
+// four of 64 x 64 (down of 2048 rows 30.5 us / 31.3); 256 x 256 outputs would spill.
+struct Instance {
+  int bm, bn;
+  Cost cost;
+};
+constexpr Instance kTiles[] = {
+    {64, 64, {3.06f, 0.0f, 0.32f, 0.07f}},   {64, 128, {0.47f, 2.44f, 0.41f, 0.07f}},  {128, 128, {0.0f, 3.34f, 0.56f, 0.08f}},
+    {128, 256, {0.0f, 4.09f, 0.92f, 0.1f}},  {192, 256, {0.0f, 3.81f, 1.29f, 0.24f}},
+};
+constexpr Instance kTilesFp8[] = {  // SwiGLU to 8 bits: 256 rows of W, the 128 columns of one scale
+    {64, 256, {0.0f, 3.54f, 0.65f, 0.1f}}, {128, 256, {0.0f, 4.56f, 0.87f, 0.07f}}, {192, 256, {0.0f, 4.45f, 1.25f, 0.16f}},
+};
+
+template <int N>
+Choice fastest(const Args& a, Form form, const Instance (&instances)[N]) {
+  Choice best{-1, INFINITY};
+  for (int i = 0; i < N; ++i) {
+    const Instance& t = instances[i];
+    const int cols = paired(form) ? t.bn / 2 : t.bn, width = paired(form) ? a.n / 2 : a.n;
+    const int64_t workgroups = static_cast<int64_t>((width + cols - 1) / cols) * ((a.m + t.bm - 1) / t.bm);
+    const float time = estimate(t.cost, workgroups, (a.k + kBlock - 1) / kBlock, a);
+    if (time < best.time) best = Choice{i, time};
+  }
+  return best;
+}
+
+template <Form E>
+int launch_index(const Args& a, int index, hipStream_t s) {
+  if constexpr (E == kSwiGLUFp8) {
+    switch (index) {
+      case 0: return launch<64, 256, 2, 4, 3, E>(a, s);
+      case 1: return launch<128, 256, 2, 4, 3, E>(a, s);
+      default: return launch<192, 256, 2, 4, 2, E>(a, s);
+    }
+  } else {
+    switch (index) {
+      case 0: return launch<64, 64, 2, 1, 4, E>(a, s);
+      case 1: return launch<64, 128, 2, 2, 4, E>(a, s);
+      case 2: return launch<128, 128, 4, 2, 4, E>(a, s);
+      case 3: return launch<128, 256, 2, 4, 3, E>(a, s);
+      default: return launch<192, 256, 2, 4, 2, E>(a, s);
+    }
+  }
+}
+
 }  // namespace
 
-int launch_tiles(const Args& a, Form form, hipStream_t s) {
+Choice choose_tile(const Args& a, Form form) {
+  return form == kSwiGLUFp8 ? fastest(a, form, kTilesFp8) : fastest(a, form, kTiles);
+}
+
+int launch_tile(const Args& a, Form form, int index, hipStream_t s) {
   switch (form) {
-    case kHalf: return launch<128, 128, 2, 2, 3, kHalf>(a, s);
-    case kSwiGLU: return launch<128, 128, 2, 2, 3, kSwiGLU>(a, s);
-    case kSwiGLUFp8: return launch<128, 256, 2, 4, 3, kSwiGLUFp8>(a, s);
-    default: return launch<128, 128, 2, 2, 3, kRope>(a, s);
+    case kHalf: return launch_index<kHalf>(a, index, s);
+    case kSwiGLU: return launch_index<kSwiGLU>(a, index, s);
+    case kSwiGLUFp8: return launch_index<kSwiGLUFp8>(a, index, s);
+    default: return launch_index<kRope>(a, index, s);
   }
 }
 
