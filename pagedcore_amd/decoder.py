@@ -32,7 +32,7 @@ from __future__ import annotations
 
 import weakref
 from dataclasses import dataclass
-from typing import Callable, Dict, Optional, Sequence, Tuple, TypeVar
+from typing import Callable, Dict, Optional, Sequence, Tuple, TypeVar, Union
 
 import numpy as np
 import torch
@@ -72,11 +72,31 @@ class LayerWeights:
 
 
 @dataclass(frozen=True, eq=False)
+class Fp8Rows:
+    """8-bit rows (_hip.quantize_fp8): a projection weight [n, k], or activations [rows, k]."""
+
+    values: Tensor  # float8_e4m3fn [rows, k]
+    scales: Tensor  # float8_e8m0fnu [rows, ceil(k / 128) rounded up to a multiple of 4]
+
+
+@dataclass(frozen=True, eq=False)
+class Fp8LayerWeights:
+    """One decoder layer with its projections in 8 bits (quantize_weights); the norms are fp16."""
+
+    input_norm: Tensor  # [2048]
+    qkv: Fp8Rows  # [2560, 2048]: q_proj | k_proj | v_proj rows
+    o_proj: Fp8Rows  # [2048, 2048]
+    post_attention_norm: Tensor  # [2048]
+    gate_up: Fp8Rows  # [2 * intermediate, 2048]: gate_proj | up_proj rows
+    down_proj: Fp8Rows  # [2048, intermediate]
+
+
+@dataclass(frozen=True, eq=False)
 class TinyLlamaWeights:
     """Embedding, layers, final norm and untied LM head (reference weights.py:64-69)."""
 
     embedding: Tensor  # [vocab, 2048]
-    layers: Tuple[LayerWeights, ...]
+    layers: Tuple[Union[LayerWeights, Fp8LayerWeights], ...]
     final_norm: Tensor  # [2048]
     lm_head: Tensor  # [vocab, 2048]
 
@@ -201,6 +221,38 @@ def pack_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
     return TinyLlamaWeights(weights.embedding, tuple(layers), weights.final_norm, weights.lm_head)
 
 
+def _quantized(rows: Tensor) -> Fp8Rows:
+    values, scales = _hip.empty_fp8(rows.shape[0], rows.shape[1], rows.device)
+    _hip.quantize_fp8(values, scales, rows)
+    return Fp8Rows(values, scales)
+
+
+def quantize_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
+    """The model with every layer's projections rounded to 8 bits, once, on the weights' GPU (the current
+    device): half the bytes that a decode step streams, and a prompt's products at the 8-bit matrix rate.
+    decode_paged, prefill_paged, DecodeGraph, PrefillGraph and DecodeWorker take the result as
+    they take the fp16 weights; the activations that enter a projection are rounded the same way, per row
+    and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. The fp16
+    projections are not kept: drop `weights` to free them."""
+    if not weights.embedding.is_cuda:
+        raise RuntimeError("quantize_weights runs on the GPU: the weights must be on a CUDA device")
+    layers = []
+    for layer in weights.layers:
+        if not isinstance(layer, LayerWeights):
+            raise ValueError("the weights are already in 8 bits")
+        if layer.down_proj.shape[1] % 16 != 0:
+            raise ValueError("8-bit projections need an MLP width that is a multiple of 16")
+        qkv = torch.cat((layer.q_proj, layer.k_proj, layer.v_proj))
+        gate_up = torch.cat((layer.gate_proj, layer.up_proj))
+        layers.append(
+            Fp8LayerWeights(
+                layer.input_norm, _quantized(qkv), _quantized(layer.o_proj), layer.post_attention_norm, _quantized(gate_up),
+                _quantized(layer.down_proj),
+            )
+        )
+    return TinyLlamaWeights(weights.embedding, tuple(layers), weights.final_norm, weights.lm_head)
+
+
 # ---------------------------------------------------------------------------------------
 # RoPE table
 # ---------------------------------------------------------------------------------------
@@ -259,6 +311,13 @@ GEMM_FEW_ROWS = 64
 QKV_SPLITS = 1
 O_PROJ_SPLITS = 4
 DOWN_SPLITS = 8
+
+
+# 8-bit projections (quantize_weights). Up to FP8_FUSED_ROWS rows o_proj and down read fp16 rows and round them on
+# the way in, as fp32 partial sums of these splits; above, their input is rounded by its producer or a launch.
+FP8_FUSED_ROWS = 32
+FP8_O_PROJ_SPLITS = 2
+FP8_DOWN_SPLITS = 4
 
 
 def _rows_splits(rows: int, n: int, k: int) -> int:
@@ -354,11 +413,15 @@ def _qkv_in_one_launch(x: Tensor, weight: Tensor) -> bool:
     return _qkv_fused(x.shape[0]) and weight.shape == (QKV_WIDTH, HIDDEN) and _kernel_operands(x, weight)
 
 
-def _qkv_projection(x: Tensor, weight: Tensor) -> Tensor:
+def _qkv_projection(x: Union[Tensor, Fp8Rows], weight: Union[Tensor, Fp8Rows]) -> Tensor:
     """q|k|v = x @ weight.T for a caller that rotates and writes it itself: the values that _qkv_rope
     rotates, bit for bit (so decode_paged and a DecodeGraph agree), as fp32 partial sums of one
     split or the fp16 product. pc_gemm_m128 and pc_gemm_rows add an unsplit product of 2560
     columns in pc_qkv_rope_append's order."""
+    if isinstance(weight, Fp8Rows):
+        qkv = torch.empty((x.values.shape[0], QKV_WIDTH), dtype=torch.float16, device=x.values.device)
+        _hip.gemm_fp8(qkv, x.values, x.scales, weight.values, weight.scales, epilogue=_hip.GEMM_HALF)
+        return qkv
     rows = x.shape[0]
     if rows <= GEMM_M128_ROWS or not _qkv_in_one_launch(x, weight):
         return _linear_parts(x, weight, QKV_SPLITS)
@@ -367,9 +430,13 @@ def _qkv_projection(x: Tensor, weight: Tensor) -> Tensor:
     return qkv
 
 
-def _qkv_rope(query: Tensor, x: Tensor, weight: Tensor, positions: Tensor, table: Tensor, **outputs) -> None:
+def _qkv_rope(query: Tensor, x: Union[Tensor, Fp8Rows], weight: Union[Tensor, Fp8Rows], positions: Tensor, table: Tensor,
+              **outputs) -> None:
     """q|k|v = x @ weight.T, RoPE and the K/V write (the outputs of _hip.rope_kv_append): one launch,
     or the projection and pc_rope_kv_append(_parts)."""
+    if isinstance(weight, Fp8Rows):
+        _hip.qkv_rope_append_fp8(query, x.values, x.scales, weight.values, weight.scales, positions, table, **outputs)
+        return
     if _qkv_in_one_launch(x, weight):
         _hip.qkv_rope_append(query, x, weight, positions, table, **outputs)
         return
@@ -417,6 +484,68 @@ def _attention_block(
     _add_rms_norm(x, hidden, _linear_parts(activated, layer.down_proj, DOWN_SPLITS // fewer), following_norm)
 
 
+def _norm_fp8(hidden: Tensor, delta: Optional[Tensor], weight: Tensor) -> Fp8Rows:
+    """hidden += delta; RMSNorm(hidden) * weight in 8 bits."""
+    values, scales = _hip.empty_fp8(hidden.shape[0], hidden.shape[1], hidden.device)
+    _hip.add_rms_norm_fp8(values, scales, None if delta is None else hidden, hidden, delta, weight, RMS_EPS)
+    return Fp8Rows(values, scales)
+
+
+def _linear_fp8(x: Union[Tensor, Fp8Rows], weight: Fp8Rows, splits: int) -> Tensor:
+    """x @ weight.T for 8-bit or fp16 x: fp32 partial sums [splits, rows, n] for a few rows of fp16 x, else the fp16
+    product, fp16 x above FP8_FUSED_ROWS rows rounded by a launch of its own."""
+    if isinstance(x, Tensor) and x.shape[0] > FP8_FUSED_ROWS:
+        x = _quantized(x)
+    values, scales = (x, None) if isinstance(x, Tensor) else (x.values, x.scales)
+    rows, n = values.shape[0], weight.values.shape[0]
+    if scales is None:
+        while splits > 1 and splits > -(-values.shape[1] // _hip.FP8_BLOCK):
+            splits //= 2
+        out = torch.empty((splits, rows, n), dtype=torch.float32, device=values.device)
+        _hip.gemm_fp8(out, values, None, weight.values, weight.scales, splits=splits)
+    else:
+        out = torch.empty((rows, n), dtype=torch.float16, device=values.device)
+        _hip.gemm_fp8(out, values, scales, weight.values, weight.scales, epilogue=_hip.GEMM_HALF)
+    return out
+
+
+def _swiglu_fp8(x: Fp8Rows, gate_up: Fp8Rows) -> Union[Tensor, Fp8Rows]:
+    """silu(x @ gate.T) * (x @ up.T), fp16 for as few rows as the down projection rounds itself, else in 8 bits."""
+    rows, width = x.values.shape[0], gate_up.values.shape[0] // 2
+    if rows <= FP8_FUSED_ROWS and width % 4 == 0:
+        activated = torch.empty((rows, width), dtype=torch.float16, device=x.values.device)
+        _hip.gemm_fp8(activated, x.values, x.scales, gate_up.values, gate_up.scales, epilogue=_hip.GEMM_SWIGLU)
+        return activated
+    values, scales = _hip.empty_fp8(rows, width, x.values.device)
+    _hip.gemm_fp8(values, x.values, x.scales, gate_up.values, gate_up.scales, out_scales=scales, epilogue=_hip.GEMM_SWIGLU_FP8)
+    return Fp8Rows(values, scales)
+
+
+def _layers(hidden: Tensor, weights: TinyLlamaWeights, attend: Callable) -> Tensor:
+    """Every decoder layer over the embedded rows `hidden` (the residual stream, in place), and the final
+    RMSNorm's fp16 rows. attend(index, x, stacked q|k|v weight) -> attention [rows, 2048] projects, rotates,
+    writes K/V and attends; x and the weight are fp16 tensors or both Fp8Rows."""
+    layers = weights.layers
+    x = torch.empty_like(hidden)
+    if isinstance(layers[0], Fp8LayerWeights):
+        rounded = _norm_fp8(hidden, None, layers[0].input_norm)
+        for index, layer in enumerate(layers):
+            attention = attend(index, rounded, layer.qkv)
+            rounded = _norm_fp8(hidden, _linear_fp8(attention, layer.o_proj, FP8_O_PROJ_SPLITS), layer.post_attention_norm)
+            activated = _swiglu_fp8(rounded, layer.gate_up)
+            delta = _linear_fp8(activated, layer.down_proj, FP8_DOWN_SPLITS)
+            if index + 1 < len(layers):
+                rounded = _norm_fp8(hidden, delta, layers[index + 1].input_norm)
+            else:
+                _add_rms_norm(x, hidden, delta, weights.final_norm)
+        return x
+    _hip.add_rms_norm(x, hidden, None, layers[0].input_norm, RMS_EPS)
+    for index, layer in enumerate(layers):
+        following = layers[index + 1].input_norm if index + 1 < len(layers) else weights.final_norm
+        _attention_block(x, hidden, layer, _fused(layer), following, lambda x, weight, index=index: attend(index, x, weight))
+    return x
+
+
 def _check_gpu(allocator: KVAllocator, weights: TinyLlamaWeights, what: str) -> None:
     """The kernels run on the GPU only: fail before any staging when the pool or the
     weights live elsewhere (there is no CPU fallback)."""
@@ -451,21 +580,17 @@ def decode_paged(
     with allocator.append_decode(request_ids):
         table = rope_table(allocator.pool.device)
         hidden = F.embedding(input_ids[:, 0], weights.embedding)  # [B, 2048]
-        x = torch.empty_like(hidden)
-        _hip.add_rms_norm(x, hidden, None, weights.layers[0].input_norm, RMS_EPS)
         batch = len(request_ids)
         workspaces: Dict[int, Tensor] = {}
-        for index, layer in enumerate(weights.layers):
 
-            def attend(x: Tensor, weight: Tensor, index: int = index) -> Tensor:
-                qkv = _qkv_projection(x, weight)
-                query = allocator.write_decode_layers_rotary(request_ids, index, qkv, table)
-                out, workspace = attend_rows(query, allocator, request_ids, index)
-                workspaces[workspace.data_ptr()] = workspace
-                return out.view(batch, HIDDEN)
+        def attend(index: int, x, weight) -> Tensor:
+            qkv = _qkv_projection(x, weight)
+            query = allocator.write_decode_layers_rotary(request_ids, index, qkv, table)
+            out, workspace = attend_rows(query, allocator, request_ids, index)
+            workspaces[workspace.data_ptr()] = workspace
+            return out.view(batch, HIDDEN)
 
-            following = weights.layers[index + 1].input_norm if index + 1 < LAYERS else weights.final_norm
-            _attention_block(x, hidden, layer, _fused(layer), following, attend)
+        x = _layers(hidden, weights, attend)
         logits = F.linear(x, weights.lm_head)
         for workspace in workspaces.values():
             _hip.check_attention_faults(workspace, "decode_paged")
@@ -593,20 +718,15 @@ class DecodeGraph:
         batch = self.batch
         ids, slots, positions = self._inputs64
         hidden = F.embedding(ids, weights.embedding)
-        x = torch.empty_like(hidden)
-        _hip.add_rms_norm(x, hidden, None, weights.layers[0].input_norm, RMS_EPS)
         query = torch.empty((batch, Q_HEADS, HEAD_DIM), dtype=torch.float16, device=pool.device)
         attention = torch.empty_like(query)
-        for index, layer in enumerate(weights.layers):
 
-            def attend(x: Tensor, weight: Tensor, index: int = index) -> Tensor:
-                _qkv_rope(query, x, weight, positions, self._table, pool=pool, layer=index, slot_mapping=slots)
-                _hip.planned_decode_attention(attention, query, pool, index, self._lens, self._plan, MAX_BLOCKS, self._workspace)
-                return attention.view(batch, HIDDEN)
+        def attend(index: int, x, weight) -> Tensor:
+            _qkv_rope(query, x, weight, positions, self._table, pool=pool, layer=index, slot_mapping=slots)
+            _hip.planned_decode_attention(attention, query, pool, index, self._lens, self._plan, MAX_BLOCKS, self._workspace)
+            return attention.view(batch, HIDDEN)
 
-            following = weights.layers[index + 1].input_norm if index + 1 < LAYERS else weights.final_norm
-            _attention_block(x, hidden, layer, _fused(layer), following, attend)
-        return F.linear(x, weights.lm_head)
+        return F.linear(_layers(hidden, weights, attend), weights.lm_head)
 
     def _take_faults(self, turn: int) -> None:
         """Wait for the step that last used staging buffer `turn` and fail closed if its copy
@@ -767,24 +887,19 @@ def _prefill_forward(ids: Tensor, positions: Tensor, slots: Tensor, weights: Tin
     tokens = ids.shape[0]
     device = ids.device
     hidden = F.embedding(ids, weights.embedding)  # [T, 2048]
-    x = torch.empty_like(hidden)
-    _hip.add_rms_norm(x, hidden, None, weights.layers[0].input_norm, RMS_EPS)
     key = torch.empty((tokens, KV_HEADS, HEAD_DIM), dtype=torch.float16, device=device)
     value = torch.empty_like(key)
     query = torch.empty((tokens, Q_HEADS, HEAD_DIM), dtype=torch.float16, device=device)
     attended = torch.empty_like(query)
-    for index, layer in enumerate(weights.layers):
 
-        def attend(x: Tensor, weight: Tensor, index: int = index) -> Tensor:
-            _qkv_rope(query, x, weight, positions, table, key_out=key, value_out=value, pool=pool, layer=index, slot_mapping=slots)
-            if on_layer is not None:
-                on_layer(index)
-            _hip.prefill_attention(attended, query, key, value)
-            return attended.view(tokens, HIDDEN)
+    def attend(index: int, x, weight) -> Tensor:
+        _qkv_rope(query, x, weight, positions, table, key_out=key, value_out=value, pool=pool, layer=index, slot_mapping=slots)
+        if on_layer is not None:
+            on_layer(index)
+        _hip.prefill_attention(attended, query, key, value)
+        return attended.view(tokens, HIDDEN)
 
-        following = weights.layers[index + 1].input_norm if index + 1 < LAYERS else weights.final_norm
-        _attention_block(x, hidden, layer, _fused(layer), following, attend)
-    return x
+    return _layers(hidden, weights, attend)
 
 
 class PrefillGraph:
