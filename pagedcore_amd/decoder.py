@@ -313,9 +313,15 @@ O_PROJ_SPLITS = 4
 DOWN_SPLITS = 8
 
 
-# 8-bit projections (quantize_weights). Up to FP8_FUSED_ROWS rows o_proj and down read fp16 rows and round them on
-# the way in, as fp32 partial sums of these splits; above, their input is rounded by its producer or a launch.
-FP8_FUSED_ROWS = 32
+# 8-bit projections (quantize_weights). Up to FP8_FUSED_ROWS rows o_proj and down round fp16 rows on the way in and give
+# fp32 partial sums of these splits; above, a launch rounds what does not come in 8 bits already. Up to
+# FP8_SWIGLU_ROWS rows SwiGLU gives fp16: its 8-bit output takes tiles of 128 columns, 44 of them a row of tiles.
+# Us per layer without attention (rounding by a launch; 8-bit SwiGLU; the fp16 projections): 1 row 30.3 (33.2, 39.2, 33.9),
+# 16 rows 31.9 (36.3, 42.7, 37.0), 64 rows 40.5 (41.7, 46.7, 45.5), 80 rows 48.3 (44.1, 46.9, 47.8), 128 rows 52.4 (46.1, 48.8,
+# 53.1); 192 rows (52.3, 52.6, 63.1), 256 rows (58.2, 57.8, 68.5), 2048 rows (173, 169, 243). Splits of 2 and 4 are within
+# 0.3 us of the best of 1, 2, 4 and 2, 4, 8 from 1 to 64 rows.
+FP8_FUSED_ROWS = 64
+FP8_SWIGLU_ROWS = 192
 FP8_O_PROJ_SPLITS = 2
 FP8_DOWN_SPLITS = 4
 
@@ -510,9 +516,9 @@ def _linear_fp8(x: Union[Tensor, Fp8Rows], weight: Fp8Rows, splits: int) -> Tens
 
 
 def _swiglu_fp8(x: Fp8Rows, gate_up: Fp8Rows) -> Union[Tensor, Fp8Rows]:
-    """silu(x @ gate.T) * (x @ up.T), fp16 for as few rows as the down projection rounds itself, else in 8 bits."""
+    """silu(x @ gate.T) * (x @ up.T): fp16 up to FP8_SWIGLU_ROWS rows, else in 8 bits."""
     rows, width = x.values.shape[0], gate_up.values.shape[0] // 2
-    if rows <= FP8_FUSED_ROWS and width % 4 == 0:
+    if rows <= FP8_SWIGLU_ROWS:
         activated = torch.empty((rows, width), dtype=torch.float16, device=x.values.device)
         _hip.gemm_fp8(activated, x.values, x.scales, gate_up.values, gate_up.scales, epilogue=_hip.GEMM_SWIGLU)
         return activated
