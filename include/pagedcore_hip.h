@@ -368,7 +368,7 @@ int32_t pc_fp8_scale_stride(int32_t width);
 
 /*
  * Rounds fp16 rows (x [rows][width], row stride x_stride elements, a multiple of 8) to 8 bits; width a
- * multiple of 16 up to 2^22. x 16-byte aligned.
+ * multiple of 16 up to 2^22, rows * ceil(width / 128) below 2^29. x 16-byte aligned.
  */
 int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride, int64_t rows, int32_t width, void* stream);
 
@@ -379,7 +379,7 @@ int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride,
  *   hidden_out = h (may be `hidden` itself; may be null where delta is null)
  *   values, scales = (h * rsqrt(mean(h^2) + eps) * weight, in fp32) rounded to 8 bits
  * The _parts form takes delta as fp32 partial sums [splits][rows][width], added in split order and
- * rounded to fp16 once, splits in [1, 64]. width a multiple of 16 up to 8192; no output may
+ * rounded to fp16 once, splits in [1, 64]. width a multiple of 16 up to 8192, rows below 2^24; no output may
  * overlap another buffer but for hidden_out and hidden; all 16-byte aligned.
  */
 int pc_add_rms_norm_fp8(void* values, void* scales, void* hidden_out, const void* hidden, const void* delta,
@@ -405,8 +405,9 @@ int pc_add_rms_norm_parts_fp8(void* values, void* scales, void* hidden_out, cons
  * splits is 1 but for PC_GEMM_PARTIALS. m in [1, 65536]; k a multiple of 16 up to 2^22; n a multiple of 4 (of 8 for
  * PC_GEMM_SWIGLU, of 32 for PC_GEMM_SWIGLU_FP8); m * k, n * k and splits * m * n up to 2^31; x, w and out 16-byte
  * aligned; out must not overlap an input. PC_GEMM_PARTIALS adds exact products in fp32. The
- * other forms may add them, above PC_FP8_STREAM_ROWS rows, on the 8-bit matrix instruction, which adds eight at a time
- * aligned to the largest: 1.5e-5 of the result's norm on normal data, beside fp16's rounding.
+ * other forms, whose outputs are rounded to fp16 or 8 bits, add them on the 8-bit matrix instruction, which takes eight
+ * at a time, aligned to the largest, and drops what lies below 2^-13 of it: at most 7 * 2^-13 of each eight's largest
+ * product, on normal data 1.5e-5 of the result's norm. The order of addition depends on m, n, k and the epilogue alone.
  */
 #define PC_GEMM_SWIGLU_FP8 4
 #define PC_FP8_STREAM_ROWS 128
@@ -416,7 +417,9 @@ int pc_gemm_fp8(void* out, void* out_scales, const void* x, const void* x_scales
 /*
  * The q|k|v projection of 8-bit rows (or fp16 ones, as above) with pc_rope_kv_append as its epilogue:
  * pc_qkv_rope_append with w [2560][k] in 8 bits, k a multiple of 16 up to 2^18. The projections are
- * PC_GEMM_HALF's, bit for bit; the other arguments and what is done with them are those of pc_qkv_rope_append.
+ * PC_GEMM_HALF's (n = 2560), bit for bit; the other arguments and what is done with them, the fp16 roundings of
+ * the rotation among it, are those of pc_qkv_rope_append: the cache holds the same bytes whichever way the product
+ * went into it.
  */
 int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, const void* x, const void* x_scales,
                            const void* w, const void* w_scales, int32_t m, int32_t k, const int64_t* positions,

@@ -641,26 +641,31 @@ def empty_fp8(rows: int, width: int, device: torch.device) -> Tuple[Tensor, Tens
     )
 
 
-def _check_fp8(name: str, values: Tensor, scales: Tensor, shape: Tuple[int, int], device: torch.device) -> None:
-    """8-bit rows of `shape` as the kernels take them."""
-    if values.dtype != _E4M3 or values.shape != shape or not values.is_contiguous() or values.device != device:
-        raise HipExtensionError(f"{name} must be contiguous float8_e4m3fn {list(shape)} on {device}")
-    expected = (shape[0], fp8_scale_stride(shape[1]))
-    if scales is None or scales.dtype != _E8M0 or scales.shape != expected or not scales.is_contiguous() or scales.device != device:
-        raise HipExtensionError(f"the scales of {name} must be contiguous float8_e8m0fnu {list(expected)} on {device}")
+def _check_fp8(name: str, values: Tensor, scales: Tensor, rows: int, width: int, device: int) -> None:
+    """8-bit rows [rows, width] as the kernels take them, on GPU `device`."""
+    if values.dtype is not _E4M3 or values.shape != (rows, width) or not values.is_contiguous() or values.get_device() != device:
+        raise HipExtensionError(f"{name} must be contiguous float8_e4m3fn [{rows}, {width}] on GPU {device}")
+    stride = (width + 511) // 512 * 4
+    if scales is None or scales.dtype is not _E8M0 or scales.shape != (rows, stride) or not scales.is_contiguous() or scales.get_device() != device:
+        raise HipExtensionError(f"the scales of {name} must be contiguous float8_e8m0fnu [{rows}, {stride}] on GPU {device}")
 
 
-def _check_half(name: str, tensor: Tensor, shape: Tuple[int, ...], device: torch.device) -> None:
-    if tensor.dtype != torch.float16 or tensor.shape != shape or not tensor.is_contiguous() or tensor.device != device:
-        raise HipExtensionError(f"{name} must be contiguous float16 {list(shape)} on {device}")
+def _check_half(name: str, tensor: Tensor, shape: Tuple[int, ...], device: int) -> None:
+    if tensor.dtype is not torch.float16 or tensor.shape != shape or not tensor.is_contiguous() or tensor.get_device() != device:
+        raise HipExtensionError(f"{name} must be contiguous float16 {list(shape)} on GPU {device}")
 
 
-def _gpu_of(tensor: Tensor) -> torch.device:
-    """The tensor's device, which has to be the current one: the launch goes to its current stream."""
-    device = tensor.device
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise HipExtensionError(f"the tensors are on {device}, which is not the current GPU")
+def _gpu_of(tensor: Tensor) -> int:
+    """The tensor's GPU, which has to be the current one: the launch goes to its current stream."""
+    device = tensor.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise HipExtensionError(f"the tensors are on {tensor.device}, which is not the current GPU")
     return device
+
+
+def _stream_of(device: int) -> int:
+    """The current stream of GPU `device`."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def quantize_fp8(values: Tensor, scales: Tensor, x: Tensor) -> None:
@@ -672,10 +677,10 @@ def quantize_fp8(values: Tensor, scales: Tensor, x: Tensor) -> None:
     if x.dim() != 2 or x.dtype != torch.float16 or (x.stride(1) != 1 and x.numel()):
         raise HipExtensionError("x must be float16 [rows, width] with unit column stride")
     rows, width = x.shape
-    _check_fp8("values", values, scales, (rows, width), device)
+    _check_fp8("values", values, scales, rows, width, device)
     lib = load()
     stride = x.stride(0) if rows > 1 else width
-    status = lib.pc_quantize_fp8(values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows, width, _stream(device))
+    status = lib.pc_quantize_fp8(values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows, width, _stream_of(device))
     if status:
         _check(lib, "pc_quantize_fp8", status)
 
@@ -690,42 +695,44 @@ def add_rms_norm_fp8(
     device = _gpu_of(hidden)
     if hidden.dim() != 2:
         raise HipExtensionError("hidden must be float16 [rows, width]")
-    rows, width = shape = tuple(hidden.shape)
+    rows, width = shape = hidden.shape
     _check_half("hidden", hidden, shape, device)
     _check_half("weight", weight, (width,), device)
-    _check_fp8("values", values, scales, shape, device)
+    _check_fp8("values", values, scales, rows, width, device)
     if hidden_out is not None:
         _check_half("hidden_out", hidden_out, shape, device)
     lib = load()
     if delta is not None and delta.dim() == 3:
-        if delta.dtype != torch.float32 or delta.shape[1:] != shape or not delta.is_contiguous() or delta.device != device:
-            raise HipExtensionError(f"partial sums must be contiguous float32 [splits, {rows}, {width}] on {device}")
+        if delta.dtype != torch.float32 or delta.shape[1:] != shape or not delta.is_contiguous() or delta.get_device() != device:
+            raise HipExtensionError(f"partial sums must be contiguous float32 [splits, {rows}, {width}] on GPU {device}")
         status = lib.pc_add_rms_norm_parts_fp8(
             values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), delta.data_ptr(), delta.shape[0],
-            weight.data_ptr(), rows, width, eps, _stream(device),
+            weight.data_ptr(), rows, width, eps, _stream_of(device),
         )
     else:
         if delta is not None:
             _check_half("delta", delta, shape, device)
         status = lib.pc_add_rms_norm_fp8(
             values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), _ptr(delta), weight.data_ptr(), rows,
-            width, eps, _stream(device),
+            width, eps, _stream_of(device),
         )
     if status:
         _check(lib, "pc_add_rms_norm_fp8", status)
 
 
-def _check_fp8_product(x: Tensor, x_scales: Optional[Tensor], w: Tensor, w_scales: Tensor) -> torch.device:
+def _check_fp8_product(x: Tensor, x_scales: Optional[Tensor], w: Tensor, w_scales: Tensor) -> Tuple[int, int, int, int]:
+    """(GPU, m, n, k) of the operands of an 8-bit projection."""
     device = _gpu_of(x)
     if x.dim() != 2 or w.dim() != 2:
         raise HipExtensionError("x and w must be [m, k] and [n, k]")
     m, k = x.shape
+    n = w.shape[0]
     if x_scales is None:
         _check_half("x without scales", x, (m, k), device)
     else:
-        _check_fp8("x", x, x_scales, (m, k), device)
-    _check_fp8("w", w, w_scales, (w.shape[0], k), device)
-    return device
+        _check_fp8("x", x, x_scales, m, k, device)
+    _check_fp8("w", w, w_scales, n, k, device)
+    return device, m, n, k
 
 
 def gemm_fp8(
@@ -737,13 +744,12 @@ def gemm_fp8(
     [splits, m, n] (GEMM_PARTIALS, up to FP8_STREAM_ROWS rows), float16 [m, n] (GEMM_HALF) or [m, n // 2]
     (GEMM_SWIGLU, w the stacked [gate | up] weight), or 8-bit rows [m, n // 2] with out_scales
     (GEMM_SWIGLU_FP8)."""
-    device = _check_fp8_product(x, x_scales, w, w_scales)
-    (m, k), n = x.shape, w.shape[0]
+    device, m, n, k = _check_fp8_product(x, x_scales, w, w_scales)
     if epilogue == GEMM_SWIGLU_FP8:
-        _check_fp8("out", out, out_scales, (m, n // 2), device)
+        _check_fp8("out", out, out_scales, m, n // 2, device)
     elif epilogue == GEMM_PARTIALS:
-        if out.dtype != torch.float32 or out.shape != (splits, m, n) or not out.is_contiguous() or out.device != device:
-            raise HipExtensionError(f"out must be contiguous float32 [{splits}, {m}, {n}] on {device}")
+        if out.dtype is not torch.float32 or out.shape != (splits, m, n) or not out.is_contiguous() or out.get_device() != device:
+            raise HipExtensionError(f"out must be contiguous float32 [{splits}, {m}, {n}] on GPU {device}")
     elif epilogue == GEMM_HALF or epilogue == GEMM_SWIGLU:
         _check_half("out", out, (m, n if epilogue == GEMM_HALF else n // 2), device)
     else:
@@ -751,7 +757,7 @@ def gemm_fp8(
     lib = load()
     status = lib.pc_gemm_fp8(
         out.data_ptr(), _ptr(out_scales), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), m, n, k, splits,
-        epilogue, _stream(device),
+        epilogue, _stream_of(device),
     )
     if status:
         _check(lib, "pc_gemm_fp8", status)
@@ -774,18 +780,19 @@ def qkv_rope_append_fp8(
 ) -> None:
     """qkv_rope_append of 8-bit rows (or float16 ones, as gemm_fp8 takes them) by the stacked q | k | v weight
     [2560, k] in 8 bits, in one launch (pc_qkv_rope_append_fp8)."""
-    device = _check_fp8_product(x, x_scales, w, w_scales)
-    m, k = x.shape
-    if w.shape[0] != 2560:
+    device, m, n, k = _check_fp8_product(x, x_scales, w, w_scales)
+    if n != 2560:
         raise HipExtensionError("w must be [2560, k]")
-    if query_out.numel() != m * 2048 or query_out.dtype != torch.float16 or not query_out.is_contiguous() or query_out.device != device:
-        raise HipExtensionError(f"query_out must be contiguous float16 [{m}, 32, 64] on {device}")
+    if query_out.numel() != m * 2048 or query_out.dtype is not torch.float16 or not query_out.is_contiguous() or query_out.get_device() != device:
+        raise HipExtensionError(f"query_out must be contiguous float16 [{m}, 32, 64] on GPU {device}")
     for name, rows in (("key_out", key_out), ("value_out", value_out)):
         if rows is not None:
             _check_half(name, rows, (m, 4, 64), device)
     for name, rows in (("positions", positions), ("slot_mapping", slot_mapping)):
-        if rows is not None and (rows.dtype != torch.int64 or rows.shape != (m,) or not rows.is_contiguous() or rows.device != device):
-            raise HipExtensionError(f"{name} must be contiguous int64 [{m}] on {device}")
+        if rows is not None and (
+            rows.dtype is not torch.int64 or rows.shape != (m,) or not rows.is_contiguous() or rows.get_device() != device
+        ):
+            raise HipExtensionError(f"{name} must be contiguous int64 [{m}] on GPU {device}")
     if rope_table.dim() != 3:
         raise HipExtensionError("rope_table must be float16 [positions, 2, 32]")
     _check_half("rope_table", rope_table, (rope_table.shape[0], 2, 32), device)
@@ -797,7 +804,7 @@ def qkv_rope_append_fp8(
     status = lib.pc_qkv_rope_append_fp8(
         query_out.data_ptr(), _ptr(key_out), _ptr(value_out), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(),
         m, k, positions.data_ptr(), rope_table.data_ptr(), rope_table.shape[0], _ptr(pool),
-        pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping), _stream(device),
+        pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping), _stream_of(device),
     )
     if status:
         _check(lib, "pc_qkv_rope_append_fp8", status)

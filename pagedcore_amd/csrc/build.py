@@ -66,6 +66,10 @@ GUARDED_KERNELS: Dict[str, int] = {
     "gemm_stream_kernelILi1ELi2ELi4ELi2E": 3,  # three (48 KB)
     "gemm_tile_kernel": 2,  # a workgroup of eight waves
     "gemm_tile_kernelILi128ELi192ELi4ELi2ELi2E": 4,  # two of them (80 KB): SwiGLU of long prompts
+    "fp8_stream_kernel": 1,  # a workgroup of four waves alone
+    "fp8_stream_kernelILi2ELi4ELi8E": 2,  # of eight
+    "fp8_stream_kernelILi1ELi2ELi4ELi2ELb0E": 3,  # three of four waves (52 KB)
+    "fp8_tile_kernel": 2,  # a workgroup of eight waves
 }
 
 _NOISE = "packed-fp32-ops' is not a recognized feature"

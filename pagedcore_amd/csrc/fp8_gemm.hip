@@ -79,11 +79,11 @@ int pc_gemm_fp8(void* out, void* out_scales, const void* x, const void* x_scales
       return set_error(PC_ERR_ARGUMENT, "splits %d outside [1, 64] or more than k's %d blocks", splits, blocks);
     }
     if (m > kStreamRows) return set_error(PC_ERR_ARGUMENT, "fp32 partial sums take up to %d rows, not %d", kStreamRows, m);
-    if (static_cast<int64_t>(splits) * m * n > (int64_t{1} << 31)) {
-      return set_error(PC_ERR_ARGUMENT, "GEMM of %d x %d x %d with %d splits too large", m, n, k, splits);
-    }
   } else if (splits != 1) {
     return set_error(PC_ERR_ARGUMENT, "only partial sums take splits");
+  }
+  if (static_cast<int64_t>(splits) * m * n > (int64_t{1} << 31)) {  // keeps a grid's threads within 32 bits, too
+    return set_error(PC_ERR_ARGUMENT, "GEMM of %d x %d x %d with %d splits too large", m, n, k, splits);
   }
   if (form == kSwiGLUFp8 && !x_scales) return set_error(PC_ERR_ARGUMENT, "PC_GEMM_SWIGLU_FP8 takes 8-bit x");
   return launch(a, form, static_cast<hipStream_t>(stream));

@@ -30,6 +30,8 @@ typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 constexpr int kMaxWidth = 1 << 22;
+constexpr int kMaxNormRows = (1 << 24) - 1;     // a workgroup each: a grid's threads stay within 32 bits
+constexpr int kMaxQuantizeBlocks = 1 << 29;    // eight threads each
 constexpr int kNormMaxChunks = 4;  // rows of up to 4 * 256 * 8 = 8192
 
 // Eight columns of a row per lane, the 16 lanes of a wave row one block: its scale, and the values.
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_fp8_kernel(const _Float
 int add_rms_norm_fp8(void* values, void* scales, void* hidden_out, const void* hidden, const void* delta,
                      const float* parts, int32_t splits, const void* weight, int64_t rows, int32_t width, float eps,
                      void* stream) {
-  if (rows < 0 || rows > INT32_MAX) return set_error(PC_ERR_ARGUMENT, "rows %lld out of range", static_cast<long long>(rows));
+  if (rows < 0 || rows > kMaxNormRows) return set_error(PC_ERR_ARGUMENT, "rows %lld out of range", static_cast<long long>(rows));
   if (width < 16 || width % 16 != 0 || width > 8 * kThreads * kNormMaxChunks) {
     return set_error(PC_ERR_ARGUMENT, "width %d must be a multiple of 16 in [16, %d]", width, 8 * kThreads * kNormMaxChunks);
   }
@@ -252,7 +254,7 @@ int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride,
   }
   const int32_t row_blocks = (width + kBlock - 1) / kBlock;
   constexpr int kPerGroup = kTurns * kThreads / 16;
-  if (rows > (INT32_MAX - kPerGroup) / row_blocks) return set_error(PC_ERR_ARGUMENT, "quantize_fp8 too large");
+  if (rows > (kMaxQuantizeBlocks - kPerGroup) / row_blocks) return set_error(PC_ERR_ARGUMENT, "quantize_fp8 too large");
   const uint32_t blocks = static_cast<uint32_t>(rows * row_blocks);
   (void)hipGetLastError();
   hipLaunchKernelGGL(quantize_fp8_kernel, dim3((blocks + kPerGroup - 1) / kPerGroup), dim3(kThreads), 0,

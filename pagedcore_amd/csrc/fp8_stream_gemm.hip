@@ -90,7 +90,7 @@ struct Shape {
   static constexpr int SUMS = WAVES * MT * NT * 1024;
   static constexpr int LDS = RING > SUMS ? RING : SUMS;
   static_assert(LDS <= 160 * 1024, "ring and accumulator exchange fit the CU's LDS");
-  static_assert((D - 1) * PER < 64 && D >= 2 && D <= 4, "vmcnt counts the later units");
+  static_assert((D - 1) * PER < 64 && D >= 1 && D <= 4, "vmcnt counts the later units");
   static_assert(NT <= 4 && MT <= 4, "one scale word per lane");
 };
 
@@ -407,7 +407,7 @@ int launch(const Args& a, hipStream_t s) {
 }
 
 // The instances, in the four cases of what X is and what the products run on. The constants are fitted to
-// the times of every instance at 8000 calls (m 1 to 2048, n 256 to 11264, k 256 to 5632, 1 to 8 splits, every form,
+// the times of every instance at 12000 calls (m 1 to 2048, n 256 to 11264, k 256 to 5632, 1 to 8 splits, every form,
 // weights from HBM): the instance taken, of these and the tiles, is 1 % off the fastest of all on average, more
 // than 20 % off at 1 % of the calls (1.8 times at worst, where a second round has few workgroups).
 struct Instance {
@@ -423,12 +423,12 @@ constexpr Instance kEightExact[] = {  // e4m3 X widened: fp32 partial sums
     {1, 2, 4, {2.16f, 0.12f, 0.47f, 0.09f}}, {2, 2, 4, {2.02f, 0.39f, 0.63f, 0.11f}}, {4, 4, 4, {0.9f, 2.5f, 1.66f, 0.2f}},
 };
 constexpr Instance kHalfX[] = {  // fp16 X rounded, on the 8-bit instruction
-    {1, 1, 4, {2.19f, 0.18f, 0.5f, 0.02f}},  {1, 2, 4, {2.22f, 0.06f, 0.56f, 0.09f}}, {1, 2, 8, {0.85f, 1.33f, 0.92f, 0.13f}},
-    {2, 3, 4, {0.93f, 1.79f, 1.13f, 0.13f}}, {2, 4, 4, {0.84f, 1.84f, 1.28f, 0.14f}},
+    {1, 1, 4, {2.15f, 0.19f, 0.5f, 0.03f}}, {1, 2, 4, {2.18f, 0.09f, 0.55f, 0.1f}},  {1, 2, 8, {0.82f, 1.35f, 0.92f, 0.13f}},
+    {2, 2, 8, {0.96f, 1.43f, 1.4f, 0.2f}},  {2, 4, 4, {0.88f, 1.81f, 1.27f, 0.15f}},
 };
 constexpr Instance kHalfXExact[] = {
-    {1, 1, 4, {1.95f, 0.36f, 0.55f, 0.04f}}, {1, 2, 4, {2.11f, 0.27f, 0.67f, 0.08f}}, {1, 2, 8, {1.04f, 1.3f, 1.17f, 0.11f}},
-    {2, 3, 4, {0.97f, 1.77f, 1.46f, 0.16f}}, {2, 4, 4, {0.9f, 1.83f, 1.72f, 0.18f}},  {4, 4, 3, {1.08f, 2.52f, 2.74f, 0.19f}},
+    {1, 1, 4, {1.95f, 0.35f, 0.56f, 0.04f}}, {1, 2, 4, {2.11f, 0.26f, 0.68f, 0.08f}}, {1, 2, 8, {1.04f, 1.3f, 1.16f, 0.12f}},
+    {2, 2, 8, {1.07f, 1.44f, 1.72f, 0.19f}}, {2, 4, 8, {1.09f, 1.89f, 2.47f, 0.19f}}, {4, 4, 4, {1.1f, 2.37f, 2.83f, 0.25f}},
 };
 
 // Whether an instance can end with the rotation, as the kernel asserts, and adds in the order of the others that can.
@@ -453,7 +453,8 @@ Choice fastest(const Args& a, Form form, const Instance (&instances)[N]) {
   return best;
 }
 
-// Rings of two units, three where one 16 x 16 tile leaves the LDS for them.
+// Rings of two units, three where a 16 x 16 tile leaves the LDS for them. An fp16 X fills it: there eight waves of one
+// unit each beat four of two (down of 64 rows at 2 splits 9.1 us / 10.8, of 128 rows 12.7 / 14.7).
 template <Form E>
 int launch_index(const Args& a, int index, hipStream_t s) {
   if constexpr (E == kPartials) {
@@ -468,9 +469,9 @@ int launch_index(const Args& a, int index, hipStream_t s) {
       case 0: return launch<1, 1, 4, 3, true, E>(a, s);
       case 1: return launch<1, 2, 4, 2, true, E>(a, s);
       case 2: return launch<1, 2, 8, 2, true, E>(a, s);
-      case 3: return launch<2, 3, 4, 2, true, E>(a, s);
-      case 4: return launch<2, 4, 4, 2, true, E>(a, s);
-      default: return launch<4, 4, 3, 2, true, E>(a, s);
+      case 3: return launch<2, 2, 8, 1, true, E>(a, s);
+      case 4: return launch<2, 4, 8, 1, true, E>(a, s);
+      default: return launch<4, 4, 4, 1, true, E>(a, s);
     }
   } else {
     if (a.x_scales) {
@@ -488,7 +489,7 @@ int launch_index(const Args& a, int index, hipStream_t s) {
         case 1: return launch<1, 2, 4, 2, true, E>(a, s);
         case 4: return launch<2, 4, 4, 2, true, E>(a, s);
       }
-      if constexpr (E != kRope) return index == 2 ? launch<1, 2, 8, 2, true, E>(a, s) : launch<2, 3, 4, 2, true, E>(a, s);
+      if constexpr (E != kRope) return index == 2 ? launch<1, 2, 8, 2, true, E>(a, s) : launch<2, 2, 8, 1, true, E>(a, s);
     }
     return pc_internal::set_error(PC_ERR_ARGUMENT, "no kernel instance %d", index);
   }

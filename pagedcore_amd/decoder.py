@@ -314,16 +314,21 @@ DOWN_SPLITS = 8
 
 
 # 8-bit projections (quantize_weights). Up to FP8_FUSED_ROWS rows o_proj and down round fp16 rows on the way in and give
-# fp32 partial sums of these splits; above, a launch rounds what does not come in 8 bits already. Up to
-# FP8_SWIGLU_ROWS rows SwiGLU gives fp16: its 8-bit output takes tiles of 128 columns, 44 of them a row of tiles.
-# Us per layer without attention (rounding by a launch; 8-bit SwiGLU; the fp16 projections): 1 row 30.3 (33.2, 39.2, 33.9),
-# 16 rows 31.9 (36.3, 42.7, 37.0), 64 rows 40.5 (41.7, 46.7, 45.5), 80 rows 48.3 (44.1, 46.9, 47.8), 128 rows 52.4 (46.1, 48.8,
-# 53.1); 192 rows (52.3, 52.6, 63.1), 256 rows (58.2, 57.8, 68.5), 2048 rows (173, 169, 243). Splits of 2 and 4 are within
-# 0.3 us of the best of 1, 2, 4 and 2, 4, 8 from 1 to 64 rows.
+# fp32 partial sums; above, a launch rounds what does not come in 8 bits already. Up to FP8_SWIGLU_ROWS
+# rows SwiGLU gives fp16: its 8-bit output takes tiles of 128 columns, 44 of them a row of tiles.
+# Us per layer without attention (rounding by a launch; 8-bit SwiGLU; the fp16 projections): 1 row 30.5 (33.6, 39.4, 34.0),
+# 16 rows 31.9 (36.2, 42.8, 37.0), 64 rows 39.7 (41.7, 46.8, 45.6), 80 rows 45.4 (44.3, 47.1, 47.9), 128 rows 47.6 (46.1, 49.0,
+# 53.1); 192 rows (52.4, 52.7, 63.0), 256 rows (58.3, 58.0, 68.7), 2048 rows (173, 169, 242). Of 1, 2 and 4 splits for o_proj
+# and 2, 4 and 8 for down, these are within 0.4 us of the best at every row count.
 FP8_FUSED_ROWS = 64
 FP8_SWIGLU_ROWS = 192
 FP8_O_PROJ_SPLITS = 2
-FP8_DOWN_SPLITS = 4
+
+
+def _fp8_down_splits(rows: int) -> int:
+    """K splits of the down projection on fp16 rows (16 rows: 32.0 us per layer, with 2 splits 33.0; 64 rows: 39.7,
+    with 4 40.5)."""
+    return 4 if rows <= 32 else 2
 
 
 def _rows_splits(rows: int, n: int, k: int) -> int:
@@ -539,7 +544,7 @@ def _layers(hidden: Tensor, weights: TinyLlamaWeights, attend: Callable) -> Tens
             attention = attend(index, rounded, layer.qkv)
             rounded = _norm_fp8(hidden, _linear_fp8(attention, layer.o_proj, FP8_O_PROJ_SPLITS), layer.post_attention_norm)
             activated = _swiglu_fp8(rounded, layer.gate_up)
-            delta = _linear_fp8(activated, layer.down_proj, FP8_DOWN_SPLITS)
+            delta = _linear_fp8(activated, layer.down_proj, _fp8_down_splits(hidden.shape[0]))
             if index + 1 < len(layers):
                 rounded = _norm_fp8(hidden, delta, layers[index + 1].input_norm)
             else:

@@ -62,7 +62,7 @@ def _refused(status: int, needle: bytes) -> None:
     ({"width": 0}, b"width"), ({"width": 24}, b"multiple of 16"), ({"width": (1 << 22) + 16}, b"width"),
     ({"rows": -1}, b"negative"), ({"stride": 48}, b"x_stride"), ({"stride": 68}, b"x_stride"),
     ({"x": P + 8}, b"aligned"), ({"values": P + 8}, b"aligned"), ({"scales": P + 2}, b"aligned"),
-    ({"rows": 1 << 60}, b"too large"),
+    ({"rows": 1 << 60}, b"too large"), ({"rows": 1 << 29}, b"too large"),
 ])
 def test_quantize_refuses(change, needle):
     a = {"values": P, "scales": P, "x": P, "stride": 64, "rows": 1, "width": 64, **change}
@@ -79,7 +79,7 @@ def test_no_rows_are_no_work():
 @pytest.mark.parametrize("change,needle", [
     ({"values": None}, b"null pointer"), ({"scales": None}, b"null pointer"), ({"hidden": None}, b"null pointer"),
     ({"weight": None}, b"null pointer"), ({"hidden_out": None}, b"hidden_out"), ({"width": 24}, b"multiple of 16"),
-    ({"width": 8208}, b"width"), ({"width": 0}, b"width"), ({"rows": -1}, b"rows"), ({"rows": 1 << 31}, b"rows"),
+    ({"width": 8208}, b"width"), ({"width": 0}, b"width"), ({"rows": -1}, b"rows"), ({"rows": 1 << 24}, b"rows"),
     ({"eps": -1.0}, b"eps"), ({"eps": float("nan")}, b"eps"), ({"hidden": P + 2}, b"aligned"), ({"delta": P + 4}, b"aligned"),
     ({"hidden_out": P + 8}, b"aligned"), ({"scales": P + 1}, b"aligned"), ({"values": P + 4}, b"aligned"),
 ])
@@ -110,7 +110,7 @@ def test_norm_parts_refuses(delta, splits, needle):
     ({"epilogue": 0, "splits": 0}, b"splits"), ({"epilogue": 0, "splits": 65}, b"splits"), ({"epilogue": 0, "splits": 3, "k": 256}, b"2 blocks"),
     ({"out": P + 8}, b"aligned"), ({"x": P + 8}, b"aligned"), ({"w": P + 4}, b"aligned"), ({"x_scales": P + 2}, b"aligned"),
     ({"w_scales": P + 1}, b"aligned"), ({"n": 1 << 20, "k": 4096}, b"too large"), ({"m": 65536, "k": 65536}, b"too large"),
-    ({"epilogue": 0, "splits": 64, "m": 128, "n": 1 << 20, "k": 8192 // 4}, b"splits"),
+    ({"epilogue": 0, "splits": 17, "k": 2048}, b"16 blocks"), ({"m": 65536, "n": 1 << 16, "k": 16}, b"too large"),
 ])
 def test_gemm_refuses(change, needle):
     a = {"out": P, "out_scales": None, "x": P, "x_scales": P, "w": P, "w_scales": P, "m": 8, "n": 64, "k": 128, "splits": 1,

@@ -402,3 +402,110 @@ def test_qkv_is_the_half_product_rotated_and_written(device, m, k, half_x):
     only = torch.empty((m, 32, 64), dtype=torch.float16, device=device)
     _hip.qkv_rope_append_fp8(only, eight, xs, w, ws, positions, table)  # no pool, no copies
     _same_bits(only, outs[0][0])
+
+
+# ---------------------------------------------------------------------------------------
+# Large buffers, graphs, refusals of the binding
+# ---------------------------------------------------------------------------------------
+
+
+def test_rows_past_32_bit_offsets(device):
+    """More than 2^31 elements, read and written: the last rows are those of a small call."""
+    rows, width = 1_100_000, 2048
+    x = torch.zeros((rows, width), dtype=torch.float16, device=device)
+    x[-5:] = _normal(device, (5, width), seed=30)
+    values, scales = _eight(x)
+    few = _eight(x[-5:].clone())
+    _same_bits(values[-5:], few[0])
+    _same_bits(scales[-5:], few[1])
+    weight = torch.ones(width, dtype=torch.float16, device=device)
+    out = torch.empty_like(x)
+    _hip.add_rms_norm_fp8(values, scales, out, x, x, weight)
+    few_out = torch.empty_like(x[-5:])
+    few = _hip.empty_fp8(5, width, device)
+    _hip.add_rms_norm_fp8(*few, few_out, x[-5:].clone(), x[-5:].clone(), weight)
+    _same_bits(values[-5:], few[0])
+    _same_bits(scales[-5:], few[1])
+    assert torch.equal(out[-5:], few_out)
+
+
+def test_products_at_the_largest_operands(device):
+    """n * k = 2^31 for one row, and 65536 rows: the ends hold what products of their own rows hold, exactly (whole numbers)."""
+    k = 2048
+    w, ws = _whole_rows(device, 1 << 20, k, seed=31)
+    x, xs = _whole_rows(device, 2, k, seed=32)
+    out = torch.empty((2, 1 << 20), dtype=torch.float16, device=device)
+    _hip.gemm_fp8(out, x, xs, w, ws, epilogue=_hip.GEMM_HALF)
+    for part in (slice(0, 40), slice(-40, None)):
+        expected = _stands(x, xs) @ _stands(w[part], ws[part]).t()
+        assert torch.equal(out[:, part].cpu(), expected.half())
+    del w, ws
+    x, xs = _whole_rows(device, 65536, k, seed=33)
+    w, ws = _whole_rows(device, 132, k, seed=34)
+    out = torch.empty((65536, 132), dtype=torch.float16, device=device)
+    _hip.gemm_fp8(out, x, xs, w, ws, epilogue=_hip.GEMM_HALF)
+    for part in (slice(0, 40), slice(-40, None)):
+        assert torch.equal(out[part].cpu(), (_stands(x[part], xs[part]) @ _stands(w, ws).t()).half())
+
+
+def test_captured_chain_replays_on_new_inputs(device):
+    """norm, SwiGLU to 8 bits and down projection in one graph, inputs changed in place between replays with eager
+    work and synchronizations: every replay equals the eager calls, bit for bit."""
+    from pagedcore_amd.decoder import capture_graph
+
+    m, width = 150, 272
+    weight = torch.ones(2048, dtype=torch.float16, device=device)
+    gate_up, down = _eight(_normal(device, (2 * width, 2048), 40, 0.05)), _eight(_normal(device, (2048, width), 41, 0.05))
+    hidden, delta = torch.empty((m, 2048), dtype=torch.float16, device=device), torch.empty((3, m, 2048), device=device)
+
+    def fill(turn):
+        hidden.copy_(_normal(device, (m, 2048), 50 + turn))
+        delta.normal_(generator=_gen(device, 60 + turn))
+
+    def chain():
+        x, xs = _hip.empty_fp8(m, 2048, device)
+        total = torch.empty_like(hidden)
+        _hip.add_rms_norm_fp8(x, xs, total, hidden, delta, weight)
+        a, a_s = _hip.empty_fp8(m, width, device)
+        _hip.gemm_fp8(a, x, xs, *gate_up, out_scales=a_s, epilogue=_hip.GEMM_SWIGLU_FP8)
+        y = torch.empty((m, 2048), dtype=torch.float16, device=device)
+        _hip.gemm_fp8(y, a, a_s, *down, epilogue=_hip.GEMM_HALF)
+        return total, y
+
+    fill(0)
+    chain()
+    graph, held = capture_graph(chain, device)
+    for turn in range(1, 5):
+        fill(turn)
+        graph.replay()
+        got = [t.clone() for t in held]
+        torch.cuda.synchronize()
+        for a, b in zip(got, chain()):
+            _same_bits(a, b)
+
+
+def test_the_binding_refuses(device):
+    x = torch.zeros((4, 64), dtype=torch.float16, device=device)
+    values, scales = _hip.empty_fp8(4, 64, device)
+    for call, needle in [
+        (lambda: _hip.quantize_fp8(values, scales, x.float()), "float16"),
+        (lambda: _hip.quantize_fp8(values, scales, x.t()), "unit column stride|float8_e4m3fn"),
+        (lambda: _hip.quantize_fp8(values[:3], scales[:3], x), "float8_e4m3fn"),
+        (lambda: _hip.quantize_fp8(values, scales[:, :0], x), "scales"),
+        (lambda: _hip.quantize_fp8(values, scales.cpu(), x), "scales"),
+        (lambda: _hip.quantize_fp8(values, scales.view(torch.uint8), x), "scales"),
+        (lambda: _hip.quantize_fp8(values, scales, x.cpu()), "not the current GPU"),
+        (lambda: _hip.quantize_fp8(values, scales, x[:1].expand(4, 64)), "x_stride"),
+        (lambda: _hip.add_rms_norm_fp8(values, scales, None, x, x, x[0].clone()), "hidden_out"),
+        (lambda: _hip.add_rms_norm_fp8(values, scales, x, x, x[:3], x[0].clone()), "delta"),
+        (lambda: _hip.add_rms_norm_fp8(values, scales, x, x, torch.zeros((2, 4, 32), device=device), x[0].clone()), "partial sums"),
+        (lambda: _hip.add_rms_norm_fp8(values, scales, x, x, None, x[0, :32].clone()), "weight"),
+        (lambda: _hip.gemm_fp8(x, values, None, values, scales, epilogue=_hip.GEMM_HALF), "without scales"),
+        (lambda: _hip.gemm_fp8(x, values, scales, values, scales, epilogue=_hip.GEMM_HALF), "out must be"),
+        (lambda: _hip.gemm_fp8(x, values, scales, values, scales, epilogue=9), "unknown"),
+        (lambda: _hip.gemm_fp8(torch.empty((1, 4, 4), device=device), values, scales, values, scales, splits=2), "out must be"),
+        (lambda: _hip.gemm_fp8(torch.empty((2, 4, 4), device=device), values, scales, values, scales, splits=2), "1 blocks"),
+        (lambda: _hip.qkv_rope_append_fp8(x, values, scales, values, scales, x, x), "2560"),
+    ]:
+        with pytest.raises(_hip.HipExtensionError, match=needle):
+            call()
