@@ -26,6 +26,9 @@ _rows_swiglu), with pc_silu_mul for the SwiGLU after F.linear. Every elementwise
 the reference's torch expression does (see the kernels' comments), so a row's result
 differs from the reference only by fp32 summation order inside the GEMMs, the norms and the
 attention.
+
+With the 8-bit projections of quantize_weights, which the reference does not have, the products are
+pc_qkv_rope_append_fp8 and pc_gemm_fp8 and the norms give 8-bit rows (pc_add_rms_norm_fp8).
 """
 
 from __future__ import annotations
@@ -232,7 +235,8 @@ def quantize_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
     device): half the bytes that a decode step streams, and a prompt's products at the 8-bit matrix rate.
     decode_paged, prefill_paged, DecodeGraph, PrefillGraph and DecodeWorker take the result as
     they take the fp16 weights; the activations that enter a projection are rounded the same way, per row
-    and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. The fp16
+    and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. A row's sums may be added in
+    another order in a batch of another size, which its activations' 8-bit roundings can enlarge. The fp16
     projections are not kept: drop `weights` to free them."""
     if not weights.embedding.is_cuda:
         raise RuntimeError("quantize_weights runs on the GPU: the weights must be on a CUDA device")
@@ -291,6 +295,8 @@ def rope_table(device: torch.device) -> Tensor:
 def _check_weights(weights: TinyLlamaWeights, what: str) -> None:
     if len(weights.layers) != LAYERS:
         raise ValueError(f"paged {what} requires 22 decoder layers")
+    if len({isinstance(layer, Fp8LayerWeights) for layer in weights.layers}) > 1:
+        raise ValueError("the layers' projections must be all in fp16 or all in 8 bits")
 
 
 # Up to GEMM_M128_ROWS rows (a decode step, a short prompt) the o_proj, gate|up and down

@@ -7,6 +7,9 @@ import torch
 
 from oracle import fp8_reference as ref
 from pagedcore_amd import _hip
+from pagedcore_amd import decoder as dec
+from pagedcore_amd.engine_types import KVReservation, RequestId
+from pagedcore_amd.kv_cache import KVAllocator
 
 
 def _every_e4m3() -> torch.Tensor:
@@ -141,3 +144,18 @@ def test_the_binding_takes_gpu_tensors_only():
     x = torch.zeros((2, 64), dtype=torch.float16)
     with pytest.raises(Exception, match="GPU|CUDA|HIP|NVIDIA|device"):
         _hip.quantize_fp8(values, scales, x)
+
+
+def test_layers_of_both_kinds_are_refused():
+    """Half a model in 8 bits is no model: refused before anything is staged."""
+    weights = dec.random_weights(device="cpu", layers=2, vocab=8, intermediate=16)
+    some = torch.zeros((1, 16), dtype=torch.float16)
+    rows = dec.Fp8Rows(some, some)
+    eight = dec.Fp8LayerWeights(weights.layers[0].input_norm, rows, rows, weights.layers[0].post_attention_norm, rows, rows)
+    mixed = dec.TinyLlamaWeights(weights.embedding, weights.layers[:1] * 21 + (eight,), weights.final_norm, weights.lm_head)
+    allocator = KVAllocator(torch.zeros((22, 2, 2, 16, 4, 64), dtype=torch.float16))
+    allocator.create(KVReservation(RequestId("a"), 1))
+    with pytest.raises(ValueError, match="all in 8 bits"):
+        dec.prefill_paged(torch.ones((1, 3), dtype=torch.int64), mixed, allocator, RequestId("a"))
+    with pytest.raises(ValueError, match="all in 8 bits"):
+        dec.decode_paged(torch.ones((1, 1), dtype=torch.int64), mixed, allocator, (RequestId("a"),))

@@ -347,6 +347,25 @@ def test_fp16_rows_are_rounded_as_quantize_does(device, m, n, k):
         _same_bits(a, b)
 
 
+@pytest.mark.parametrize("m,splits", [(3, 1), (20, 2), (70, 3)])
+def test_nonfinite_fp16_rows_are_rounded_as_quantize_does(device, m, splits):
+    """Infinities and NaN in fp16 x, beside values that set the scale and beside none: the rows become NaN, others keep
+    their bits, whatever forms the products take."""
+    x = _normal(device, (m, 400), seed=70)
+    x[0, 5], x[1, 399] = float("inf"), float("nan")
+    x[1, 130:140] = -float("inf")
+    x[2, 128:256] = float("inf")
+    eight, xs = _eight(x)
+    w, ws = _eight(_normal(device, (72, 400), seed=71))
+    for epilogue, shape, dtype, count in ((_hip.GEMM_PARTIALS, (splits, m, 72), torch.float32, splits), (_hip.GEMM_HALF, (m, 72), torch.float16, 1)):
+        a, b = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        _hip.gemm_fp8(a, x, None, w, ws, splits=count, epilogue=epilogue)
+        _hip.gemm_fp8(b, eight, xs, w, ws, splits=count, epilogue=epilogue)
+        assert torch.equal(a.isnan(), b.isnan())
+        bad = a.isnan().any(0) if a.ndim == 3 else a.isnan()
+        assert bad[:3].all() and not bad[3:].any()
+
+
 @pytest.mark.parametrize("m", [4, 140])
 def test_nan_stays_in_its_row_and_column(device, m):
     x = _normal(device, (m, 272), seed=11)
