@@ -407,7 +407,8 @@ int pc_add_rms_norm_parts_fp8(void* values, void* scales, void* hidden_out, cons
  * aligned; out must not overlap an input. PC_GEMM_PARTIALS adds exact products in fp32. The
  * other forms, whose outputs are rounded to fp16 or 8 bits, add them on the 8-bit matrix instruction, which takes eight
  * at a time, aligned to the largest, and drops what lies below 2^-13 of it: at most 7 * 2^-13 of each eight's largest
- * product, on normal data 1.5e-5 of the result's norm. The order of addition depends on m, n, k and the epilogue alone.
+ * product, on normal data 1.5e-5 of the result's norm. The order of addition depends on the
+ * sizes, the splits, the epilogue and whether x is fp16, on nothing else.
  */
 #define PC_GEMM_SWIGLU_FP8 4
 #define PC_FP8_STREAM_ROWS 128

@@ -11,13 +11,12 @@
 // of D slots of its own (LDS DMA, whole 128-byte lines), with no barrier in the loop. The waves' sums
 // are added in wave order at the end.
 //
-// The products run on the fp16 matrix instruction, the operands widened from e4m3 in registers
-// (exact). The 8-bit instruction would add eight products at a time aligned to the largest and drop what lies
-// below about 2^-14 of it (measured: 1.5e-5 of the result's norm; fp32 sums of fp16 products: 5e-8), and
-// its rate is not needed here: the conversions (16 per 16 rows and block) and the narrower matrix
-// instruction hide behind the weight's stream at a decode step's rows. An fp16 X is rounded
-// to 8 bits in the same registers, with the values and scales of pc_quantize_fp8, so that a decode step
-// needs no launch for it.
+// fp16 outputs run on the 8-bit matrix instruction of 128 columns, which takes the powers of two itself.
+// It adds eight products at a time aligned to the largest and drops what lies below about 2^-14 of it
+// (measured: 1.5e-5 of the result's norm), far less than the rounding to fp16 that follows. The fp32 partial sums
+// run on the fp16 instruction, the operands widened from e4m3 in registers (exact; 5e-8), since what
+// adds them decides what they are rounded to. An fp16 X is rounded to 8 bits in registers, with the values and
+// scales of pc_quantize_fp8, so that a decode step needs no launch for it.
 
 #include "fp8_gemm.h"
 
@@ -407,28 +406,34 @@ int launch(const Args& a, hipStream_t s) {
 }
 
 // The instances, in the four cases of what X is and what the products run on. The constants are fitted to
-// the times of every instance at 12000 calls (m 1 to 2048, n 256 to 11264, k 256 to 5632, 1 to 8 splits, every form,
-// weights from HBM): the instance taken, of these and the tiles, is 1 % off the fastest of all on average, more
-// than 20 % off at 1 % of the calls (1.8 times at worst, where a second round has few workgroups).
+// the times of every instance at 19000 calls (m 1 to 2048, n 256 to 11264, k 256 to 5632, 1 to 8 splits, every form,
+// weights from HBM): the instance taken, of these and the tiles, is 1.5 % off the fastest of all that were measured on
+// average, more than 20 % off at 2 % of the calls (1.7 times at worst, where a second round has few workgroups).
+// Rings of two units, three where a 16 x 16 tile leaves the LDS for them, and of one where that lets a second workgroup
+// onto the CU, which hides more than a second unit: fp32 partial sums of 8-bit rows a seventh faster over
+// the calls above, of fp16 rows, which fill twice the LDS, a seventh (down of 128 rows at 4 splits 14.4 -> 12.8 us); SwiGLU of
+// 37 rows 9.6 -> 8.7. Where a workgroup per CU is all there is, more in flight in it is faster: a second unit, or eight
+// waves (down of 16 rows at 4 splits 6.8 us / 5.8).
 struct Instance {
-  int mt, nt, waves;
+  int mt, nt, waves, units;
   Cost cost;
 };
 constexpr Instance kEight[] = {  // e4m3 X on the 8-bit instruction
-    {1, 1, 4, {2.15f, 0.16f, 0.22f, 0.09f}}, {1, 2, 4, {2.22f, 0.0f, 0.32f, 0.13f}},  {2, 2, 4, {2.04f, 0.31f, 0.41f, 0.13f}},
-    {3, 2, 4, {0.93f, 1.55f, 0.55f, 0.13f}}, {4, 2, 4, {0.91f, 1.71f, 0.64f, 0.14f}}, {4, 3, 4, {0.87f, 2.21f, 0.77f, 0.13f}},
-    {4, 4, 4, {0.96f, 2.26f, 0.93f, 0.14f}},
+    {1, 1, 4, 3, {2.07f, 0.17f, 0.22f, 0.08f}}, {1, 2, 4, 2, {2.14f, 0.01f, 0.33f, 0.12f}},
+    {2, 2, 4, 2, {1.98f, 0.33f, 0.41f, 0.12f}}, {3, 2, 4, 2, {0.92f, 1.54f, 0.55f, 0.12f}},
+    {4, 2, 4, 2, {0.91f, 1.68f, 0.64f, 0.13f}}, {2, 3, 4, 1, {2.81f, 0.0f, 0.6f, 0.15f}},
+    {4, 3, 4, 2, {0.92f, 2.18f, 0.78f, 0.13f}}, {4, 4, 4, 2, {0.96f, 2.24f, 0.94f, 0.14f}},
 };
 constexpr Instance kEightExact[] = {  // e4m3 X widened: fp32 partial sums
-    {1, 2, 4, {2.16f, 0.12f, 0.47f, 0.09f}}, {2, 2, 4, {2.02f, 0.39f, 0.63f, 0.11f}}, {4, 4, 4, {0.9f, 2.5f, 1.66f, 0.2f}},
+    {1, 2, 4, 2, {2.17f, 0.1f, 0.47f, 0.09f}}, {2, 2, 4, 1, {2.47f, 0.0f, 0.6f, 0.11f}}, {4, 2, 4, 1, {2.83f, 0.02f, 0.96f, 0.14f}},
 };
 constexpr Instance kHalfX[] = {  // fp16 X rounded, on the 8-bit instruction
-    {1, 1, 4, {2.15f, 0.19f, 0.5f, 0.03f}}, {1, 2, 4, {2.18f, 0.09f, 0.55f, 0.1f}},  {1, 2, 8, {0.82f, 1.35f, 0.92f, 0.13f}},
-    {2, 2, 8, {0.96f, 1.43f, 1.4f, 0.2f}},  {2, 4, 4, {0.88f, 1.81f, 1.27f, 0.15f}},
+    {1, 1, 4, 3, {2.15f, 0.19f, 0.5f, 0.03f}},  {1, 2, 4, 2, {2.18f, 0.09f, 0.55f, 0.1f}}, {2, 4, 4, 2, {0.88f, 1.81f, 1.27f, 0.15f}},
+    {1, 2, 8, 2, {0.82f, 1.35f, 0.92f, 0.13f}}, {2, 2, 8, 1, {0.96f, 1.43f, 1.4f, 0.2f}},
 };
 constexpr Instance kHalfXExact[] = {
-    {1, 1, 4, {1.95f, 0.35f, 0.56f, 0.04f}}, {1, 2, 4, {2.11f, 0.26f, 0.68f, 0.08f}}, {1, 2, 8, {1.04f, 1.3f, 1.16f, 0.12f}},
-    {2, 2, 8, {1.07f, 1.44f, 1.72f, 0.19f}}, {2, 4, 8, {1.09f, 1.89f, 2.47f, 0.19f}}, {4, 4, 4, {1.1f, 2.37f, 2.83f, 0.25f}},
+    {1, 1, 4, 3, {1.95f, 0.35f, 0.55f, 0.04f}}, {1, 2, 4, 1, {2.56f, 0.0f, 0.58f, 0.11f}},  {1, 2, 4, 2, {2.11f, 0.26f, 0.68f, 0.08f}},
+    {1, 2, 8, 2, {1.04f, 1.3f, 1.17f, 0.11f}},  {2, 2, 8, 1, {1.07f, 1.46f, 1.71f, 0.19f}}, {2, 4, 4, 1, {2.79f, 0.0f, 1.7f, 0.12f}},
 };
 
 // Whether an instance can end with the rotation, as the kernel asserts, and adds in the order of the others that can.
@@ -453,45 +458,25 @@ Choice fastest(const Args& a, Form form, const Instance (&instances)[N]) {
   return best;
 }
 
-// Rings of two units, three where a 16 x 16 tile leaves the LDS for them. An fp16 X fills it: there eight waves of one
-// unit each beat four of two (down of 64 rows at 2 splits 9.1 us / 10.8, of 128 rows 12.7 / 14.7).
-template <Form E>
-int launch_index(const Args& a, int index, hipStream_t s) {
-  if constexpr (E == kPartials) {
-    if (a.x_scales) {
-      switch (index) {
-        case 0: return launch<1, 2, 4, 2, false, E>(a, s);
-        case 1: return launch<2, 2, 4, 2, false, E>(a, s);
-        default: return launch<4, 4, 4, 2, false, E>(a, s);
-      }
-    }
-    switch (index) {
-      case 0: return launch<1, 1, 4, 3, true, E>(a, s);
-      case 1: return launch<1, 2, 4, 2, true, E>(a, s);
-      case 2: return launch<1, 2, 8, 2, true, E>(a, s);
-      case 3: return launch<2, 2, 8, 1, true, E>(a, s);
-      case 4: return launch<2, 4, 8, 1, true, E>(a, s);
-      default: return launch<4, 4, 4, 1, true, E>(a, s);
-    }
+template <Form E, bool HALFX, const auto& INSTANCES, size_t I = 0>
+int launch_index(const Args& a, size_t index, hipStream_t s) {
+  if constexpr (I == sizeof(INSTANCES) / sizeof(Instance)) {
+    return pc_internal::set_error(PC_ERR_ARGUMENT, "no kernel instance %d", static_cast<int>(index));
   } else {
-    if (a.x_scales) {
-      switch (index) {
-        case 0: return launch<1, 1, 4, 3, false, E>(a, s);
-        case 1: return launch<1, 2, 4, 2, false, E>(a, s);
-        case 2: return launch<2, 2, 4, 2, false, E>(a, s);
-        case 3: return launch<3, 2, 4, 2, false, E>(a, s);
-        case 4: return launch<4, 2, 4, 2, false, E>(a, s);
-      }
-      if constexpr (E != kRope) return index == 5 ? launch<4, 3, 4, 2, false, E>(a, s) : launch<4, 4, 4, 2, false, E>(a, s);
-    } else {
-      switch (index) {
-        case 0: return launch<1, 1, 4, 3, true, E>(a, s);
-        case 1: return launch<1, 2, 4, 2, true, E>(a, s);
-        case 4: return launch<2, 4, 4, 2, true, E>(a, s);
-      }
-      if constexpr (E != kRope) return index == 2 ? launch<1, 2, 8, 2, true, E>(a, s) : launch<2, 2, 8, 1, true, E>(a, s);
+    constexpr Instance t = INSTANCES[I];
+    if constexpr (E != kRope || rotates(t)) {
+      if (index == I) return launch<t.mt, t.nt, t.waves, t.units, HALFX, E>(a, s);
     }
-    return pc_internal::set_error(PC_ERR_ARGUMENT, "no kernel instance %d", index);
+    return launch_index<E, HALFX, INSTANCES, I + 1>(a, index, s);
+  }
+}
+
+template <Form E>
+int launch_form(const Args& a, int index, hipStream_t s) {
+  if constexpr (E == kPartials) {
+    return a.x_scales ? launch_index<E, false, kEightExact>(a, index, s) : launch_index<E, true, kHalfXExact>(a, index, s);
+  } else {
+    return a.x_scales ? launch_index<E, false, kEight>(a, index, s) : launch_index<E, true, kHalfX>(a, index, s);
   }
 }
 
@@ -504,10 +489,10 @@ Choice choose_stream(const Args& a, Form form) {
 
 int launch_stream(const Args& a, Form form, int index, hipStream_t s) {
   switch (form) {
-    case kPartials: return launch_index<kPartials>(a, index, s);
-    case kHalf: return launch_index<kHalf>(a, index, s);
-    case kSwiGLU: return launch_index<kSwiGLU>(a, index, s);
-    default: return launch_index<kRope>(a, index, s);
+    case kPartials: return launch_form<kPartials>(a, index, s);
+    case kHalf: return launch_form<kHalf>(a, index, s);
+    case kSwiGLU: return launch_form<kSwiGLU>(a, index, s);
+    default: return launch_form<kRope>(a, index, s);
   }
 }
 
