@@ -14,6 +14,8 @@ Contents (each function cites the reference lines it restates):
   paged_reference.LifoFreeList                kv_cache.py:86,158,197-201,297 (block choice)
   paged_reference.dense_attention_fp64        tests/unit/test_attention.py:173-179 (FP64 oracle)
   decoder_reference.*                         dense.py, decoder.py:70-100,202-240 (TinyLlama forward, generate)
+  fp8_reference.*                             none: 8-bit rows and their projections in 64 bits, from the format's definition
+                                              (pinned in tests/test_fp8_host.py by torch's own casts and by hand)
 
 How each one is pinned (tests/test_oracle.py): the reference tests' known answers (exact
 3, exact 100*(h//8)+16, exact 0.25, tiny probabilities > 0, +-1000 scores) and FP64
