@@ -404,7 +404,8 @@ int pc_add_rms_norm_parts_fp8(void* values, void* scales, void* hidden_out, cons
  *                         other epilogues); 8-bit x
  * splits is 1 but for PC_GEMM_PARTIALS. m in [1, 65536]; k a multiple of 16 up to 2^22; n a multiple of 4 (of 8 for
  * PC_GEMM_SWIGLU, of 32 for PC_GEMM_SWIGLU_FP8); m * k, n * k and splits * m * n up to 2^31; x, w and out 16-byte
- * aligned; out must not overlap an input. PC_GEMM_PARTIALS adds exact products in fp32. The
+ * aligned; out must not overlap an input. PC_GEMM_PARTIALS adds exact products in fp32, a block's sum first times x's
+ * power and then times w's (each within fp32's range for rows that the entry points above wrote). The
  * other forms, whose outputs are rounded to fp16 or 8 bits, add them on the 8-bit matrix instruction, which takes eight
  * at a time, aligned to the largest, and drops what lies below 2^-13 of it: at most 7 * 2^-13 of each eight's largest
  * product, on normal data 1.5e-5 of the result's norm. The order of addition depends on the

@@ -42,8 +42,8 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 
 // silu(gate) * up in fp32, silu(x) = x / (1 + e^-x), with the hardware's base-2 exponential and reciprocal (one
 // ulp each; the exponent's own rounding adds |x| 2^-24). The outputs are rounded to fp16 or to 8 bits; expf and
-// a correctly rounded quotient take as long as an eighth of the product before them (SwiGLU of 2048 rows 64.0 us
-// on 128 x 256 tiles, 56.5 us so).
+// a correctly rounded quotient are several times the instructions beside the tiles' products (without them, and with the
+// next stage read before the refill, SwiGLU of 2048 rows 63.4 -> 56.6 us).
 __device__ __forceinline__ float silu_mul(float gate, float up) {
   const float e = __builtin_amdgcn_exp2f(gate * -1.44269504088896340736f);
   return gate * __builtin_amdgcn_rcpf(1.0f + e) * up;

@@ -528,3 +528,44 @@ def test_the_binding_refuses(device):
     ]:
         with pytest.raises(_hip.HipExtensionError, match=needle):
             call()
+
+
+def test_streams_at_once(device):
+    """Calls of two streams, interleaved, give what they give alone: no entry point has a buffer of its own."""
+    def chain(m, seed, outputs):
+        hidden, weight = _normal(device, (m, 512), seed=seed), _normal(device, (512,), seed=seed + 1)
+        w, ws = _eight(_normal(device, (384, 512), seed=seed + 2, std=0.05))
+        down, ds = _eight(_normal(device, (512, 192), seed=seed + 3, std=0.05))
+
+        def run():
+            rows = _hip.empty_fp8(m, 512, device)
+            _hip.add_rms_norm_fp8(*rows, None, hidden, None, weight)
+            active = torch.empty((m, 192), dtype=torch.float16, device=device)
+            _hip.gemm_fp8(active, *rows, w, ws, epilogue=_hip.GEMM_SWIGLU)
+            parts = torch.empty((2, m, 512), device=device)
+            _hip.gemm_fp8(parts, active, None, down, ds, splits=2)
+            eight = _hip.empty_fp8(m, 192, device)
+            _hip.quantize_fp8(*eight, active)
+            half = torch.empty((m, 512), dtype=torch.float16, device=device)
+            _hip.gemm_fp8(half, *eight, down, ds, epilogue=_hip.GEMM_HALF)
+            outputs.append((active, parts, *eight, half))
+        return run
+
+    alone, together = ([], []), ([], [])
+    sides = [(chain(37, 80, alone[0]), chain(37, 80, together[0])), (chain(100, 90, alone[1]), chain(100, 90, together[1]))]
+    for first, _ in sides:
+        first()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sides]
+    for _ in range(10):
+        for stream, (_, again) in zip(streams, sides):
+            with torch.cuda.stream(stream):
+                again()
+    torch.cuda.synchronize()
+    for expected, got in zip(alone, together):
+        assert len(got) == 10
+        for outputs in got:
+            for a, b in zip(expected[0], outputs):
+                if a.dtype == torch.float8_e8m0fnu:  # a row's bytes past its blocks are not written
+                    a, b = a[:, :2], b[:, :2]
+                _same_bits(a, b)
