@@ -294,8 +294,15 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           acc[i][j][e] = silu_mul(acc[i][j][e], acc[i + P][j][e]);
-          most = fmaxf(most, finite_magnitude(acc[i][j][e]));
+          most = fmaxf(most, fabsf(acc[i][j][e]));  // of a NaN and a number the number
         }
+      }
+      if (__builtin_amdgcn_ballot_w64(most == INFINITY)) {  // an infinity: the largest of the others
+        most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_magnitude(acc[i][j][e]));
       }
       const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
       most = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));

@@ -326,6 +326,30 @@ def test_swiglu_to_eight_bits(device, m, n, k):
     assert (past == 0x5A).all()
 
 
+@pytest.mark.parametrize("m", [5, 200])
+def test_swiglu_to_eight_bits_past_fp32(device, m):
+    """Activations past fp32's range become NaN and leave the scale to the block's others: the even columns, whose
+    weights are zero where x is huge."""
+    x, xs = _eight(_normal(device, (m, 256), seed=21))
+    xs.view(torch.uint8)[1::2, 0] = 127 + 80  # 2^80: gate and up far past 2^64, or the gate below -2^64 and the output 0
+    weight = _normal(device, (320, 256), seed=22, std=0.125)
+    weight[::2, :128] = 0.0
+    w, ws = _eight(weight)
+    x64, w64 = _stands(x, xs), _stands(w, ws)
+    exact, slack = _swiglu_slack(x64, w64, x64 @ w64.t())
+    lost = torch.zeros((m, 160), dtype=torch.bool)
+    lost[1::2, 1::2] = (x64 @ w64.t())[1::2, 1:160:2] > 0.0
+    empty = torch.zeros_like(lost)
+    empty[1::2, 1::2] = True
+    assert (exact[lost].abs() > 2.0**130).all() and lost.any()
+    out, scales = _hip.empty_fp8(m, 160, device)
+    _hip.gemm_fp8(out, x, xs, w, ws, out_scales=scales, epilogue=_hip.GEMM_SWIGLU_FP8)
+    got = out.cpu().double()
+    assert torch.equal(got.isnan(), lost)
+    zero = torch.zeros((), dtype=torch.float64)
+    _check_rounded(got.nan_to_num(nan=0.0), scales, torch.where(empty, zero, exact), torch.where(empty, zero, slack))
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 64, 2048), (5, 36, 112), (16, 128, 1328), (31, 64, 5632), (64, 96, 400), (65, 32, 144), (128, 72, 272)])
 def test_fp16_rows_are_rounded_as_quantize_does(device, m, n, k):
     x = _normal(device, (m, k), seed=m + 7)
