@@ -205,11 +205,24 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
     const int4v_t p = lds_chunk(at[s][0] + row_base), q = lds_chunk(at[s][1] + row_base);
     return int8v_t{p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
   };
+  auto read_one = [&](Half& f, uint32_t slot, int s, int part) {
+    if (part < NT) f.w[part] = fragment(slot + S::XB + (wn * TN + 32 * part) * 128, s);
+    else f.x[part - NT] = fragment(slot + (wm * TM + 32 * (part - NT)) * 128, s);
+  };
   auto read = [&](Half& f, uint32_t slot, int s) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) f.w[i] = fragment(slot + S::XB + (wn * TN + 32 * i) * 128, s);
+    for (int p = 0; p < NT + MT; ++p) read_one(f, slot, s, p);
+  };
+  constexpr int kAtOnce = 2;
+  // Operands of the next half between this one's products.
+  auto reading = [&](Half& f, uint32_t slot, int s) {
+    return [&, slot, s](int product) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) f.x[j] = fragment(slot + (wm * TM + 32 * j) * 128, s);
+      for (int p = 0; p < NT + MT; ++p)
+        if (p / kAtOnce == product || (product == NT * MT - 1 && p / kAtOnce > product)) read_one(f, slot, s, p);
+      __builtin_amdgcn_sched_barrier(0);
+    };
   };
   struct Scales {
     int x[MT], w[NT];
@@ -221,12 +234,14 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
 #pragma unroll
     for (int j = 0; j < MT; ++j) f.x[j] = lds_byte(base + (wm * TM + 32 * j) * 16);
   };
-  auto multiply = [&](const Half& f, const Scales& scales) {
+  auto multiply = [&](const Half& f, const Scales& scales, auto between) {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < MT; ++j)
+      for (int j = 0; j < MT; ++j) {
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.w[i], f.x[j], acc[i][j], 0, 0, 0, scales.w[i], 0, scales.x[j]);
+        between(i * MT + j);
+      }
     // Nothing but this keeps the compiler from moving the products behind the barrier that follows.
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -252,18 +267,15 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
   read_scales(now, 0);
   int slot = 0;
   auto step = [&](int t, auto refill) {
-    read(two, slot * S::STAGE, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(one, now);
+    multiply(one, now, reading(two, slot * S::STAGE, 1));
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int following = slot + 1 == ST ? 0 : slot + 1;
     landed(decltype(refill)::value ? ST - 2 : min(ST - 2, steps - 2 - t));
-    read(one, following * S::STAGE, 0);
     read_scales(next, t + 1);
     if constexpr (decltype(refill)::value) issue(smem + slot * S::STAGE, t + ST);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(two, now);
+    multiply(two, now, reading(one, following * S::STAGE, 0));
     __builtin_amdgcn_sched_barrier(0);
     now = next;
     slot = following;
@@ -274,8 +286,9 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(const void* x, c
 #pragma nounroll
   for (; t + 1 < steps; ++t) step(t, std::false_type{});
   read(two, slot * S::STAGE, 1);
-  multiply(one, now);
-  multiply(two, now);
+  auto nothing = [](int) {};
+  multiply(one, now, nothing);
+  multiply(two, now, nothing);
 
   // acc[i][j] of lane (r32, h), element 4 q + e: X row wm TM + 32 j + r32, W row wn TN + 32 i + 8 q + 4 h + e
   // of the tile.
