@@ -322,18 +322,18 @@ DOWN_SPLITS = 8
 # 8-bit projections (quantize_weights). Up to FP8_FUSED_ROWS rows o_proj and down round fp16 rows on the way in and give
 # fp32 partial sums; above, a launch rounds what does not come in 8 bits already. Up to FP8_SWIGLU_ROWS
 # rows SwiGLU gives fp16: its 8-bit output takes tiles of 128 columns, 44 of them a row of tiles.
-# Us per layer without attention (rounding by a launch; 8-bit SwiGLU; the fp16 projections): 1 row 30.5 (33.6, 39.4, 34.0),
-# 16 rows 31.9 (36.2, 42.8, 37.0), 64 rows 39.7 (41.7, 46.8, 45.6), 80 rows 45.4 (44.3, 47.1, 47.9), 128 rows 47.6 (46.1, 49.0,
-# 53.1); 192 rows (52.4, 52.7, 63.0), 256 rows (58.3, 58.0, 68.7), 2048 rows (173, 169, 242). Of 1, 2 and 4 splits for o_proj
-# and 2, 4 and 8 for down, these are within 0.4 us of the best at every row count.
+# Us per layer without attention (rounding by a launch; 8-bit SwiGLU; the fp16 projections): 1 row 30.3 (34.0, 39.3, 34.0),
+# 16 rows 31.9 (36.9, 42.0, 36.8), 64 rows 39.7 (41.7, 46.9, 45.6), 80 rows 45.1 (44.3, 47.0, 47.7), 128 rows 51.2 (46.0, 48.9,
+# 53.3); 192 rows (51.8, 52.5, 63.1), 256 rows (57.6, 57.2, 68.9), 2048 rows (165, 161, 242). Of 1, 2 and 4 splits for o_proj
+# and 1 to 8 for down, these are within 0.5 us of the best at every row count.
 FP8_FUSED_ROWS = 64
 FP8_SWIGLU_ROWS = 192
 FP8_O_PROJ_SPLITS = 2
 
 
 def _fp8_down_splits(rows: int) -> int:
-    """K splits of the down projection on fp16 rows (16 rows: 32.0 us per layer, with 2 splits 33.0; 64 rows: 39.7,
-    with 4 40.5)."""
+    """K splits of the down projection on fp16 rows (16 rows: 31.9 us per layer, with 2 splits 33.1; 64 rows: 39.7,
+    with 4 41.0)."""
     return 4 if rows <= 32 else 2
 
 
