@@ -208,9 +208,12 @@ def random_weights(
 
 def pack_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
     """A copy whose q/k/v and gate/up projections are stacked in memory (for weights loaded
-    as separate tensors), so decode runs its fused GEMMs without per-call concatenation."""
+    as separate tensors), so decode runs its fused GEMMs without per-call concatenation.
+    quantize_weights stacks them itself: its result is refused."""
     layers = []
     for layer in weights.layers:
+        if isinstance(layer, Fp8LayerWeights):
+            raise ValueError("the weights are already in 8 bits, their projections stacked")
         layers.append(
             _layer_from_stacks(
                 layer.input_norm,
