@@ -245,7 +245,7 @@ def quantize_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
         raise RuntimeError("quantize_weights runs on the GPU: the weights must be on a CUDA device")
     layers = []
     for layer in weights.layers:
-        if not isinstance(layer, LayerWeights):
+        if isinstance(layer, Fp8LayerWeights):
             raise ValueError("the weights are already in 8 bits")
         if layer.down_proj.shape[1] % 16 != 0:
             raise ValueError("8-bit projections need an MLP width that is a multiple of 16")
