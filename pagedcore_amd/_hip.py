@@ -656,16 +656,23 @@ def _check_half(name: str, tensor: Tensor, shape: Tuple[int, ...], device: int) 
 
 
 def _gpu_of(tensor: Tensor) -> int:
-    """The tensor's GPU, which has to be the current one: the launch goes to its current stream."""
+    """The tensor's GPU, to whose current stream the call goes."""
     device = tensor.get_device()
-    if device < 0 or device != torch.cuda.current_device():
-        raise HipExtensionError(f"the tensors are on {tensor.device}, which is not the current GPU")
+    if device < 0:
+        raise HipExtensionError(f"the tensors are on {tensor.device}, which is not the current GPU nor another one")
     return device
 
 
-def _stream_of(device: int) -> int:
-    """The current stream of GPU `device`."""
-    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+def _call_on(device: int, lib: ctypes.CDLL, name: str, *args) -> None:
+    """The entry point `name` on the current stream of GPU `device`, which is made current for the call where another
+    one is (the library sets its kernels' LDS limits on the current GPU)."""
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call_on(device, lib, name, *args)
+    stream = _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    status = getattr(lib, name)(*args, stream)
+    if status:
+        _check(lib, name, status)
 
 
 def quantize_fp8(values: Tensor, scales: Tensor, x: Tensor) -> None:
@@ -680,9 +687,7 @@ def quantize_fp8(values: Tensor, scales: Tensor, x: Tensor) -> None:
     _check_fp8("values", values, scales, rows, width, device)
     lib = load()
     stride = x.stride(0) if rows > 1 else width
-    status = lib.pc_quantize_fp8(values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows, width, _stream_of(device))
-    if status:
-        _check(lib, "pc_quantize_fp8", status)
+    _call_on(device, lib, "pc_quantize_fp8", values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows, width)
 
 
 def add_rms_norm_fp8(
@@ -705,19 +710,17 @@ def add_rms_norm_fp8(
     if delta is not None and delta.dim() == 3:
         if delta.dtype != torch.float32 or delta.shape[1:] != shape or not delta.is_contiguous() or delta.get_device() != device:
             raise HipExtensionError(f"partial sums must be contiguous float32 [splits, {rows}, {width}] on GPU {device}")
-        status = lib.pc_add_rms_norm_parts_fp8(
-            values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), delta.data_ptr(), delta.shape[0],
-            weight.data_ptr(), rows, width, eps, _stream_of(device),
+        _call_on(
+            device, lib, "pc_add_rms_norm_parts_fp8", values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(),
+            delta.data_ptr(), delta.shape[0], weight.data_ptr(), rows, width, eps,
         )
     else:
         if delta is not None:
             _check_half("delta", delta, shape, device)
-        status = lib.pc_add_rms_norm_fp8(
-            values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), _ptr(delta), weight.data_ptr(), rows,
-            width, eps, _stream_of(device),
+        _call_on(
+            device, lib, "pc_add_rms_norm_fp8", values.data_ptr(), scales.data_ptr(), _ptr(hidden_out), hidden.data_ptr(), _ptr(delta),
+            weight.data_ptr(), rows, width, eps,
         )
-    if status:
-        _check(lib, "pc_add_rms_norm_fp8", status)
 
 
 def _check_fp8_product(x: Tensor, x_scales: Optional[Tensor], w: Tensor, w_scales: Tensor) -> Tuple[int, int, int, int]:
@@ -755,12 +758,10 @@ def gemm_fp8(
     else:
         raise HipExtensionError(f"unknown GEMM epilogue {epilogue}")
     lib = load()
-    status = lib.pc_gemm_fp8(
-        out.data_ptr(), _ptr(out_scales), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), m, n, k, splits,
-        epilogue, _stream_of(device),
+    _call_on(
+        device, lib, "pc_gemm_fp8", out.data_ptr(), _ptr(out_scales), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(), m,
+        n, k, splits, epilogue,
     )
-    if status:
-        _check(lib, "pc_gemm_fp8", status)
 
 
 def qkv_rope_append_fp8(
@@ -801,10 +802,8 @@ def qkv_rope_append_fp8(
             raise HipExtensionError("pool must be float16 [22, 2, blocks, 16, 4, 64]")
         _check_half("pool", pool, (22, 2, pool.shape[2], 16, 4, 64), device)
     lib = load()
-    status = lib.pc_qkv_rope_append_fp8(
-        query_out.data_ptr(), _ptr(key_out), _ptr(value_out), x.data_ptr(), _ptr(x_scales), w.data_ptr(), w_scales.data_ptr(),
-        m, k, positions.data_ptr(), rope_table.data_ptr(), rope_table.shape[0], _ptr(pool),
-        pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping), _stream_of(device),
+    _call_on(
+        device, lib, "pc_qkv_rope_append_fp8", query_out.data_ptr(), _ptr(key_out), _ptr(value_out), x.data_ptr(), _ptr(x_scales),
+        w.data_ptr(), w_scales.data_ptr(), m, k, positions.data_ptr(), rope_table.data_ptr(), rope_table.shape[0], _ptr(pool),
+        pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping),
     )
-    if status:
-        _check(lib, "pc_qkv_rope_append_fp8", status)

@@ -234,8 +234,8 @@ def _quantized(rows: Tensor) -> Fp8Rows:
 
 
 def quantize_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
-    """The model with every layer's projections rounded to 8 bits, once, on the weights' GPU (the current
-    device): half the bytes that a decode step streams, and a prompt's products at the 8-bit matrix rate.
+    """The model with every layer's projections rounded to 8 bits, once, on the weights' GPU:
+    half the bytes that a decode step streams, and a prompt's products at the 8-bit matrix rate.
     decode_paged, prefill_paged, DecodeGraph, PrefillGraph and DecodeWorker take the result as
     they take the fp16 weights; the activations that enter a projection are rounded the same way, per row
     and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. A row's sums may be added in
