@@ -428,6 +428,15 @@ int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, cons
                            const void* rope_table, int32_t rope_positions, void* pool, int64_t num_blocks, int32_t layer,
                            const int64_t* slot_mapping, void* stream);
 
+/*
+ * Which of its kernels pc_gemm_fp8 takes for a call of these sizes (half_x: fp16 x), or pc_qkv_rope_append_fp8 for
+ * epilogue PC_GEMM_QKV_ROPE (n = 2560, splits 1): an index below pc_gemm_fp8_kernels(epilogue, half_x), -1 for sizes that
+ * are refused. Both are the host's alone. What reads a profile, or is to run every kernel, needs them; no call does.
+ */
+#define PC_GEMM_QKV_ROPE 5
+int32_t pc_gemm_fp8_kernel(int32_t m, int32_t n, int32_t k, int32_t splits, int32_t epilogue, int32_t half_x);
+int32_t pc_gemm_fp8_kernels(int32_t epilogue, int32_t half_x);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 LIBRARY_NAME = "libpagedcore_hip.so"
 
 _lock = threading.Lock()
@@ -151,6 +151,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pc_add_rms_norm_parts_fp8.argtypes = [_p, _p, _p, _p, _p, _i32, _p, _i64, _i32, ctypes.c_float, _p]
     lib.pc_gemm_fp8.restype = ctypes.c_int
     lib.pc_gemm_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]
+    lib.pc_gemm_fp8_kernel.restype = _i32
+    lib.pc_gemm_fp8_kernel.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32]
+    lib.pc_gemm_fp8_kernels.restype = _i32
+    lib.pc_gemm_fp8_kernels.argtypes = [_i32, _i32]
     lib.pc_qkv_rope_append_fp8.restype = ctypes.c_int
     lib.pc_qkv_rope_append_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _i32, _p, _i64, _i32, _p, _p]
 

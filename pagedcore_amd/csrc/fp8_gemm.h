@@ -16,7 +16,7 @@ enum Form : int32_t {
   kHalf = PC_GEMM_HALF,
   kSwiGLU = PC_GEMM_SWIGLU,
   kSwiGLUFp8 = PC_GEMM_SWIGLU_FP8,
-  kRope,  // pc_qkv_rope_append_fp8
+  kRope = PC_GEMM_QKV_ROPE,
 };
 // The forms whose tiles hold pairs of W rows: gate and up, or a head's d and d + 32.
 constexpr bool paired(Form f) { return f == kSwiGLU || f == kSwiGLUFp8 || f == kRope; }
@@ -53,8 +53,11 @@ inline float estimate(const Cost& c, int64_t workgroups, int blocks, const Args&
 // A q|k|v product, as fp16 or rotated: both take the same instance, so that they have the same bits.
 inline bool qkv_product(const Args& a, Form form) { return form == kRope || (form == kHalf && a.n == rope_device::kQkvElems); }
 
-Choice choose_stream(const Args& a, Form form);  // not kSwiGLUFp8
-Choice choose_tile(const Args& a, Form form);    // not kPartials, e4m3 x
+// Of the sizes in `a` and of whether x is fp16, and of nothing else in it.
+Choice choose_stream(const Args& a, Form form, bool half_x);  // not kSwiGLUFp8
+Choice choose_tile(const Args& a, Form form);                 // not kPartials, e4m3 x
+int stream_kernels(Form form, bool half_x);                   // how many each chooses among
+int tile_kernels(Form form);
 int launch_stream(const Args& a, Form form, int index, hipStream_t s);
 int launch_tile(const Args& a, Form form, int index, hipStream_t s);
 

@@ -21,6 +21,8 @@
 
 #include "fp8_gemm.h"
 
+#include <iterator>
+
 namespace fp8_gemm {
 namespace {
 
@@ -483,9 +485,14 @@ int launch_form(const Args& a, int index, hipStream_t s) {
 
 }  // namespace
 
-Choice choose_stream(const Args& a, Form form) {
-  if (form == kPartials) return a.x_scales ? fastest(a, form, kEightExact) : fastest(a, form, kHalfXExact);
-  return a.x_scales ? fastest(a, form, kEight) : fastest(a, form, kHalfX);
+Choice choose_stream(const Args& a, Form form, bool half_x) {
+  if (form == kPartials) return half_x ? fastest(a, form, kHalfXExact) : fastest(a, form, kEightExact);
+  return half_x ? fastest(a, form, kHalfX) : fastest(a, form, kEight);
+}
+
+int stream_kernels(Form form, bool half_x) {
+  return static_cast<int>(form == kPartials ? (half_x ? std::size(kHalfXExact) : std::size(kEightExact))
+                                            : (half_x ? std::size(kHalfX) : std::size(kEight)));
 }
 
 int launch_stream(const Args& a, Form form, int index, hipStream_t s) {

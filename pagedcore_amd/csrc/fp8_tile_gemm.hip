@@ -20,6 +20,7 @@
 
 #include "fp8_gemm.h"
 
+#include <iterator>
 #include <type_traits>
 
 namespace fp8_gemm {
@@ -443,6 +444,8 @@ int launch_index(const Args& a, int index, hipStream_t s) {
 Choice choose_tile(const Args& a, Form form) {
   return form == kSwiGLUFp8 ? fastest(a, form, kTilesFp8) : fastest(a, form, kTiles);
 }
+
+int tile_kernels(Form form) { return static_cast<int>(form == kSwiGLUFp8 ? std::size(kTilesFp8) : std::size(kTiles)); }
 
 int launch_tile(const Args& a, Form form, int index, hipStream_t s) {
   switch (form) {
