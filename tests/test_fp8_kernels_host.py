@@ -5,8 +5,10 @@ from __future__ import annotations
 import pytest
 
 from pagedcore_amd import _hip
+from pagedcore_amd import decoder as dec
+from tests import fp8_sizes
+from tests.fp8_sizes import HALF, PARTIALS, ROPE, SWIGLU, SWIGLU_FP8
 
-PARTIALS, HALF, SWIGLU, SWIGLU_FP8, ROPE = 0, 1, 2, 4, 5
 FORMS = [(PARTIALS, 0), (PARTIALS, 1), (HALF, 0), (HALF, 1), (SWIGLU, 0), (SWIGLU, 1), (SWIGLU_FP8, 0), (ROPE, 0), (ROPE, 1)]
 
 
@@ -42,3 +44,36 @@ def test_sizes_that_are_refused_have_no_kernel(form, m, n, k, splits):
 def test_q_k_v_takes_one_kernel_rotated_or_not(m):
     """So that a cache holds the same bytes whichever way the product went into it."""
     assert kernel(HALF, 0, m, 2560, 2048) == kernel(ROPE, 0, m, 2560, 2048)
+
+
+def _kernels(form, half_x, group):
+    return {kernel(form, half_x, *size) for size in fp8_sizes.GROUPS[group].get((form, half_x), [])}
+
+
+@pytest.mark.parametrize("group", ["RAGGED", "WHOLE"])
+@pytest.mark.parametrize("form,half_x", FORMS)
+def test_the_tests_sizes_run_every_kernel(form, half_x, group):
+    """A change of the choice's constants that takes the sizes off a kernel fails here: other sizes for it are due in
+    tests/fp8_sizes.py, or the kernel is one that no call takes."""
+    every = set(range(_hip.load().pc_gemm_fp8_kernels(form, half_x)))
+    if form == ROPE:
+        every -= {5, 6, 7} if not half_x else {3, 4}  # tiles of 24 columns, more quads than threads; waves of eight
+    assert _kernels(form, half_x, group) == every
+    for m, n, k, *_ in fp8_sizes.GROUPS[group][form, half_x]:
+        assert (m % 16 and k % 128 and (n % 64 or form == ROPE)) if group == "RAGGED" else m % 16 == n % 64 == k % 128 == 0
+
+
+def test_the_tests_sizes_run_every_kernel_of_the_model():
+    """Of the decoder's calls at 1 to 2048 rows, at its own widths."""
+    taken = {}
+    for m in range(1, 2049):
+        calls = [(ROPE, 0, m, 2560, 2048, 1), (HALF, 0, m, 2560, 2048, 1)]
+        if m <= dec.FP8_FUSED_ROWS:
+            calls += [(PARTIALS, 1, m, 2048, 2048, dec.FP8_O_PROJ_SPLITS), (PARTIALS, 1, m, 2048, 5632, dec._fp8_down_splits(m))]
+        else:
+            calls += [(HALF, 0, m, 2048, 2048, 1), (HALF, 0, m, 2048, 5632, 1)]
+        calls.append((SWIGLU if m <= dec.FP8_SWIGLU_ROWS else SWIGLU_FP8, 0, m, 11264, 2048, 1))
+        for form, half_x, *size in calls:
+            taken.setdefault((form, half_x), set()).add(kernel(form, half_x, *size))
+    for (form, half_x), kernels in taken.items():
+        assert kernels <= _kernels(form, half_x, "MODEL"), (form, half_x)
