@@ -77,3 +77,12 @@ def test_the_tests_sizes_run_every_kernel_of_the_model():
             taken.setdefault((form, half_x), set()).add(kernel(form, half_x, *size))
     for (form, half_x), kernels in taken.items():
         assert kernels <= _kernels(form, half_x, "MODEL"), (form, half_x)
+
+
+def test_the_tests_sizes_wrap_every_tile_kernels_scales():
+    """Its ring holds the scales of 16 blocks twice: a second fetch behind 2048 columns, the first slot again behind 4096."""
+    for form, depths in ((HALF, (2064, 4112, 5632)), (SWIGLU_FP8, (2064, 4112, 5632)), (SWIGLU, (4112,)), (ROPE, (4112,))):
+        count = _hip.load().pc_gemm_fp8_kernels(form, 0)
+        tiles = set(range(count)) if form == SWIGLU_FP8 else set(range(count - 5, count))
+        for depth in depths:
+            assert {kernel(form, 0, m, n, k) for m, n, k in fp8_sizes.DEEP[form, 0] if k == depth} == tiles
