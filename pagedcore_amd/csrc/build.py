@@ -69,7 +69,6 @@ GUARDED_KERNELS: Dict[str, int] = {
     "fp8_stream_kernel": 1,  # a workgroup of four waves alone
     "fp8_stream_kernelILi2ELi2ELi8E": 2,  # of eight
     "fp8_stream_kernelILi2ELi4ELi4ELi1E": 2,  # two of four waves (66 KB)
-    "fp8_stream_kernelILi2ELi3ELi4ELi1E": 3,  # three (42 KB)
     "fp8_stream_kernelILi4ELi2ELi4ELi1E": 3,  # three (52 KB)
     "fp8_stream_kernelILi1ELi2ELi4ELi2ELb0E": 3,  # three of four waves (52 KB)
     "fp8_tile_kernel": 2,  # a workgroup of eight waves
