@@ -368,7 +368,7 @@ int32_t pc_fp8_scale_stride(int32_t width);
 
 /*
  * Rounds fp16 rows (x [rows][width], row stride x_stride elements, a multiple of 8) to 8 bits; width a
- * multiple of 16 up to 2^22, rows * ceil(width / 128) below 2^29. x 16-byte aligned.
+ * multiple of 16 up to 2^22, rows * ceil(width / 128) up to 2^29 - 32. x 16-byte aligned.
  */
 int pc_quantize_fp8(void* values, void* scales, const void* x, int64_t x_stride, int64_t rows, int32_t width, void* stream);
 
@@ -408,7 +408,8 @@ int pc_add_rms_norm_parts_fp8(void* values, void* scales, void* hidden_out, cons
  * power and then times w's (each within fp32's range for rows that the entry points above wrote). The
  * other forms, whose outputs are rounded to fp16 or 8 bits, add them on the 8-bit matrix instruction, which takes eight
  * at a time, aligned to the largest, and drops what lies below 2^-13 of it: at most 7 * 2^-13 of each eight's largest
- * product, on normal data 1.5e-5 of the result's norm. The order of addition depends on the
+ * product, on normal data 1.5e-5 of the result's norm. An output in fp16 that passes 65504 is an infinity; rounded to
+ * 8 bits (PC_GEMM_SWIGLU_FP8) fp32's range holds. The order of addition depends on the
  * sizes, the splits, the epilogue and whether x is fp16, on nothing else.
  */
 #define PC_GEMM_SWIGLU_FP8 4

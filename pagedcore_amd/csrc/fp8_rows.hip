@@ -98,10 +98,11 @@ constexpr int kAnySplits = 64;                // a count without its own instanc
 // One workgroup per row, eight columns per thread and chunk. The sum of the residual stream is an
 // fp16 row (the next layer's residual), rounded as the fp16 form rounds it; the mean of squares and the
 // norm are fp32. What bounds it: at decode sizes one round trip of memory (every load is issued
-// before the first wait; the split counts of a decode step have instances of their own for that), at
-// prompt sizes HBM. FULL: every thread has all its chunks (no branch around the loads). 1 row of 2048 and 4 splits: 2.2 us
-// (a launch alone is 1.9), 128 rows and 8 splits 3.6 (2660 GB/s), 2048 rows and an fp16 delta 6.9 (4270 GB/s; 8.2 where
-// the loads allocate in the caches, which partial sums, read where they were just written, do better with).
+// before the first wait; 1, 2, 4 and 8 splits have instances of their own for that), at
+// prompt sizes HBM. FULL: every thread has all its chunks (no branch around the loads). 1 row of 2048 and 4 splits: 2.1 us
+// (a launch alone is 1.9), 128 rows and 8 splits 3.6 (2660 GB/s from the caches; 4.0 from HBM), 2048 rows and an fp16 delta
+// 6.9 (4270 GB/s; 8.2 where the loads allocate in the caches, which partial sums, read where they were just written, do
+// better with).
 template <int CHUNKS, bool FULL, int DELTA>
 __global__ __launch_bounds__(kThreads) void add_rms_norm_fp8_kernel(const _Float16* hidden, const void* delta,
                                                                     int64_t parts_stride, const _Float16* weight,
@@ -225,7 +226,7 @@ int add_rms_norm_fp8(void* values, void* scales, void* hidden_out, const void* h
       default: return launch(add_rms_norm_fp8_kernel<4, false, D>);
     }
   };
-  // Two to eight parts at once where a thread has one chunk of them (the registers of more do not repay).
+  // Two, four or eight parts at once where a thread has one chunk of them (the registers of more do not repay).
   const bool one_chunk = width <= 8 * kThreads;
   if (!parts && !delta) with_delta(std::integral_constant<int, kNoDelta>{});
   else if (delta) with_delta(std::integral_constant<int, kHalfDelta>{});

@@ -10,11 +10,12 @@
 // so every byte of the tile is fetched by exactly one wave, through a ring
 // of D slots of its own (LDS DMA, whole 128-byte lines), with no barrier in the loop. The waves' sums
 // are added in wave order at the end. SwiGLU of 1 row (11264 x 2048) 6.6 us, of which a launch is 1.9: 4.9 TB/s behind it, a
-// large copy's rate; of 64 rows 9.1 us, where the X that every workgroup fetches again counts as much as W.
+// large copy's rate; of 24 rows 7.9-8.1 us, where the X that every workgroup fetches again counts too.
 //
 // fp16 outputs run on the 8-bit matrix instruction of 128 columns, which takes the powers of two itself.
-// It adds eight products at a time aligned to the largest and drops what lies below about 2^-14 of it
-// (measured: 1.5e-5 of the result's norm), far less than the rounding to fp16 that follows. The fp32 partial sums
+// It adds eight products at a time aligned to the largest and drops what lies below 2^-13 of it: measured 1.5e-5 of the
+// result's norm on normal data, 3e-5 where one column in a hundred is ten times as large. The rounding to fp16 that
+// follows is 2.1e-4 (together 2.10e-4 against 2.07e-4). The fp32 partial sums
 // run on the fp16 instruction, the operands widened from e4m3 in registers (exact; 5e-8), since what
 // adds them decides what they are rounded to. An fp16 X is rounded to 8 bits in registers, with the values and
 // scales of pc_quantize_fp8, so that a decode step needs no launch for it.
@@ -414,7 +415,8 @@ int launch(const Args& a, hipStream_t s) {
 // average, more than 20 % off at 2 % of the calls (1.7 times at worst, where a second round has few workgroups).
 // Rings of two units, three where a 16 x 16 tile leaves the LDS for them, and of one where that lets a second workgroup
 // onto the CU, which hides more than a second unit: fp32 partial sums of 8-bit rows a seventh faster over
-// the calls above, of fp16 rows, which fill twice the LDS, a seventh (down of 128 rows at 4 splits 14.4 -> 12.8 us). On the
+// the calls above, of fp16 rows, which fill twice the LDS, a seventh (down of 128 rows at 4 splits 14.4 -> 12.8 us, 13.2 with
+// outputs that are not in the caches). On the
 // 8-bit instruction a second unit is as good or better (32 x 48 tiles of one unit, for SwiGLU of 17 to 32 rows: 8.7 us, the 32 x 32
 // tiles of two 7.7 to 8.2). Where a workgroup per CU is all there is, more in flight in it is faster: a second unit, or eight
 // waves (down of 16 rows at 4 splits 6.8 us / 5.8).
