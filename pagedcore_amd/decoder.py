@@ -238,9 +238,15 @@ def quantize_weights(weights: TinyLlamaWeights) -> TinyLlamaWeights:
     half the bytes that a decode step streams, and a prompt's products at the 8-bit matrix rate.
     decode_paged, prefill_paged, DecodeGraph, PrefillGraph and DecodeWorker take the result as
     they take the fp16 weights; the activations that enter a projection are rounded the same way, per row
-    and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. A row's sums may be added in
-    another order in a batch of another size, which its activations' 8-bit roundings can enlarge. The fp16
-    projections are not kept: drop `weights` to free them."""
+    and 128 columns. Embedding, norms, attention, the KV cache and the LM head stay fp16. The fp16 projections are not kept:
+    drop `weights` to free them.
+
+    A row's last bits depend on the batch that it is in, which its activations' 8-bit roundings can enlarge: products add
+    in another order at another row count; up to FP8_FUSED_ROWS rows o_proj and down add in fp32 what goes to the residual
+    sum, above on the 8-bit matrix instruction, rounded to fp16 (3e-5 and 2.1e-4 of the norm, beside 2.6e-2 of the rounding to
+    8 bits); up to FP8_SWIGLU_ROWS rows the MLP's activations are rounded to fp16 and then to 8 bits, above once. So an
+    activation past fp16's 65504 is an infinity in a decode step, as in the fp16 model, and makes its row NaN; a long prompt's
+    is not."""
     if not weights.embedding.is_cuda:
         raise RuntimeError("quantize_weights runs on the GPU: the weights must be on a CUDA device")
     layers = []
