@@ -358,7 +358,7 @@ int pc_prefill_attention(void* out, const void* query, const void* key, const vo
  * 448 * 2^(s - 127) (1 for a block of zeros); value = e4m3(x * 2^(127 - s)), to nearest even.
  * An infinity or NaN becomes a NaN, and leaves the scale of its block alone.
  * None of this is in the reference, whose weights and activations are fp16; the entry points stand
- * where those below are cited.
+ * where those below are cited. Their `stream` must belong to the current device.
  */
 #define PC_FP8_BLOCK 128
 
