@@ -438,6 +438,65 @@ int pc_qkv_rope_append_fp8(void* query_out, void* key_out, void* value_out, cons
 int32_t pc_gemm_fp8_kernel(int32_t m, int32_t n, int32_t k, int32_t splits, int32_t epilogue, int32_t half_x);
 int32_t pc_gemm_fp8_kernels(int32_t epilogue, int32_t half_x);
 
+/*
+ * The pool in 4 bits: a K or V row (the 64 values of one token and kv head) as 16 levels between its smallest and its
+ * largest value, 36 bytes instead of 128. For a row x
+ *   lo = min(x),  s = the smallest fp16 with 15 s >= max(x) - lo,  n = round((x - lo) / s) (half to even; 0 where s = 0)
+ * (the differences in fp32; a lo of zero is +0) and the row stands for lo + s n. A row that holds an infinity or NaN is (lo, s) = (NaN, 0): all its values are NaN.
+ *
+ *   pool: contiguous, 128-byte aligned [22 layers][num_blocks][4 kv heads][PC_Q4_UNIT_BYTES], a block of 16 slots; each unit:
+ *     bytes 0-511      K's levels: slot 4 i + e, dims 32 x + 8 g + j (i, e, g in 0..3, x in 0..1, j in 0..7) in the 32-bit word
+ *                      at 256 (i / 2) + 64 e + 16 g + 8 (i % 2) + 4 x, bits 4 (j / 2) + 16 (j % 2) and the next three
+ *     bytes 512-1023   V's levels: slot 4 q + t, dims 32 p + r in the low and 32 p + 16 + r in the high half (r in 0..15) of
+ *                      the byte at 512 + 256 (q / 2) + 16 r + 8 (q % 2) + 4 p + {0, 2, 1, 3}[t]
+ *     bytes 1024-1087  (lo, s) of slot t's K row, two fp16 at 1024 + 4 t; bytes 1088-1151 the same of the V rows
+ *   (the order in which the attention's matrix products take them; every slot has bytes of its own).
+ *
+ * The reference's pool is fp16 only (src/pagedcore/kv_cache.py:39-43); the entry points stand where those named below do.
+ */
+#define PC_Q4_UNIT_BYTES 1152
+
+/*
+ * KV append into the 4-bit pool: pc_kv_append (reference src/pagedcore/kv_cache.py:161-172, 242-245) with each row quantised
+ * as it is written. Arguments as there: key/value rows are [4][64] fp16 with contiguous heads and dims, layer and token
+ * strides free; a token whose slot lies outside [0, num_blocks * 16) is not written, nor is any byte of another slot. A slot
+ * named twice holds one of its tokens' rows, or bytes of both. num_layers * num_tokens up to 2^28.
+ */
+int pc_kv_append_q4(void* pool, int64_t num_blocks, int32_t layer_begin, int32_t num_layers, const void* key,
+                    int64_t key_layer_stride, int64_t key_token_stride, const void* value, int64_t value_layer_stride,
+                    int64_t value_token_stride, const int64_t* slot_mapping, int64_t num_tokens, void* stream);
+
+/*
+ * The rows of given slots read back as fp16, in place of the pool views of KVAllocator.read_block (reference
+ * src/pagedcore/kv_cache.py:272-284): for layer l and token t
+ *   key[l][t] = the K row of slot_mapping[t] in layer layer_begin + l, value[l][t] its V row, lo + s n rounded to fp16
+ *               (65504 where it passes that, as it may by s / 2 where s was rounded up)
+ * laid out as pc_kv_append_q4 takes them. The rows of a token whose slot lies outside the pool are not written. The outputs
+ * must not overlap each other or the pool.
+ */
+int pc_kv_read_q4(void* key, int64_t key_layer_stride, int64_t key_token_stride, void* value, int64_t value_layer_stride,
+                  int64_t value_token_stride, const void* pool, int64_t num_blocks, int32_t layer_begin, int32_t num_layers,
+                  const int64_t* slot_mapping, int64_t num_tokens, void* stream);
+
+/*
+ * Paged decode attention of one layer over the 4-bit pool: pc_paged_decode_attn with the same plan, workspace, faults and
+ * rules, over the values lo + s n that the rows stand for (not rounded to fp16). Scores, softmax and sums are fp32, the
+ * weights that multiply V's levels are held in 16 bits of significand, the output is rounded once. Slots past a sequence's
+ * length never reach the output, whatever their bytes are.
+ */
+int pc_paged_decode_attn_q4(void* out, const void* query, const void* pool, int64_t num_blocks, int32_t layer,
+                            const int32_t* context_lens, int32_t batch, int32_t max_blocks, const int32_t* plan,
+                            int32_t num_records, void* workspace, void* stream);
+
+/*
+ * The same with each sequence's newest token quantised and written in the launch: pc_kv_append_paged_decode_attn for the
+ * 4-bit pool, bit-identical to pc_kv_append_q4 of those slots followed by pc_paged_decode_attn_q4.
+ */
+int pc_kv_append_paged_decode_attn_q4(void* out, const void* query, void* pool, int64_t num_blocks, int32_t layer,
+                                      const int32_t* context_lens, int32_t batch, int32_t max_blocks, const int32_t* plan,
+                                      int32_t num_records, const void* new_key, const void* new_value, void* workspace,
+                                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 LIBRARY_NAME = "libpagedcore_hip.so"
 
 _lock = threading.Lock()
@@ -155,6 +155,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pc_gemm_fp8_kernel.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32]
     lib.pc_gemm_fp8_kernels.restype = _i32
     lib.pc_gemm_fp8_kernels.argtypes = [_i32, _i32]
+    lib.pc_kv_append_q4.restype = ctypes.c_int
+    lib.pc_kv_append_q4.argtypes = [_p, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p]
+    lib.pc_kv_read_q4.restype = ctypes.c_int
+    lib.pc_kv_read_q4.argtypes = [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _i32, _p, _i64, _p]
+    lib.pc_paged_decode_attn_q4.restype = ctypes.c_int
+    lib.pc_paged_decode_attn_q4.argtypes = [_p, _p, _p, _i64, _i32, _p, _i32, _i32, _p, _i32, _p, _p]
+    lib.pc_kv_append_paged_decode_attn_q4.restype = ctypes.c_int
+    lib.pc_kv_append_paged_decode_attn_q4.argtypes = [_p, _p, _p, _i64, _i32, _p, _i32, _i32, _p, _i32, _p, _p, _p, _p]
     lib.pc_qkv_rope_append_fp8.restype = ctypes.c_int
     lib.pc_qkv_rope_append_fp8.argtypes = [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _i32, _p, _i64, _i32, _p, _p]
 
@@ -810,4 +818,143 @@ def qkv_rope_append_fp8(
         device, lib, "pc_qkv_rope_append_fp8", query_out.data_ptr(), _ptr(key_out), _ptr(value_out), x.data_ptr(), _ptr(x_scales),
         w.data_ptr(), w_scales.data_ptr(), m, k, positions.data_ptr(), rope_table.data_ptr(), rope_table.shape[0], _ptr(pool),
         pool.shape[2] if pool is not None else 0, layer, _ptr(slot_mapping),
+    )
+
+
+# The KV pool in 4 bits (include/pagedcore_hip.h): per block of 16 tokens and kv head a unit of 1152 bytes.
+Q4_UNIT_BYTES = 1152
+
+
+def empty_q4_pool(blocks: int, device: torch.device) -> Tensor:
+    """An uninitialised 4-bit KV pool, uint8 [22, blocks, 4, 1152]."""
+    return torch.empty((22, blocks, 4, Q4_UNIT_BYTES), dtype=torch.uint8, device=device)
+
+
+def is_q4_pool(pool: Tensor) -> bool:
+    """Whether `pool` has the type and shape of a 4-bit pool, contiguous."""
+    return (
+        pool.dtype is torch.uint8
+        and pool.dim() == 4
+        and pool.shape[1] > 0
+        and pool.shape == (22, pool.shape[1], 4, Q4_UNIT_BYTES)
+        and pool.is_contiguous()
+    )
+
+
+def _check_q4_pool(pool: Tensor) -> int:
+    """The pool's GPU."""
+    device = _gpu_of(pool)
+    if not is_q4_pool(pool):
+        raise HipExtensionError("pool must be contiguous uint8 [22, blocks, 4, 1152]")
+    return device
+
+
+def _check_q4_rows(names: Tuple[str, str], key: Tensor, value: Tensor, layer_begin: int, slot_mapping: Tensor, device: int) -> None:
+    """K and V rows [layers, tokens, 4, 64] and the slots of the tokens, on GPU `device`."""
+    shape = key.shape
+    if len(shape) != 4 or shape[2] != 4 or shape[3] != 64 or value.shape != shape or not 1 <= shape[0] <= 22 - layer_begin or layer_begin < 0:
+        raise HipExtensionError(f"{names[0]} and {names[1]} must share [layers, tokens, 4, 64], with the layers from {layer_begin} on within 22")
+    for tensor in (key, value):
+        if tensor.dtype is not torch.float16 or tensor.get_device() != device:
+            raise HipExtensionError(f"{names[0]} and {names[1]} must be float16 on GPU {device}")
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (shape[1],) or not slot_mapping.is_contiguous() or slot_mapping.get_device() != device:
+        raise HipExtensionError(f"slot_mapping must be contiguous int64 [{shape[1]}] on GPU {device}")
+
+
+def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
+    """kv_append into a 4-bit pool (uint8 [22, blocks, 4, 1152]): each row [64] of key/value[l, t] quantised to 16 levels
+    between its smallest and its largest value and written to slot slot_mapping[t] of layer layer_begin + l.
+
+    key/value: float16 [layers, tokens, 4, 64]; layer and token strides are free. slot_mapping: int64 [tokens], each slot at
+    most once; a slot outside the pool is skipped. A row with an infinity or NaN becomes a row of NaN. Enqueued on the current
+    stream of the pool's device."""
+    device = _check_q4_pool(pool)
+    _check_q4_rows(("key", "value"), key, value, layer_begin, slot_mapping, device)
+    if key.stride(3) != 1 or key.stride(2) != 64:
+        key = key.contiguous()
+    if value.stride(3) != 1 or value.stride(2) != 64:
+        value = value.contiguous()
+    _call_on(
+        device, load(), "pc_kv_append_q4", pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], key.data_ptr(), key.stride(0),
+        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), slot_mapping.data_ptr(), key.shape[1],
+    )
+
+
+def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_mapping: Tensor) -> None:
+    """key/value[l, t] = the values of slot slot_mapping[t] in layer layer_begin + l of a 4-bit pool, rounded to float16.
+
+    key/value: float16 [layers, tokens, 4, 64] to write, each [4, 64] row contiguous, layer and token strides free; the rows of
+    a slot outside the pool are left as they are. slot_mapping: int64 [tokens]. On the current stream of the pool's device."""
+    device = _check_q4_pool(pool)
+    _check_q4_rows(("key", "value"), key, value, layer_begin, slot_mapping, device)
+    for tensor in (key, value):
+        if tensor.stride(3) != 1 or tensor.stride(2) != 64:
+            raise HipExtensionError("each [4, 64] row of key and value must be contiguous")
+    _call_on(
+        device, load(), "pc_kv_read_q4", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+        value.stride(1), pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], slot_mapping.data_ptr(), key.shape[1],
+    )
+
+
+def paged_decode_attention_q4(
+    out: Tensor,
+    query: Tensor,
+    pool: Tensor,
+    layer: int,
+    block_tables: Tensor,
+    context_lens: Tensor,
+    *,
+    plan: Optional[Tensor] = None,
+    workspace: Optional[Tensor] = None,
+) -> Tensor:
+    """paged_decode_attention over a 4-bit pool: the same arguments, plan, workspace and fault word."""
+    batch, max_blocks = block_tables.shape
+    nbytes = workspace_bytes(batch, max_blocks)
+    if nbytes <= 0:
+        raise HipExtensionError(f"invalid attention shape batch={batch} max_blocks={max_blocks}")
+    if workspace is None:
+        workspace = attention_workspace(pool.device, nbytes)
+    if plan is None:
+        plan = torch.from_numpy(decode_plan(context_lens.cpu().numpy(), block_tables.cpu().numpy())).to(pool.device)
+    planned_decode_attention_q4(out, query, pool, layer, context_lens, plan, max_blocks, workspace)
+    return workspace
+
+
+def planned_decode_attention_q4(
+    out: Tensor, query: Tensor, pool: Tensor, layer: int, context_lens: Tensor, plan: Tensor, max_blocks: int,
+    workspace: Tensor, *, new_key: Optional[Tensor] = None, new_value: Optional[Tensor] = None,
+) -> None:
+    """planned_decode_attention over a 4-bit pool (uint8 [22, blocks, 4, 1152]): out/query float16 [batch, 32, 64] contiguous
+    (a dimension of 1 more between is taken), the plan, lengths and workspace as there. With new_key and new_value (float16
+    [batch, 4, 64]) each sequence's newest token is quantised and written in the same launch, with the results of
+    kv_append_q4 followed by attention."""
+    device = _check_q4_pool(pool)
+    batch = context_lens.shape[0]
+    for name, rows in (("out", out), ("query", query)):
+        if rows.dtype is not torch.float16 or rows.numel() != batch * 2048 or rows.shape[0] != batch or not rows.is_contiguous() or rows.get_device() != device:
+            raise HipExtensionError(f"{name} must be contiguous float16 [{batch}, 32, 64] on GPU {device}")
+    lib = load()
+    nbytes = lib.pc_attn_workspace_bytes(batch, max_blocks)
+    if nbytes <= 0:
+        raise HipExtensionError(f"invalid attention shape batch={batch} max_blocks={max_blocks}")
+    if workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.get_device() != device:
+        raise HipExtensionError(f"workspace needs {nbytes} contiguous bytes on GPU {device}")
+    if context_lens.dtype is not torch.int32 or context_lens.dim() != 1 or not context_lens.is_contiguous() or context_lens.get_device() != device:
+        raise HipExtensionError(f"context_lens must be contiguous int32 [batch] on GPU {device}")
+    if plan.dtype is not torch.int32 or plan.dim() != 2 or plan.shape[1] != lib.pc_attn_plan_record_ints() or not plan.is_contiguous() or plan.get_device() != device:
+        raise HipExtensionError(f"plan must be a contiguous int32 decode_plan() array on GPU {device}")
+    if new_key is None and new_value is None:
+        _call_on(
+            device, lib, "pc_paged_decode_attn_q4", out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer,
+            context_lens.data_ptr(), batch, max_blocks, plan.data_ptr(), plan.shape[0], workspace.data_ptr(),
+        )
+        return
+    for name, rows in (("new_key", new_key), ("new_value", new_value)):
+        if rows is None:
+            raise HipExtensionError("new_key and new_value are given together")
+        _check_half(name, rows, (batch, 4, 64), device)
+    _call_on(
+        device, lib, "pc_kv_append_paged_decode_attn_q4", out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer,
+        context_lens.data_ptr(), batch, max_blocks, plan.data_ptr(), plan.shape[0], new_key.data_ptr(), new_value.data_ptr(),
+        workspace.data_ptr(),
     )

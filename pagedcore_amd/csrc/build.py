@@ -24,7 +24,7 @@ ROOT = os.path.dirname(PACKAGE)
 SOURCES = [
     os.path.join(HERE, name)
     for name in ("pagedcore_hip.hip", "decode_step.hip", "prefill.hip", "skinny_gemm.hip", "tile_gemm.hip", "fp8_rows.hip",
-                 "fp8_gemm.hip", "fp8_stream_gemm.hip", "fp8_tile_gemm.hip", "fault_word.hip")
+                 "fp8_gemm.hip", "fp8_stream_gemm.hip", "fp8_tile_gemm.hip", "fault_word.hip", "q4_rows.hip", "q4_attention.hip")
 ]
 OUTPUT = os.path.join(PACKAGE, "libpagedcore_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

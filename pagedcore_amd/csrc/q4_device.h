@@ -1,0 +1,167 @@
+// Device helpers of the 4-bit KV pool, shared by the kernels that write and read it (not part of the
+// C ABI): a row's quantisation and where its bytes lie.
+//
+// A row (64 values of one token, kv head and kind) is held as lo = min(x), s = the smallest fp16 with
+// 15 s >= max(x) - lo and the levels n = round_half_even((x - lo) / s), for the values lo + s n. s is
+// rounded up, so no level passes 15 and none needs a clamp; lo is one of the values, so it needs no rounding. The two
+// differences are fp32's: exact but in rows whose magnitudes span more than 2^13.
+// Scale and minimum belong to a row, not to a channel: they then leave the attention's products, which
+// multiply the levels alone (s and lo enter once per token, in fp32).
+//
+// A unit (one block of 16 tokens, one kv head) is 1152 bytes, nine 128-byte lines: K's levels (512 bytes), V's
+// (512), then (lo, s) as fp16 pairs of the 16 K rows (64) and of the 16 V rows (64). Within them the levels lie as
+// the matrix instruction's lanes take them, 16 bytes a lane, and every token has bytes of its own, so that rows are
+// written without reading their neighbours:
+//   K: token 4i + e (i, e in 0..3), dims 32 x + 8 g + j (x in 0..1, g in 0..3, j in 0..7): the word at
+//      256 (i / 2) + 64 e + 16 g + 8 (i % 2) + 4 x, bits 4 (j / 2) + 16 (j % 2)
+//   V: token 4q + t, dims 32 p + r (low half) and 32 p + 16 + r (high half of the byte, r in 0..15): the byte at
+//      256 (q / 2) + 16 r + 8 (q % 2) + 4 p + {0, 2, 1, 3}[t]
+// In both, a 16-bit half of (word >> 4 n) & 0x000F000F is one of two neighbours of the product's inner index.
+#ifndef PAGEDCORE_Q4_DEVICE_H
+#define PAGEDCORE_Q4_DEVICE_H
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include "attn_plan.h"
+#include "pc_device.h"
+#include "pagedcore_hip.h"
+
+namespace q4_device {
+
+using attn_plan::kHeadDim;
+using attn_plan::kKVHeads;
+using attn_plan::kLayers;
+using attn_plan::kSlots;
+using pc_device::half8_t;
+
+constexpr int kUnitBytes = PC_Q4_UNIT_BYTES;
+constexpr int kValueOffset = 512;
+constexpr int kPairOffset = 1024;       // (lo, s) of the K rows; the V rows' follow
+constexpr int kPairBytes = 4 * kSlots;  // 64
+constexpr int64_t kBlockBytes = kKVHeads * kUnitBytes;
+constexpr int kRowLanes = 8;  // lanes of a row, 8 values each
+static_assert(kUnitBytes == kPairOffset + 2 * kPairBytes, "K, V, and the pairs of both");
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(x)));
+}
+constexpr int kSwap1 = 0xB1;     // quad_perm [1, 0, 3, 2]
+constexpr int kSwap2 = 0x4E;     // quad_perm [2, 3, 0, 1]
+constexpr int kMirror8 = 0x141;  // row_half_mirror: lane 7 - l of its eight
+constexpr int kRotate8 = 0x128;  // row_ror 8: lane l ^ 8 of a row of 16
+
+// One eighth of a quantised row: its 8 levels as the K word above, and the row's (lo, s) as the pair's bits.
+struct Levels {
+  uint32_t word;
+  uint32_t pair;
+};
+
+// Lane a of eight (aligned) holds values 8a .. 8a + 7 of a row. The quotient is the correctly rounded one: with
+// the correctly rounded reciprocal and a product within an ulp, one residual step gives it (Markstein), and
+// only the exact quotient lies at a half where it does, so that ties go to the even level. (lo, s) of a row with
+// an infinity or NaN is (NaN, 0): all its values are NaN.
+__device__ __forceinline__ Levels quantize8(half8_t x) {
+#pragma clang fp contract(off)
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(x[j]);
+  float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
+  float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  float zero = 0.f;  // NaN if a value is not finite (min and max pass over a NaN)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) zero = fmaf(f[j], 0.f, zero);
+  lo = fminf(lo, dpp<kSwap1>(lo));
+  hi = fmaxf(hi, dpp<kSwap1>(hi));
+  zero += dpp<kSwap1>(zero);
+  lo = fminf(lo, dpp<kSwap2>(lo));
+  hi = fmaxf(hi, dpp<kSwap2>(hi));
+  zero += dpp<kSwap2>(zero);
+  lo = fminf(lo, dpp<kMirror8>(lo));
+  hi = fmaxf(hi, dpp<kMirror8>(hi));
+  zero += dpp<kMirror8>(zero);
+  lo += 0.f;  // a zero of either sign is +0: the row's bytes do not depend on the order of its values
+  const float span = hi - lo;
+  uint16_t step_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(span * (1.0f / 15.0f)));
+  // 15 s is exact in fp32 (4 and 11 bits).
+  if (static_cast<float>(__builtin_bit_cast(_Float16, step_bits)) * 15.0f < span) ++step_bits;
+  const float step = static_cast<float>(__builtin_bit_cast(_Float16, step_bits));
+  const float inverse = step > 0.f ? 1.0f / step : 0.f;
+  uint32_t low = 0, high = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = f[j] - lo;
+    float y = t * inverse;
+    y = fmaf(fmaf(-y, step, t), inverse, y);
+    const uint32_t n = __float_as_uint(y + 8388608.0f) & 15u;  // to an integer, to nearest even
+    if (j % 2 == 0) low |= n << (2 * j);
+    else high |= n << (2 * (j - 1));
+  }
+  Levels r;
+  const uint32_t lo_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo));
+  r.word = low | high << 16;
+  r.pair = lo_bits | static_cast<uint32_t>(step_bits) << 16;
+  if (!(zero == 0.f)) {
+    r.word = 0;
+    r.pair = 0x7e00u;  // (NaN, 0)
+  }
+  return r;
+}
+
+// The level of value j of a lane's word.
+__device__ __forceinline__ uint32_t level(uint32_t word, int j) { return word >> (4 * (j / 2) + 16 * (j % 2)) & 15u; }
+
+// Offsets within a unit: lane a's K word of token t, the first of lane a's V bytes (dims r = 8 (a % 2) + j at + 16 j), and
+// the row's pair.
+__device__ __forceinline__ int key_word(int t, int a) {
+  return 256 * (t >> 3) + 64 * (t & 3) + 16 * (a & 3) + 8 * (t >> 2 & 1) + 4 * (a >> 2);
+}
+__device__ __forceinline__ int value_byte(int t, int a) {
+  const int place = (t & 1) << 1 | (t >> 1 & 1);  // 0, 2, 1, 3
+  return kValueOffset + 256 * (t >> 3) + 128 * (a & 1) + 8 * (t >> 2 & 1) + 4 * (a >> 2) + place;
+}
+__device__ __forceinline__ int pair_offset(int kind, int t) { return kPairOffset + kPairBytes * kind + 4 * t; }
+
+// Stores token t's row (lane a of eight, all of them here) into its unit. A V byte holds values of two lanes, a and
+// a ^ 2: each stores the bytes of four of their eight columns.
+__device__ __forceinline__ void store_row(char* unit, int kind, int t, int a, const Levels& q) {
+  const uint32_t other = dpp<kSwap2>(q.word);
+  if (kind == 0) {
+    *reinterpret_cast<uint32_t*>(unit + key_word(t, a)) = q.word;
+  } else {
+    const bool upper = (a & 2) != 0;
+    const uint32_t lo_word = upper ? other : q.word, hi_word = upper ? q.word : other;
+    char* at = unit + value_byte(t, a) + (upper ? 64 : 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t n = upper ? level(lo_word, j + 4) | level(hi_word, j + 4) << 4 : level(lo_word, j) | level(hi_word, j) << 4;
+      at[16 * j] = static_cast<char>(n);
+    }
+  }
+  if (a == 0) *reinterpret_cast<uint32_t*>(unit + pair_offset(kind, t)) = q.pair;
+}
+
+// Values 8a .. 8a + 7 of a row, in fp16: the exact lo + s n, rounded to fp32 (it has at most 40 bits) and to fp16. s is
+// rounded up, so lo + 15 s may pass 65504 where the row's largest value did not: it reads as 65504.
+__device__ __forceinline__ half8_t row_values(uint32_t pair, const uint32_t n[8]) {
+  const float lo = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair)));
+  const float step = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> 16)));
+  half8_t x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = fmaf(step, static_cast<float>(n[j]), lo);
+    x[j] = static_cast<_Float16>(v > 65504.f ? 65504.f : v);
+  }
+  return x;
+}
+
+}  // namespace q4_device
+
+#endif  // PAGEDCORE_Q4_DEVICE_H

@@ -1,0 +1,390 @@
+"""The 4-bit KV pool on the GPU: appended bytes equal the definition's bit for bit, rows read back are its values rounded
+once, attention stays within a bound derived from its operations, the fused append equals the pair of calls."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import q4_reference as ref
+from pagedcore_amd import _hip
+from pagedcore_amd.decoder import capture_graph
+from tests.support import flags_clear
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(rng, *shape):
+    """K or V rows float16 [..., 4, 64] of several scales, some constant, some with ties."""
+    x = rng.standard_normal((*shape, 4, 64)) * 2.0 ** rng.integers(-6, 4, (*shape, 4, 1)) + rng.standard_normal((*shape, 4, 1))
+    x = x.astype(np.float16)
+    flat = x.reshape(-1, 64)
+    flat[3::17] = flat[3::17, :1]  # constant rows
+    flat[5::13] = np.float16(0.5) * rng.integers(-16, 16, flat[5::13].shape)  # whole halves: many ties
+    return x
+
+
+def _pool(rng, blocks):
+    return rng.integers(0, 256, (22, blocks, 4, ref.UNIT), dtype=np.uint8)
+
+
+def _up(array, device):
+    return torch.from_numpy(np.ascontiguousarray(array)).to(device)
+
+
+def _tables(rng, lengths, spare=3):
+    need = -(-np.asarray(lengths) // 16)
+    blocks = int(need.sum()) + spare
+    ids = rng.permutation(blocks).astype(np.int32)
+    tables = np.zeros((len(lengths), max(1, int(need.max()))), dtype=np.int32)
+    at = 0
+    for b, n in enumerate(need):
+        tables[b, :n] = ids[at : at + n]
+        at += n
+    return tables, blocks
+
+
+def _filled(rng, blocks, layer):
+    """A pool whose layer holds quantised rows in every slot, other bytes random (whatever they stand for)."""
+    pool = _pool(rng, blocks)
+    key, value = _rows(rng, 1, blocks * 16), _rows(rng, 1, blocks * 16)
+    ref.write(pool, layer, key, value, range(blocks * 16))
+    return pool
+
+
+@pytest.mark.parametrize("layers,begin,tokens,start", [(1, 21, 1, 0), (22, 0, 17, 5), (3, 7, 64, 0), (2, 20, 131, 15), (5, 0, 4, 2)])
+def test_append_bytes(device, layers, begin, tokens, start):
+    rng = np.random.default_rng(tokens)
+    blocks = -(-(start + tokens) // 16) + 2
+    table = rng.permutation(blocks)
+    at = np.arange(start, start + tokens)
+    slots = table[at // 16] * 16 + at % 16
+    pool = _pool(rng, blocks)
+    key, value = _rows(rng, layers, tokens), _rows(rng, layers, tokens)
+    expected = pool.copy()
+    ref.write(expected, begin, key, value, slots)
+    got = _up(pool, device)
+    _hip.kv_append_q4(got, begin, _up(key, device), _up(value, device), _up(slots, device))
+    assert torch.equal(got.cpu(), torch.from_numpy(expected))
+
+
+@pytest.mark.parametrize("offset", [0, 8, 1])
+def test_append_strided_and_skipped(device, offset):
+    """Rows as views of wider ones (16-byte aligned or not), slots in any order, some outside the pool."""
+    rng = np.random.default_rng(7)
+    tokens, blocks = 50, 6
+    wide = np.zeros((2, tokens, 600 + offset), dtype=np.float16)
+    wide[:, :, offset : offset + 256] = _rows(rng, 2, tokens).reshape(2, tokens, 256)
+    wide[:, :, offset + 256 : offset + 512] = _rows(rng, 2, tokens).reshape(2, tokens, 256)
+    slots = rng.permutation(blocks * 16)[:tokens].astype(np.int64)
+    slots[[3, 11, 12]] = (-1, blocks * 16, 1 << 40)
+    pool = _pool(rng, blocks)
+    on = _up(wide, device)
+    key, value = (on[:, :, at : at + 256].unflatten(-1, (4, 64)) for at in (offset, offset + 256))
+    got = _up(pool, device)
+    _hip.kv_append_q4(got, 4, key, value, _up(slots, device))
+    expected = pool.copy()
+    ref.write(expected, 4, key.cpu().numpy(), value.cpu().numpy(), slots)
+    assert torch.equal(got.cpu(), torch.from_numpy(expected))
+    # Read back into views of the same alignment; skipped tokens' rows keep what they held.
+    back = torch.full((2, 2, tokens, 600 + offset), 7.0, dtype=torch.float16, device=device)
+    rows = [back[i, :, :, offset : offset + 256].unflatten(-1, (4, 64)) for i in range(2)]
+    _hip.kv_read_q4(rows[0], rows[1], got, 4, _up(slots, device))
+    inside = (slots >= 0) & (slots < blocks * 16)
+    for kind in range(2):
+        want = np.stack([ref.rows(expected[4 + layer], kind, np.where(inside, slots, 0)) for layer in range(2)])
+        _assert_read(rows[kind].cpu().numpy()[:, inside], want[:, inside])
+        assert (rows[kind].cpu().numpy()[:, ~inside] == 7.0).all()
+    back[..., offset : offset + 256] = 7.0
+    assert (back == 7.0).all()
+
+
+def _assert_read(got, want):
+    """One rounding to fp16 behind one to fp32 (half steps 2^-11 and 2^-24 of the value; 2^-25 below fp16's normal range); what
+    lies past fp16's largest value is that value."""
+    want = np.minimum(want, 65504.0)
+    fine = np.isfinite(want)
+    assert (np.isnan(got) == ~fine).all()
+    off = np.abs(got.astype(np.float64) - want)[fine]
+    assert (off <= (2.0**-11 + 2.0**-23) * np.abs(want[fine]) + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("layers,begin,tokens", [(1, 3, 1), (22, 0, 33), (2, 20, 300)])
+def test_read_rows(device, layers, begin, tokens):
+    rng = np.random.default_rng(tokens)
+    blocks = tokens // 16 + 3
+    pool = _pool(rng, blocks)
+    for layer in range(layers):
+        ref.write(pool, begin + layer, _rows(rng, 1, blocks * 16), _rows(rng, 1, blocks * 16), range(blocks * 16))
+    slots = rng.integers(0, blocks * 16, tokens)  # a slot may be read twice
+    key = torch.zeros((layers, tokens, 4, 64), dtype=torch.float16, device=device)
+    value = torch.zeros_like(key)
+    _hip.kv_read_q4(key, value, _up(pool, device), begin, _up(slots, device))
+    for kind, got in enumerate((key, value)):
+        _assert_read(got.cpu().numpy(), np.stack([ref.rows(pool[begin + layer], kind, slots) for layer in range(layers)]))
+
+
+def test_rows_of_every_kind(device):
+    """Infinities and NaN, the widest and the narrowest spans, subnormal steps, zeros of both signs."""
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((1, 16, 4, 64)).astype(np.float16)
+    f = x.reshape(-1, 64)
+    f[0], f[1, 5], f[2, 63], f[3, :2] = np.nan, np.inf, -np.inf, (np.inf, -np.inf)
+    f[4], f[5] = 65504, np.where(np.arange(64) % 2, 65504, -65504)
+    f[6] = np.where(np.arange(64) % 2, -0.0, 0.0)
+    f[7] = (np.arange(64) % 23) * np.float16(2.0**-24)  # a span whose fifteenth lies between two subnormals
+    f[8] = (np.arange(64) % 16) * np.float16(2.0**-24)
+    f[9] = np.arange(64) * np.float16(2.0**-14)
+    f[10] = np.where(np.arange(64) == 17, 2.0**-24, 0)
+    f[11] = -(np.arange(64).astype(np.float16))
+    pool = _pool(rng, 2)
+    expected = pool.copy()
+    ref.write(expected, 0, x, x[..., ::-1].copy(), range(16))
+    got = _up(pool, device)
+    slots = torch.arange(16, device=device)
+    _hip.kv_append_q4(got, 0, _up(x, device), _up(x[..., ::-1], device), slots)
+    key = torch.zeros((1, 16, 4, 64), dtype=torch.float16, device=device)
+    value = torch.zeros_like(key)
+    _hip.kv_read_q4(key, value, got, 0, slots)
+    got = got.cpu().numpy()
+    bad = [i for i in range(64) if not np.isfinite(f[i]).all()]
+    for kind, rows in enumerate((key, value)):
+        want = ref.rows(expected[0], kind, np.arange(16))
+        _assert_read(rows.cpu().numpy()[0], want)
+        assert np.isnan(rows.cpu().numpy()[0].reshape(-1, 64)[bad]).all()
+    assert (got == expected).all()
+
+
+def _attend(device, pool, layer, query, tables, lengths, new=None, out=None, workspace=None):
+    batch = len(lengths)
+    lens, tabs = np.asarray(lengths, dtype=np.int32), np.asarray(tables, dtype=np.int32)
+    plan = _up(_hip.decode_plan(lens, tabs), device)
+    if workspace is None:
+        workspace = torch.zeros(_hip.workspace_bytes(batch, tabs.shape[1]), dtype=torch.uint8, device=device)
+    if out is None:
+        out = torch.full((batch, 32, 64), 3.0, dtype=torch.float16, device=device)
+    key, value = new if new is not None else (None, None)
+    _hip.planned_decode_attention_q4(out, query, pool, layer, _up(lens, device), plan, tabs.shape[1], workspace, new_key=key, new_value=value)
+    torch.cuda.synchronize()
+    _hip.check_attention_faults(workspace, "test")
+    assert flags_clear(workspace)
+    return out
+
+
+def _check_rows(out, query, units, tables, lengths, rows=None):
+    got = out.cpu().numpy().astype(np.float64)
+    q = query.cpu().numpy()
+    for b in range(len(lengths)) if rows is None else rows:
+        if lengths[b] == 0:
+            assert (got[b] == 3.0).all()  # left as it was
+            continue
+        want, bound = ref.attention(q[b], units, tables[b], int(lengths[b]))
+        off = np.abs(got[b] - want)
+        assert (off <= bound).all(), f"row {b} of length {lengths[b]}: {np.max(off / bound):.3g} of the bound"
+
+
+CASES = {
+    "one": [1],
+    "short": [1, 2, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65],
+    "block_ends": [128, 127, 129, 112, 80, 96, 16, 64],
+    "with_empty_rows": [0, 5, 0, 200, 0],
+    "cut": [2048, 3, 1500, 700],
+    "long": [9001],
+    "many_short": [1 + i % 48 for i in range(300)],
+}
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_attention(device, name):
+    rng = np.random.default_rng(len(name))
+    lengths = CASES[name]
+    tables, blocks = _tables(rng, lengths)
+    layer = 5
+    pool = _filled(rng, blocks, layer)
+    # Slots past a length hold anything, rows of NaN among it.
+    for b, n in enumerate(lengths):
+        if n % 16:
+            unit = pool[layer, tables[b, n // 16]]
+            for t in range(n % 16, 16):
+                for kind in range(2):
+                    at = ref.pair_place(kind, t)
+                    unit[:, at : at + 4] = np.frombuffer(np.array([np.nan, np.inf], dtype=np.float16).tobytes(), dtype=np.uint8)
+    query = _up(rng.standard_normal((len(lengths), 32, 64)).astype(np.float16), device)
+    out = _attend(device, _up(pool, device), layer, query, tables, lengths)
+    rows = range(0, len(lengths), 7) if len(lengths) > 100 else None
+    _check_rows(out, query, pool[layer], tables, lengths, rows)
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0**-20, 30.0, 1000.0])
+def test_attention_of_sharp_and_flat_scores(device, scale):
+    rng = np.random.default_rng(3)
+    lengths = [77, 400]
+    tables, blocks = _tables(rng, lengths)
+    pool = _filled(rng, blocks, 0)
+    query = _up((rng.standard_normal((2, 32, 64)) * scale).astype(np.float16), device)
+    out = _attend(device, _up(pool, device), 0, query, tables, lengths)
+    _check_rows(out, query, pool[0], tables, lengths)
+
+
+def test_constant_values_come_back_exactly(device):
+    rng = np.random.default_rng(4)
+    lengths = [333, 16]
+    tables, blocks = _tables(rng, lengths)
+    pool = _pool(rng, blocks)
+    value = np.full((1, blocks * 16, 4, 64), 3.140625, dtype=np.float16)
+    ref.write(pool, 2, _rows(rng, 1, blocks * 16), value, range(blocks * 16))
+    query = _up(rng.standard_normal((2, 32, 64)).astype(np.float16), device)
+    out = _attend(device, _up(pool, device), 2, query, tables, lengths)
+    assert (out == 3.140625).all()
+
+
+def test_nan_rows_stay_in_their_head_and_sequence(device):
+    rng = np.random.default_rng(5)
+    lengths = [40, 70, 90]
+    tables, blocks = _tables(rng, lengths)
+    pool = _filled(rng, blocks, 1)
+    query = rng.standard_normal((3, 32, 64)).astype(np.float16)
+    query[2, 9] = np.nan
+    on = _up(pool, device)
+    clean = _attend(device, on, 1, _up(query, device), tables, lengths)
+    x = _rows(rng, 1, 2)
+    x[0, 0, 2, 7], x[0, 1, 3, 0] = np.nan, np.inf
+    fine = _rows(rng, 1, 2)
+    slots = np.array([tables[1, 33 // 16] * 16 + 33 % 16, tables[0, 5 // 16] * 16 + 5 % 16], dtype=np.int64)
+    _hip.kv_append_q4(on, 1, _up(x, device), _up(fine, device), _up(slots, device))
+    out = _attend(device, on, 1, _up(query, device), tables, lengths)
+    nan = torch.isnan(out).all(-1).cpu()
+    assert (torch.isnan(out).any(-1).cpu() == nan).all()
+    expected = torch.zeros((3, 32), dtype=torch.bool)
+    expected[1, 16:24] = expected[0, 24:32] = expected[2, 9] = True
+    assert torch.equal(nan, expected)
+    assert torch.equal(out[2, :9].view(torch.int16), clean[2, :9].view(torch.int16))
+
+
+def test_block_ids_outside_the_pool(device):
+    rng = np.random.default_rng(6)
+    lengths = [50, 300, 20]
+    tables, blocks = _tables(rng, lengths)
+    pool = _up(_filled(rng, blocks, 0), device)
+    query = _up(rng.standard_normal((3, 32, 64)).astype(np.float16), device)
+    clean = _attend(device, pool, 0, query, tables, lengths)
+    for bad in (blocks, -1, 1 << 30):
+        broken = tables.copy()
+        broken[1, 7] = bad
+        lens = np.array(lengths, dtype=np.int32)
+        workspace = torch.zeros(_hip.workspace_bytes(3, tables.shape[1]), dtype=torch.uint8, device=device)
+        out = torch.zeros_like(query)
+        _hip.planned_decode_attention_q4(out, query, pool, 0, _up(lens, device), _up(_hip.decode_plan(lens, broken), device), tables.shape[1], workspace)
+        torch.cuda.synchronize()
+        with pytest.raises(_hip.AttentionFaultError, match="block id"):
+            _hip.check_attention_faults(workspace, "test")
+        assert torch.isnan(out[1]).all()
+        assert torch.equal(out[[0, 2]].view(torch.int16), clean[[0, 2]].view(torch.int16))
+
+
+@pytest.mark.parametrize("name", ["one", "short", "block_ends", "cut", "many_short", "with_empty_rows"])
+def test_fused_append_equals_the_pair(device, name):
+    rng = np.random.default_rng(10 + len(name))
+    lengths = CASES[name]
+    tables, blocks = _tables(rng, lengths)
+    layer = 20
+    pool = _up(_filled(rng, blocks, layer), device)
+    query = _up(rng.standard_normal((len(lengths), 32, 64)).astype(np.float16), device)
+    new = [_up(_rows(rng, len(lengths)), device) for _ in range(2)]
+    slots = np.array([tables[b, (n - 1) // 16] * 16 + (n - 1) % 16 if n else -1 for b, n in enumerate(lengths)], dtype=np.int64)
+    pair = pool.clone()
+    _hip.kv_append_q4(pair, layer, new[0][None], new[1][None], _up(slots, device))
+    expected = _attend(device, pair, layer, query, tables, lengths)
+    for _ in range(2):  # a second call writes the same bytes
+        out = _attend(device, pool, layer, query, tables, lengths, new)
+        assert torch.equal(out.view(torch.int16), expected.view(torch.int16))
+        assert torch.equal(pool, pair)
+
+
+def test_decode_steps_in_a_graph(device):
+    """Append, attention and read back over several steps, captured once over static buffers and replayed with eager work
+    between, against the same calls made one by one."""
+    rng = np.random.default_rng(12)
+    batch, start = 5, np.array([1, 15, 16, 40, 200], dtype=np.int32)
+    tables, blocks = _tables(rng, start + 8)
+    width = tables.shape[1]
+    pool = _up(_filled(rng, blocks, 3), device)
+    eager = pool.clone()
+    capacity = _hip.plan_capacity(batch, width)
+    fields = _hip.load().pc_attn_plan_record_ints()
+    plan = torch.zeros((capacity, fields), dtype=torch.int32, device=device)
+    lens = torch.zeros(batch, dtype=torch.int32, device=device)
+    slots = torch.full((batch,), -1, dtype=torch.int64, device=device)
+    query, key, value = (torch.zeros((batch, n, 64), dtype=torch.float16, device=device) for n in (32, 4, 4))
+    workspace = torch.zeros(_hip.workspace_bytes(batch, width), dtype=torch.uint8, device=device)
+
+    def step():
+        out = torch.zeros_like(query)
+        back = torch.zeros((2, 1, batch, 4, 64), dtype=torch.float16, device=device)
+        _hip.planned_decode_attention_q4(out, query, pool, 3, lens, plan, width, workspace, new_key=key, new_value=value)
+        _hip.kv_read_q4(back[0], back[1], pool, 3, slots)
+        return out, back
+
+    graph, (out, back) = capture_graph(step, device)
+    for turn in range(6):
+        lengths = start + 1 + turn
+        host = np.zeros((capacity, fields), dtype=np.int32)
+        _hip.decode_plan_into(lengths, tables, host)
+        plan.copy_(torch.from_numpy(host))
+        lens.copy_(torch.from_numpy(lengths))
+        at = np.array([tables[b, (n - 1) // 16] * 16 + (n - 1) % 16 for b, n in enumerate(lengths)], dtype=np.int64)
+        slots.copy_(torch.from_numpy(at))
+        for t in (query, key, value):
+            t.copy_(torch.from_numpy(rng.standard_normal(tuple(t.shape)).astype(np.float16)))
+        graph.replay()
+        torch.cuda.synchronize()
+        expected = _attend(device, eager, 3, query, tables, lengths, (key, value))
+        assert torch.equal(out.view(torch.int16), expected.view(torch.int16))
+        assert torch.equal(pool, eager)
+        read = torch.zeros_like(back)
+        _hip.kv_read_q4(read[0], read[1], eager, 3, slots)
+        assert torch.equal(back.view(torch.int16), read.view(torch.int16))
+    _hip.check_attention_faults(workspace, "test")
+
+
+def test_offsets_past_32_bits(device):
+    """A pool of over 4 GiB: blocks at its end, in its last layer."""
+    blocks = 46000  # 22 * 46000 * 4608 bytes
+    pool = _hip.empty_q4_pool(blocks, device)
+    pool[21].zero_()
+    rng = np.random.default_rng(13)
+    length = 100
+    table = np.array([[blocks - 1 - 3 * i for i in range(7)]], dtype=np.int32)
+    slots = np.array([table[0, p // 16] * 16 + p % 16 for p in range(length)], dtype=np.int64)
+    key, value = _rows(rng, 1, length), _rows(rng, 1, length)
+    _hip.kv_append_q4(pool, 21, _up(key, device), _up(value, device), _up(slots, device))
+    last = pool[21].cpu().numpy()
+    expected = np.zeros((22, blocks, 4, ref.UNIT), dtype=np.uint8)[21:]
+    ref.write(expected, 0, key, value, slots)
+    assert (last == expected[0]).all()
+    query = _up(rng.standard_normal((1, 32, 64)).astype(np.float16), device)
+    out = _attend(device, pool, 21, query, table, [length])
+    _check_rows(out, query, last, table, [length])
+    back = torch.zeros((2, 1, length, 4, 64), dtype=torch.float16, device=device)
+    _hip.kv_read_q4(back[0], back[1], pool, 21, _up(slots, device))
+    for kind in range(2):
+        _assert_read(back[kind, 0].cpu().numpy(), ref.rows(last, kind, slots))
+
+
+def test_another_stream(device):
+    rng = np.random.default_rng(14)
+    lengths = [600, 31]
+    tables, blocks = _tables(rng, lengths)
+    pool = _filled(rng, blocks, 0)
+    on = _up(pool, device)
+    query = _up(rng.standard_normal((2, 32, 64)).astype(np.float16), device)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        out = torch.full_like(query, 3.0)
+        lens = np.array(lengths, dtype=np.int32)
+        workspace = _hip.paged_decode_attention_q4(out, query, on, 0, _up(tables, device), _up(lens, device))
+    stream.synchronize()
+    _hip.check_attention_faults(workspace, "test")
+    _check_rows(out, query, pool[0], tables, lengths)
