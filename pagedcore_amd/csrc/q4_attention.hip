@@ -46,7 +46,12 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 64 * kKVHeads;
+constexpr int kParts = 2;  // waves of a kv head
+constexpr int kWaves = kParts * kKVHeads;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
+constexpr int kMergeParts = 4;   // partials a round trip
+constexpr int kMergeGroup = 16;  // parts of a long span that one of them folds
 constexpr int kStepBlocks = 4;
 // A raw score, in units of 2^-24, to a base-2 exponent: 2^24 log2(e) / 8.
 constexpr float kRawToLog2 = 16777216.0f * kScoreToLog2;
@@ -113,6 +118,26 @@ __device__ __forceinline__ Part load_part(const char* slot, int lane) {
   return p;
 }
 
+// A partial in LDS: O at 16 L and 1024 + 16 L of lane L, (m, l) at 2048 + 8 L.
+__device__ __forceinline__ void put_part(char* area, int lane, const Part& p) {
+  *reinterpret_cast<float4_t*>(area + 16 * lane) = float4_t{p.o[0], p.o[1], p.o[2], p.o[3]};
+  *reinterpret_cast<float4_t*>(area + 1024 + 16 * lane) = float4_t{p.o[4], p.o[5], p.o[6], p.o[7]};
+  reinterpret_cast<float*>(area + 2048)[2 * lane] = p.m;
+  reinterpret_cast<float*>(area + 2048)[2 * lane + 1] = p.l;
+}
+__device__ __forceinline__ Part take_part(const char* area, int lane) {
+  const float4_t a = *reinterpret_cast<const float4_t*>(area + 16 * lane), b = *reinterpret_cast<const float4_t*>(area + 1024 + 16 * lane);
+  Part p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p.o[i] = a[i];
+    p.o[4 + i] = b[i];
+  }
+  p.m = reinterpret_cast<const float*>(area + 2048)[2 * lane];
+  p.l = reinterpret_cast<const float*>(area + 2048)[2 * lane + 1];
+  return p;
+}
+
 // Eight levels of a word as fp16 subnormals n 2^-24.
 __device__ __forceinline__ half8_t key_levels(uint32_t w) {
   uint4_t r = {w & 0x000F000Fu, w >> 4 & 0x000F000Fu, w >> 8 & 0x000F000Fu, w >> 12 & 0x000F000Fu};
@@ -142,237 +167,353 @@ __device__ __forceinline__ uint32_t take_half(uint32_t x, uint32_t y) {
       __builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(y), kRotate8, 0xf, UPPER ? 0xc : 0x3, false));
 }
 
+// The workspace slots of the parts of one cut sequence that a bin waits for: parts first, first + stride, ... (count of them).
+struct Waited {
+  int first, stride, count;
+};
+
+// Folds the waited parts into `total`, in order, as their flags rise, and lowers the flags. Returns PC_ATTN_FAULT_* bits.
+__device__ __forceinline__ int merge_parts(Part& total, char* slots, int slot0, const Waited& parts, int h, int lane, int key) {
+  const int want = key | (xcc_id() + 1);
+  bool timeout = false, foreign = false;
+  for (int base = 0; base < parts.count; base += 64) {
+    const int n = min(64, parts.count - base);
+    // Lane k polls the flag of part k (lanes past the span repeat the last one).
+    int32_t* flag = reinterpret_cast<int32_t*>(part_slot(slots, slot0, parts.first + parts.stride * (base + min(lane, n - 1)), h) + kFlagOffset);
+    int f = 0;
+    for (int spins = 0; spins < kMaxSpins; ++spins) {
+      f = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) == 0) break;
+      __builtin_amdgcn_s_sleep(1);
+    }
+    timeout |= __builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) != 0;
+    foreign |= __builtin_amdgcn_ballot_w64(flag_of_call(f, key) && f != want) != 0;
+    asm volatile("" ::: "memory");
+    // Four parts a round trip; past the last one the last is loaded again and not folded.
+    for (int k = 0; k < n; k += kMergeParts) {
+      Part p[kMergeParts];
+#pragma unroll
+      for (int i = 0; i < kMergeParts; ++i) p[i] = load_part(part_slot(slots, slot0, parts.first + parts.stride * (base + min(k + i, n - 1)), h), lane);
+#pragma unroll
+      for (int i = 0; i < kMergeParts; ++i) {
+        if (k + i < n) fold_part(total, p[i]);
+      }
+    }
+    if (lane < n) __hip_atomic_store(flag, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (timeout || foreign) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) total.o[i] = NAN;
+  }
+  return (timeout ? PC_ATTN_FAULT_MERGE_TIMEOUT : 0) | (foreign ? PC_ATTN_FAULT_FOREIGN_XCD : 0);
+}
+
+// One step's bytes: four blocks of one head. The parts of the next step are loaded as this one's are used up.
+struct Step {
+  uint4_t k[2], v[2], kp[2], vp[2];
+
+  __device__ __forceinline__ void load_keys(const char* kb) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) k[a] = *reinterpret_cast<const uint4_t*>(kb + 256 * a);
+  }
+  __device__ __forceinline__ void load_pairs(const char* vb, int c) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) kp[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::pair_offset(0, 8 * a + 4 * (c >> 3)));
+#pragma unroll
+    for (int a = 0; a < 2; ++a) vp[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::pair_offset(1, 8 * a + 4 * (c >> 3)));
+  }
+  __device__ __forceinline__ void load_values(const char* vb, int c) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) v[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::kValueOffset + 256 * a + 16 * c);
+  }
+};
+
+// Where a lane finds its bytes of a step: its K row's chunk (of block c / 4 of the four) and block g's unit. Ids outside the
+// pool are never dereferenced (block 0 is read); blocks past the segment's repeat its last one.
+struct Block4 {
+  const int32_t* ids;  // of the segment, in LDS
+  int nblk;
+  const char* lbase;
+  int64_t num_blocks;
+  int c, g;
+
+  // Returns whether one of the step's ids lies outside the pool.
+  __device__ __forceinline__ bool addresses(int u, const char*& kb, const char*& vb) const {
+    const uint32_t idk = static_cast<uint32_t>(ids[min(u + (c >> 2), nblk - 1)]);
+    const uint32_t idv = static_cast<uint32_t>(ids[min(u + g, nblk - 1)]);
+    kb = lbase + static_cast<int64_t>(idk >= static_cast<uint64_t>(num_blocks) ? 0 : idk) * kBlockBytes + 64 * (c & 3) + 16 * g;
+    vb = lbase + static_cast<int64_t>(idv >= static_cast<uint64_t>(num_blocks) ? 0 : idv) * kBlockBytes;
+    return __builtin_amdgcn_ballot_w64(idv >= static_cast<uint64_t>(num_blocks)) != 0;
+  }
+};
+
 template <bool APPEND>
-__global__ __launch_bounds__(kThreads) void paged_decode_q4_kernel(const int32_t* plan, const _Float16* query, char* pool,
-                                                                  int64_t num_blocks, int layer, int batch, int nslots,
-                                                                  _Float16* out, char* workspace, const _Float16* new_key,
-                                                                  const _Float16* new_value) {
-  const int h = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int32_t* __restrict__ plan, const _Float16* query, char* pool,
+                                                                     int64_t num_blocks, int layer, int batch, int nslots,
+                                                                     _Float16* out, char* workspace, const _Float16* new_key,
+                                                                     const _Float16* new_value) {
+  __shared__ int32_t ids[kMaxUnits];
+  __shared__ __attribute__((aligned(16))) char shared_parts[kWaves * 2 * kPartBytes];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = wave % kKVHeads, part = wave / kKVHeads;
   const int lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
   const int32_t* row = plan + static_cast<int64_t>(blockIdx.x) * kRowInts;
-  const int32_t* ids = row + kRecordInts;
   char* const slots = workspace + kWorkspaceHeader;
   int32_t rec[kRecordInts];
 #pragma unroll
   for (int i = 0; i < kRecordInts; ++i) rec[i] = row[i];
+  const int32_t my_id = row[kRecordInts + (threadIdx.x & (kMaxUnits - 1))];
   const int nseg = rec[0], nunits = rec[1];
   if (nseg <= 0 || nseg > kMaxSegs || nunits <= 0 || nunits > kMaxUnits) return;  // padding rows do nothing
+  auto field = [&](int s, int f) { return row[kHeaderInts + s * kSegInts + f]; };  // of a segment, by a scalar load
+  // The segments' blocks and steps; a record whose segments are not its blocks does nothing.
+  int steps = 0;
+  {
+    int64_t blocks = 0;
+    bool sound = true;
+#pragma unroll
+    for (int s = 0; s < kMaxSegs; ++s) {
+      if (s < nseg) {
+        const int n = rec[kHeaderInts + s * kSegInts + 3];
+        sound &= n > 0;
+        blocks += n;
+        steps += (n + kStepBlocks - 1) / kStepBlocks;
+      }
+    }
+    if (!sound || blocks != nunits) return;
+  }
+  if (threadIdx.x < kMaxUnits) ids[threadIdx.x] = my_id;
   const int key = flag_key(rec[2], layer);
   char* const lbase = pool + static_cast<int64_t>(layer) * num_blocks * kBlockBytes + h * kUnitBytes;
-
-  auto field = [&](int s, int f) {
-    return s == 0 ? rec[8 + f] : s == 1 ? rec[16 + f] : s == 2 ? rec[24 + f] : rec[32 + f];
-  };
+  __syncthreads();
 
   // APPEND: lanes (c, g) quantise and store the new K (c < 8) and V row of segment g, if the bin holds its sequence's last
-  // block, before this wave (which alone reads the unit) reads it: a wave's memory operations are done in order.
+  // block, before anything reads the unit.
   if constexpr (APPEND) {
-    int first = 0, sb = 0, len = 0, j0 = 0, nblk = 0;
+    if (part == 0) {
+      int first = 0, sb = 0, len = 0, j0 = 0, nblk = 0;
 #pragma unroll
-    for (int s = 0, at = 0; s < kMaxSegs; ++s) {
-      if (s == g) {
-        first = at;
-        sb = field(s, 0);
-        len = field(s, 1);
-        j0 = field(s, 2);
-        nblk = field(s, 3);
+      for (int s = 0, at = 0; s < kMaxSegs; ++s) {
+        if (s == g) {
+          first = at;
+          sb = rec[kHeaderInts + s * kSegInts + 0];
+          len = rec[kHeaderInts + s * kSegInts + 1];
+          j0 = rec[kHeaderInts + s * kSegInts + 2];
+          nblk = rec[kHeaderInts + s * kSegInts + 3];
+        }
+        if (s < nseg) at += rec[kHeaderInts + s * kSegInts + 3];
       }
-      at += max(field(s, 3), 1);
+      const bool mine = g < nseg && len > 0 && j0 + nblk == blocks_of(len) && sb >= 0 && sb < batch;
+      const uint32_t id = static_cast<uint32_t>(ids[mine ? first + nblk - 1 : 0]);
+      const int a = c & 7, kind = c >> 3;
+      const _Float16* src = (kind ? new_value : new_key) + (static_cast<int64_t>(mine ? sb : 0) * kKVHeads + h) * kHeadDim + 8 * a;
+      const q4_device::Levels q = q4_device::quantize8(*reinterpret_cast<const half8_t*>(src));
+      if (mine && id < static_cast<uint64_t>(num_blocks)) {
+        q4_device::store_row(lbase + static_cast<int64_t>(id) * kBlockBytes, kind, (len - 1) % kSlots, a, q);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const int last = first + nblk - 1;
-    const bool mine = g < nseg && nblk > 0 && len > 0 && j0 + nblk == blocks_of(len) && sb >= 0 && sb < batch && last < nunits;
-    const uint32_t id = static_cast<uint32_t>(ids[mine ? last : 0]);
-    const int a = c & 7, kind = c >> 3;
-    const _Float16* src = (kind ? new_value : new_key) + (static_cast<int64_t>(mine ? sb : 0) * kKVHeads + h) * kHeadDim + 8 * a;
-    const q4_device::Levels q = q4_device::quantize8(*reinterpret_cast<const half8_t*>(src));
-    if (mine && id < static_cast<uint64_t>(num_blocks)) {
-      q4_device::store_row(lbase + static_cast<int64_t>(id) * kBlockBytes, kind, (len - 1) % kSlots, a, q);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
   }
 
-  Part first_part, last_part;
-  bool any_bad = false;
-  int seg = 0, seg_end = 0;
-  for (; seg < nseg; ++seg) {
-    const int seg_begin = seg_end;
+  // This wave's steps [begin, end) of the bin's.
+  const int begin = part * steps / kParts, end = (part + 1) * steps / kParts;
+  char* const areas = shared_parts + wave * 2 * kPartBytes;
+  // The wave's first and last segment, if it holds their first step but cannot write their rows by itself (-1: none): what
+  // the wave did of them is in its first and second area.
+  int first_seg = -1, last_seg = -1;
+  bool any_bad = false, first = true;
+  int seg_begin = 0, seg_step = 0;
+  for (int seg = 0; seg < nseg; ++seg) {
     const int sb = field(seg, 0), len = field(seg, 1), j0 = field(seg, 2), nblk = field(seg, 3), nspan = field(seg, 6);
-    seg_end = seg_begin + max(nblk, 1);
-    if (nblk <= 0 || seg_end > nunits) break;  // malformed record
-    // Q of head c % 8 in the columns of the first (c < 8) or of the second tile of a pair; sum(q) 2^-24.
-    const int qb = sb < 0 || sb >= batch ? 0 : sb;
-    const half8_t* src = reinterpret_cast<const half8_t*>(query + (static_cast<int64_t>(qb) * kQHeads + kGroup * h + (c & 7)) * kHeadDim) + g;
-    const half8_t qa = src[0], qb8 = src[4];
-    const half8_t none = {0, 0, 0, 0, 0, 0, 0, 0};
-    const half8_t q0a = c < 8 ? qa : none, q0b = c < 8 ? qb8 : none, q1a = c < 8 ? none : qa, q1b = c < 8 ? none : qb8;
-    float qsum = 0.f;
+    const int seg_steps = (nblk + kStepBlocks - 1) / kStepBlocks;
+    const int from = max(begin - seg_step, 0), to = min(end - seg_step, seg_steps);
+    if (from < to) {
+      const Block4 at{ids + seg_begin, nblk, lbase, num_blocks, c, g};
+      Step d;
+      const char *kb, *vb;
+      bool bad = at.addresses(from * kStepBlocks, kb, vb);
+      d.load_keys(kb);
+      d.load_pairs(vb, c);
+      d.load_values(vb, c);
+      // Q of head c % 8, dims 8 g and 32 + 8 g on; sum(q) 2^-24.
+      const int qrow = sb < 0 || sb >= batch ? 0 : sb;
+      const half8_t* src = reinterpret_cast<const half8_t*>(query + (static_cast<int64_t>(qrow) * kQHeads + kGroup * h + (c & 7)) * kHeadDim) + g;
+      const half8_t qa = src[0], qb = src[4];
+      float qsum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) qsum += static_cast<float>(qa[j]) + static_cast<float>(qb8[j]);
-    qsum = sum_over_groups(qsum) * (1.0f / 16777216.0f);
+      for (int j = 0; j < 8; ++j) qsum += static_cast<float>(qa[j]) + static_cast<float>(qb[j]);
+      qsum = sum_over_groups(qsum) * (1.0f / 16777216.0f);
 
-    float m = 0.f, lsum = 0.f, usum = 0.f;
-    float4_t acc[4], wacc = {0.f, 0.f, 0.f, 0.f};
+      float m = 0.f, lsum = 0.f, usum = 0.f;
+      float4_t acc[4], wacc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-    bool bad = false;
-
-    for (int u = 0; u < nblk; u += kStepBlocks) {
-      const uint32_t idk = static_cast<uint32_t>(ids[seg_begin + min(u + (c >> 2), nblk - 1)]);
-      const uint32_t idv = static_cast<uint32_t>(ids[seg_begin + min(u + g, nblk - 1)]);
-      const bool out_of_pool = idv >= static_cast<uint64_t>(num_blocks);
-      bad |= __builtin_amdgcn_ballot_w64(out_of_pool) != 0;
-      // never dereferenced out of the pool
-      const char* kb = lbase + static_cast<int64_t>(idk >= static_cast<uint64_t>(num_blocks) ? 0 : idk) * kBlockBytes + 64 * (c & 3) + 16 * g;
-      const char* vb = lbase + static_cast<int64_t>(out_of_pool ? 0 : idv) * kBlockBytes;
-      uint4_t kw[2], vw[2], kp[2], vp[2];
+      for (int t = 0; t < 4; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma nounroll
+      for (int x = from; x < to; ++x) {
+        const int u = x * kStepBlocks;
+        const bool more = x + 1 < to;
+        if (more) bad |= at.addresses(u + kStepBlocks, kb, vb);
+        float4_t s[2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        kw[a] = *reinterpret_cast<const uint4_t*>(kb + 256 * a);
-        vw[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::kValueOffset + 256 * a + 16 * c);
-        kp[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::pair_offset(0, 8 * a + 4 * (c >> 3)));
-        vp[a] = *reinterpret_cast<const uint4_t*>(vb + q4_device::pair_offset(1, 8 * a + 4 * (c >> 3)));
-      }
-      float y[2][4];
+        for (int a = 0; a < 2; ++a) {
+          float4_t even = {0.f, 0.f, 0.f, 0.f}, odd = even;
+          even = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][0]), qa, even, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][2]), qa, odd, 0, 0, 0);
+          even = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][1]), qb, even, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][3]), qb, odd, 0, 0, 0);
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        float4_t s = {0.f, 0.f, 0.f, 0.f};
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(kw[a][0]), q0a, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(kw[a][1]), q0b, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(kw[a][2]), q1a, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(kw[a][3]), q1b, s, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[a][e] = fmaf(pair_low(kp[a][e]), qsum, pair_step(kp[a][e]) * s[e]);
-      }
-      // Tokens of block u + g that exist; the score of one that does not is -inf and its weights are 0, whatever its bytes are.
-      const int valid = u + g < nblk ? len - (j0 + u + g) * kSlots : 0;
-      const bool full = __builtin_amdgcn_ballot_w64(valid < kSlots) == 0;
-      if (!full) {
+          for (int e = 0; e < 4; ++e) s[a][e] = c < 8 ? even[e] : odd[e];
+        }
+        if (more) d.load_keys(kb);
+        float y[2][4];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[a][e] = 8 * a + 4 * (c >> 3) + e < valid ? y[a][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) y[a][e] = fmaf(pair_low(d.kp[a][e]), qsum, pair_step(d.kp[a][e]) * s[a][e]);
+        // Tokens of block u + g that exist; the score of one that does not is -inf and its weights are 0, whatever its bytes are.
+        const int valid = u + g < nblk ? len - (j0 + u + g) * kSlots : 0;
+        const bool full = __builtin_amdgcn_ballot_w64(valid < kSlots) == 0;
+        if (!full) {
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool there = 8 * a + 4 * (c >> 3) + e < valid;
+              y[a][e] = there ? y[a][e] : -INFINITY;
+              d.vp[a][e] = there ? d.vp[a][e] : 0u;
+            }
+        }
+        const float bm = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])), fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
+        if (x == from) {
+          m = max_halves(max_over_groups(bm));  // token 0 of a step's first block is valid
+        } else if (__builtin_amdgcn_ballot_w64((bm - m) * kRawToLog2 > kLazyLog2) != 0) {
+          const float mn = fmaxf(m, max_halves(max_over_groups(bm)));
+          const float alpha = exp2_fast((m - mn) * kRawToLog2);
+          lsum *= alpha;
+          usum *= alpha;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t][e] *= alpha;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wacc[e] *= alpha;
+          m = mn;
+        }
+        bf16x8_t weights[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_fast((y[a][e] - m) * kRawToLog2);
+            lsum += p;
+            w[e] = p * pair_step(d.vp[a][e]);
+            usum = fmaf(p, pair_low(d.vp[a][e]), usum);
+          }
+          const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
+          const uint32_t lo0 = pack_bf16(w[0] - low_bf16(hi0), w[1] - high_bf16(hi0));
+          const uint32_t lo1 = pack_bf16(w[2] - low_bf16(hi1), w[3] - high_bf16(hi1));
+          // Columns 0-7: the weights of both tiles' tokens, columns 8-15 their remainders.
+          const uint4_t wp = {take_half<true>(hi0, lo0), take_half<true>(hi1, lo1), take_half<false>(lo0, hi0), take_half<false>(lo1, hi1)};
+          weights[a] = __builtin_bit_cast(bf16x8_t, wp);
+        }
+        if (more) d.load_pairs(vb, c);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(d.v[a][t >> 1], d.v[a][2 + (t >> 1)], 4 * (t & 1)), weights[a], acc[t], 0, 0, 0);
+          }
+          const uint4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+          wacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), weights[a], wacc, 0, 0, 0);
+        }
+        if (more) d.load_values(vb, c);
       }
-      const float bm = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])), fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
-      if (u == 0) {
-        m = max_halves(max_over_groups(bm));  // token 0 of the first block is valid
-      } else if (__builtin_amdgcn_ballot_w64((bm - m) * kRawToLog2 > kLazyLog2) != 0) {
-        const float mn = fmaxf(m, max_halves(max_over_groups(bm)));
-        const float alpha = exp2_fast((m - mn) * kRawToLog2);
-        lsum *= alpha;
-        usum *= alpha;
+      Part p;
+      p.m = m;
+      p.l = add_halves(sum_over_groups(lsum));
+      const float shift = fmaf(-128.f, add_halves(wacc[0]), add_halves(sum_over_groups(usum)));
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[t][e] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) wacc[e] *= alpha;
-        m = mn;
-      }
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        float w[4];
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp2_fast((y[a][e] - m) * kRawToLog2);
-          lsum += p;
-          float low = pair_low(vp[a][e]);
-          w[e] = p * pair_step(vp[a][e]);
-          if (!full && 8 * a + 4 * (c >> 3) + e >= valid) low = w[e] = 0.f;
-          usum = fmaf(p, low, usum);
+          const float x = add_halves(acc[k][e]), z = add_halves(acc[2 + k][e]);
+          p.o[4 * k + e] = bad ? NAN : (c < 8 ? x : z) + shift;
         }
-        const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
-        const uint32_t lo0 = pack_bf16(w[0] - low_bf16(hi0), w[1] - high_bf16(hi0));
-        const uint32_t lo1 = pack_bf16(w[2] - low_bf16(hi1), w[3] - high_bf16(hi1));
-        // Columns 0-7: the weights of both tiles' tokens, columns 8-15 their remainders.
-        const uint4_t wp = {take_half<true>(hi0, lo0), take_half<true>(hi1, lo1), take_half<false>(lo0, hi0), take_half<false>(lo1, hi1)};
-        const bf16x8_t weights = __builtin_bit_cast(bf16x8_t, wp);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(vw[a][t >> 1], vw[a][2 + (t >> 1)], 4 * (t & 1)), weights, acc[t], 0, 0, 0);
+      any_bad |= bad;
+      if (from == 0 && to == seg_steps && nspan == 1) {
+        if (sb >= 0 && sb < batch) store_output(out + (static_cast<int64_t>(sb) * kQHeads + kGroup * h) * kHeadDim, lane, p);
+      } else {
+        put_part(areas + (first ? 0 : kPartBytes), lane, p);
+        if (from == 0) {
+          first_seg = first ? seg : first_seg;
+          last_seg = first ? last_seg : seg;
         }
-        const uint4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-        wacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), weights, wacc, 0, 0, 0);
       }
+      first = false;
     }
-    Part p;
-    p.m = m;
-    p.l = add_halves(sum_over_groups(lsum));
-    const float shift = fmaf(-128.f, add_halves(wacc[0]), add_halves(sum_over_groups(usum)));
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = add_halves(acc[k][e]), z = add_halves(acc[2 + k][e]);
-        p.o[4 * k + e] = bad ? NAN : (c < 8 ? x : z) + shift;
-      }
-    any_bad |= bad;
-    if (nspan == 1) {
-      if (sb >= 0 && sb < batch) {
-        store_output(out + (static_cast<int64_t>(sb) * kQHeads + kGroup * h) * kHeadDim, lane, p);
-      }
-    } else {
-      if (seg == 0) first_part = p;
-      if (seg == nseg - 1) last_part = p;
-    }
-  }
-  const bool complete = seg == nseg && seg_end == nunits;  // the record's segments cover its blocks
-
-  const int b0 = rec[8], k00 = rec[12], kidx0 = rec[13], nspan0 = rec[14], slot0 = rec[15];
-  const int sl = nseg - 1;
-  const int kidxl = field(sl, 5), nspanl = field(sl, 6), slotl = field(sl, 7);
-  // The span's slots [first, first + parts - 1) lie in the workspace.
-  auto slots_ok = [&](int first, int parts) { return first >= 0 && parts >= 2 && first + static_cast<int64_t>(parts) - 1 <= nslots; };
-
-  // A part that is not the last of its span: store it, wait for the acknowledgement, then raise its flag.
-  if (complete && nspanl > 1 && kidxl < nspanl - 1 && kidxl >= 0 && slots_ok(slotl, nspanl)) {
-    char* slot = part_slot(slots, slotl, kidxl, h);
-    store_part(slot, lane, last_part);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (lane == 0) {
-      __hip_atomic_store(reinterpret_cast<int32_t*>(slot + kFlagOffset), key | (xcc_id() + 1), __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-    }
+    seg_begin += nblk;
+    seg_step += seg_steps;
   }
   int fault = any_bad ? PC_ATTN_FAULT_BLOCK_ID : 0;
-  // The last part of a cut sequence: the other parts in order as their flags rise, and this bin's part last. The bins of a
-  // sequence run on one XCD, whose L2 their partials meet in; the earlier ones were dispatched first and wait for nothing.
-  if (complete && nspan0 > 1 && kidx0 == nspan0 - 1 && slots_ok(slot0, nspan0) &&
-      k00 + static_cast<int64_t>(kGroups) * kidx0 == static_cast<int64_t>(blockIdx.x) && k00 >= 0) {
-    const int want = key | (xcc_id() + 1);
-    bool timeout = false, foreign = false;
-    Part total;
+  __syncthreads();
+  int tail_lane = lane;  // what is computed from it below is not carried through the loop above
+  asm volatile("" : "+v"(tail_lane));
+  // The later segment first: another bin may wait for its part, and the bin's first segment may have to wait itself.
+#pragma nounroll
+  for (int r = 1; r >= 0; --r) {
+    const int seg = r ? last_seg : first_seg;
+    if (seg < 0) continue;
+    const int sb = field(seg, 0), kidx = field(seg, 5), nspan = field(seg, 6), slot0 = field(seg, 7), k00 = field(seg, 4);
+    int seg_end = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) total.o[i] = 0.f;
-    total.m = -INFINITY;
-    total.l = 0.f;
-    for (int k = 0; k < nspan0 - 1; ++k) {
-      const char* slot = part_slot(slots, slot0, k, h);
-      int f = 0;
-      for (int spins = 0; spins < kMaxSpins && !timeout; ++spins) {
-        f = __builtin_amdgcn_readfirstlane(
-            __hip_atomic_load(reinterpret_cast<const int32_t*>(slot + kFlagOffset), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        if (flag_of_call(f, key)) break;
-        __builtin_amdgcn_s_sleep(2);
+    for (int s = 0; s < kMaxSegs; ++s) {
+      if (s <= seg) seg_end += (rec[kHeaderInts + s * kSegInts + 3] + kStepBlocks - 1) / kStepBlocks;
+    }
+    Part total = take_part(areas + r * kPartBytes, tail_lane);
+    // The waves behind this one whose first segment this is.
+    for (int p = part + 1; p < kParts && p * steps / kParts < seg_end; ++p) {
+      if ((p + 1) * steps / kParts > p * steps / kParts) {
+        const char* area = shared_parts + (p * kKVHeads + h) * 2 * kPartBytes;
+        fold_part(total, take_part(area, tail_lane));
       }
-      timeout |= !flag_of_call(f, key);
-      foreign |= flag_of_call(f, key) && f != want;  // raised on another XCD: its partial is not visible here
-      asm volatile("" ::: "memory");
-      fold_part(total, load_part(slot, lane));
     }
-    fold_part(total, first_part);
-    if (timeout || foreign) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) total.o[i] = NAN;
-      fault |= (timeout ? PC_ATTN_FAULT_MERGE_TIMEOUT : 0) | (foreign ? PC_ATTN_FAULT_FOREIGN_XCD : 0);
+    bool last = true;
+    if (nspan != 1) {
+      // The span's slots [slot0, slot0 + parts - 1) lie in the workspace, and the part in the span.
+      if (slot0 < 0 || nspan < 2 || slot0 + static_cast<int64_t>(nspan) - 1 > nslots || kidx < 0 || kidx >= nspan || k00 < 0 ||
+          k00 + static_cast<int64_t>(kGroups) * kidx != static_cast<int64_t>(blockIdx.x)) {
+        continue;
+      }
+      last = kidx == nspan - 1;
+      // Long spans are folded in two levels: the last part of every kMergeGroup takes its group's others, and the span's last
+      // part its own group's and then those.
+      const bool two_levels = nspan > 2 * kMergeGroup;
+      const int group = two_levels ? kidx / kMergeGroup * kMergeGroup : 0;
+      const bool heads = last && two_levels;
+      if (last || (two_levels && kidx % kMergeGroup == kMergeGroup - 1)) {
+#pragma nounroll
+        for (int level = 0; level < (heads ? 2 : 1); ++level) {
+          const Waited waited = level == 0 ? Waited{group, 1, kidx - group} : Waited{kMergeGroup - 1, kMergeGroup, group / kMergeGroup};
+          fault |= merge_parts(total, slots, slot0, waited, h, tail_lane, key);
+        }
+      }
     }
-    for (int k = lane; k < nspan0 - 1; k += 64) {
-      __hip_atomic_store(reinterpret_cast<int32_t*>(part_slot(slots, slot0, k, h) + kFlagOffset), 0, __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
+    if (last) {
+      if (sb >= 0 && sb < batch) store_output(out + (static_cast<int64_t>(sb) * kQHeads + kGroup * h) * kHeadDim, tail_lane, total);
+    } else {
+      char* slot = part_slot(slots, slot0, kidx, h);
+      store_part(slot, tail_lane, total);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (tail_lane == 0) {
+        __hip_atomic_store(reinterpret_cast<int32_t*>(slot + kFlagOffset), key | (xcc_id() + 1), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
-    if (b0 >= 0 && b0 < batch) store_output(out + (static_cast<int64_t>(b0) * kQHeads + kGroup * h) * kHeadDim, lane, total);
   }
-  if (fault != 0 && lane == 0) {
+  if (fault != 0 && tail_lane == 0) {
     __hip_atomic_fetch_or(reinterpret_cast<int32_t*>(workspace), fault, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
