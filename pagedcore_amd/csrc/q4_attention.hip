@@ -53,12 +53,12 @@ constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
 constexpr int kMergeParts = 4;   // partials a round trip
 constexpr int kMergeGroup = 16;  // parts of a long span that one of them folds
 constexpr int kStepBlocks = 4;
-// A raw score, in units of 2^-24, to a base-2 exponent: 2^24 log2(e) / 8.
-constexpr float kRawToLog2 = 16777216.0f * kScoreToLog2;
+constexpr int64_t kMaxBlocks = 1 << 26;  // a block's place in a layer, in 128-byte lines, in 32 bits
+static_assert(kMaxUnits == 256, "four vectors of block ids");
 constexpr float kLazyLog2 = 8.0f;  // headroom (log2 of p) before the running max is raised
 
 // Partial of one (sequence, kv head): lane (c, g) holds head c % 8, dims 16 T + 4 g + e, T = 2 (c / 8) + {0, 1}:
-// unnormalized O, and the head's max (raw) and sum.
+// unnormalized O, and the head's max (a base-2 exponent) and sum.
 struct Part {
   float o[8];
   float m, l;
@@ -70,8 +70,8 @@ __device__ __forceinline__ float max_halves(float x) { return fmaxf(x, dpp<kRota
 // acc <- acc (+) p, the online-softmax fold.
 __device__ __forceinline__ void fold_part(Part& acc, const Part& p) {
   const float mn = fmaxf(acc.m, p.m);
-  const float so = exp2_fast((acc.m - mn) * kRawToLog2);
-  const float sn = exp2_fast((p.m - mn) * kRawToLog2);
+  const float so = exp2_fast(acc.m - mn);
+  const float sn = exp2_fast(p.m - mn);
   acc.l = fmaf(p.l, sn, acc.l * so);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc.o[i] = fmaf(p.o[i], sn, acc.o[i] * so);
@@ -138,17 +138,32 @@ __device__ __forceinline__ Part take_part(const char* area, int lane) {
   return p;
 }
 
-// Eight levels of a word as fp16 subnormals n 2^-24.
+// Eight levels of a word as fp16 subnormals: n 2^-24 for j = 0, 1, 4, 5 and, left where they are in the byte, n 2^-20 for
+// j = 2, 3, 6, 7 (the query's elements make up for it, see scaled_query).
 __device__ __forceinline__ half8_t key_levels(uint32_t w) {
-  uint4_t r = {w & 0x000F000Fu, w >> 4 & 0x000F000Fu, w >> 8 & 0x000F000Fu, w >> 12 & 0x000F000Fu};
+  const uint32_t z = w >> 8;
+  uint4_t r = {w & 0x000F000Fu, w & 0x00F000F0u, z & 0x000F000Fu, z & 0x00F000F0u};
   return __builtin_bit_cast(half8_t, r);
 }
 
-// Levels of two words (tokens 0-3 and 4-7; `high`: the byte's upper half) as bf16 128 + n.
-__device__ __forceinline__ bf16x8_t value_levels(uint32_t a, uint32_t b, int shift) {
-  uint4_t r = {(a >> shift & 0x000F000Fu) | 0x43004300u, (a >> (8 + shift) & 0x000F000Fu) | 0x43004300u,
-               (b >> shift & 0x000F000Fu) | 0x43004300u, (b >> (8 + shift) & 0x000F000Fu) | 0x43004300u};
+// Levels of two words (tokens 0-3 and 4-7; shift 4: the byte's upper half) as bf16 128 + n. `bias` is 0x43004300 in a vector
+// register: an and-or takes one constant from the scalar ones.
+__device__ __forceinline__ bf16x8_t value_levels(uint32_t a, uint32_t b, int shift, uint32_t bias) {
+  uint4_t r = {(a >> shift & 0x000F000Fu) | bias, (a >> (8 + shift) & 0x000F000Fu) | bias, (b >> shift & 0x000F000Fu) | bias,
+               (b >> (8 + shift) & 0x000F000Fu) | bias};
   return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// q with its elements j = 0, 1, 4, 5 of every eight times `even` and the others times `odd`.
+__device__ __forceinline__ half8_t scaled_query(half8_t q, _Float16 even, _Float16 odd) {
+  return q * half8_t{even, even, odd, odd, even, even, odd, odd};
+}
+
+// x times the pair's upper half (the step), one instruction: written as a product the compiler converts first.
+__device__ __forceinline__ float times_step(uint32_t pair, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(x));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -228,22 +243,17 @@ struct Step {
   }
 };
 
-// Where a lane finds its bytes of a step: its K row's chunk (of block c / 4 of the four) and block g's unit. Ids outside the
-// pool are never dereferenced (block 0 is read); blocks past the segment's repeat its last one.
-struct Block4 {
-  const int32_t* ids;  // of the segment, in LDS
+// Where a lane finds its bytes of a step: its K row's chunk (of block c / 4 of the four) and block g's unit. Blocks past the
+// segment's repeat its last one.
+struct Blocks {
+  const uint32_t* lines;  // of the segment's blocks in the layer, in units of 128 bytes (in LDS)
   int nblk;
   const char* lbase;
-  int64_t num_blocks;
   int c, g;
 
-  // Returns whether one of the step's ids lies outside the pool.
-  __device__ __forceinline__ bool addresses(int u, const char*& kb, const char*& vb) const {
-    const uint32_t idk = static_cast<uint32_t>(ids[min(u + (c >> 2), nblk - 1)]);
-    const uint32_t idv = static_cast<uint32_t>(ids[min(u + g, nblk - 1)]);
-    kb = lbase + static_cast<int64_t>(idk >= static_cast<uint64_t>(num_blocks) ? 0 : idk) * kBlockBytes + 64 * (c & 3) + 16 * g;
-    vb = lbase + static_cast<int64_t>(idv >= static_cast<uint64_t>(num_blocks) ? 0 : idv) * kBlockBytes;
-    return __builtin_amdgcn_ballot_w64(idv >= static_cast<uint64_t>(num_blocks)) != 0;
+  __device__ __forceinline__ void addresses(int u, const char*& kb, const char*& vb) const {
+    kb = lbase + (static_cast<uint64_t>(lines[min(u + (c >> 2), nblk - 1)]) << 7) + 64 * (c & 3) + 16 * g;
+    vb = lbase + (static_cast<uint64_t>(lines[min(u + g, nblk - 1)]) << 7);
   }
 };
 
@@ -252,22 +262,24 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
                                                                      int64_t num_blocks, int layer, int batch, int nslots,
                                                                      _Float16* out, char* workspace, const _Float16* new_key,
                                                                      const _Float16* new_value) {
-  __shared__ int32_t ids[kMaxUnits];
+  __shared__ uint32_t shared_lines[kWaves * kMaxUnits];
   __shared__ __attribute__((aligned(16))) char shared_parts[kWaves * 2 * kPartBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = wave % kKVHeads, part = wave / kKVHeads;
   const int lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
   const int32_t* row = plan + static_cast<int64_t>(blockIdx.x) * kRowInts;
-  char* const slots = workspace + kWorkspaceHeader;
+  // The record (scalar loads) and the bin's block ids (lane L of vector k holds id 64 k + L) in one round trip.
   int32_t rec[kRecordInts];
 #pragma unroll
   for (int i = 0; i < kRecordInts; ++i) rec[i] = row[i];
-  const int32_t my_id = row[kRecordInts + (threadIdx.x & (kMaxUnits - 1))];
+  int32_t idv[kMaxUnits / 64];
+#pragma unroll
+  for (int k = 0; k < kMaxUnits / 64; ++k) idv[k] = row[kRecordInts + 64 * k + lane];
   const int nseg = rec[0], nunits = rec[1];
   if (nseg <= 0 || nseg > kMaxSegs || nunits <= 0 || nunits > kMaxUnits) return;  // padding rows do nothing
   auto field = [&](int s, int f) { return row[kHeaderInts + s * kSegInts + f]; };  // of a segment, by a scalar load
-  // The segments' blocks and steps; a record whose segments are not its blocks does nothing.
+  // The segments' steps; a record whose segments are not its blocks does nothing.
   int steps = 0;
   {
     int64_t blocks = 0;
@@ -283,68 +295,93 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     }
     if (!sound || blocks != nunits) return;
   }
-  if (threadIdx.x < kMaxUnits) ids[threadIdx.x] = my_id;
-  const int key = flag_key(rec[2], layer);
-  char* const lbase = pool + static_cast<int64_t>(layer) * num_blocks * kBlockBytes + h * kUnitBytes;
-  __syncthreads();
-
-  // APPEND: lanes (c, g) quantise and store the new K (c < 8) and V row of segment g, if the bin holds its sequence's last
-  // block, before anything reads the unit.
-  if constexpr (APPEND) {
-    if (part == 0) {
-      int first = 0, sb = 0, len = 0, j0 = 0, nblk = 0;
+  // Each wave keeps the blocks' places for itself: no barrier before its first load. An id outside the pool is never
+  // dereferenced (block 0 is read).
+  uint32_t* const lines = shared_lines + wave * kMaxUnits;
+  uint64_t outside[kMaxUnits / 64];
 #pragma unroll
-      for (int s = 0, at = 0; s < kMaxSegs; ++s) {
-        if (s == g) {
-          first = at;
-          sb = rec[kHeaderInts + s * kSegInts + 0];
-          len = rec[kHeaderInts + s * kSegInts + 1];
-          j0 = rec[kHeaderInts + s * kSegInts + 2];
-          nblk = rec[kHeaderInts + s * kSegInts + 3];
-        }
-        if (s < nseg) at += rec[kHeaderInts + s * kSegInts + 3];
-      }
-      const bool mine = g < nseg && len > 0 && j0 + nblk == blocks_of(len) && sb >= 0 && sb < batch;
-      const uint32_t id = static_cast<uint32_t>(ids[mine ? first + nblk - 1 : 0]);
-      const int a = c & 7, kind = c >> 3;
-      const _Float16* src = (kind ? new_value : new_key) + (static_cast<int64_t>(mine ? sb : 0) * kKVHeads + h) * kHeadDim + 8 * a;
-      const q4_device::Levels q = q4_device::quantize8(*reinterpret_cast<const half8_t*>(src));
-      if (mine && id < static_cast<uint64_t>(num_blocks)) {
-        q4_device::store_row(lbase + static_cast<int64_t>(id) * kBlockBytes, kind, (len - 1) % kSlots, a, q);
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __syncthreads();
+  for (int k = 0; k < kMaxUnits / 64; ++k) {
+    const uint32_t id = static_cast<uint32_t>(idv[k]);
+    const bool bad = 64 * k + lane < nunits && id >= static_cast<uint64_t>(num_blocks);
+    outside[k] = __builtin_amdgcn_ballot_w64(bad);
+    lines[64 * k + lane] = (bad ? 0 : id) * static_cast<uint32_t>(kBlockBytes / 128);
   }
+  wave_lds_fence();
+  char* const lbase = pool + static_cast<int64_t>(layer) * num_blocks * kBlockBytes + h * kUnitBytes;
 
   // This wave's steps [begin, end) of the bin's.
   const int begin = part * steps / kParts, end = (part + 1) * steps / kParts;
+
+  // APPEND: lanes (c, g) quantise and store the new K (c < 8) and V row of segment g, if it ends its sequence and this wave has
+  // its last step: the wave alone reads the unit, after this, and a wave's memory operations are done in order.
+  if constexpr (APPEND) {
+    int first = 0, sb = 0, len = 0, j0 = 0, nblk = 0, ends = 0;
+#pragma unroll
+    for (int s = 0, at = 0, step = 0; s < kMaxSegs; ++s) {
+      const int n = s < nseg ? rec[kHeaderInts + s * kSegInts + 3] : 0;
+      step += (n + kStepBlocks - 1) / kStepBlocks;
+      if (s == g) {
+        first = at;
+        sb = rec[kHeaderInts + s * kSegInts];
+        len = rec[kHeaderInts + s * kSegInts + 1];
+        j0 = rec[kHeaderInts + s * kSegInts + 2];
+        nblk = n;
+        ends = step;
+      }
+      at += n;
+    }
+    const int last = nblk > 0 ? first + nblk - 1 : 0;
+    const bool mine = nblk > 0 && len > 0 && j0 + nblk == blocks_of(len) && sb >= 0 && sb < batch && ends > begin && ends <= end;
+    const int a = c & 7, kind = c >> 3;
+    const _Float16* src = (kind ? new_value : new_key) + (static_cast<int64_t>(mine ? sb : 0) * kKVHeads + h) * kHeadDim + 8 * a;
+    const uint32_t line = lines[last];
+    const bool in_pool = (outside[last >> 6] >> (last & 63) & 1) == 0;
+    if (__builtin_amdgcn_ballot_w64(mine) != 0) {
+      const q4_device::Levels q = q4_device::quantize8(*reinterpret_cast<const half8_t*>(src));
+      if (mine && in_pool) q4_device::store_row(lbase + (static_cast<uint64_t>(line) << 7), kind, (len - 1) % kSlots, a, q);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  }
+
+  uint32_t bias;
+  asm("v_mov_b32 %0, 0x43004300" : "=v"(bias));
   char* const areas = shared_parts + wave * 2 * kPartBytes;
   // The wave's first and last segment, if it holds their first step but cannot write their rows by itself (-1: none): what
   // the wave did of them is in its first and second area.
   int first_seg = -1, last_seg = -1;
-  bool any_bad = false, first = true;
+  bool first = true;
   int seg_begin = 0, seg_step = 0;
   for (int seg = 0; seg < nseg; ++seg) {
     const int sb = field(seg, 0), len = field(seg, 1), j0 = field(seg, 2), nblk = field(seg, 3), nspan = field(seg, 6);
     const int seg_steps = (nblk + kStepBlocks - 1) / kStepBlocks;
     const int from = max(begin - seg_step, 0), to = min(end - seg_step, seg_steps);
     if (from < to) {
-      const Block4 at{ids + seg_begin, nblk, lbase, num_blocks, c, g};
+      const Blocks at{lines + seg_begin, nblk, lbase, c, g};
       Step d;
       const char *kb, *vb;
-      bool bad = at.addresses(from * kStepBlocks, kb, vb);
+      at.addresses(from * kStepBlocks, kb, vb);
       d.load_keys(kb);
-      d.load_pairs(vb, c);
-      d.load_values(vb, c);
-      // Q of head c % 8, dims 8 g and 32 + 8 g on; sum(q) 2^-24.
+      // Q of head c % 8, dims 8 g and 32 + 8 g on.
       const int qrow = sb < 0 || sb >= batch ? 0 : sb;
       const half8_t* src = reinterpret_cast<const half8_t*>(query + (static_cast<int64_t>(qrow) * kQHeads + kGroup * h + (c & 7)) * kHeadDim) + g;
-      const half8_t qa = src[0], qb = src[4];
-      float qsum = 0.f;
+      half8_t qa = src[0], qb = src[4];
+      d.load_pairs(vb, c);
+      d.load_values(vb, c);
+      // The products give 2^-20 (q . n) with 16 q at the places of n 2^-24; for a head whose 16 q passes fp16's range 2^-24 (q . n)
+      // with q / 16 at the others (what that rounds off is 2^-36 of the largest). `to_log2`: a score in this unit as a
+      // base-2 exponent, log2(e) / 8 over the unit.
+      float qmax = 0.f, qsum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) qsum += static_cast<float>(qa[j]) + static_cast<float>(qb[j]);
-      qsum = sum_over_groups(qsum) * (1.0f / 16777216.0f);
+      for (int j = 0; j < 8; ++j) {
+        qmax = fmaxf(qmax, fmaxf(fabsf(static_cast<float>(qa[j])), fabsf(static_cast<float>(qb[j]))));
+        qsum += static_cast<float>(qa[j]) + static_cast<float>(qb[j]);
+      }
+      const bool large = max_over_groups(qmax) > 4094.f;
+      qsum = sum_over_groups(qsum) * (large ? 1.f / 16777216.f : 1.f / 1048576.f);
+      const float to_log2 = large ? 16777216.f * kScoreToLog2 : 1048576.f * kScoreToLog2;
+      const _Float16 even = static_cast<_Float16>(large ? 1.f : 16.f), odd = static_cast<_Float16>(large ? 0.0625f : 1.f);
+      qa = scaled_query(qa, even, odd);
+      qb = scaled_query(qb, even, odd);
 
       float m = 0.f, lsum = 0.f, usum = 0.f;
       float4_t acc[4], wacc = {0.f, 0.f, 0.f, 0.f};
@@ -354,28 +391,24 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
       for (int x = from; x < to; ++x) {
         const int u = x * kStepBlocks;
         const bool more = x + 1 < to;
-        if (more) bad |= at.addresses(u + kStepBlocks, kb, vb);
-        float4_t s[2];
+        if (more) at.addresses(u + kStepBlocks, kb, vb);
+        float y[2][4];  // scores less the running max
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          float4_t even = {0.f, 0.f, 0.f, 0.f}, odd = even;
-          even = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][0]), qa, even, 0, 0, 0);
-          odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][2]), qa, odd, 0, 0, 0);
-          even = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][1]), qb, even, 0, 0, 0);
-          odd = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][3]), qb, odd, 0, 0, 0);
+          const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+          float4_t even_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][0]), qa, zero, 0, 0, 0);
+          float4_t odd_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][2]), qa, zero, 0, 0, 0);
+          even_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][1]), qb, even_tile, 0, 0, 0);
+          odd_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][3]), qb, odd_tile, 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[a][e] = c < 8 ? even[e] : odd[e];
+          for (int e = 0; e < 4; ++e) {
+            y[a][e] = fmaf(pair_step(d.kp[a][e]), c < 8 ? even_tile[e] : odd_tile[e], fmaf(pair_low(d.kp[a][e]), qsum, -m));
+          }
         }
         if (more) d.load_keys(kb);
-        float y[2][4];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[a][e] = fmaf(pair_low(d.kp[a][e]), qsum, pair_step(d.kp[a][e]) * s[a][e]);
         // Tokens of block u + g that exist; the score of one that does not is -inf and its weights are 0, whatever its bytes are.
         const int valid = u + g < nblk ? len - (j0 + u + g) * kSlots : 0;
-        const bool full = __builtin_amdgcn_ballot_w64(valid < kSlots) == 0;
-        if (!full) {
+        if (__builtin_amdgcn_ballot_w64(valid < kSlots) != 0) {
 #pragma unroll
           for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -385,21 +418,26 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
               d.vp[a][e] = there ? d.vp[a][e] : 0u;
             }
         }
-        const float bm = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])), fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
-        if (x == from) {
-          m = max_halves(max_over_groups(bm));  // token 0 of a step's first block is valid
-        } else if (__builtin_amdgcn_ballot_w64((bm - m) * kRawToLog2 > kLazyLog2) != 0) {
-          const float mn = fmaxf(m, max_halves(max_over_groups(bm)));
-          const float alpha = exp2_fast((m - mn) * kRawToLog2);
-          lsum *= alpha;
-          usum *= alpha;
+        float bm = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])), fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
+        if (x == from || __builtin_amdgcn_ballot_w64(bm * to_log2 > kLazyLog2) != 0) {
+          bm = max_halves(max_over_groups(bm));  // of a first step finite: token 0 of its first block is valid
+          if (x != from) {
+            bm = fmaxf(bm, 0.f);
+            const float alpha = exp2_fast(-bm * to_log2);
+            lsum *= alpha;
+            usum *= alpha;
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[t][e] *= alpha;
+              for (int e = 0; e < 4; ++e) acc[t][e] *= alpha;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) wacc[e] *= alpha;
-          m = mn;
+            for (int e = 0; e < 4; ++e) wacc[e] *= alpha;
+          }
+          m += bm;
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[a][e] -= bm;
         }
         bf16x8_t weights[2];
 #pragma unroll
@@ -407,9 +445,9 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
           float w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = exp2_fast((y[a][e] - m) * kRawToLog2);
+            const float p = exp2_fast(y[a][e] * to_log2);
             lsum += p;
-            w[e] = p * pair_step(d.vp[a][e]);
+            w[e] = times_step(d.vp[a][e], p);
             usum = fmaf(p, pair_low(d.vp[a][e]), usum);
           }
           const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
@@ -424,15 +462,22 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
         for (int a = 0; a < 2; ++a) {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(d.v[a][t >> 1], d.v[a][2 + (t >> 1)], 4 * (t & 1)), weights[a], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(d.v[a][t >> 1], d.v[a][2 + (t >> 1)], 4 * (t & 1), bias), weights[a], acc[t], 0, 0, 0);
           }
           const uint4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
           wacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), weights[a], wacc, 0, 0, 0);
         }
         if (more) d.load_values(vb, c);
       }
+      // A block id outside the pool among the segment's blocks here.
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < kMaxUnits / 64; ++k) {
+        const int at_block = 64 * k + lane - seg_begin;
+        bad |= (outside[k] & __builtin_amdgcn_ballot_w64(at_block >= kStepBlocks * from && at_block < min(kStepBlocks * to, nblk))) != 0;
+      }
       Part p;
-      p.m = m;
+      p.m = m * to_log2;
       p.l = add_halves(sum_over_groups(lsum));
       const float shift = fmaf(-128.f, add_halves(wacc[0]), add_halves(sum_over_groups(usum)));
 #pragma unroll
@@ -442,7 +487,6 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
           const float x = add_halves(acc[k][e]), z = add_halves(acc[2 + k][e]);
           p.o[4 * k + e] = bad ? NAN : (c < 8 ? x : z) + shift;
         }
-      any_bad |= bad;
       if (from == 0 && to == seg_steps && nspan == 1) {
         if (sb >= 0 && sb < batch) store_output(out + (static_cast<int64_t>(sb) * kQHeads + kGroup * h) * kHeadDim, lane, p);
       } else {
@@ -457,8 +501,10 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     seg_begin += nblk;
     seg_step += seg_steps;
   }
-  int fault = any_bad ? PC_ATTN_FAULT_BLOCK_ID : 0;
+  int fault = (outside[0] | outside[1] | outside[2] | outside[3]) != 0 ? PC_ATTN_FAULT_BLOCK_ID : 0;
   __syncthreads();
+  char* const slots = workspace + kWorkspaceHeader;
+  const int key = flag_key(rec[2], layer);
   int tail_lane = lane;  // what is computed from it below is not carried through the loop above
   asm volatile("" : "+v"(tail_lane));
   // The later segment first: another bin may wait for its part, and the bin's first segment may have to wait itself.
@@ -525,7 +571,7 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
   if (!out || !query || !pool || !context_lens || !plan) return set_error(PC_ERR_ARGUMENT, "null pointer");
   if (APPEND && (!new_key || !new_value)) return set_error(PC_ERR_ARGUMENT, "null pointer");
   if (!workspace) return set_error(PC_ERR_ARGUMENT, "workspace required (null pointer)");
-  if (num_blocks < 1 || num_blocks > INT32_MAX) return set_error(PC_ERR_ARGUMENT, "num_blocks out of range");
+  if (num_blocks < 1 || num_blocks > kMaxBlocks) return set_error(PC_ERR_ARGUMENT, "num_blocks out of range [1, 2^26]");
   if (layer < 0 || layer >= kLayers) return set_error(PC_ERR_ARGUMENT, "layer %d outside [0, 22)", layer);
   if (int rc = check_attn_shape(batch, max_blocks)) return rc;
   if (!aligned(query, 16) || !aligned(out, 16) || !aligned(pool, 128) || !aligned(workspace, 256) || !aligned(plan, 16) ||
