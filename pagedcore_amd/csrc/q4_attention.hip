@@ -51,6 +51,7 @@ constexpr int kWaves = kParts * kKVHeads;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
 constexpr int kMergeParts = 4;   // partials a round trip
+constexpr int kSpreadBins = 64;  // bins of a group above which a long sequence's are spread over the XCDs
 constexpr int kMergeGroup = 16;  // parts of a long span that one of them folds
 constexpr int kStepBlocks = 4;
 constexpr int64_t kMaxBlocks = 1 << 26;  // a block's place in a layer, in 128-byte lines, in 32 bits
@@ -91,30 +92,35 @@ __device__ __forceinline__ void store_output(_Float16* rows, int lane, const Par
   }
 }
 
-// A partial in a workspace slot: lane L's O at byte 32 L, then (m, l) of the 8 heads at 2048.
-__device__ __forceinline__ void store_part(char* slot, int lane, const Part& p) {
-  float4_t* d = reinterpret_cast<float4_t*>(slot + lane * 32);
-  d[0] = float4_t{p.o[0], p.o[1], p.o[2], p.o[3]};
-  d[1] = float4_t{p.o[4], p.o[5], p.o[6], p.o[7]};
-  if (lane < kGroup) {
-    reinterpret_cast<float*>(slot + 2048)[2 * lane] = p.m;
-    reinterpret_cast<float*>(slot + 2048)[2 * lane + 1] = p.l;
-  }
+// A partial in a workspace slot: lane L's O at byte 32 L, then (m, l) of the 8 heads at 2048. Where the bins of a sequence run
+// on one XCD, its L2 is where their partials meet, by plain stores and loads; on several XCDs (SPREAD), whose L2s are not
+// coherent with each other, stores and loads are agent-scope ones.
+template <bool SPREAD>
+__device__ __forceinline__ void store_words(char* at, float a, float b) {
+  const uint64_t v = static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
+  if constexpr (SPREAD) __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else *reinterpret_cast<uint64_t*>(at) = v;
 }
-
+template <bool SPREAD>
+__device__ __forceinline__ void load_words(const char* at, float& a, float& b) {
+  uint64_t v;
+  if constexpr (SPREAD) v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else v = *reinterpret_cast<const uint64_t*>(at);
+  a = __uint_as_float(static_cast<uint32_t>(v));
+  b = __uint_as_float(static_cast<uint32_t>(v >> 32));
+}
+template <bool SPREAD>
+__device__ __forceinline__ void store_part(char* slot, int lane, const Part& p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) store_words<SPREAD>(slot + 32 * lane + 8 * i, p.o[2 * i], p.o[2 * i + 1]);
+  if (lane < kGroup) store_words<SPREAD>(slot + 2048 + 8 * lane, p.m, p.l);
+}
+template <bool SPREAD>
 __device__ __forceinline__ Part load_part(const char* slot, int lane) {
-  const float4_t* d = reinterpret_cast<const float4_t*>(slot + lane * 32);
-  const float4_t a = d[0], b = d[1];
-  const float* e = reinterpret_cast<const float*>(slot + 2048) + 2 * (lane & 7);
   Part p;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p.o[i] = a[i];
-    p.o[4 + i] = b[i];
-  }
-  // The flag shares this line and has been polled: read past the L1.
-  p.m = __hip_atomic_load(e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  p.l = __hip_atomic_load(e + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = 0; i < 4; ++i) load_words<SPREAD>(slot + 32 * lane + 8 * i, p.o[2 * i], p.o[2 * i + 1]);
+  load_words<true>(slot + 2048 + 8 * (lane & 7), p.m, p.l);  // beside the flag, which has been polled: past the L1
   return p;
 }
 
@@ -159,13 +165,6 @@ __device__ __forceinline__ half8_t scaled_query(half8_t q, _Float16 even, _Float
   return q * half8_t{even, even, odd, odd, even, even, odd, odd};
 }
 
-// x times the pair's upper half (the step), one instruction: written as a product the compiler converts first.
-__device__ __forceinline__ float times_step(uint32_t pair, float x) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(x));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   bf16x2_t v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, v);
@@ -187,9 +186,17 @@ struct Waited {
   int first, stride, count;
 };
 
+// A raised flag's low bits: the XCD where its part is to be seen; on all of them 1.
+template <bool SPREAD>
+__device__ __forceinline__ int flag_id() {
+  if constexpr (SPREAD) return 1;
+  else return xcc_id() + 1;
+}
+
 // Folds the waited parts into `total`, in order, as their flags rise, and lowers the flags. Returns PC_ATTN_FAULT_* bits.
+template <bool SPREAD>
 __device__ __forceinline__ int merge_parts(Part& total, char* slots, int slot0, const Waited& parts, int h, int lane, int key) {
-  const int want = key | (xcc_id() + 1);
+  const int want = key | flag_id<SPREAD>();
   bool timeout = false, foreign = false;
   for (int base = 0; base < parts.count; base += 64) {
     const int n = min(64, parts.count - base);
@@ -208,7 +215,7 @@ __device__ __forceinline__ int merge_parts(Part& total, char* slots, int slot0, 
     for (int k = 0; k < n; k += kMergeParts) {
       Part p[kMergeParts];
 #pragma unroll
-      for (int i = 0; i < kMergeParts; ++i) p[i] = load_part(part_slot(slots, slot0, parts.first + parts.stride * (base + min(k + i, n - 1)), h), lane);
+      for (int i = 0; i < kMergeParts; ++i) p[i] = load_part<SPREAD>(part_slot(slots, slot0, parts.first + parts.stride * (base + min(k + i, n - 1)), h), lane);
 #pragma unroll
       for (int i = 0; i < kMergeParts; ++i) {
         if (k + i < n) fold_part(total, p[i]);
@@ -257,9 +264,9 @@ struct Blocks {
   }
 };
 
-template <bool APPEND>
+template <bool APPEND, bool SPREAD>
 __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int32_t* __restrict__ plan, const _Float16* query, char* pool,
-                                                                     int64_t num_blocks, int layer, int batch, int nslots,
+                                                                     int64_t num_blocks, int layer, int rows, int batch, int nslots,
                                                                      _Float16* out, char* workspace, const _Float16* new_key,
                                                                      const _Float16* new_value) {
   __shared__ uint32_t shared_lines[kWaves * kMaxUnits];
@@ -268,7 +275,15 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
   const int h = wave % kKVHeads, part = wave / kKVHeads;
   const int lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
-  const int32_t* row = plan + static_cast<int64_t>(blockIdx.x) * kRowInts;
+  // The hardware deals consecutive workgroups to the XCDs in turn, and the plan's rows are in this order: a group of bins to
+  // an XCD. SPREAD: consecutive workgroups take consecutive bins of one group.
+  int64_t row_index = blockIdx.x;
+  if constexpr (SPREAD) {
+    const uint32_t bins = gridDim.x / kGroups;
+    row_index = static_cast<int64_t>(blockIdx.x % bins) * kGroups + blockIdx.x / bins;
+    if (row_index >= rows) return;
+  }
+  const int32_t* row = plan + row_index * kRowInts;
   // The record (scalar loads) and the bin's block ids (lane L of vector k holds id 64 k + L) in one round trip.
   int32_t rec[kRecordInts];
 #pragma unroll
@@ -345,6 +360,9 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
 
   uint32_t bias;
   asm("v_mov_b32 %0, 0x43004300" : "=v"(bias));
+  // A zero that the compiler does not see through: p s + 0 is one instruction on the pair's half, p s a conversion and a product.
+  float none;
+  asm("s_mov_b32 %0, 0" : "=s"(none));
   char* const areas = shared_parts + wave * 2 * kPartBytes;
   // The wave's first and last segment, if it holds their first step but cannot write their rows by itself (-1: none): what
   // the wave did of them is in its first and second area.
@@ -447,7 +465,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
           for (int e = 0; e < 4; ++e) {
             const float p = exp2_fast(y[a][e] * to_log2);
             lsum += p;
-            w[e] = times_step(d.vp[a][e], p);
+            w[e] = fmaf(p, pair_step(d.vp[a][e]), none);
             usum = fmaf(p, pair_low(d.vp[a][e]), usum);
           }
           const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
@@ -530,7 +548,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     if (nspan != 1) {
       // The span's slots [slot0, slot0 + parts - 1) lie in the workspace, and the part in the span.
       if (slot0 < 0 || nspan < 2 || slot0 + static_cast<int64_t>(nspan) - 1 > nslots || kidx < 0 || kidx >= nspan || k00 < 0 ||
-          k00 + static_cast<int64_t>(kGroups) * kidx != static_cast<int64_t>(blockIdx.x)) {
+          k00 + static_cast<int64_t>(kGroups) * kidx != row_index) {
         continue;
       }
       last = kidx == nspan - 1;
@@ -543,7 +561,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
 #pragma nounroll
         for (int level = 0; level < (heads ? 2 : 1); ++level) {
           const Waited waited = level == 0 ? Waited{group, 1, kidx - group} : Waited{kMergeGroup - 1, kMergeGroup, group / kMergeGroup};
-          fault |= merge_parts(total, slots, slot0, waited, h, tail_lane, key);
+          fault |= merge_parts<SPREAD>(total, slots, slot0, waited, h, tail_lane, key);
         }
       }
     }
@@ -551,10 +569,10 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
       if (sb >= 0 && sb < batch) store_output(out + (static_cast<int64_t>(sb) * kQHeads + kGroup * h) * kHeadDim, tail_lane, total);
     } else {
       char* slot = part_slot(slots, slot0, kidx, h);
-      store_part(slot, tail_lane, total);
+      store_part<SPREAD>(slot, tail_lane, total);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (tail_lane == 0) {
-        __hip_atomic_store(reinterpret_cast<int32_t*>(slot + kFlagOffset), key | (xcc_id() + 1), __ATOMIC_RELAXED,
+        __hip_atomic_store(reinterpret_cast<int32_t*>(slot + kFlagOffset), key | flag_id<SPREAD>(), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
       }
     }
@@ -582,10 +600,14 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
     return set_error(PC_ERR_ARGUMENT, "num_records %d outside [0, pc_attn_plan_capacity]", num_records);
   }
   if (batch == 0 || num_records == 0) return ok();
+  // Fewer bins a group, or of a sequence, and each of an XCD's CUs has at most two of them.
+  const bool spread = num_records > kGroups * kSpreadBins && max_blocks > kMinBinBlocks * kSpreadBins;
+  const auto kernel = spread ? paged_decode_q4_kernel<APPEND, true> : paged_decode_q4_kernel<APPEND, false>;
+  const unsigned grid = static_cast<unsigned>(spread ? (num_records + kGroups - 1) / kGroups * kGroups : num_records);
   (void)hipGetLastError();
-  hipLaunchKernelGGL(paged_decode_q4_kernel<APPEND>, dim3(static_cast<unsigned>(num_records)), dim3(kThreads), 0,
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), plan, static_cast<const _Float16*>(query), static_cast<char*>(pool), num_blocks,
-                     layer, batch, static_cast<int>(slots_bound(batch, max_blocks)), static_cast<_Float16*>(out),
+                     layer, num_records, batch, static_cast<int>(slots_bound(batch, max_blocks)), static_cast<_Float16*>(out),
                      static_cast<char*>(workspace), static_cast<const _Float16*>(new_key), static_cast<const _Float16*>(new_value));
   return check_launch(APPEND ? "kv_append_paged_decode_q4" : "paged_decode_q4");
 }
