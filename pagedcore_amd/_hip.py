@@ -821,44 +821,59 @@ def qkv_rope_append_fp8(
     )
 
 
-# The KV pool in 4 bits (include/pagedcore_hip.h): per block of 16 tokens and kv head a unit of 1152 bytes.
+# The KV pool in 4 bits (include/pagedcore_hip.h): per block of 16 tokens and kv head a unit of 1152 bytes. A decode step
+# calls these once a layer, so each call tests everything in one expression and looks for what is wrong only if that fails.
 Q4_UNIT_BYTES = 1152
+_F16, _I32, _I64, _U8 = torch.float16, torch.int32, torch.int64, torch.uint8
 
 
 def empty_q4_pool(blocks: int, device: torch.device) -> Tensor:
     """An uninitialised 4-bit KV pool, uint8 [22, blocks, 4, 1152]."""
-    return torch.empty((22, blocks, 4, Q4_UNIT_BYTES), dtype=torch.uint8, device=device)
+    return torch.empty((22, blocks, 4, Q4_UNIT_BYTES), dtype=_U8, device=device)
 
 
 def is_q4_pool(pool: Tensor) -> bool:
     """Whether `pool` has the type and shape of a 4-bit pool, contiguous."""
     return (
-        pool.dtype is torch.uint8
-        and pool.dim() == 4
-        and pool.shape[1] > 0
-        and pool.shape == (22, pool.shape[1], 4, Q4_UNIT_BYTES)
+        pool.dtype is _U8 and pool.dim() == 4 and pool.shape[1] > 0 and pool.shape == (22, pool.shape[1], 4, Q4_UNIT_BYTES)
         and pool.is_contiguous()
     )
 
 
+def _q4_launch(device: int, fn, *args) -> int:
+    """fn(*args, the current stream of GPU `device`), with that GPU current."""
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _q4_launch(device, fn, *args)
+    return fn(*args, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+
+
 def _check_q4_pool(pool: Tensor) -> int:
-    """The pool's GPU."""
     device = _gpu_of(pool)
     if not is_q4_pool(pool):
         raise HipExtensionError("pool must be contiguous uint8 [22, blocks, 4, 1152]")
     return device
 
 
-def _check_q4_rows(names: Tuple[str, str], key: Tensor, value: Tensor, layer_begin: int, slot_mapping: Tensor, device: int) -> None:
-    """K and V rows [layers, tokens, 4, 64] and the slots of the tokens, on GPU `device`."""
+def _q4_rows_fit(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> bool:
+    device, shape = pool.get_device(), key.shape
+    return (
+        device >= 0 and is_q4_pool(pool)
+        and len(shape) == 4 and shape[2] == 4 and shape[3] == 64 and value.shape == shape and 0 <= layer_begin and 1 <= shape[0] <= 22 - layer_begin
+        and key.dtype is _F16 and value.dtype is _F16 and key.get_device() == device and value.get_device() == device
+        and slot_mapping.dtype is _I64 and slot_mapping.dim() == 1 and slot_mapping.shape[0] == shape[1] and slot_mapping.is_contiguous()
+        and slot_mapping.get_device() == device
+    )
+
+
+def _refuse_q4_rows(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
+    device = _check_q4_pool(pool)
     shape = key.shape
-    if len(shape) != 4 or shape[2] != 4 or shape[3] != 64 or value.shape != shape or not 1 <= shape[0] <= 22 - layer_begin or layer_begin < 0:
-        raise HipExtensionError(f"{names[0]} and {names[1]} must share [layers, tokens, 4, 64], with the layers from {layer_begin} on within 22")
-    for tensor in (key, value):
-        if tensor.dtype is not torch.float16 or tensor.get_device() != device:
-            raise HipExtensionError(f"{names[0]} and {names[1]} must be float16 on GPU {device}")
-    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (shape[1],) or not slot_mapping.is_contiguous() or slot_mapping.get_device() != device:
-        raise HipExtensionError(f"slot_mapping must be contiguous int64 [{shape[1]}] on GPU {device}")
+    if len(shape) != 4 or shape[2:] != (4, 64) or value.shape != shape or not 0 <= layer_begin < 22 or not 1 <= shape[0] <= 22 - layer_begin:
+        raise HipExtensionError(f"key and value must share [layers, tokens, 4, 64], the layers from {layer_begin} on within 22")
+    if any(tensor.dtype is not _F16 or tensor.get_device() != device for tensor in (key, value)):
+        raise HipExtensionError(f"key and value must be float16 on GPU {device}")
+    raise HipExtensionError(f"slot_mapping must be contiguous int64 [{shape[1]}] on GPU {device}")
 
 
 def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
@@ -868,16 +883,22 @@ def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slo
     key/value: float16 [layers, tokens, 4, 64]; layer and token strides are free. slot_mapping: int64 [tokens], each slot at
     most once; a slot outside the pool is skipped. A row with an infinity or NaN becomes a row of NaN. Enqueued on the current
     stream of the pool's device."""
-    device = _check_q4_pool(pool)
-    _check_q4_rows(("key", "value"), key, value, layer_begin, slot_mapping, device)
-    if key.stride(3) != 1 or key.stride(2) != 64:
+    if not _q4_rows_fit(pool, layer_begin, key, value, slot_mapping):
+        _refuse_q4_rows(pool, layer_begin, key, value, slot_mapping)
+    ks, vs = key.stride(), value.stride()
+    if ks[3] != 1 or ks[2] != 64:
         key = key.contiguous()
-    if value.stride(3) != 1 or value.stride(2) != 64:
+        ks = key.stride()
+    if vs[3] != 1 or vs[2] != 64:
         value = value.contiguous()
-    _call_on(
-        device, load(), "pc_kv_append_q4", pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], key.data_ptr(), key.stride(0),
-        key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), slot_mapping.data_ptr(), key.shape[1],
+        vs = value.stride()
+    lib = load()
+    status = _q4_launch(
+        pool.get_device(), lib.pc_kv_append_q4, pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], key.data_ptr(), ks[0], ks[1],
+        value.data_ptr(), vs[0], vs[1], slot_mapping.data_ptr(), key.shape[1],
     )
+    if status:
+        _check(lib, "pc_kv_append_q4", status)
 
 
 def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_mapping: Tensor) -> None:
@@ -885,15 +906,18 @@ def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_
 
     key/value: float16 [layers, tokens, 4, 64] to write, each [4, 64] row contiguous, layer and token strides free; the rows of
     a slot outside the pool are left as they are. slot_mapping: int64 [tokens]. On the current stream of the pool's device."""
-    device = _check_q4_pool(pool)
-    _check_q4_rows(("key", "value"), key, value, layer_begin, slot_mapping, device)
-    for tensor in (key, value):
-        if tensor.stride(3) != 1 or tensor.stride(2) != 64:
-            raise HipExtensionError("each [4, 64] row of key and value must be contiguous")
-    _call_on(
-        device, load(), "pc_kv_read_q4", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-        value.stride(1), pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], slot_mapping.data_ptr(), key.shape[1],
+    if not _q4_rows_fit(pool, layer_begin, key, value, slot_mapping):
+        _refuse_q4_rows(pool, layer_begin, key, value, slot_mapping)
+    ks, vs = key.stride(), value.stride()
+    if ks[3] != 1 or ks[2] != 64 or vs[3] != 1 or vs[2] != 64:
+        raise HipExtensionError("each [4, 64] row of key and value must be contiguous")
+    lib = load()
+    status = _q4_launch(
+        pool.get_device(), lib.pc_kv_read_q4, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], pool.data_ptr(),
+        pool.shape[1], layer_begin, key.shape[0], slot_mapping.data_ptr(), key.shape[1],
     )
+    if status:
+        _check(lib, "pc_kv_read_q4", status)
 
 
 def paged_decode_attention_q4(
@@ -920,6 +944,28 @@ def paged_decode_attention_q4(
     return workspace
 
 
+_PLAN_INTS = 296  # pc_attn_plan_record_ints()
+
+
+def _refuse_q4_attention(out, query, pool, context_lens, plan, max_blocks, workspace, nbytes, new_key, new_value) -> None:
+    device = _check_q4_pool(pool)
+    if context_lens.dtype is not _I32 or context_lens.dim() != 1 or not context_lens.is_contiguous() or context_lens.get_device() != device:
+        raise HipExtensionError(f"context_lens must be contiguous int32 [batch] on GPU {device}")
+    batch = context_lens.shape[0]
+    if nbytes <= 0:
+        raise HipExtensionError(f"invalid attention shape batch={batch} max_blocks={max_blocks}")
+    for name, rows, heads in (("out", out, 32), ("query", query, 32), ("new_key", new_key, 4), ("new_value", new_value, 4)):
+        if rows is None and heads == 4:
+            if new_key is not None or new_value is not None:
+                raise HipExtensionError("new_key and new_value are given together")
+            continue
+        if rows.dtype is not _F16 or rows.dim() < 2 or rows.shape[0] != batch or rows.numel() != batch * heads * 64 or not rows.is_contiguous() or rows.get_device() != device:
+            raise HipExtensionError(f"{name} must be contiguous float16 [{batch}, {heads}, 64] on GPU {device}")
+    if plan.dtype is not _I32 or plan.dim() != 2 or plan.shape[1] != _PLAN_INTS or not plan.is_contiguous() or plan.get_device() != device:
+        raise HipExtensionError(f"plan must be a contiguous int32 decode_plan() array on GPU {device}")
+    raise HipExtensionError(f"workspace needs {nbytes} contiguous bytes on GPU {device}")
+
+
 def planned_decode_attention_q4(
     out: Tensor, query: Tensor, pool: Tensor, layer: int, context_lens: Tensor, plan: Tensor, max_blocks: int,
     workspace: Tensor, *, new_key: Optional[Tensor] = None, new_value: Optional[Tensor] = None,
@@ -928,33 +974,36 @@ def planned_decode_attention_q4(
     (a dimension of 1 more between is taken), the plan, lengths and workspace as there. With new_key and new_value (float16
     [batch, 4, 64]) each sequence's newest token is quantised and written in the same launch, with the results of
     kv_append_q4 followed by attention."""
-    device = _check_q4_pool(pool)
-    batch = context_lens.shape[0]
-    for name, rows in (("out", out), ("query", query)):
-        if rows.dtype is not torch.float16 or rows.numel() != batch * 2048 or rows.shape[0] != batch or not rows.is_contiguous() or rows.get_device() != device:
-            raise HipExtensionError(f"{name} must be contiguous float16 [{batch}, 32, 64] on GPU {device}")
     lib = load()
-    nbytes = lib.pc_attn_workspace_bytes(batch, max_blocks)
-    if nbytes <= 0:
-        raise HipExtensionError(f"invalid attention shape batch={batch} max_blocks={max_blocks}")
-    if workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.get_device() != device:
-        raise HipExtensionError(f"workspace needs {nbytes} contiguous bytes on GPU {device}")
-    if context_lens.dtype is not torch.int32 or context_lens.dim() != 1 or not context_lens.is_contiguous() or context_lens.get_device() != device:
-        raise HipExtensionError(f"context_lens must be contiguous int32 [batch] on GPU {device}")
-    if plan.dtype is not torch.int32 or plan.dim() != 2 or plan.shape[1] != lib.pc_attn_plan_record_ints() or not plan.is_contiguous() or plan.get_device() != device:
-        raise HipExtensionError(f"plan must be a contiguous int32 decode_plan() array on GPU {device}")
-    if new_key is None and new_value is None:
-        _call_on(
-            device, lib, "pc_paged_decode_attn_q4", out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer,
-            context_lens.data_ptr(), batch, max_blocks, plan.data_ptr(), plan.shape[0], workspace.data_ptr(),
+    device, batch = pool.get_device(), context_lens.shape[0] if context_lens.dim() == 1 else -1
+    nbytes = lib.pc_attn_workspace_bytes(batch, max_blocks) if batch >= 0 else 0
+    if not (
+        device >= 0 and is_q4_pool(pool) and nbytes > 0
+        and context_lens.dtype is _I32 and context_lens.is_contiguous() and context_lens.get_device() == device
+        and out.dtype is _F16 and out.dim() > 1 and out.shape[0] == batch and out.numel() == batch * 2048 and out.is_contiguous() and out.get_device() == device
+        and query.dtype is _F16 and query.dim() > 1 and query.shape[0] == batch and query.numel() == batch * 2048 and query.is_contiguous()
+        and query.get_device() == device
+        and plan.dtype is _I32 and plan.dim() == 2 and plan.shape[1] == _PLAN_INTS and plan.is_contiguous() and plan.get_device() == device
+        and workspace.nbytes >= nbytes and workspace.is_contiguous() and workspace.get_device() == device
+        and (
+            (new_key is None and new_value is None)
+            or (
+                new_key is not None and new_value is not None
+                and new_key.dtype is _F16 and new_key.dim() > 1 and new_key.shape[0] == batch and new_key.numel() == batch * 256
+                and new_key.is_contiguous() and new_key.get_device() == device
+                and new_value.dtype is _F16 and new_value.dim() > 1 and new_value.shape[0] == batch and new_value.numel() == batch * 256
+                and new_value.is_contiguous() and new_value.get_device() == device
+            )
         )
+    ):
+        _refuse_q4_attention(out, query, pool, context_lens, plan, max_blocks, workspace, nbytes, new_key, new_value)
+    args = (out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer, context_lens.data_ptr(), batch, max_blocks,
+            plan.data_ptr(), plan.shape[0])
+    if new_key is None:
+        status = _q4_launch(device, lib.pc_paged_decode_attn_q4, *args, workspace.data_ptr())
+        if status:
+            _check(lib, "pc_paged_decode_attn_q4", status)
         return
-    for name, rows in (("new_key", new_key), ("new_value", new_value)):
-        if rows is None:
-            raise HipExtensionError("new_key and new_value are given together")
-        _check_half(name, rows, (batch, 4, 64), device)
-    _call_on(
-        device, lib, "pc_kv_append_paged_decode_attn_q4", out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer,
-        context_lens.data_ptr(), batch, max_blocks, plan.data_ptr(), plan.shape[0], new_key.data_ptr(), new_value.data_ptr(),
-        workspace.data_ptr(),
-    )
+    status = _q4_launch(device, lib.pc_kv_append_paged_decode_attn_q4, *args, new_key.data_ptr(), new_value.data_ptr(), workspace.data_ptr())
+    if status:
+        _check(lib, "pc_kv_append_paged_decode_attn_q4", status)

@@ -40,6 +40,8 @@ using pc_internal::set_error;
 using q4_device::dpp;
 using q4_device::kRotate8;
 using q4_device::kUnitBytes;
+using q4_device::pair_low;
+using q4_device::pair_step;
 using q4_device::kBlockBytes;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -171,8 +173,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 __device__ __forceinline__ float low_bf16(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-__device__ __forceinline__ float pair_low(uint32_t x) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x))); }
-__device__ __forceinline__ float pair_step(uint32_t x) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x >> 16))); }
 
 // x with lanes 8-15 of each row of 16 replaced by lanes 0-7 of y (UPPER), or lanes 0-7 by lanes 8-15 of y.
 template <bool UPPER>

@@ -64,51 +64,55 @@ struct Levels {
   uint32_t pair;
 };
 
-// Lane a of eight (aligned) holds values 8a .. 8a + 7 of a row. The quotient is the correctly rounded one: with
-// the correctly rounded reciprocal and a product within an ulp, one residual step gives it (Markstein), and
-// only the exact quotient lies at a half where it does, so that ties go to the even level. (lo, s) of a row with
-// an infinity or NaN is (NaN, 0): all its values are NaN.
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+
+template <int CTRL>
+__device__ __forceinline__ half2_t dpp(half2_t x) {
+  return __builtin_bit_cast(half2_t, dpp<CTRL>(__builtin_bit_cast(uint32_t, x)));
+}
+
+// Lane a of eight (aligned) holds values 8a .. 8a + 7 of a row. Its minimum and maximum are taken on pairs, by the forms that
+// hand a NaN on. The quotient t / s ends correctly rounded: t s^-1 with a reciprocal good to an ulp, and one step with the
+// exact residual (Markstein): what is left of the error is 2^-45 of it, and a quotient at a half (a tie, to the even level)
+// or next to one is 2^-21 from any other value that 24 bits of t and 11 of s give. (lo, s) of a row with an infinity or NaN
+// is (NaN, 0): all its values are NaN.
 __device__ __forceinline__ Levels quantize8(half8_t x) {
 #pragma clang fp contract(off)
-  float f[8];
+  half2_t lo2 = {x[0], x[1]}, hi2 = lo2;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(x[j]);
-  float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
-  float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-  float zero = 0.f;  // NaN if a value is not finite (min and max pass over a NaN)
-#pragma unroll
-  for (int j = 0; j < 8; ++j) zero = fmaf(f[j], 0.f, zero);
-  lo = fminf(lo, dpp<kSwap1>(lo));
-  hi = fmaxf(hi, dpp<kSwap1>(hi));
-  zero += dpp<kSwap1>(zero);
-  lo = fminf(lo, dpp<kSwap2>(lo));
-  hi = fmaxf(hi, dpp<kSwap2>(hi));
-  zero += dpp<kSwap2>(zero);
-  lo = fminf(lo, dpp<kMirror8>(lo));
-  hi = fmaxf(hi, dpp<kMirror8>(hi));
-  zero += dpp<kMirror8>(zero);
-  lo += 0.f;  // a zero of either sign is +0: the row's bytes do not depend on the order of its values
-  const float span = hi - lo;
-  uint16_t step_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(span * (1.0f / 15.0f)));
+  for (int j = 2; j < 8; j += 2) {
+    const half2_t v = {x[j], x[j + 1]};
+    lo2 = __builtin_elementwise_minimum(lo2, v);
+    hi2 = __builtin_elementwise_maximum(hi2, v);
+  }
+  lo2 = __builtin_elementwise_minimum(lo2, dpp<kSwap1>(lo2));
+  hi2 = __builtin_elementwise_maximum(hi2, dpp<kSwap1>(hi2));
+  lo2 = __builtin_elementwise_minimum(lo2, dpp<kSwap2>(lo2));
+  hi2 = __builtin_elementwise_maximum(hi2, dpp<kSwap2>(hi2));
+  lo2 = __builtin_elementwise_minimum(lo2, dpp<kMirror8>(lo2));
+  hi2 = __builtin_elementwise_maximum(hi2, dpp<kMirror8>(hi2));
+  // + 0: a zero of either sign is +0, the row's bytes do not depend on the order of its values.
+  const float lo = static_cast<float>(__builtin_elementwise_minimum(lo2[0], lo2[1])) + 0.f;
+  const float span = static_cast<float>(__builtin_elementwise_maximum(hi2[0], hi2[1])) - lo;
+  uint32_t step_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(span * (1.0f / 15.0f)));
   // 15 s is exact in fp32 (4 and 11 bits).
-  if (static_cast<float>(__builtin_bit_cast(_Float16, step_bits)) * 15.0f < span) ++step_bits;
-  const float step = static_cast<float>(__builtin_bit_cast(_Float16, step_bits));
-  const float inverse = step > 0.f ? 1.0f / step : 0.f;
-  uint32_t low = 0, high = 0;
+  if (static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(step_bits))) * 15.0f < span) ++step_bits;
+  const float step = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(step_bits)));
+  const float inverse = step > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
+  uint32_t low = 0, high = 0;  // the levels of even and of odd j, in the low 16 bits
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float t = f[j] - lo;
+    const float t = static_cast<float>(x[j]) - lo;
     float y = t * inverse;
     y = fmaf(fmaf(-y, step, t), inverse, y);
-    const uint32_t n = __float_as_uint(y + 8388608.0f) & 15u;  // to an integer, to nearest even
+    const uint32_t n = __float_as_uint(y + 8388608.0f);  // an integer, to nearest even, below bits 24 and on
     if (j % 2 == 0) low |= n << (2 * j);
     else high |= n << (2 * (j - 1));
   }
   Levels r;
-  const uint32_t lo_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo));
-  r.word = low | high << 16;
-  r.pair = lo_bits | static_cast<uint32_t>(step_bits) << 16;
-  if (!(zero == 0.f)) {
+  r.word = __builtin_amdgcn_perm(high, low, 0x05040100u);
+  r.pair = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo)) | step_bits << 16;
+  if (!(span < INFINITY)) {
     r.word = 0;
     r.pair = 0x7e00u;  // (NaN, 0)
   }
@@ -148,17 +152,32 @@ __device__ __forceinline__ void store_row(char* unit, int kind, int t, int a, co
   if (a == 0) *reinterpret_cast<uint32_t*>(unit + pair_offset(kind, t)) = q.pair;
 }
 
-// Values 8a .. 8a + 7 of a row, in fp16: the exact lo + s n, rounded to fp32 (it has at most 40 bits) and to fp16. s is
-// rounded up, so lo + 15 s may pass 65504 where the row's largest value did not: it reads as 65504.
-__device__ __forceinline__ half8_t row_values(uint32_t pair, const uint32_t n[8]) {
-  const float lo = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair)));
-  const float step = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> 16)));
+__device__ __forceinline__ float pair_low(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair))); }
+__device__ __forceinline__ float pair_step(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> 16))); }
+
+// A value in fp16: the exact lo + s n, rounded to fp32 (it has at most 40 bits) and to fp16. s is rounded up, so lo + 15 s may
+// pass 65504 where the row's largest value did not: it reads as 65504.
+__device__ __forceinline__ _Float16 row_value(float lo, float step, float n) {
+  const float v = fmaf(step, n, lo);
+  return static_cast<_Float16>(v > 65504.f ? 65504.f : v);
+}
+
+// Values 8a .. 8a + 7 of token t's row, lane a of eight.
+__device__ __forceinline__ half8_t load_row(const char* unit, int kind, int t, int a) {
+  const uint32_t pair = *reinterpret_cast<const uint32_t*>(unit + pair_offset(kind, t));
+  uint32_t n[8];
+  if (kind == 0) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(unit + key_word(t, a));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n[j] = level(word, j);
+  } else {
+    const char* at = unit + value_byte(t, a);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n[j] = static_cast<uint8_t>(at[16 * j]) >> (a & 2 ? 4 : 0) & 15u;
+  }
   half8_t x;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float v = fmaf(step, static_cast<float>(n[j]), lo);
-    x[j] = static_cast<_Float16>(v > 65504.f ? 65504.f : v);
-  }
+  for (int j = 0; j < 8; ++j) x[j] = row_value(pair_low(pair), pair_step(pair), static_cast<float>(n[j]));
   return x;
 }
 

@@ -53,7 +53,7 @@ def _filled(rng, blocks, layer):
     return pool
 
 
-@pytest.mark.parametrize("layers,begin,tokens,start", [(1, 21, 1, 0), (22, 0, 17, 5), (3, 7, 64, 0), (2, 20, 131, 15), (5, 0, 4, 2)])
+@pytest.mark.parametrize("layers,begin,tokens,start", [(1, 21, 1, 0), (22, 0, 17, 5), (3, 7, 64, 0), (2, 20, 131, 15), (5, 0, 4, 2), (22, 0, 27, 7), (1, 4, 700, 0)])
 def test_append_bytes(device, layers, begin, tokens, start):
     rng = np.random.default_rng(tokens)
     blocks = -(-(start + tokens) // 16) + 2
@@ -100,6 +100,46 @@ def test_append_strided_and_skipped(device, offset):
     assert (back == 7.0).all()
 
 
+@pytest.mark.parametrize("kind", ["start_0", "start_8", "start_13", "backwards", "holes", "swapped", "across"])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_prompt_rows(device, kind, offset):
+    """Enough rows that eight tokens go together where their slots do: whole halves of blocks, halves cut at both ends, slots in
+    another order, tokens that are skipped; rows as views of wider ones, aligned to 16 bytes or not."""
+    rng = np.random.default_rng(len(kind))
+    layers, tokens = 4, 203
+    table = rng.permutation(16)
+    at = np.arange({"start_8": 8, "start_13": 13}.get(kind, 0), 240)[:tokens]
+    slots = (table[at // 16] * 16 + at % 16).astype(np.int64)
+    if kind == "backwards":
+        slots = slots[::-1].copy()
+    elif kind == "holes":
+        slots[[0, 9, 63, 64, 100, 202]] = (-1, 256, -5, 1 << 33, -1, 300)
+    elif kind == "swapped":
+        slots[[16, 17]], slots[[40, 48]] = slots[[17, 16]], slots[[48, 40]]
+    elif kind == "across":  # consecutive slots that go on from one block into the next
+        slots = np.arange(4, 4 + tokens, dtype=np.int64)
+    wide = np.zeros((2, layers, tokens, 264 + offset), dtype=np.float16)
+    wide[..., offset : offset + 256] = _rows(rng, 2, layers, tokens).reshape(2, layers, tokens, 256)
+    on = _up(wide, device)
+    key, value = (on[i, ..., offset : offset + 256].unflatten(-1, (4, 64)) for i in range(2))
+    pool = _pool(rng, 16)
+    expected = pool.copy()
+    ref.write(expected, 9, key.cpu().numpy(), value.cpu().numpy(), slots)
+    got = _up(pool, device)
+    _hip.kv_append_q4(got, 9, key, value, _up(slots, device))
+    assert torch.equal(got.cpu(), torch.from_numpy(expected))
+    back = torch.full((2, layers, tokens, 264 + offset), 7.0, dtype=torch.float16, device=device)
+    rows = [back[i, ..., offset : offset + 256].unflatten(-1, (4, 64)) for i in range(2)]
+    _hip.kv_read_q4(rows[0], rows[1], got, 9, _up(slots, device))
+    inside = (slots >= 0) & (slots < 256)
+    for i in range(2):
+        want = np.stack([ref.rows(expected[9 + layer], i, np.where(inside, slots, 0)) for layer in range(layers)])
+        _assert_read(rows[i].cpu().numpy()[:, inside], want[:, inside])
+        assert (rows[i].cpu().numpy()[:, ~inside] == 7.0).all()
+    back[..., offset : offset + 256] = 7.0
+    assert (back == 7.0).all()
+
+
 def _assert_read(got, want):
     """One rounding to fp16 behind one to fp32 (half steps 2^-11 and 2^-24 of the value; 2^-25 below fp16's normal range); what
     lies past fp16's largest value is that value."""
@@ -110,7 +150,7 @@ def _assert_read(got, want):
     assert (off <= (2.0**-11 + 2.0**-23) * np.abs(want[fine]) + 2.0**-25).all()
 
 
-@pytest.mark.parametrize("layers,begin,tokens", [(1, 3, 1), (22, 0, 33), (2, 20, 300)])
+@pytest.mark.parametrize("layers,begin,tokens", [(1, 3, 1), (22, 0, 20), (22, 0, 33), (2, 20, 300)])
 def test_read_rows(device, layers, begin, tokens):
     rng = np.random.default_rng(tokens)
     blocks = tokens // 16 + 3
