@@ -229,6 +229,7 @@ def kv_append(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_m
     device. Enqueued on the current stream of the pool's device.
     """
     lib = load()
+    _check_fp16_pool(pool)
     rows = []
     for tensor in (key, value):
         if tensor.stride(3) != 1 or tensor.stride(2) != 64:
@@ -251,6 +252,11 @@ def kv_append(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_m
         _stream(pool.device),
     )
     _check(lib, "pc_kv_append", status)
+
+
+def _check_fp16_pool(pool: Optional[Tensor]) -> None:
+    if pool is not None and pool.dtype is not torch.float16:
+        raise HipExtensionError("pool must be float16 [22, 2, blocks, 16, 4, 64] (the _q4 calls take a 4-bit pool)")
 
 
 _workspaces: Dict[Tuple[int, int], Tensor] = {}
@@ -385,6 +391,7 @@ def planned_decode_attention(
 def _launch_planned(out, query, pool, layer, context_lens, plan, max_blocks, workspace, nbytes, new_key, new_value) -> None:
     """planned_decode_attention for a shape whose workspace takes `nbytes`."""
     lib = load()
+    _check_fp16_pool(pool)
     batch = int(context_lens.shape[0])
     if nbytes <= 0:
         raise HipExtensionError(f"invalid attention shape batch={batch} max_blocks={max_blocks}")
@@ -444,6 +451,7 @@ def rope_kv_append(
     not read back here: callers check them on the host.
     """
     lib = load()
+    _check_fp16_pool(pool)
     if qkv.dim() != 2 or qkv.stride(1) != 1:
         raise HipExtensionError("qkv must be [tokens, columns] with unit column stride")
     status = lib.pc_rope_kv_append(
@@ -480,6 +488,7 @@ def rope_kv_append_parts(
     """rope_kv_append with the q | k | v row given as split-K partial sums: qkv_parts
     contiguous fp32 [splits, tokens, 2560] (gemm_m128's partials), rounded to fp16 once."""
     lib = load()
+    _check_fp16_pool(pool)
     if qkv_parts.dim() != 3 or qkv_parts.dtype != torch.float32 or not qkv_parts.is_contiguous():
         raise HipExtensionError("qkv_parts must be contiguous fp32 [splits, tokens, 2560]")
     status = lib.pc_rope_kv_append_parts(
@@ -517,6 +526,7 @@ def qkv_rope_append(
     """rope_kv_append of the q | k | v projection x @ w.T, in one launch (pc_qkv_rope_append): x
     contiguous fp16 [tokens, k], w contiguous fp16 [2560, k]; the outputs of rope_kv_append."""
     lib = load()
+    _check_fp16_pool(pool)
     m, k = x.shape
     if x.dtype != torch.float16 or w.dtype != torch.float16 or tuple(w.shape) != (2560, k):
         raise HipExtensionError("x and w must be fp16 [tokens, k] and [2560, k]")

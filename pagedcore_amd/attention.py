@@ -14,7 +14,7 @@ for the launch, read the workspace's fault word and raise
 AttentionFaultError (a RuntimeError) instead of returning NaN rows.
 
 ``paged_attention_batch`` is the batched form the decode loop needs (one launch for all
-rows of a layer). The reference's ``eager_rounding=True`` path replays HF fp16 rounding for
+rows of a layer). Over a 4-bit pool (allocate_kv_pool(bits=4)) both attend to the values that its rows stand for. The reference's ``eager_rounding=True`` path replays HF fp16 rounding for
 forensic comparisons; it is not part of the serving path and is rejected here.
 """
 
@@ -57,7 +57,8 @@ def attend_rows(
     q = query if query.is_contiguous() else query.contiguous()
     out = torch.empty((batch, Q_HEADS, 1, HEAD_DIM), dtype=torch.float16, device=query.device)
     plan = allocator.rows_plan(rows)
-    workspace = _hip.paged_decode_attention(out, q, pool, layer_index, rows.tables, rows.lengths, plan=plan)
+    attend = _hip.paged_decode_attention_q4 if allocator.quantized else _hip.paged_decode_attention
+    workspace = attend(out, q, pool, layer_index, rows.tables, rows.lengths, plan=plan)
     return out, workspace
 
 

@@ -27,6 +27,10 @@ the reference's torch expression does (see the kernels' comments), so a row's re
 differs from the reference only by fp32 summation order inside the GEMMs, the norms and the
 attention.
 
+Over a 4-bit pool (allocate_kv_pool(bits=4), which the reference does not have) q|k|v leave the rotated K and V rows beside the
+queries: a DecodeGraph's attention quantises and writes them in its launch, prompts and eager steps in one of their own
+(pc_kv_append_q4). A prompt attends to its own K and V before they are rounded; later steps read them in 4 bits.
+
 With the 8-bit projections of quantize_weights, which the reference does not have, the products are
 pc_qkv_rope_append_fp8 and pc_gemm_fp8 and the norms give 8-bit rows (pc_add_rms_norm_fp8).
 """
@@ -746,6 +750,17 @@ class DecodeGraph:
         hidden = F.embedding(ids, weights.embedding)
         query = torch.empty((batch, Q_HEADS, HEAD_DIM), dtype=torch.float16, device=pool.device)
         attention = torch.empty_like(query)
+        if self._allocator.quantized:  # the new rows are quantised and written by the attention's launch
+            key, value = torch.empty((2, batch, KV_HEADS, HEAD_DIM), dtype=torch.float16, device=pool.device)
+
+            def attend_q4(index: int, x, weight) -> Tensor:
+                _qkv_rope(query, x, weight, positions, self._table, key_out=key, value_out=value)
+                _hip.planned_decode_attention_q4(
+                    attention, query, pool, index, self._lens, self._plan, MAX_BLOCKS, self._workspace, new_key=key, new_value=value
+                )
+                return attention.view(batch, HIDDEN)
+
+            return F.linear(_layers(hidden, weights, attend_q4), weights.lm_head)
 
         def attend(index: int, x, weight) -> Tensor:
             _qkv_rope(query, x, weight, positions, self._table, pool=pool, layer=index, slot_mapping=slots)
@@ -918,8 +933,14 @@ def _prefill_forward(ids: Tensor, positions: Tensor, slots: Tensor, weights: Tin
     query = torch.empty((tokens, Q_HEADS, HEAD_DIM), dtype=torch.float16, device=device)
     attended = torch.empty_like(query)
 
+    quantized = pool.dtype == torch.uint8  # a 4-bit pool
+
     def attend(index: int, x, weight) -> Tensor:
-        _qkv_rope(query, x, weight, positions, table, key_out=key, value_out=value, pool=pool, layer=index, slot_mapping=slots)
+        if quantized:
+            _qkv_rope(query, x, weight, positions, table, key_out=key, value_out=value)
+            _hip.kv_append_q4(pool, index, key.unsqueeze(0), value.unsqueeze(0), slots)
+        else:
+            _qkv_rope(query, x, weight, positions, table, key_out=key, value_out=value, pool=pool, layer=index, slot_mapping=slots)
         if on_layer is not None:
             on_layer(index)
         _hip.prefill_attention(attended, query, key, value)

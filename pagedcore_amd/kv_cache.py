@@ -13,7 +13,9 @@ Additions to the reference API (additive, for batched callers):
     one launch;
   * ``gather_block_tables`` returns the device block table and context lengths that the
     attention kernel walks, with the same staged-layer rules as ``iter_layer_blocks``;
-  * ``KVAllocator(pool, kv_writer=...)`` lets host-logic tests substitute the writer.
+  * ``KVAllocator(pool, kv_writer=...)`` lets host-logic tests substitute the writer;
+  * ``allocate_kv_pool(config, bits=4)`` gives a pool that holds K and V in 4 bits, 3.6 times as many blocks in the same
+    memory and as few bytes for attention to read; an allocator over it has the same methods and rules.
 """
 
 from __future__ import annotations
@@ -42,13 +44,18 @@ QKV_COLUMNS = (32 + 2 * KV_HEADS) * HEAD_DIM  # 2560: one token's q | k | v proj
 MAX_BLOCKS_PER_REQUEST = CONTEXT_LIMIT // BLOCK_TOKENS  # 128
 
 
-def allocate_kv_pool(config: PagedCoreConfig, *, device: str | torch.device = "cuda:0") -> Tensor:
+def allocate_kv_pool(config: PagedCoreConfig, *, device: str | torch.device = "cuda:0", bits: int = 16) -> Tensor:
     """Allocate the fp16 pool [22, 2, blocks, 16, 4, 64] once; keep it for the worker's life.
 
     Same sizing and memory checks as the reference (src/pagedcore/kv_cache.py:17-47):
     whole 352 KiB blocks within ``kv_pool_mib``, free memory for pool + margin checked
     before, margin re-checked after. Storage is uninitialised.
+
+    ``bits=4`` allocates the 4-bit pool, uint8 [22, blocks, 4, 1152], whose blocks take 99 KiB: KVAllocator, and all that
+    runs on one, quantises K and V rows as it writes them (_hip.kv_append_q4). The reference has no such pool.
     """
+    if type(bits) is not int or bits not in (4, 16):
+        raise ValueError("a KV pool holds 16 or 4 bits a value")
     target = torch.device(device)
     if target.type != "cuda":
         raise ValueError("KV pool requires a CUDA device")
@@ -57,17 +64,20 @@ def allocate_kv_pool(config: PagedCoreConfig, *, device: str | torch.device = "c
 
     pool_bytes = config.kv_pool_mib * 2**20
     margin_bytes = config.workspace_margin_mib * 2**20
-    block_bytes = LAYERS * 2 * config.block_tokens * KV_HEADS * HEAD_DIM * 2
+    block_bytes = LAYERS * (2 * config.block_tokens * KV_HEADS * HEAD_DIM * 2 if bits == 16 else KV_HEADS * _hip.Q4_UNIT_BYTES)
     num_blocks = pool_bytes // block_bytes
     free_bytes, _ = torch.cuda.mem_get_info(target)
     if free_bytes < pool_bytes + margin_bytes:
         raise RuntimeError("configured KV pool and workspace margin do not fit in GPU memory")
 
-    pool = torch.empty(
-        (LAYERS, 2, num_blocks, config.block_tokens, KV_HEADS, HEAD_DIM),
-        dtype=torch.float16,
-        device=target,
-    )
+    if bits == 16:
+        pool = torch.empty(
+            (LAYERS, 2, num_blocks, config.block_tokens, KV_HEADS, HEAD_DIM),
+            dtype=torch.float16,
+            device=target,
+        )
+    else:
+        pool = _hip.empty_q4_pool(num_blocks, target)
     if torch.cuda.mem_get_info(target)[0] < margin_bytes:
         del pool
         raise RuntimeError("KV pool allocation leaves less than the configured workspace margin")
@@ -113,6 +123,27 @@ class HipKVWriter:
             _hip.rope_kv_append_parts(query_out, qkv, positions, rope_table, pool=pool, layer=layer, slot_mapping=slots)
         else:
             _hip.rope_kv_append(query_out, qkv, positions, rope_table, pool=pool, layer=layer, slot_mapping=slots)
+
+
+class HipQ4Writer(HipKVWriter):
+    """The same on a 4-bit pool: rows are quantised as they are written."""
+
+    def append(
+        self, pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slots: Sequence[int]
+    ) -> None:
+        if not isinstance(slots, Tensor):
+            slots = torch.as_tensor(np.asarray(slots, dtype=np.int64)).to(pool.device)
+        _hip.kv_append_q4(pool, layer_begin, key, value, slots)
+
+    def rope_append(
+        self, pool: Tensor, layer: int, qkv: Tensor, rope_table: Tensor, positions: Tensor, slots: Tensor,
+        query_out: Tensor,
+    ) -> None:
+        tokens = slots.shape[0]
+        rows = torch.empty((2, 1, tokens, KV_HEADS, HEAD_DIM), dtype=torch.float16, device=pool.device)
+        rope = _hip.rope_kv_append_parts if qkv.ndim == 3 else _hip.rope_kv_append
+        rope(query_out, qkv, positions, rope_table, key_out=rows[0], value_out=rows[1])
+        _hip.kv_append_q4(pool, layer, rows[0], rows[1], slots)
 
 
 class _HostOnlyWriter:
@@ -265,10 +296,12 @@ class KVAllocator:
     CUDA work stays on the stream current at construction. Block reads borrow pool
     storage: treat them as read-only and do not keep them past an append or release.
     CPU pools support the bookkeeping (tests); their KV writes need an explicit writer.
+    Over a 4-bit pool K and V rows are quantised as they are written, and block reads are copies.
     """
 
     def __init__(self, pool: Tensor, *, kv_writer: Optional[KVWriter] = None) -> None:
-        if (
+        self._quantized = _hip.is_q4_pool(pool) and pool.device.type in ("cpu", "cuda")
+        if not self._quantized and (
             pool.ndim != 6
             or pool.shape[:2] != (LAYERS, 2)
             or pool.shape[2] < 1
@@ -280,13 +313,13 @@ class KVAllocator:
         ):
             raise ValueError("KV pool must be contiguous FP16 [22, 2, blocks, 16, 4, 64] storage")
         if kv_writer is None:
-            kv_writer = HipKVWriter() if pool.is_cuda else _HostOnlyWriter()
+            kv_writer = _HostOnlyWriter() if not pool.is_cuda else HipQ4Writer() if self._quantized else HipKVWriter()
         self._pool = pool
         self._writer = kv_writer
         self._worker = current_thread()
         self._stream = torch.cuda.current_stream(pool.device) if pool.is_cuda else None
         self._stream_handle = self._stream.cuda_stream if self._stream is not None else None
-        self._free_blocks = _CountingList(BlockId(index) for index in reversed(range(pool.shape[2])))
+        self._free_blocks = _CountingList(BlockId(index) for index in reversed(range(self.total_blocks)))
         self._sequences: Dict[RequestId, _SequenceCache] = _CountingDict()
         # Tables are checked against the owners recorded when blocks are assigned.
         self._block_owners: Dict[BlockId, RequestId] = _CountingDict()
@@ -302,6 +335,15 @@ class KVAllocator:
     @property
     def pool(self) -> Tensor:
         return self._pool
+
+    @property
+    def quantized(self) -> bool:
+        """Whether the pool holds 4 bits a value (allocate_kv_pool(bits=4))."""
+        return self._quantized
+
+    @property
+    def total_blocks(self) -> int:
+        return self._pool.shape[1 if self._quantized else 2]
 
     def create(self, reservation: KVReservation) -> None:
         """Grant credits at admission without assigning physical blocks."""
@@ -709,8 +751,15 @@ class KVAllocator:
     def iter_layer_blocks(
         self, request_id: RequestId, *, layer_index: int
     ) -> Iterator[Tuple[Tensor, Tensor]]:
-        """Borrow valid [slots, 4, 64] pages, including a completed staged layer."""
+        """Borrow valid [slots, 4, 64] pages, including a completed staged layer. Of a 4-bit pool: copies of their values in
+        fp16, read back in one launch when the first is asked for."""
         sequence = self._layer_sequence(request_id, layer_index)
+        if self._quantized:
+            key, value = self._read_back(layer_index, 1, _slot_mapping(sequence.blocks, 0, sequence.length))
+            for start in range(0, sequence.length, BLOCK_TOKENS):
+                self._check_worker()
+                yield key[0, start : start + BLOCK_TOKENS], value[0, start : start + BLOCK_TOKENS]
+            return
         for logical_block, physical_block in enumerate(sequence.blocks):
             self._check_worker()
             valid = min(BLOCK_TOKENS, sequence.length - logical_block * BLOCK_TOKENS)
@@ -811,7 +860,7 @@ class KVAllocator:
         return result
 
     def read_block(self, request_id: RequestId, logical_block: int) -> Tuple[Tensor, Tensor]:
-        """Borrow K/V views [22, valid slots, 4, 64] for one logical block."""
+        """Borrow K/V views [22, valid slots, 4, 64] for one logical block (of a 4-bit pool: copies of their values in fp16)."""
         self._check_worker()
         self._assert_accounting()
         sequence = self._sequences[request_id]
@@ -819,10 +868,20 @@ class KVAllocator:
             raise ValueError("logical block must identify a cached block")
         physical_block = sequence.blocks[logical_block]
         valid = min(BLOCK_TOKENS, sequence.length - logical_block * BLOCK_TOKENS)
+        if self._quantized:
+            return self._read_back(0, LAYERS, np.arange(valid, dtype=np.int64) + physical_block * BLOCK_TOKENS)
         return (
             self._pool[:, 0, physical_block, :valid],
             self._pool[:, 1, physical_block, :valid],
         )
+
+    def _read_back(self, layer_begin: int, layers: int, slots: np.ndarray) -> Tuple[Tensor, Tensor]:
+        """K and V of the slots in a 4-bit pool's layers, FP16 [layers, slots, 4, 64]."""
+        if not self._pool.is_cuda:
+            raise RuntimeError("reads of a 4-bit pool run on the GPU: this allocator's pool is on the CPU")
+        rows = torch.empty((2, layers, slots.shape[0], KV_HEADS, HEAD_DIM), dtype=torch.float16, device=self._pool.device)
+        _hip.kv_read_q4(rows[0], rows[1], self._pool, layer_begin, _upload(slots, self._pool.device))
+        return rows[0], rows[1]
 
     def release_all(self, request_id: RequestId) -> None:
         """Release once on the worker stream; unknown/released requests raise KeyError."""
@@ -935,7 +994,7 @@ class KVAllocator:
         return counts
 
     def _full_accounting(self) -> CapacityCounts:
-        total = self._pool.shape[2]
+        total = self.total_blocks
         for request_id, sequence in self._sequences.items():
             if (
                 sequence.reservation.request_id != request_id

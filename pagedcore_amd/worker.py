@@ -190,7 +190,7 @@ class DecodeWorker:
             raise ValueError("request IDs must be unique")
         if self._vocab is not None and max(request.input_ids) >= self._vocab:
             raise ValueError(f"input_ids must be below the vocabulary size {self._vocab}")
-        if request.block_credits > self._allocator.pool.shape[2]:
+        if request.block_credits > self._allocator.total_blocks:
             raise ValueError("request exceeds total KV pool capacity")
         self._known.add(request.request_id)
         self._pending.append((request, np.fromiter(request.input_ids, dtype=np.int64, count=len(request.input_ids))))
