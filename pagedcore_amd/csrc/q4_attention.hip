@@ -12,16 +12,17 @@
 //     remainder in the two halves of the columns (16 bits of it; bf16 because p s' spans fp32's range), and
 //     128 sum(p s') of the same rounded weights, from one more product with ones, is taken off at the end.
 //
-// Each of the four waves of a workgroup takes one kv head of its bin, four blocks (64 tokens) a step. The row of a
-// product's tile is chosen so that no data crosses lanes: tile i's row 4b + e is token 4i + e of the step's block
-// b, which leaves lane (c, g) the scores of block g for one head. The group has 8 query heads and a tile 16
-// columns, so two tiles share an accumulator: columns 0-7 hold the heads for tile 2a, columns 8-15 for tile
-// 2a + 1 (the operand's other half is zero), and the softmax runs on 32 tokens x 8 heads per four values of a lane.
+// Two waves of a workgroup take a kv head of its bin, four blocks (64 tokens) a step. The row of a product's tile is
+// chosen so that no data crosses lanes: tile i's row 4b + e is token 4i + e of the step's block b, which leaves lane
+// (c, g) the scores of block g for head c % 8. The group has 8 query heads and a tile 16 columns (the heads twice), so
+// the softmax takes tile 2a from columns 0-7 and tile 2a + 1 from columns 8-15: 32 tokens x 8 heads per four values
+// of a lane, and each exponential is computed once.
 
 #include <hip/hip_runtime.h>
 
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "attn_plan.h"
 #include "pagedcore_hip.h"
@@ -47,6 +48,7 @@ using q4_device::kBlockBytes;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+typedef int32_t int8_vt __attribute__((ext_vector_type(8), aligned(4)));
 
 constexpr int kParts = 2;  // waves of a kv head
 constexpr int kWaves = kParts * kKVHeads;
@@ -181,6 +183,17 @@ __device__ __forceinline__ uint32_t take_half(uint32_t x, uint32_t y) {
       __builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(y), kRotate8, 0xf, UPPER ? 0xc : 0x3, false));
 }
 
+// The largest of eight, none of them fresh from a matrix instruction. (fmaxf of values that the compiler cannot tell to be
+// quiet costs an instruction each to make them so.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max8(const float (&y)[2][4]) {
+  return max3(max3(max3(y[0][0], y[0][1], y[0][2]), y[0][3], y[1][0]), max3(y[1][1], y[1][2], y[1][3]), y[1][3]);
+}
+
 // The workspace slots of the parts of one cut sequence that a bin waits for: parts first, first + stride, ... (count of them).
 struct Waited {
   int first, stride, count;
@@ -266,7 +279,7 @@ struct Blocks {
 
 template <bool APPEND, bool SPREAD>
 __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int32_t* __restrict__ plan, const _Float16* query, char* pool,
-                                                                     int64_t num_blocks, int layer, int rows, int batch, int nslots,
+                                                                     uint32_t num_blocks, int layer, int rows, int batch, int nslots,
                                                                      _Float16* out, char* workspace, const _Float16* new_key,
                                                                      const _Float16* new_value) {
   __shared__ uint32_t shared_lines[kWaves * kMaxUnits];
@@ -284,45 +297,45 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     if (row_index >= rows) return;
   }
   const int32_t* row = plan + row_index * kRowInts;
-  // The record (scalar loads) and the bin's block ids (lane L of vector k holds id 64 k + L) in one round trip.
-  int32_t rec[kRecordInts];
-#pragma unroll
-  for (int i = 0; i < kRecordInts; ++i) rec[i] = row[i];
+  // The record (scalar loads) and the bin's block ids (lane L of vector k holds id 64 k + L) in one round trip: all of them are
+  // wanted at one place, before any is looked at.
   int32_t idv[kMaxUnits / 64];
 #pragma unroll
   for (int k = 0; k < kMaxUnits / 64; ++k) idv[k] = row[kRecordInts + 64 * k + lane];
-  const int nseg = rec[0], nunits = rec[1];
+  const int8_vt* fields = reinterpret_cast<const int8_vt*>(row);
+  int8_vt header = fields[0], seg0 = fields[1], seg1 = fields[2], seg2 = fields[3], seg3 = fields[4];
+  asm volatile("" : "+s"(header), "+s"(seg0), "+s"(seg1), "+s"(seg2), "+s"(seg3), "+v"(idv[0]), "+v"(idv[1]), "+v"(idv[2]), "+v"(idv[3]));
+  const int nseg = header[0], nunits = header[1];
   if (nseg <= 0 || nseg > kMaxSegs || nunits <= 0 || nunits > kMaxUnits) return;  // padding rows do nothing
-  auto field = [&](int s, int f) { return row[kHeaderInts + s * kSegInts + f]; };  // of a segment, by a scalar load
-  // The segments' steps; a record whose segments are not its blocks does nothing.
-  int steps = 0;
-  {
-    int64_t blocks = 0;
-    bool sound = true;
-#pragma unroll
-    for (int s = 0; s < kMaxSegs; ++s) {
-      if (s < nseg) {
-        const int n = rec[kHeaderInts + s * kSegInts + 3];
-        sound &= n > 0;
-        blocks += n;
-        steps += (n + kStepBlocks - 1) / kStepBlocks;
-      }
-    }
-    if (!sound || blocks != nunits) return;
-  }
+  // Field f of segment s.
+  auto field = [&](int s, int f) {
+    int v = seg0[f];
+    v = s == 1 ? seg1[f] : v;
+    v = s == 2 ? seg2[f] : v;
+    return s == 3 ? seg3[f] : v;
+  };
+  // Its steps; a record whose segments are not its blocks does nothing.
+  auto steps_of = [](int blocks) { return static_cast<int>(static_cast<uint32_t>(blocks + kStepBlocks - 1) / kStepBlocks); };
+  const uint32_t n0 = seg0[3], n1 = nseg > 1 ? seg1[3] : 0, n2 = nseg > 2 ? seg2[3] : 0, n3 = nseg > 3 ? seg3[3] : 0;
+  const uint32_t most = max(max(n0, n1), max(n2, n3)), least = min(min(n0, nseg > 1 ? n1 : n0), min(nseg > 2 ? n2 : n0, nseg > 3 ? n3 : n0));
+  if (least == 0 || most > kMaxUnits || n0 + n1 + n2 + n3 != static_cast<uint32_t>(nunits)) return;
+  const int steps = steps_of(n0) + steps_of(n1) + steps_of(n2) + steps_of(n3);
   // Each wave keeps the blocks' places for itself: no barrier before its first load. An id outside the pool is never
   // dereferenced (block 0 is read).
   uint32_t* const lines = shared_lines + wave * kMaxUnits;
-  uint64_t outside[kMaxUnits / 64];
+  uint64_t outside[kMaxUnits / 64] = {};
 #pragma unroll
   for (int k = 0; k < kMaxUnits / 64; ++k) {
-    const uint32_t id = static_cast<uint32_t>(idv[k]);
-    const bool bad = 64 * k + lane < nunits && id >= static_cast<uint64_t>(num_blocks);
-    outside[k] = __builtin_amdgcn_ballot_w64(bad);
-    lines[64 * k + lane] = (bad ? 0 : id) * static_cast<uint32_t>(kBlockBytes / 128);
+    if (64 * k < nunits) {
+      const uint32_t id = static_cast<uint32_t>(idv[k]);
+      const uint64_t there = nunits >= 64 * (k + 1) ? ~uint64_t{0} : (uint64_t{1} << (nunits - 64 * k)) - 1;
+      outside[k] = __builtin_amdgcn_ballot_w64(id >= num_blocks) & there;
+      lines[64 * k + lane] = (id >= num_blocks ? 0 : id) * static_cast<uint32_t>(kBlockBytes / 128);
+    }
   }
+  const bool any_outside = (outside[0] | outside[1] | outside[2] | outside[3]) != 0;
   wave_lds_fence();
-  char* const lbase = pool + static_cast<int64_t>(layer) * num_blocks * kBlockBytes + h * kUnitBytes;
+  char* const lbase = pool + static_cast<int64_t>(layer) * static_cast<int64_t>(num_blocks) * kBlockBytes + h * kUnitBytes;
 
   // This wave's steps [begin, end) of the bin's.
   const int begin = part * steps / kParts, end = (part + 1) * steps / kParts;
@@ -333,13 +346,13 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     int first = 0, sb = 0, len = 0, j0 = 0, nblk = 0, ends = 0;
 #pragma unroll
     for (int s = 0, at = 0, step = 0; s < kMaxSegs; ++s) {
-      const int n = s < nseg ? rec[kHeaderInts + s * kSegInts + 3] : 0;
-      step += (n + kStepBlocks - 1) / kStepBlocks;
+      const int n = s < nseg ? field(s, 3) : 0;
+      step += steps_of(n);
       if (s == g) {
         first = at;
-        sb = rec[kHeaderInts + s * kSegInts];
-        len = rec[kHeaderInts + s * kSegInts + 1];
-        j0 = rec[kHeaderInts + s * kSegInts + 2];
+        sb = field(s, 0);
+        len = field(s, 1);
+        j0 = field(s, 2);
         nblk = n;
         ends = step;
       }
@@ -371,7 +384,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
   int seg_begin = 0, seg_step = 0;
   for (int seg = 0; seg < nseg; ++seg) {
     const int sb = field(seg, 0), len = field(seg, 1), j0 = field(seg, 2), nblk = field(seg, 3), nspan = field(seg, 6);
-    const int seg_steps = (nblk + kStepBlocks - 1) / kStepBlocks;
+    const int seg_steps = steps_of(nblk);
     const int from = max(begin - seg_step, 0), to = min(end - seg_step, seg_steps);
     if (from < to) {
       const Blocks at{lines + seg_begin, nblk, lbase, c, g};
@@ -385,35 +398,39 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
       half8_t qa = src[0], qb = src[4];
       d.load_pairs(vb, c);
       d.load_values(vb, c);
-      // The products give 2^-20 (q . n) with 16 q at the places of n 2^-24; for a head whose 16 q passes fp16's range 2^-24 (q . n)
-      // with q / 16 at the others (what that rounds off is 2^-36 of the largest). `to_log2`: a score in this unit as a
-      // base-2 exponent, log2(e) / 8 over the unit.
-      float qmax = 0.f, qsum = 0.f;
+      float m = 0.f, lsum = 0.f, usum = 0.f;
+      float4_t acc[4], wacc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        qmax = fmaxf(qmax, fmaxf(fabsf(static_cast<float>(qa[j])), fabsf(static_cast<float>(qb[j]))));
-        qsum += static_cast<float>(qa[j]) + static_cast<float>(qb[j]);
-      }
-      const bool large = max_over_groups(qmax) > 4094.f;
-      qsum = sum_over_groups(qsum) * (large ? 1.f / 16777216.f : 1.f / 1048576.f);
+      for (int t = 0; t < 4; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+      // (Set here, while the loads are on their way, and not behind the wait for them.)
+      asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(wacc));
+      // sum(q) of every head, by a product with ones, and the heads' products with each other, which tell if any of them may
+      // have an element of 4095 or more (none is larger than a head's own, and that is at least its largest element's square).
+      // The products give 2^-20 (q . n) with 16 q at the places of n 2^-24; where 16 q might pass fp16's range 2^-24 (q . n) with
+      // q / 16 at the others (what that rounds off is at most 2^-25). `to_log2`: a score in this unit as a base-2 exponent,
+      // log2(e) / 8 over the unit.
+      const _Float16 o = static_cast<_Float16>(1.f);
+      const half8_t ones = {o, o, o, o, o, o, o, o};
+      const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+      float4_t sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qa, zero, 0, 0, 0);
+      float4_t gram = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa, qa, zero, 0, 0, 0);
+      sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qb, sums, 0, 0, 0);
+      gram = __builtin_amdgcn_mfma_f32_16x16x32_f16(qb, qb, gram, 0, 0, 0);
+      const bool large = __builtin_amdgcn_ballot_w64(!(fmaxf(fmaxf(gram[0], gram[1]), fmaxf(gram[2], gram[3])) < 4094.f * 4094.f)) != 0;
+      const float qsum = sums[0] * (large ? 1.f / 16777216.f : 1.f / 1048576.f);
       const float to_log2 = large ? 16777216.f * kScoreToLog2 : 1048576.f * kScoreToLog2;
       const _Float16 even = static_cast<_Float16>(large ? 1.f : 16.f), odd = static_cast<_Float16>(large ? 0.0625f : 1.f);
       qa = scaled_query(qa, even, odd);
       qb = scaled_query(qb, even, odd);
 
-      float m = 0.f, lsum = 0.f, usum = 0.f;
-      float4_t acc[4], wacc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma nounroll
-      for (int x = from; x < to; ++x) {
+      // One step, MORE: of which there is a next, whose loads go out behind the uses of the registers that they fill.
+      auto one_step = [&](int x, auto more_steps) __attribute__((always_inline)) {
+        constexpr bool MORE = decltype(more_steps)::value;
         const int u = x * kStepBlocks;
-        const bool more = x + 1 < to;
-        if (more) at.addresses(u + kStepBlocks, kb, vb);
+        if constexpr (MORE) at.addresses(u + kStepBlocks, kb, vb);
         float y[2][4];  // scores less the running max
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          const float4_t zero = {0.f, 0.f, 0.f, 0.f};
           float4_t even_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][0]), qa, zero, 0, 0, 0);
           float4_t odd_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][2]), qa, zero, 0, 0, 0);
           even_tile = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_levels(d.k[a][1]), qb, even_tile, 0, 0, 0);
@@ -423,7 +440,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
             y[a][e] = fmaf(pair_step(d.kp[a][e]), c < 8 ? even_tile[e] : odd_tile[e], fmaf(pair_low(d.kp[a][e]), qsum, -m));
           }
         }
-        if (more) d.load_keys(kb);
+        if constexpr (MORE) d.load_keys(kb);
         // Tokens of block u + g that exist; the score of one that does not is -inf and its weights are 0, whatever its bytes are.
         const int valid = u + g < nblk ? len - (j0 + u + g) * kSlots : 0;
         if (__builtin_amdgcn_ballot_w64(valid < kSlots) != 0) {
@@ -436,7 +453,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
               d.vp[a][e] = there ? d.vp[a][e] : 0u;
             }
         }
-        float bm = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])), fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
+        float bm = max8(y);
         if (x == from || __builtin_amdgcn_ballot_w64(bm * to_log2 > kLazyLog2) != 0) {
           bm = max_halves(max_over_groups(bm));  // of a first step finite: token 0 of its first block is valid
           if (x != from) {
@@ -475,7 +492,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
           const uint4_t wp = {take_half<true>(hi0, lo0), take_half<true>(hi1, lo1), take_half<false>(lo0, hi0), take_half<false>(lo1, hi1)};
           weights[a] = __builtin_bit_cast(bf16x8_t, wp);
         }
-        if (more) d.load_pairs(vb, c);
+        if constexpr (MORE) d.load_pairs(vb, c);
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
 #pragma unroll
@@ -485,14 +502,19 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
           const uint4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
           wacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), weights[a], wacc, 0, 0, 0);
         }
-        if (more) d.load_values(vb, c);
-      }
+        if constexpr (MORE) d.load_values(vb, c);
+      };
+#pragma nounroll
+      for (int x = from; x + 1 < to; ++x) one_step(x, std::true_type{});
+      one_step(to - 1, std::false_type{});
       // A block id outside the pool among the segment's blocks here.
       bool bad = false;
+      if (any_outside) {
 #pragma unroll
-      for (int k = 0; k < kMaxUnits / 64; ++k) {
-        const int at_block = 64 * k + lane - seg_begin;
-        bad |= (outside[k] & __builtin_amdgcn_ballot_w64(at_block >= kStepBlocks * from && at_block < min(kStepBlocks * to, nblk))) != 0;
+        for (int k = 0; k < kMaxUnits / 64; ++k) {
+          const int at_block = 64 * k + lane - seg_begin;
+          bad |= (outside[k] & __builtin_amdgcn_ballot_w64(at_block >= kStepBlocks * from && at_block < min(kStepBlocks * to, nblk))) != 0;
+        }
       }
       Part p;
       p.m = m * to_log2;
@@ -519,10 +541,10 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     seg_begin += nblk;
     seg_step += seg_steps;
   }
-  int fault = (outside[0] | outside[1] | outside[2] | outside[3]) != 0 ? PC_ATTN_FAULT_BLOCK_ID : 0;
+  int fault = any_outside ? PC_ATTN_FAULT_BLOCK_ID : 0;
   __syncthreads();
   char* const slots = workspace + kWorkspaceHeader;
-  const int key = flag_key(rec[2], layer);
+  const int key = flag_key(header[2], layer);
   int tail_lane = lane;  // what is computed from it below is not carried through the loop above
   asm volatile("" : "+v"(tail_lane));
   // The later segment first: another bin may wait for its part, and the bin's first segment may have to wait itself.
@@ -531,11 +553,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     const int seg = r ? last_seg : first_seg;
     if (seg < 0) continue;
     const int sb = field(seg, 0), kidx = field(seg, 5), nspan = field(seg, 6), slot0 = field(seg, 7), k00 = field(seg, 4);
-    int seg_end = 0;
-#pragma unroll
-    for (int s = 0; s < kMaxSegs; ++s) {
-      if (s <= seg) seg_end += (rec[kHeaderInts + s * kSegInts + 3] + kStepBlocks - 1) / kStepBlocks;
-    }
+    const int seg_end = steps_of(n0) + (seg > 0 ? steps_of(n1) : 0) + (seg > 1 ? steps_of(n2) : 0) + (seg > 2 ? steps_of(n3) : 0);
     Part total = take_part(areas + r * kPartBytes, tail_lane);
     // The waves behind this one whose first segment this is.
     for (int p = part + 1; p < kParts && p * steps / kParts < seg_end; ++p) {
@@ -606,7 +624,7 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
   const unsigned grid = static_cast<unsigned>(spread ? (num_records + kGroups - 1) / kGroups * kGroups : num_records);
   (void)hipGetLastError();
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0,
-                     static_cast<hipStream_t>(stream), plan, static_cast<const _Float16*>(query), static_cast<char*>(pool), num_blocks,
+                     static_cast<hipStream_t>(stream), plan, static_cast<const _Float16*>(query), static_cast<char*>(pool), static_cast<uint32_t>(num_blocks),
                      layer, num_records, batch, static_cast<int>(slots_bound(batch, max_blocks)), static_cast<_Float16*>(out),
                      static_cast<char*>(workspace), static_cast<const _Float16*>(new_key), static_cast<const _Float16*>(new_value));
   return check_launch(APPEND ? "kv_append_paged_decode_q4" : "paged_decode_q4");
