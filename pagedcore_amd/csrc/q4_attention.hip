@@ -55,8 +55,7 @@ constexpr int kWaves = kParts * kKVHeads;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
 constexpr int kMergeParts = 4;   // partials a round trip
-constexpr int kSpreadBins = 64;  // bins of a group above which a long sequence's are spread over the XCDs
-constexpr int kMergeGroup = 16;  // parts of a long span that one of them folds
+constexpr int kSpreadBins = 32;  // bins of a group above which a long sequence's are spread over the XCDs
 constexpr int kStepBlocks = 4;
 constexpr int64_t kMaxBlocks = 1 << 26;  // a block's place in a layer, in 128-byte lines, in 32 bits
 static_assert(kMaxUnits == 256, "four vectors of block ids");
@@ -96,35 +95,44 @@ __device__ __forceinline__ void store_output(_Float16* rows, int lane, const Par
   }
 }
 
-// A partial in a workspace slot: lane L's O at byte 32 L, then (m, l) of the 8 heads at 2048. Where the bins of a sequence run
-// on one XCD, its L2 is where their partials meet, by plain stores and loads; on several XCDs (SPREAD), whose L2s are not
-// coherent with each other, stores and loads are agent-scope ones.
-template <bool SPREAD>
-__device__ __forceinline__ void store_words(char* at, float a, float b) {
+// A partial in a workspace slot: O in 2 KiB, then (m, l) of the 8 heads at 2048. Where the bins of a sequence run on one XCD,
+// its L2 is where their partials meet, by plain stores and loads of 16 bytes (lane L's at 32 L); on several
+// XCDs (SPREAD), whose L2s are not coherent with each other, by agent-scope ones of 8 bytes (at 8 L, 512 + 8 L, ...).
+__device__ __forceinline__ void store_pair(char* at, float a, float b) {
   const uint64_t v = static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
-  if constexpr (SPREAD) __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  else *reinterpret_cast<uint64_t*>(at) = v;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <bool SPREAD>
-__device__ __forceinline__ void load_words(const char* at, float& a, float& b) {
-  uint64_t v;
-  if constexpr (SPREAD) v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  else v = *reinterpret_cast<const uint64_t*>(at);
+__device__ __forceinline__ void load_pair(const char* at, float& a, float& b) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   a = __uint_as_float(static_cast<uint32_t>(v));
   b = __uint_as_float(static_cast<uint32_t>(v >> 32));
 }
 template <bool SPREAD>
 __device__ __forceinline__ void store_part(char* slot, int lane, const Part& p) {
+  if constexpr (SPREAD) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) store_words<SPREAD>(slot + 32 * lane + 8 * i, p.o[2 * i], p.o[2 * i + 1]);
-  if (lane < kGroup) store_words<SPREAD>(slot + 2048 + 8 * lane, p.m, p.l);
+    for (int i = 0; i < 4; ++i) store_pair(slot + 512 * i + 8 * lane, p.o[2 * i], p.o[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<float4_t*>(slot + 32 * lane + 16 * i) = float4_t{p.o[4 * i], p.o[4 * i + 1], p.o[4 * i + 2], p.o[4 * i + 3]};
+  }
+  if (lane < kGroup) store_pair(slot + 2048 + 8 * lane, p.m, p.l);
 }
 template <bool SPREAD>
 __device__ __forceinline__ Part load_part(const char* slot, int lane) {
   Part p;
+  if constexpr (SPREAD) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) load_words<SPREAD>(slot + 32 * lane + 8 * i, p.o[2 * i], p.o[2 * i + 1]);
-  load_words<true>(slot + 2048 + 8 * (lane & 7), p.m, p.l);  // beside the flag, which has been polled: past the L1
+    for (int i = 0; i < 4; ++i) load_pair(slot + 512 * i + 8 * lane, p.o[2 * i], p.o[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4_t x = *reinterpret_cast<const float4_t*>(slot + 32 * lane + 16 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p.o[4 * i + e] = x[e];
+    }
+  }
+  load_pair(slot + 2048 + 8 * (lane & 7), p.m, p.l);  // beside the flag, which has been polled: past the L1
   return p;
 }
 
@@ -194,7 +202,7 @@ __device__ __forceinline__ float max8(const float (&y)[2][4]) {
   return max3(max3(max3(y[0][0], y[0][1], y[0][2]), y[0][3], y[1][0]), max3(y[1][1], y[1][2], y[1][3]), y[1][3]);
 }
 
-// The workspace slots of the parts of one cut sequence that a bin waits for: parts first, first + stride, ... (count of them).
+// The parts of one cut sequence that a bin waits for: first, first + stride, ... (count of them, at most 64).
 struct Waited {
   int first, stride, count;
 };
@@ -211,31 +219,31 @@ template <bool SPREAD>
 __device__ __forceinline__ int merge_parts(Part& total, char* slots, int slot0, const Waited& parts, int h, int lane, int key) {
   const int want = key | flag_id<SPREAD>();
   bool timeout = false, foreign = false;
-  for (int base = 0; base < parts.count; base += 64) {
-    const int n = min(64, parts.count - base);
-    // Lane k polls the flag of part k (lanes past the span repeat the last one).
-    int32_t* flag = reinterpret_cast<int32_t*>(part_slot(slots, slot0, parts.first + parts.stride * (base + min(lane, n - 1)), h) + kFlagOffset);
-    int f = 0;
-    for (int spins = 0; spins < kMaxSpins; ++spins) {
-      f = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (__builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) == 0) break;
-      __builtin_amdgcn_s_sleep(1);
-    }
-    timeout |= __builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) != 0;
-    foreign |= __builtin_amdgcn_ballot_w64(flag_of_call(f, key) && f != want) != 0;
-    asm volatile("" ::: "memory");
-    // Four parts a round trip; past the last one the last is loaded again and not folded.
-    for (int k = 0; k < n; k += kMergeParts) {
-      Part p[kMergeParts];
-#pragma unroll
-      for (int i = 0; i < kMergeParts; ++i) p[i] = load_part<SPREAD>(part_slot(slots, slot0, parts.first + parts.stride * (base + min(k + i, n - 1)), h), lane);
-#pragma unroll
-      for (int i = 0; i < kMergeParts; ++i) {
-        if (k + i < n) fold_part(total, p[i]);
-      }
-    }
-    if (lane < n) __hip_atomic_store(flag, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int n = parts.count;
+  if (n <= 0) return 0;
+  // Lane k polls the flag of part k (lanes past the last one repeat it).
+  int32_t* flag = reinterpret_cast<int32_t*>(part_slot(slots, slot0, parts.first + parts.stride * min(lane, n - 1), h) + kFlagOffset);
+  int f = 0;
+  for (int spins = 0; spins < kMaxSpins; ++spins) {
+    f = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) == 0) break;
+    __builtin_amdgcn_s_sleep(1);
   }
+  timeout = __builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) != 0;
+  foreign = __builtin_amdgcn_ballot_w64(flag_of_call(f, key) && f != want) != 0;
+  asm volatile("" ::: "memory");
+  // Past the last part it is loaded again and not folded.
+#pragma nounroll
+  for (int k = 0; k < n; k += kMergeParts) {
+    Part p[kMergeParts];
+#pragma unroll
+    for (int i = 0; i < kMergeParts; ++i) p[i] = load_part<SPREAD>(part_slot(slots, slot0, parts.first + parts.stride * min(k + i, n - 1), h), lane);
+#pragma unroll
+    for (int i = 0; i < kMergeParts; ++i) {
+      if (k + i < n) fold_part(total, p[i]);
+    }
+  }
+  if (lane < n) __hip_atomic_store(flag, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (timeout || foreign) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) total.o[i] = NAN;
@@ -570,17 +578,14 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
         continue;
       }
       last = kidx == nspan - 1;
-      // Long spans are folded in two levels: the last part of every kMergeGroup takes its group's others, and the span's last
-      // part its own group's and then those.
-      const bool two_levels = nspan > 2 * kMergeGroup;
-      const int group = two_levels ? kidx / kMergeGroup * kMergeGroup : 0;
-      const bool heads = last && two_levels;
-      if (last || (two_levels && kidx % kMergeGroup == kMergeGroup - 1)) {
+      // A tree: at every level the last part of 2^bits (and the span's last part) folds the others', by now of 2^bits times as
+      // many parts each. A level costs a flag's way and one trip for every kMergeParts partials: spread, four at a time are
+      // best (32763 tokens, 256 parts: 13.6 us; eight 15.4, sixteen 16.4); on one XCD eight (4096 tokens, 32 parts: 8.8 us;
+      // four 9.4, sixteen 9.7), and up to sixteen at once (8 ragged sequences: 8.1 us; eight 8.9).
+      const int bits = SPREAD ? 2 : (nspan <= 16 ? 4 : 3), others = (1 << bits) - 1;
 #pragma nounroll
-        for (int level = 0; level < (heads ? 2 : 1); ++level) {
-          const Waited waited = level == 0 ? Waited{group, 1, kidx - group} : Waited{kMergeGroup - 1, kMergeGroup, group / kMergeGroup};
-          fault |= merge_parts<SPREAD>(total, slots, slot0, waited, h, tail_lane, key);
-        }
+      for (int shift = 0, at = kidx; at > 0 && (last || (at & others) == others); shift += bits, at >>= bits) {
+        fault |= merge_parts<SPREAD>(total, slots, slot0, {((at & ~others) + 1 << shift) - 1, 1 << shift, at & others}, h, tail_lane, key);
       }
     }
     if (last) {
