@@ -203,8 +203,9 @@ __device__ __forceinline__ float max8(const float (&y)[2][4]) {
 }
 
 // The parts of one cut sequence that a bin waits for: first, first + stride, ... (count of them, at most 64).
+// `spins`: how long; a level of the tree waits longer than all before it, which may have waited for a part that never came.
 struct Waited {
-  int first, stride, count;
+  int first, stride, count, spins;
 };
 
 // A raised flag's low bits: the XCD where its part is to be seen; on all of them 1.
@@ -224,7 +225,7 @@ __device__ __forceinline__ int merge_parts(Part& total, char* slots, int slot0, 
   // Lane k polls the flag of part k (lanes past the last one repeat it).
   int32_t* flag = reinterpret_cast<int32_t*>(part_slot(slots, slot0, parts.first + parts.stride * min(lane, n - 1), h) + kFlagOffset);
   int f = 0;
-  for (int spins = 0; spins < kMaxSpins; ++spins) {
+  for (int spins = 0; spins < parts.spins; ++spins) {
     f = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (__builtin_amdgcn_ballot_w64(!flag_of_call(f, key)) == 0) break;
     __builtin_amdgcn_s_sleep(1);
@@ -584,8 +585,9 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
       // four 9.4, sixteen 9.7), and up to sixteen at once (8 ragged sequences: 8.1 us; eight 8.9).
       const int bits = SPREAD ? 2 : (nspan <= 16 ? 4 : 3), others = (1 << bits) - 1;
 #pragma nounroll
-      for (int shift = 0, at = kidx; at > 0 && (last || (at & others) == others); shift += bits, at >>= bits) {
-        fault |= merge_parts<SPREAD>(total, slots, slot0, {((at & ~others) + 1 << shift) - 1, 1 << shift, at & others}, h, tail_lane, key);
+      for (int shift = 0, at = kidx, spins = kMaxSpins; at > 0 && (last || (at & others) == others); shift += bits, at >>= bits, spins = min(2 * spins, 16 * kMaxSpins)) {
+        const Waited waited = {(((at & ~others) + 1) << shift) - 1, 1 << shift, at & others, spins};
+        fault |= merge_parts<SPREAD>(total, slots, slot0, waited, h, tail_lane, key);
       }
     }
     if (last) {

@@ -10,7 +10,7 @@ import torch
 from oracle import q4_reference as ref
 from pagedcore_amd import _hip
 from pagedcore_amd.decoder import capture_graph
-from tests.support import flags_clear
+from tests.support import fault_word, flags_clear, workspace_flags
 
 pytestmark = pytest.mark.gpu
 
@@ -231,6 +231,8 @@ CASES = {
     "with_empty_rows": [0, 5, 0, 200, 0],
     "cut": [2048, 3, 1500, 700],
     "long": [9001],
+    "long_ragged": [5000, 4097, 1, 0, 12003, 17, 8191],
+    "group_of_32": [4000],
     "many_short": [1 + i % 48 for i in range(300)],
 }
 
@@ -256,15 +258,29 @@ def test_attention(device, name):
     _check_rows(out, query, pool[layer], tables, lengths, rows)
 
 
-@pytest.mark.parametrize("scale", [0.0, 2.0**-20, 30.0, 1000.0])
+@pytest.mark.parametrize("scale", [0.0, 2.0**-20, 30.0, 1000.0, 20000.0])
 def test_attention_of_sharp_and_flat_scores(device, scale):
     rng = np.random.default_rng(3)
     lengths = [77, 400]
     tables, blocks = _tables(rng, lengths)
     pool = _filled(rng, blocks, 0)
-    query = _up((rng.standard_normal((2, 32, 64)) * scale).astype(np.float16), device)
+    query = _up(np.clip(rng.standard_normal((2, 32, 64)) * scale, -65504, 65504).astype(np.float16), device)
     out = _attend(device, _up(pool, device), 0, query, tables, lengths)
     _check_rows(out, query, pool[0], tables, lengths)
+
+
+@pytest.mark.parametrize("exponent", [-24, -20, -14, 12])
+def test_attention_over_rows_of_tiny_and_large_steps(device, exponent):
+    """Steps that are fp16 subnormals (down to the smallest) and steps and minima of thousands."""
+    rng = np.random.default_rng(8)
+    lengths = [77, 1000, 3]
+    tables, blocks = _tables(rng, lengths)
+    pool = _pool(rng, blocks)
+    key, value = (np.clip(rng.standard_normal((1, blocks * 16, 4, 64)) * 2.0**exponent, -60000, 60000).astype(np.float16) for _ in range(2))
+    ref.write(pool, 4, key, value, range(blocks * 16))
+    query = _up((rng.standard_normal((3, 32, 64)) * (30 if exponent < 0 else 2.0**-8)).astype(np.float16), device)
+    out = _attend(device, _up(pool, device), 4, query, tables, lengths)
+    _check_rows(out, query, pool[4], tables, lengths)
 
 
 def test_constant_values_come_back_exactly(device):
@@ -302,9 +318,9 @@ def test_nan_rows_stay_in_their_head_and_sequence(device):
     assert torch.equal(out[2, :9].view(torch.int16), clean[2, :9].view(torch.int16))
 
 
-def test_block_ids_outside_the_pool(device):
+@pytest.mark.parametrize("lengths", [[50, 300, 20], [50, 9000, 20]])
+def test_block_ids_outside_the_pool(device, lengths):
     rng = np.random.default_rng(6)
-    lengths = [50, 300, 20]
     tables, blocks = _tables(rng, lengths)
     pool = _up(_filled(rng, blocks, 0), device)
     query = _up(rng.standard_normal((3, 32, 64)).astype(np.float16), device)
@@ -323,7 +339,7 @@ def test_block_ids_outside_the_pool(device):
         assert torch.equal(out[[0, 2]].view(torch.int16), clean[[0, 2]].view(torch.int16))
 
 
-@pytest.mark.parametrize("name", ["one", "short", "block_ends", "cut", "many_short", "with_empty_rows"])
+@pytest.mark.parametrize("name", ["one", "short", "block_ends", "cut", "many_short", "with_empty_rows", "long_ragged"])
 def test_fused_append_equals_the_pair(device, name):
     rng = np.random.default_rng(10 + len(name))
     lengths = CASES[name]
@@ -340,6 +356,104 @@ def test_fused_append_equals_the_pair(device, name):
         out = _attend(device, pool, layer, query, tables, lengths, new)
         assert torch.equal(out.view(torch.int16), expected.view(torch.int16))
         assert torch.equal(pool, pair)
+
+
+def _spans(plan):
+    """Of every cut sequence its parts: {part: (plan row, segment)}."""
+    spans = {}
+    for row in range(plan.shape[0]):
+        for s in range(int(plan[row, 0])):
+            b, _, _, _, _, part, parts, _ = (int(v) for v in plan[row, 8 + 8 * s : 16 + 8 * s])
+            if parts > 1:
+                spans.setdefault(b, {})[part] = (row, s)
+    return spans
+
+
+@pytest.mark.parametrize("fault", ["first part", "part that folds", "last part", "slots outside the workspace", "sequence outside the batch"])
+@pytest.mark.parametrize("lengths", [[300, 40, 2048, 1500], [4000], [40, 9000, 700]])
+def test_plans_that_do_not_match(device, lengths, fault):
+    """A plan without one of a cut sequence's parts: the fold waits for it a bounded time, its row is NaN and the fault is
+    reported; without the last part, or with its partials outside the workspace, or under another number, its row is left alone.
+    Rows that the change does not touch keep their bits, and the next call on the workspace is right."""
+    rng = np.random.default_rng(16)
+    tables, blocks = _tables(rng, lengths)
+    lens, layer, width = np.asarray(lengths, dtype=np.int32), 7, tables.shape[1]
+    pool = _up(_filled(rng, blocks, layer), device)
+    query = _up(rng.standard_normal((len(lengths), 32, 64)).astype(np.float16), device)
+    workspace = torch.zeros(_hip.workspace_bytes(len(lengths), width), dtype=torch.uint8, device=device)
+    good = _attend(device, pool, layer, query, tables, lengths, workspace=workspace)
+    plan = _hip.decode_plan(lens, tables)
+    spans = _spans(plan)
+    b = int(np.argmax(lens))
+    parts = spans[b]
+    last = max(parts)
+    nan_rows, left_alone = set(), {b}
+    if fault in ("first part", "part that folds", "last part"):
+        row = parts[{"first part": 0, "part that folds": min(7, last - 1), "last part": last}[fault]][0]
+        inside = {int(x) for x in plan[row, 8 : 8 + 8 * int(plan[row, 0]) : 8]}
+        nan_rows = {x for x in inside if x in spans and spans[x][max(spans[x])][0] != row}
+        left_alone = inside - nan_rows
+        plan[row] = 0
+    elif fault == "slots outside the workspace":
+        for row, s in parts.values():
+            plan[row, 8 + 8 * s + 7] = 1 << 30
+    else:
+        for row, s in parts.values():
+            plan[row, 8 + 8 * s] = len(lengths) + 5
+    out = torch.full_like(good, 3.0)
+    _hip.planned_decode_attention_q4(out, query, pool, layer, _up(lens, device), _up(plan, device), width, workspace)
+    torch.cuda.synchronize()
+    for x in range(len(lengths)):
+        if x in nan_rows:
+            assert torch.isnan(out[x]).all(), x
+        elif x in left_alone:
+            assert (out[x] == 3.0).all(), x
+        else:
+            assert torch.equal(out[x].view(torch.int16), good[x].view(torch.int16)), x
+    assert fault_word(workspace) == (_hip.FAULT_MERGE_TIMEOUT if nan_rows else 0)
+    if nan_rows:
+        with pytest.raises(_hip.AttentionFaultError, match="bounded wait"):
+            _hip.check_attention_faults(workspace, "test")
+    elif fault == "last part":
+        assert workspace_flags(workspace).any()
+    again = _attend(device, pool, layer, query, tables, lengths, workspace=workspace)
+    assert torch.equal(again.view(torch.int16), good.view(torch.int16))
+
+
+def test_two_graphs_share_a_workspace(device):
+    """Graphs of two layers' attention, replayed in turn on one stream over one workspace, and a plan padded to its capacity."""
+    rng = np.random.default_rng(17)
+    lengths = [2000, 9, 700, 4500]
+    tables, blocks = _tables(rng, lengths)
+    width = tables.shape[1]
+    lens = _up(np.asarray(lengths, dtype=np.int32), device)
+    pool = _up(_pool(rng, blocks), device)
+    for layer in (0, 1):
+        key, value = (_up(_rows(rng, 1, blocks * 16), device) for _ in range(2))
+        _hip.kv_append_q4(pool, layer, key, value, torch.arange(blocks * 16, device=device))
+    host = np.zeros((_hip.plan_capacity(len(lengths), width), _hip.load().pc_attn_plan_record_ints()), dtype=np.int32)
+    _hip.decode_plan_into(np.asarray(lengths, dtype=np.int32), tables, host)
+    plan = _up(host, device)
+    workspace = torch.zeros(_hip.workspace_bytes(len(lengths), width), dtype=torch.uint8, device=device)
+    query = torch.zeros((len(lengths), 32, 64), dtype=torch.float16, device=device)
+    runs = []
+    for layer in (0, 1):
+
+        def step(layer=layer):
+            out = torch.zeros_like(query)
+            _hip.planned_decode_attention_q4(out, query, pool, layer, lens, plan, width, workspace)
+            return out
+
+        runs.append(capture_graph(step, device))
+    for turn in range(3):
+        query.copy_(torch.from_numpy(rng.standard_normal(tuple(query.shape)).astype(np.float16)))
+        for graph, _ in runs:
+            graph.replay()
+        for layer, (_, out) in enumerate(runs):
+            expected = _attend(device, pool, layer, query, tables, lengths)
+            assert torch.equal(out.view(torch.int16), expected.view(torch.int16))
+    _hip.check_attention_faults(workspace, "test")
+    assert flags_clear(workspace)
 
 
 def test_decode_steps_in_a_graph(device):
