@@ -12,7 +12,7 @@
 //     remainder in the two halves of the columns (16 bits of it; bf16 because p s' spans fp32's range), and
 //     128 sum(p s') of the same rounded weights, from one more product with ones, is taken off at the end.
 //
-// Two waves of a workgroup take a kv head of its bin, four blocks (64 tokens) a step. The row of a product's tile is
+// One or two waves of a workgroup take a kv head of its bin, four blocks (64 tokens) a step. The row of a product's tile is
 // chosen so that no data crosses lanes: tile i's row 4b + e is token 4i + e of the step's block b, which leaves lane
 // (c, g) the scores of block g for head c % 8. The group has 8 query heads and a tile 16 columns (the heads twice), so
 // the softmax takes tile 2a from columns 0-7 and tile 2a + 1 from columns 8-15: 32 tokens x 8 heads per four values
@@ -50,9 +50,6 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef int32_t int8_vt __attribute__((ext_vector_type(8), aligned(4)));
 
-constexpr int kParts = 2;  // waves of a kv head
-constexpr int kWaves = kParts * kKVHeads;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
 constexpr int kMergeParts = 4;   // partials a round trip
 constexpr int kSpreadBins = 32;  // bins of a group above which a long sequence's are spread over the XCDs
@@ -286,11 +283,19 @@ struct Blocks {
   }
 };
 
-template <bool APPEND, bool SPREAD>
-__global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int32_t* __restrict__ plan, const _Float16* query, char* pool,
-                                                                     uint32_t num_blocks, int layer, int rows, int batch, int nslots,
-                                                                     _Float16* out, char* workspace, const _Float16* new_key,
-                                                                     const _Float16* new_value) {
+// PARTS waves a kv head, each its share of the bin's steps. With much to read it is bound by HBM: 256 sequences of 2048 tokens
+// (151 MB) take 30.1 us with the launch, 5.0 TB/s (a large read: 6.3); vector instructions are half of that time. With little,
+// by latency: 128 tokens 3.9 us, of which a launch that does nothing is 1.9, then record, rows, products in turn; a cut sequence
+// adds its tree of partials (2048 tokens 7.9 us, 32763 12.9).
+//   Two waves a head have more loads in flight and halve a bin's chain of steps: 256 sequences of 2048 tokens 30.1 us (one wave
+// 37.2, four 31.0), 64 ragged ones 10.5 (11.1, 12.6), 256 of at most 64 tokens 8.6 (10.3, 8.0). One wave needs no barrier and no
+// fold: 128 tokens 3.9 us (two 4.6), eight ragged sequences 7.8 (8.1), one of 8192 tokens 10.4 (10.9).
+//   126 registers leave two workgroups of eight waves on a CU, which a plan of more bins than CUs needs.
+template <bool APPEND, bool SPREAD, int PARTS>
+__global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kernel(
+    const int32_t* __restrict__ plan, const _Float16* query, char* pool, uint32_t num_blocks, int layer, int rows, int batch, int nslots,
+    _Float16* out, char* workspace, const _Float16* new_key, const _Float16* new_value) {
+  constexpr int kWaves = PARTS * kKVHeads;
   __shared__ uint32_t shared_lines[kWaves * kMaxUnits];
   __shared__ __attribute__((aligned(16))) char shared_parts[kWaves * 2 * kPartBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
   char* const lbase = pool + static_cast<int64_t>(layer) * static_cast<int64_t>(num_blocks) * kBlockBytes + h * kUnitBytes;
 
   // This wave's steps [begin, end) of the bin's.
-  const int begin = part * steps / kParts, end = (part + 1) * steps / kParts;
+  const int begin = part * steps / PARTS, end = (part + 1) * steps / PARTS;
 
   // APPEND: lanes (c, g) quantise and store the new K (c < 8) and V row of segment g, if it ends its sequence and this wave has
   // its last step: the wave alone reads the unit, after this, and a wave's vector memory operations are done in order (the fence
@@ -549,7 +554,8 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     seg_step += seg_steps;
   }
   int fault = any_outside ? PC_ATTN_FAULT_BLOCK_ID : 0;
-  __syncthreads();
+  if constexpr (PARTS > 1) __syncthreads();
+  else wave_lds_fence();
   char* const slots = workspace + kWorkspaceHeader;
   const int key = flag_key(row[2], layer);
   int tail_lane = lane;  // what is computed from it below is not carried through the loop above
@@ -564,8 +570,8 @@ __global__ __launch_bounds__(kThreads, 4) void paged_decode_q4_kernel(const int3
     const int seg_end = r ? last_end : first_end;
     Part total = take_part(areas + r * kPartBytes, tail_lane);
     // The waves behind this one whose first segment this is.
-    for (int p = part + 1; p < kParts && p * steps / kParts < seg_end; ++p) {
-      if ((p + 1) * steps / kParts > p * steps / kParts) {
+    for (int p = part + 1; p < PARTS && p * steps / PARTS < seg_end; ++p) {
+      if ((p + 1) * steps / PARTS > p * steps / PARTS) {
         const char* area = shared_parts + (p * kKVHeads + h) * 2 * kPartBytes;
         fold_part(total, take_part(area, tail_lane));
       }
@@ -626,10 +632,13 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
   if (batch == 0 || num_records == 0) return ok();
   // Fewer bins a group, or of a sequence, and each of an XCD's CUs has at most two of them.
   const bool spread = num_records > kGroups * kSpreadBins && max_blocks > kMinBinBlocks * kSpreadBins;
-  const auto kernel = spread ? paged_decode_q4_kernel<APPEND, true> : paged_decode_q4_kernel<APPEND, false>;
+  // Bins of one segment and, at their least, two steps.
+  const bool single = batch <= kGroups && static_cast<int64_t>(batch) * max_blocks <= kTargetBins * kMinBinBlocks;
+  const auto kernel = spread ? (single ? paged_decode_q4_kernel<APPEND, true, 1> : paged_decode_q4_kernel<APPEND, true, 2>)
+                             : (single ? paged_decode_q4_kernel<APPEND, false, 1> : paged_decode_q4_kernel<APPEND, false, 2>);
   const unsigned grid = static_cast<unsigned>(spread ? (num_records + kGroups - 1) / kGroups * kGroups : num_records);
   (void)hipGetLastError();
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0,
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * kKVHeads * (single ? 1 : 2)), 0,
                      static_cast<hipStream_t>(stream), plan, static_cast<const _Float16*>(query), static_cast<char*>(pool), static_cast<uint32_t>(num_blocks),
                      layer, num_records, batch, static_cast<int>(slots_bound(batch, max_blocks)), static_cast<_Float16*>(out),
                      static_cast<char*>(workspace), static_cast<const _Float16*>(new_key), static_cast<const _Float16*>(new_value));

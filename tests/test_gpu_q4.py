@@ -53,6 +53,14 @@ def _filled(rng, blocks, layer):
     return pool
 
 
+def _written(rng, blocks, layer, device):
+    """The same, on the device and quantised there, where no definition is compared with."""
+    pool = torch.randint(0, 256, (22, blocks, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    key, value = (_up(rng.standard_normal((1, blocks * 16, 4, 64)).astype(np.float16), device) for _ in range(2))
+    _hip.kv_append_q4(pool, layer, key, value, torch.arange(blocks * 16, device=device))
+    return pool
+
+
 @pytest.mark.parametrize("layers,begin,tokens,start", [(1, 21, 1, 0), (22, 0, 17, 5), (3, 7, 64, 0), (2, 20, 131, 15), (5, 0, 4, 2), (22, 0, 27, 7), (1, 4, 700, 0)])
 def test_append_bytes(device, layers, begin, tokens, start):
     rng = np.random.default_rng(tokens)
@@ -233,6 +241,7 @@ CASES = {
     "long": [9001],
     "long_ragged": [5000, 4097, 1, 0, 12003, 17, 8191],
     "group_of_32": [4000],
+    "long_few": [8191, 9, 5000],
     "many_short": [1 + i % 48 for i in range(300)],
 }
 
@@ -322,7 +331,7 @@ def test_nan_rows_stay_in_their_head_and_sequence(device):
 def test_block_ids_outside_the_pool(device, lengths):
     rng = np.random.default_rng(6)
     tables, blocks = _tables(rng, lengths)
-    pool = _up(_filled(rng, blocks, 0), device)
+    pool = _written(rng, blocks, 0, device)
     query = _up(rng.standard_normal((3, 32, 64)).astype(np.float16), device)
     clean = _attend(device, pool, 0, query, tables, lengths)
     for bad in (blocks, -1, 1 << 30):
@@ -339,13 +348,13 @@ def test_block_ids_outside_the_pool(device, lengths):
         assert torch.equal(out[[0, 2]].view(torch.int16), clean[[0, 2]].view(torch.int16))
 
 
-@pytest.mark.parametrize("name", ["one", "short", "block_ends", "cut", "many_short", "with_empty_rows", "long_ragged"])
+@pytest.mark.parametrize("name", ["one", "short", "block_ends", "cut", "many_short", "with_empty_rows", "long_ragged", "long_few"])
 def test_fused_append_equals_the_pair(device, name):
     rng = np.random.default_rng(10 + len(name))
     lengths = CASES[name]
     tables, blocks = _tables(rng, lengths)
     layer = 20
-    pool = _up(_filled(rng, blocks, layer), device)
+    pool = _written(rng, blocks, layer, device)
     query = _up(rng.standard_normal((len(lengths), 32, 64)).astype(np.float16), device)
     new = [_up(_rows(rng, len(lengths)), device) for _ in range(2)]
     slots = np.array([tables[b, (n - 1) // 16] * 16 + (n - 1) % 16 if n else -1 for b, n in enumerate(lengths)], dtype=np.int64)
@@ -370,7 +379,7 @@ def _spans(plan):
 
 
 @pytest.mark.parametrize("fault", ["first part", "part that folds", "last part", "slots outside the workspace", "sequence outside the batch"])
-@pytest.mark.parametrize("lengths", [[300, 40, 2048, 1500], [4000], [40, 9000, 700]])
+@pytest.mark.parametrize("lengths", [[300, 40, 2048, 1500], [4000], [40, 9000, 700], [300, 40, 2048, 1500, 1, 64, 7, 900, 30, 5], [40, 9000, 12000, 700]])
 def test_plans_that_do_not_match(device, lengths, fault):
     """A plan without one of a cut sequence's parts: the fold waits for it a bounded time, its row is NaN and the fault is
     reported; without the last part, or with its partials outside the workspace, or under another number, its row is left alone.
@@ -378,7 +387,7 @@ def test_plans_that_do_not_match(device, lengths, fault):
     rng = np.random.default_rng(16)
     tables, blocks = _tables(rng, lengths)
     lens, layer, width = np.asarray(lengths, dtype=np.int32), 7, tables.shape[1]
-    pool = _up(_filled(rng, blocks, layer), device)
+    pool = _written(rng, blocks, layer, device)
     query = _up(rng.standard_normal((len(lengths), 32, 64)).astype(np.float16), device)
     workspace = torch.zeros(_hip.workspace_bytes(len(lengths), width), dtype=torch.uint8, device=device)
     good = _attend(device, pool, layer, query, tables, lengths, workspace=workspace)
@@ -427,10 +436,8 @@ def test_two_graphs_share_a_workspace(device):
     tables, blocks = _tables(rng, lengths)
     width = tables.shape[1]
     lens = _up(np.asarray(lengths, dtype=np.int32), device)
-    pool = _up(_pool(rng, blocks), device)
-    for layer in (0, 1):
-        key, value = (_up(_rows(rng, 1, blocks * 16), device) for _ in range(2))
-        _hip.kv_append_q4(pool, layer, key, value, torch.arange(blocks * 16, device=device))
+    pool = _written(rng, blocks, 0, device)
+    pool[1] = pool[0].flip(0)
     host = np.zeros((_hip.plan_capacity(len(lengths), width), _hip.load().pc_attn_plan_record_ints()), dtype=np.int32)
     _hip.decode_plan_into(np.asarray(lengths, dtype=np.int32), tables, host)
     plan = _up(host, device)
