@@ -16,6 +16,8 @@ Contents (each function cites the reference lines it restates):
   decoder_reference.*                         dense.py, decoder.py:70-100,202-240 (TinyLlama forward, generate)
   fp8_reference.*                             none: 8-bit rows and their projections in 64 bits, from the format's definition
                                               (pinned in tests/test_fp8_host.py by torch's own casts and by hand)
+  q4_reference.*                              none: 4-bit KV rows and attention over them in 64 bits, from the format's definition
+                                              (pinned in tests/test_q4_host.py by hand)
 
 How each one is pinned (tests/test_oracle.py): the reference tests' known answers (exact
 3, exact 100*(h//8)+16, exact 0.25, tiny probabilities > 0, +-1000 scores) and FP64

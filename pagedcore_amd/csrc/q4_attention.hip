@@ -6,8 +6,8 @@
 //   y_t = s_t (q . n_t) + lo_t sum(q),   p_t = exp((y_t - max y) / 8)
 //   out = (sum_t (p_t s'_t) n'_t + sum_t p_t lo'_t) / sum_t p_t
 // so scales and minima enter once per token and head, and the products run on the levels themselves:
-//   * q . n on the fp16 instruction, n taken as the fp16 whose bits are n (the subnormal n 2^-24: exact, and one
-//     mask and shift for two of them);
+//   * q . n on the fp16 instruction, n taken as the fp16 whose bits are n or 16 n (the subnormals n 2^-24 and n 2^-20:
+//     exact, and one mask and at most one shift for two of them; the query's elements make up for the factor);
 //   * (p s') n' on the bf16 instruction, n' as 128 + n' (bf16 bits 0x4300 | n'), p s' as bf16 and the bf16 of its
 //     remainder in the two halves of the columns (16 bits of it; bf16 because p s' spans fp32's range), and
 //     128 sum(p s') of the same rounded weights, from one more product with ones, is taken off at the end.
