@@ -460,7 +460,8 @@ int32_t pc_gemm_fp8_kernels(int32_t epilogue, int32_t half_x);
  * KV append into the 4-bit pool: pc_kv_append (reference src/pagedcore/kv_cache.py:161-172, 242-245) with each row quantised
  * as it is written. Arguments as there: key/value rows are [4][64] fp16 with contiguous heads and dims, layer and token
  * strides free; a token whose slot lies outside [0, num_blocks * 16) is not written, nor is any byte of another slot. A slot
- * named twice holds one of its tokens' rows, or bytes of both. num_layers * num_tokens up to 2^28.
+ * named twice holds one of its tokens' rows, or bytes of both. num_layers * num_tokens up to 2^28; with no tokens key, value and
+ * slot_mapping may be null.
  */
 int pc_kv_append_q4(void* pool, int64_t num_blocks, int32_t layer_begin, int32_t num_layers, const void* key,
                     int64_t key_layer_stride, int64_t key_token_stride, const void* value, int64_t value_layer_stride,
@@ -482,7 +483,8 @@ int pc_kv_read_q4(void* key, int64_t key_layer_stride, int64_t key_token_stride,
  * Paged decode attention of one layer over the 4-bit pool: pc_paged_decode_attn with the same plan, workspace, faults and
  * rules, over the values lo + s n that the rows stand for (not rounded to fp16). Scores, softmax and sums are fp32, the
  * weights that multiply V's levels are held in 16 bits of significand, the output is rounded once. Slots past a sequence's
- * length never reach the output, whatever their bytes are.
+ * length never reach the output, whatever their bytes are. Without sequences or plan rows the call does nothing and their pointers
+ * may be null.
  */
 int pc_paged_decode_attn_q4(void* out, const void* query, const void* pool, int64_t num_blocks, int32_t layer,
                             const int32_t* context_lens, int32_t batch, int32_t max_blocks, const int32_t* plan,

@@ -255,7 +255,7 @@ def kv_append(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_m
 
 
 def _check_fp16_pool(pool: Optional[Tensor]) -> None:
-    if pool is not None and pool.dtype is not torch.float16:
+    if pool is not None and pool.dtype is _U8:
         raise HipExtensionError("pool must be float16 [22, 2, blocks, 16, 4, 64] (the _q4 calls take a 4-bit pool)")
 
 
@@ -886,6 +886,14 @@ def _refuse_q4_rows(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, 
     raise HipExtensionError(f"slot_mapping must be contiguous int64 [{shape[1]}] on GPU {device}")
 
 
+def _refuse_overlapping_rows(layers: int, tokens: int, *strides: Tuple[int, ...]) -> None:
+    for outer, inner, *_ in strides:  # each layer's rows behind the last one's, or each token's
+        if (tokens > 1 and inner < 256) or (layers > 1 and outer < 256) or (
+            tokens > 1 and layers > 1 and outer < 256 + inner * (tokens - 1) and inner < 256 + outer * (layers - 1)
+        ):
+            raise HipExtensionError("the rows of key and value must not overlap")
+
+
 def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
     """kv_append into a 4-bit pool (uint8 [22, blocks, 4, 1152]): each row [64] of key/value[l, t] quantised to 16 levels
     between its smallest and its largest value and written to slot slot_mapping[t] of layer layer_begin + l.
@@ -914,17 +922,21 @@ def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slo
 def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_mapping: Tensor) -> None:
     """key/value[l, t] = the values of slot slot_mapping[t] in layer layer_begin + l of a 4-bit pool, rounded to float16.
 
-    key/value: float16 [layers, tokens, 4, 64] to write, each [4, 64] row contiguous, layer and token strides free; the rows of
-    a slot outside the pool are left as they are. slot_mapping: int64 [tokens]. On the current stream of the pool's device."""
+    key/value: float16 [layers, tokens, 4, 64] to write, each [4, 64] row contiguous, layer and token strides free but for rows
+    that overlap; the rows of a slot outside the pool are left as they are. slot_mapping: int64 [tokens]. On the current stream
+    of the pool's device."""
     if not _q4_rows_fit(pool, layer_begin, key, value, slot_mapping):
         _refuse_q4_rows(pool, layer_begin, key, value, slot_mapping)
     ks, vs = key.stride(), value.stride()
     if ks[3] != 1 or ks[2] != 64 or vs[3] != 1 or vs[2] != 64:
         raise HipExtensionError("each [4, 64] row of key and value must be contiguous")
+    layers, tokens = key.shape[0], key.shape[1]
+    if ks[1] < 256 or vs[1] < 256 or ks[0] < ks[1] * tokens or vs[0] < vs[1] * tokens:  # not layer behind layer
+        _refuse_overlapping_rows(layers, tokens, ks, vs)
     lib = load()
     status = _q4_launch(
         pool.get_device(), lib.pc_kv_read_q4, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], pool.data_ptr(),
-        pool.shape[1], layer_begin, key.shape[0], slot_mapping.data_ptr(), key.shape[1],
+        pool.shape[1], layer_begin, layers, slot_mapping.data_ptr(), tokens,
     )
     if status:
         _check(lib, "pc_kv_read_q4", status)

@@ -616,8 +616,8 @@ template <bool APPEND>
 int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t layer, const int32_t* context_lens, int32_t batch,
            int32_t max_blocks, const int32_t* plan, int32_t num_records, const void* new_key, const void* new_value,
            void* workspace, void* stream) {
-  if (!out || !query || !pool || !context_lens || !plan) return set_error(PC_ERR_ARGUMENT, "null pointer");
-  if (APPEND && (!new_key || !new_value)) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (!pool || (num_records != 0 && !plan)) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (batch != 0 && (!out || !query || !context_lens || (APPEND && (!new_key || !new_value)))) return set_error(PC_ERR_ARGUMENT, "null pointer");
   if (!workspace) return set_error(PC_ERR_ARGUMENT, "workspace required (null pointer)");
   if (num_blocks < 1 || num_blocks > kMaxBlocks) return set_error(PC_ERR_ARGUMENT, "num_blocks out of range [1, 2^26]");
   if (layer < 0 || layer >= kLayers) return set_error(PC_ERR_ARGUMENT, "layer %d outside [0, 22)", layer);

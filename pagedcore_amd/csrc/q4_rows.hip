@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(Row
 int row_args(RowArgs& args, const void* pool, int64_t num_blocks, int32_t layer_begin, int32_t num_layers, const void* key,
              int64_t key_layer_stride, int64_t key_token_stride, const void* value, int64_t value_layer_stride,
              int64_t value_token_stride, const int64_t* slot_mapping, int64_t num_tokens) {
-  if (!pool || !key || !value || !slot_mapping) return set_error(PC_ERR_ARGUMENT, "null pointer");
+  if (!pool || (num_tokens != 0 && (!key || !value || !slot_mapping))) return set_error(PC_ERR_ARGUMENT, "null pointer");
   if (num_blocks < 1 || num_blocks > (1 << 26)) return set_error(PC_ERR_ARGUMENT, "num_blocks %lld out of range [1, 2^26]", static_cast<long long>(num_blocks));
   if (num_layers < 1 || layer_begin < 0 || num_layers > kLayers || layer_begin > kLayers - num_layers) {
     return set_error(PC_ERR_ARGUMENT, "layers [%d, %d + %d) outside [0, %d)", layer_begin, layer_begin, num_layers, kLayers);

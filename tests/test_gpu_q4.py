@@ -533,6 +533,29 @@ def test_offsets_past_32_bits(device):
         _assert_read(back[kind, 0].cpu().numpy(), ref.rows(last, kind, slots))
 
 
+def test_nothing_to_do(device):
+    """No tokens, no sequences, sequences that are all empty: the pool and the outputs stay as they were."""
+    pool = torch.randint(0, 256, (22, 4, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    before = pool.clone()
+    rows = [torch.empty((3, 0, 4, 64), dtype=torch.float16, device=device) for _ in range(2)]
+    slots = torch.empty(0, dtype=torch.int64, device=device)
+    _hip.kv_append_q4(pool, 0, *rows, slots)
+    _hip.kv_read_q4(*rows, pool, 0, slots)
+    for lengths in ([], [0], [0, 0, 0]):
+        n = len(lengths)
+        lens, tables = torch.zeros(n, dtype=torch.int32, device=device), torch.zeros((n, 2), dtype=torch.int32, device=device)
+        query = torch.zeros((n, 32, 64), dtype=torch.float16, device=device)
+        out = torch.full_like(query, 3.0)
+        workspace = torch.zeros(_hip.workspace_bytes(n, 2), dtype=torch.uint8, device=device)
+        _hip.paged_decode_attention_q4(out, query, pool, 1, tables, lens, workspace=workspace)
+        new = torch.ones((n, 4, 64), dtype=torch.float16, device=device)
+        plan = _up(_hip.decode_plan(np.zeros(n, dtype=np.int32), np.zeros((n, 2), dtype=np.int32)), device)
+        _hip.planned_decode_attention_q4(out, query, pool, 1, lens, plan, 2, workspace, new_key=new, new_value=new)
+        torch.cuda.synchronize()
+        assert (out == 3.0).all() and not workspace.any()
+    assert torch.equal(pool, before)
+
+
 def test_another_stream(device):
     rng = np.random.default_rng(14)
     lengths = [600, 31]

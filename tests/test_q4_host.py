@@ -125,6 +125,23 @@ def test_rows_to_read_into_must_be_whole(calls):  # noqa: F811
     assert calls == []
 
 
+@pytest.mark.parametrize("rows", [
+    torch.zeros((1, 5, 4, 64), dtype=torch.float16).expand(2, 5, 4, 64),
+    torch.zeros((2, 1, 4, 64), dtype=torch.float16).expand(2, 5, 4, 64),
+    torch.zeros(2000, dtype=torch.float16).as_strided((2, 5, 4, 64), (400, 128, 64, 1)),
+])
+def test_rows_to_read_into_must_not_overlap(calls, rows):  # noqa: F811
+    pool, _, value, slots, _ = _call()
+    for pair in ((OnGpu(rows, 0), value), (value, OnGpu(rows, 0))):
+        with pytest.raises(_hip.HipExtensionError, match="overlap"):
+            _hip.kv_read_q4(*pair, pool, 0, slots)
+    assert calls == []
+    single = OnGpu(torch.zeros((1, 1, 4, 64), dtype=torch.float16).as_strided((1, 1, 4, 64), (0, 0, 64, 1)), 0)
+    _hip.kv_read_q4(single, single, pool, 0, _on((1,), torch.int64))  # one row: its strides are of no account
+    _hip.kv_append_q4(pool, 0, OnGpu(rows, 0), value, slots)  # what is only read may
+    assert [name for name, *_ in calls] == ["pc_kv_read_q4", "pc_kv_append_q4"]
+
+
 def test_calls_go_to_the_pools_gpu(calls):  # noqa: F811
     for gpu in (0, 2):
         on = lambda shape, dtype=torch.float16: _on(shape, dtype, gpu)  # noqa: E731
@@ -179,6 +196,13 @@ def test_attention_refused(monkeypatch):
     assert len(launched) == 2
 
 
+def test_the_fp16_calls_look_at_no_other_type():
+    """Their rows are 16-bit words: what they took before there were 4-bit pools, they still take."""
+    for dtype in (torch.float16, torch.int16, torch.bfloat16):
+        _hip._check_fp16_pool(torch.zeros((22, 2, 1, 16, 4, 64), dtype=dtype))
+    _hip._check_fp16_pool(None)
+
+
 def test_the_fp16_calls_refuse_a_4_bit_pool():
     pool = torch.zeros((22, 3, 4, 1152), dtype=torch.uint8)
     rows = torch.zeros((1, 2, 4, 64), dtype=torch.float16)
@@ -213,7 +237,7 @@ def test_library_refusals():
         )
 
     for call in (append, read):
-        assert call(tokens=0) == 0
+        assert call(tokens=0) == 0 and call(tokens=0, key=None, value=None, slots=None) == 0  # as empty tensors' pointers are
         for change, text in (
             ({"pool": None}, b"null"), ({"key": None}, b"null"), ({"value": None}, b"null"), ({"slots": None}, b"null"),
             ({"blocks": 0}, b"num_blocks"), ({"blocks": (1 << 26) + 1}, b"num_blocks"), ({"begin": -1}, b"layers"),
@@ -232,6 +256,8 @@ def test_library_refusals():
 
     for fused in (False, True):
         assert attend(fused, rows=0) == 0 and attend(fused, batch=0) == 0
+        assert attend(fused, rows=0, plan=None) == 0  # nothing but empty sequences
+        assert attend(fused, batch=0, rows=0, out=None, query=None, lens=None, plan=None, key=None, value=None) == 0
         for change, text in (
             ({"out": None}, b"null"), ({"plan": None}, b"null"), ({"workspace": None}, b"workspace"), ({"blocks": 0}, b"num_blocks"),
             ({"blocks": (1 << 26) + 1}, b"num_blocks"), ({"layer": 22}, b"layer"), ({"layer": -1}, b"layer"), ({"batch": -1}, b"batch"),
