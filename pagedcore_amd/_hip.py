@@ -844,8 +844,9 @@ def empty_q4_pool(blocks: int, device: torch.device) -> Tensor:
 
 def is_q4_pool(pool: Tensor) -> bool:
     """Whether `pool` has the type and shape of a 4-bit pool, contiguous."""
+    shape = pool.shape
     return (
-        pool.dtype is _U8 and pool.dim() == 4 and pool.shape[1] > 0 and pool.shape == (22, pool.shape[1], 4, Q4_UNIT_BYTES)
+        pool.dtype is _U8 and len(shape) == 4 and shape[0] == 22 and shape[1] > 0 and shape[2] == 4 and shape[3] == Q4_UNIT_BYTES
         and pool.is_contiguous()
     )
 
@@ -999,13 +1000,14 @@ def planned_decode_attention_q4(
     lib = load()
     device, batch = pool.get_device(), context_lens.shape[0] if context_lens.dim() == 1 else -1
     nbytes = lib.pc_attn_workspace_bytes(batch, max_blocks) if batch >= 0 else 0
+    plan_shape = plan.shape
     if not (
         device >= 0 and is_q4_pool(pool) and nbytes > 0
         and context_lens.dtype is _I32 and context_lens.is_contiguous() and context_lens.get_device() == device
         and out.dtype is _F16 and out.dim() > 1 and out.shape[0] == batch and out.numel() == batch * 2048 and out.is_contiguous() and out.get_device() == device
         and query.dtype is _F16 and query.dim() > 1 and query.shape[0] == batch and query.numel() == batch * 2048 and query.is_contiguous()
         and query.get_device() == device
-        and plan.dtype is _I32 and plan.dim() == 2 and plan.shape[1] == _PLAN_INTS and plan.is_contiguous() and plan.get_device() == device
+        and plan.dtype is _I32 and len(plan_shape) == 2 and plan_shape[1] == _PLAN_INTS and plan.is_contiguous() and plan.get_device() == device
         and workspace.nbytes >= nbytes and workspace.is_contiguous() and workspace.get_device() == device
         and (
             (new_key is None and new_value is None)
@@ -1020,7 +1022,7 @@ def planned_decode_attention_q4(
     ):
         _refuse_q4_attention(out, query, pool, context_lens, plan, max_blocks, workspace, nbytes, new_key, new_value)
     args = (out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer, context_lens.data_ptr(), batch, max_blocks,
-            plan.data_ptr(), plan.shape[0])
+            plan.data_ptr(), plan_shape[0])
     if new_key is None:
         status = _q4_launch(device, lib.pc_paged_decode_attn_q4, *args, workspace.data_ptr())
         if status:

@@ -14,7 +14,8 @@ for the launch, read the workspace's fault word and raise
 AttentionFaultError (a RuntimeError) instead of returning NaN rows.
 
 ``paged_attention_batch`` is the batched form the decode loop needs (one launch for all
-rows of a layer). Over a 4-bit pool (allocate_kv_pool(bits=4)) both attend to the values that its rows stand for. The reference's ``eager_rounding=True`` path replays HF fp16 rounding for
+rows of a layer). Over a 4-bit pool (allocate_kv_pool(bits=4)) both attend to the values that
+its rows stand for. The reference's ``eager_rounding=True`` path replays HF fp16 rounding for
 forensic comparisons; it is not part of the serving path and is rejected here.
 """
 
