@@ -51,7 +51,11 @@ typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef int32_t int8_vt __attribute__((ext_vector_type(8), aligned(4)));
 
 constexpr int kPartBytes = 2048 + 512;  // a wave's partial in LDS
-constexpr int kMergeParts = 4;   // partials a round trip
+// Partials a round trip (seven: 2048 tokens 8.3 us instead of 7.95, 64 ragged sequences 10.7 instead of 10.4, 32763 13.8 instead of 12.9).
+constexpr int kMergeParts = 4;
+// Bins of a group above which a long sequence's are spread over the XCDs. On one XCD its bins share 32 CUs, on all of them their
+// partials meet in memory instead of in the L2. One call, us on one XCD / spread: 4096 tokens 8.9 / 9.5, 8192 11.1 / 10.3,
+// six of 9000 14.3 / 13.4; 64 ragged sequences 10.4 / 13.1.
 constexpr int kSpreadBins = 32;  // bins of a group above which a long sequence's are spread over the XCDs
 constexpr int kStepBlocks = 4;
 constexpr int64_t kMaxBlocks = 1 << 26;  // a block's place in a layer, in 128-byte lines, in 32 bits
@@ -586,8 +590,8 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
       last = kidx == nspan - 1;
       // A tree: at every level the last part of 2^bits (and the span's last part) folds the others', by now of 2^bits times as
       // many parts each. A level costs a flag's way and one trip for every kMergeParts partials: spread, four at a time are
-      // best (32763 tokens, 256 parts: 13.6 us; eight 15.4, sixteen 16.4); on one XCD eight (4096 tokens, 32 parts: 8.8 us;
-      // four 9.4, sixteen 9.7), and up to sixteen at once (8 ragged sequences: 8.1 us; eight 8.9).
+      // best (32763 tokens, 256 parts: 12.9 us; eight 14.5, sixteen 15.6); on one XCD eight (4096 tokens, 32 parts: 8.9 us;
+      // four 9.2, sixteen 9.6), and up to sixteen at once (8 ragged sequences: 7.85 us; four 8.2, eight 8.8).
       const int bits = SPREAD ? 2 : (nspan <= 16 ? 4 : 3), others = (1 << bits) - 1;
 #pragma nounroll
       for (int shift = 0, at = kidx, spins = kMaxSpins; at > 0 && (last || (at & others) == others); shift += bits, at >>= bits, spins = min(2 * spins, 16 * kMaxSpins)) {
