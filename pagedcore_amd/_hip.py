@@ -851,12 +851,12 @@ def is_q4_pool(pool: Tensor) -> bool:
     )
 
 
-def _q4_launch(device: int, fn, *args) -> int:
+def _q4_launch(device: int, fn, args: tuple) -> int:
     """fn(*args, the current stream of GPU `device`), with that GPU current."""
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _q4_launch(device, fn, *args)
-    return fn(*args, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+    if device == torch.cuda.current_device():
+        return fn(*args, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return _q4_launch(device, fn, args)
 
 
 def _check_q4_pool(pool: Tensor) -> int:
@@ -912,10 +912,9 @@ def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slo
         value = value.contiguous()
         vs = value.stride()
     lib = load()
-    status = _q4_launch(
-        pool.get_device(), lib.pc_kv_append_q4, pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], key.data_ptr(), ks[0], ks[1],
-        value.data_ptr(), vs[0], vs[1], slot_mapping.data_ptr(), key.shape[1],
-    )
+    args = (pool.data_ptr(), pool.shape[1], layer_begin, key.shape[0], key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1],
+            slot_mapping.data_ptr(), key.shape[1])
+    status = _q4_launch(pool.get_device(), lib.pc_kv_append_q4, args)
     if status:
         _check(lib, "pc_kv_append_q4", status)
 
@@ -935,10 +934,9 @@ def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_
     if ks[1] < 256 or vs[1] < 256 or ks[0] < ks[1] * tokens or vs[0] < vs[1] * tokens:  # not layer behind layer
         _refuse_overlapping_rows(layers, tokens, ks, vs)
     lib = load()
-    status = _q4_launch(
-        pool.get_device(), lib.pc_kv_read_q4, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], pool.data_ptr(),
-        pool.shape[1], layer_begin, layers, slot_mapping.data_ptr(), tokens,
-    )
+    args = (key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], pool.data_ptr(), pool.shape[1], layer_begin, layers,
+            slot_mapping.data_ptr(), tokens)
+    status = _q4_launch(pool.get_device(), lib.pc_kv_read_q4, args)
     if status:
         _check(lib, "pc_kv_read_q4", status)
 
@@ -1004,8 +1002,8 @@ def planned_decode_attention_q4(
     if not (
         device >= 0 and is_q4_pool(pool) and nbytes > 0
         and context_lens.dtype is _I32 and context_lens.is_contiguous() and context_lens.get_device() == device
-        and out.dtype is _F16 and out.dim() > 1 and out.shape[0] == batch and out.numel() == batch * 2048 and out.is_contiguous() and out.get_device() == device
-        and query.dtype is _F16 and query.dim() > 1 and query.shape[0] == batch and query.numel() == batch * 2048 and query.is_contiguous()
+        and out.dtype is _F16 and out.numel() == batch * 2048 and out.shape[0] == batch and out.is_contiguous() and out.get_device() == device
+        and query.dtype is _F16 and query.numel() == batch * 2048 and query.shape[0] == batch and query.is_contiguous()
         and query.get_device() == device
         and plan.dtype is _I32 and len(plan_shape) == 2 and plan_shape[1] == _PLAN_INTS and plan.is_contiguous() and plan.get_device() == device
         and workspace.nbytes >= nbytes and workspace.is_contiguous() and workspace.get_device() == device
@@ -1013,9 +1011,9 @@ def planned_decode_attention_q4(
             (new_key is None and new_value is None)
             or (
                 new_key is not None and new_value is not None
-                and new_key.dtype is _F16 and new_key.dim() > 1 and new_key.shape[0] == batch and new_key.numel() == batch * 256
+                and new_key.dtype is _F16 and new_key.numel() == batch * 256 and new_key.shape[0] == batch
                 and new_key.is_contiguous() and new_key.get_device() == device
-                and new_value.dtype is _F16 and new_value.dim() > 1 and new_value.shape[0] == batch and new_value.numel() == batch * 256
+                and new_value.dtype is _F16 and new_value.numel() == batch * 256 and new_value.shape[0] == batch
                 and new_value.is_contiguous() and new_value.get_device() == device
             )
         )
@@ -1024,10 +1022,10 @@ def planned_decode_attention_q4(
     args = (out.data_ptr(), query.data_ptr(), pool.data_ptr(), pool.shape[1], layer, context_lens.data_ptr(), batch, max_blocks,
             plan.data_ptr(), plan_shape[0])
     if new_key is None:
-        status = _q4_launch(device, lib.pc_paged_decode_attn_q4, *args, workspace.data_ptr())
+        status = _q4_launch(device, lib.pc_paged_decode_attn_q4, (*args, workspace.data_ptr()))
         if status:
             _check(lib, "pc_paged_decode_attn_q4", status)
         return
-    status = _q4_launch(device, lib.pc_kv_append_paged_decode_attn_q4, *args, new_key.data_ptr(), new_value.data_ptr(), workspace.data_ptr())
+    status = _q4_launch(device, lib.pc_kv_append_paged_decode_attn_q4, (*args, new_key.data_ptr(), new_value.data_ptr(), workspace.data_ptr()))
     if status:
         _check(lib, "pc_kv_append_paged_decode_attn_q4", status)

@@ -56,7 +56,7 @@ constexpr int kMergeParts = 4;
 // Bins of a group above which a long sequence's are spread over the XCDs. On one XCD its bins share 32 CUs, on all of them their
 // partials meet in memory instead of in the L2. One call, us on one XCD / spread: 4096 tokens 8.9 / 9.5, 8192 11.1 / 10.3,
 // six of 9000 14.3 / 13.4; 64 ragged sequences 10.4 / 13.1.
-constexpr int kSpreadBins = 32;  // bins of a group above which a long sequence's are spread over the XCDs
+constexpr int kSpreadBins = 32;
 constexpr int kStepBlocks = 4;
 constexpr int64_t kMaxBlocks = 1 << 26;  // a block's place in a layer, in 128-byte lines, in 32 bits
 static_assert(kMaxUnits == 256, "four vectors of block ids");
