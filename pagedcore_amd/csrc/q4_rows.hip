@@ -1,7 +1,7 @@
 // Rows of the 4-bit KV pool: quantised as they are written (pc_kv_append_q4), and read back as fp16
 // (pc_kv_read_q4). The format and its bytes are in q4_device.h. Both are bound by HBM: 1024 bytes of fp16 and
-// 288 of the pool per token and layer: 2048 tokens of 22 layers (59 MB) are appended in 15.6 us and read back in 15.1
-// with the launch, 16384 read back in 95.6 (4.95 TB/s, a large copy's rate).
+// 288 of the pool per token and layer: 2048 tokens of 22 layers (59 MB) are appended in 15.6 us and read back in 12.8
+// with the launch, 16384 read back in 71.9 (6.6 TB/s; a large fill reaches 6.9, a large copy 4.9).
 
 #include <hip/hip_runtime.h>
 
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(RowArgs args) {
 constexpr int kGroupTokens = 8;
 constexpr int kGroupWaves = 4;
 // Rows (8 a token and layer) above which they pay: 1024 tokens of 1, 2 and 5 layers take 4.6, 4.6 and 4.8 us in groups, 3.2, 3.5 and 5.2
-// a token at a time; 2048 of 22 layers 15.6 and 22.2, read back 15.1 and 21.5, 16384 read back 95.6 and 196.
+// a token at a time; 2048 of 22 layers 15.6 and 22.2, read back 12.8 and 21.5, 16384 read back 71.9 and 196.
 constexpr uint32_t kGroupRows = 8 * 4400;
 
 struct Group {
@@ -214,6 +214,11 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_append_q4_groups_kernel(R
   *reinterpret_cast<uint32_t*>(unit + pair_offset(kind, kGroupTokens * half + a)) = pair;
 }
 
+// The rows are whole lines that nothing reads soon, 9 MB and more of them: stored non-temporally 2048 tokens of 22 layers take 12.8 us
+// instead of 15.1, 16384 71.9 instead of 95.4, and with a sum of K and V that reads them at once 27.6 instead of 30.0 and 182
+// instead of 199. (Of the append's 13 MB of pool, which attention reads next, the same made 333 tokens slower, 5.0 to 5.4.)
+__device__ __forceinline__ void store_past_caches(char* at, half8_t row) { __builtin_nontemporal_store(row, reinterpret_cast<half8_t*>(at)); }
+
 __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(RowArgs args) {
   Group group;
   if (!group_of(args, group)) return;
@@ -228,8 +233,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(Row
           static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(group.slot >> 32), i))) << 32 |
           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(group.slot), i)));
       if (slot >= 0) {
-        *reinterpret_cast<half8_t*>(rows + stride * (group.token0 + i)) =
-            load_row(layer + slot / kSlots * kBlockBytes, kind, static_cast<int>(slot % kSlots), a);
+        store_past_caches(rows + stride * (group.token0 + i), load_row(layer + slot / kSlots * kBlockBytes, kind, static_cast<int>(slot % kSlots), a));
       }
     }
     return;
@@ -271,7 +275,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(Row
         const float lo = pair_low(pairs[4 * q + t]), step = pair_step(pairs[4 * q + t]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) row[j] = row_value(lo, step, static_cast<float>(n[q][j] >> shift & 255u));
-        *reinterpret_cast<half8_t*>(rows + stride * (group.token0 + 4 * q + t)) = row;
+        store_past_caches(rows + stride * (group.token0 + 4 * q + t), row);
       }
   } else {
 #pragma unroll
@@ -284,7 +288,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(Row
         const uint32_t from = (j & 2) != 0 ? high : low;
         row[j] = row_value(lo, step, static_cast<float>(from >> (8 * ((j >> 2) + 2 * (j & 1))) & 255u));
       }
-      *reinterpret_cast<half8_t*>(rows + stride * (group.token0 + i)) = row;
+      store_past_caches(rows + stride * (group.token0 + i), row);
     }
   }
 }
