@@ -47,7 +47,7 @@ static_assert(kUnitBytes == kPairOffset + 2 * kPairBytes, "K, V, and the pairs o
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, false));
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), CTRL, 0xf, 0xf, true));  // every lane has a source
 }
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
@@ -99,10 +99,13 @@ __device__ __forceinline__ Levels quantize8(half8_t x) {
   if (static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(step_bits))) * 15.0f < span) ++step_bits;
   const float step = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(step_bits)));
   const float inverse = step > 0.f ? __builtin_amdgcn_rcpf(step) : 0.f;
+  // A one that the compiler does not see through: x 1 - lo is one instruction on the half, x - lo a conversion and a difference.
+  float one;
+  asm("s_mov_b32 %0, 1.0" : "=s"(one));
   uint32_t low = 0, high = 0;  // the levels of even and of odd j, in the low 16 bits
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float t = static_cast<float>(x[j]) - lo;
+    const float t = fmaf(static_cast<float>(x[j]), one, -lo);
     float y = t * inverse;
     y = fmaf(fmaf(-y, step, t), inverse, y);
     const uint32_t n = __float_as_uint(y + 8388608.0f);  // an integer, to nearest even, below bits 24 and on
@@ -155,11 +158,14 @@ __device__ __forceinline__ void store_row(char* unit, int kind, int t, int a, co
 __device__ __forceinline__ float pair_low(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair))); }
 __device__ __forceinline__ float pair_step(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> 16))); }
 
-// A value in fp16: the exact lo + s n, rounded to fp32 (it has at most 40 bits) and to fp16. s is rounded up, so lo + 15 s may
-// pass 65504 where the row's largest value did not: it reads as 65504.
-__device__ __forceinline__ _Float16 row_value(float lo, float step, float n) {
-  const float v = fmaf(step, n, lo);
-  return static_cast<_Float16>(v > 65504.f ? 65504.f : v);
+// Eight values in fp16: the exact lo + s n, rounded to fp32 (it has at most 40 bits) and to fp16. s is rounded up, so lo + 15 s may
+// pass 65504 where the row's largest value did not: it reads as 65504 (by a minimum that hands a NaN on, two values an instruction).
+__device__ __forceinline__ half8_t row_values(float lo, float step, const float (&n)[8]) {
+  half8_t x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = static_cast<_Float16>(fmaf(step, n[j], lo));
+  const _Float16 most = static_cast<_Float16>(65504.f);
+  return __builtin_elementwise_minimum(x, half8_t{most, most, most, most, most, most, most, most});
 }
 
 // Values 8a .. 8a + 7 of token t's row, lane a of eight.
@@ -175,10 +181,10 @@ __device__ __forceinline__ half8_t load_row(const char* unit, int kind, int t, i
 #pragma unroll
     for (int j = 0; j < 8; ++j) n[j] = static_cast<uint8_t>(at[16 * j]) >> (a & 2 ? 4 : 0) & 15u;
   }
-  half8_t x;
+  float levels[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = row_value(pair_low(pair), pair_step(pair), static_cast<float>(n[j]));
-  return x;
+  for (int j = 0; j < 8; ++j) levels[j] = static_cast<float>(n[j]);
+  return row_values(pair_low(pair), pair_step(pair), levels);
 }
 
 }  // namespace q4_device

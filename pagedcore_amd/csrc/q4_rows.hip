@@ -1,7 +1,8 @@
 // Rows of the 4-bit KV pool: quantised as they are written (pc_kv_append_q4), and read back as fp16
-// (pc_kv_read_q4). The format and its bytes are in q4_device.h. Both are bound by HBM: 1024 bytes of fp16 and
-// 288 of the pool per token and layer: 2048 tokens of 22 layers (59 MB) are appended in 15.6 us and read back in 12.8
-// with the launch, 16384 read back in 71.9 (6.6 TB/s; a large fill reaches 6.9, a large copy 4.9).
+// (pc_kv_read_q4). The format and its bytes are in q4_device.h. Both are bound by HBM, with vector instructions close behind
+// (a thousand a wave of 64 rows; taking 240 of them out made a long read back 15 % faster): 1024 bytes of fp16 and
+// 288 of the pool per token and layer: 2048 tokens of 22 layers (59 MB) are appended in 14.5 us and read back in 10.7
+// with the launch, 16384 in 88 and 69 (5.4 and 6.8 TB/s; a large fill reaches 6.9, a large copy 4.9).
 
 #include <hip/hip_runtime.h>
 
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(RowArgs args) {
 constexpr int kGroupTokens = 8;
 constexpr int kGroupWaves = 4;
 // Rows (8 a token and layer) above which they pay: 1024 tokens of 1, 2 and 5 layers take 4.6, 4.6 and 4.8 us in groups, 3.2, 3.5 and 5.2
-// a token at a time; 2048 of 22 layers 15.6 and 22.2, read back 12.8 and 21.5, 16384 read back 71.9 and 196.
+// a token at a time; 2048 of 22 layers 14.5 and 22.2, read back 10.7 and 21.5, 16384 read back 69 and 196.
 constexpr uint32_t kGroupRows = 8 * 4400;
 
 struct Group {
@@ -152,7 +153,8 @@ __device__ __forceinline__ int chunk_offset(int kind, int half, int a) {
 }
 __device__ __forceinline__ int chunk_stride(int kind) { return kind ? 16 : 64; }
 
-__global__ __launch_bounds__(64 * kGroupWaves) void kv_append_q4_groups_kernel(RowArgs args) {
+// Eight waves a SIMD: 22 groups of a long prompt on each CU at once (89 registers and five waves: 2048 tokens 16.5 us, not 14.5).
+__global__ __launch_bounds__(64 * kGroupWaves, 8) void kv_append_q4_groups_kernel(RowArgs args) {
   Group group;
   if (!group_of(args, group)) return;
   const int a = threadIdx.x % kRowLanes, h = threadIdx.x / kRowLanes % kKVHeads, kind = threadIdx.x / (kRowLanes * kKVHeads) % 2;
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_append_q4_groups_kernel(R
   *reinterpret_cast<uint32_t*>(unit + pair_offset(kind, kGroupTokens * half + a)) = pair;
 }
 
-// The rows are whole lines that nothing reads soon, 9 MB and more of them: stored non-temporally 2048 tokens of 22 layers take 12.8 us
+// The rows are whole lines that nothing reads soon, 9 MB and more of them: stored non-temporally 2048 tokens of 22 layers took 12.8 us
 // instead of 15.1, 16384 71.9 instead of 95.4, and with a sum of K and V that reads them at once 27.6 instead of 30.0 and 182
 // instead of 199. (Of the append's 13 MB of pool, which attention reads next, the same made 333 tokens slower, 5.0 to 5.4.)
 __device__ __forceinline__ void store_past_caches(char* at, half8_t row) { __builtin_nontemporal_store(row, reinterpret_cast<half8_t*>(at)); }
@@ -271,24 +273,22 @@ __global__ __launch_bounds__(64 * kGroupWaves) void kv_read_q4_groups_kernel(Row
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int shift = t == 0 ? 0 : t == 1 ? 16 : t == 2 ? 8 : 24;
-        half8_t row;
-        const float lo = pair_low(pairs[4 * q + t]), step = pair_step(pairs[4 * q + t]);
+        float levels[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) row[j] = row_value(lo, step, static_cast<float>(n[q][j] >> shift & 255u));
-        store_past_caches(rows + stride * (group.token0 + 4 * q + t), row);
+        for (int j = 0; j < 8; ++j) levels[j] = static_cast<float>(n[q][j] >> shift & 255u);
+        store_past_caches(rows + stride * (group.token0 + 4 * q + t), row_values(pair_low(pairs[4 * q + t]), pair_step(pairs[4 * q + t]), levels));
       }
   } else {
 #pragma unroll
     for (int i = 0; i < kGroupTokens; ++i) {
       const uint32_t low = w[i] & 0x0F0F0F0Fu, high = w[i] >> 4 & 0x0F0F0F0Fu;  // j = 0 4 1 5 and 2 6 3 7
-      const float lo = pair_low(pairs[i]), step = pair_step(pairs[i]);
-      half8_t row;
+      float levels[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t from = (j & 2) != 0 ? high : low;
-        row[j] = row_value(lo, step, static_cast<float>(from >> (8 * ((j >> 2) + 2 * (j & 1))) & 255u));
+        levels[j] = static_cast<float>(from >> (8 * ((j >> 2) + 2 * (j & 1))) & 255u);
       }
-      store_past_caches(rows + stride * (group.token0 + i), row);
+      store_past_caches(rows + stride * (group.token0 + i), row_values(pair_low(pairs[i]), pair_step(pairs[i]), levels));
     }
   }
 }

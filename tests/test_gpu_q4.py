@@ -173,6 +173,33 @@ def test_read_rows(device, layers, begin, tokens):
         _assert_read(got.cpu().numpy(), np.stack([ref.rows(pool[begin + layer], kind, slots) for layer in range(layers)]))
 
 
+def test_a_row_is_the_same_whichever_call_writes_or_reads_it(device):
+    """Eight tokens a wave, a token a wave, rows aligned to 16 bytes or not: the same bytes and the same values bit for bit."""
+    rng = np.random.default_rng(18)
+    layers, tokens, blocks = 3, 2048, 128
+    key, value = (_up(rng.standard_normal((layers, tokens, 4, 64)).astype(np.float16), device) for _ in range(2))
+    slots = torch.arange(tokens, device=device)
+    pools = [torch.zeros((22, blocks, 4, ref.UNIT), dtype=torch.uint8, device=device) for _ in range(3)]
+    wide = torch.empty((2, layers, tokens, 4 * 64 + 1), dtype=torch.float16, device=device)
+    odd = [x[..., 1:].unflatten(-1, (4, 64)) for x in wide]
+    odd[0].copy_(key)
+    odd[1].copy_(value)
+    _hip.kv_append_q4(pools[0], 0, key, value, slots)
+    _hip.kv_append_q4(pools[1], 0, *odd, slots)
+    back = torch.zeros((2, layers, tokens, 4, 64), dtype=torch.float16, device=device)
+    _hip.kv_read_q4(back[0], back[1], pools[0], 0, slots)
+    for at in range(0, tokens, 100):
+        some = slice(at, at + 100)
+        _hip.kv_append_q4(pools[2], 0, key[:, some], value[:, some], slots[some])
+        part = torch.zeros_like(back[:, :, some])
+        _hip.kv_read_q4(part[0], part[1], pools[0], 0, slots[some])
+        assert torch.equal(part.view(torch.int16), back[:, :, some].view(torch.int16))
+    assert torch.equal(pools[0], pools[1]) and torch.equal(pools[0], pools[2])
+    wide.zero_()
+    _hip.kv_read_q4(*odd, pools[0], 0, slots)
+    assert all(torch.equal(x, y) for x, y in zip(odd, back))
+
+
 def test_rows_of_every_kind(device):
     """Infinities and NaN, the widest and the narrowest spans, subnormal steps, zeros of both signs."""
     rng = np.random.default_rng(1)
