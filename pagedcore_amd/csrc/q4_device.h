@@ -93,7 +93,7 @@ __device__ __forceinline__ Levels quantize8(half8_t x) {
   hi2 = __builtin_elementwise_maximum(hi2, dpp<kMirror8>(hi2));
   // + 0: a zero of either sign is +0, the row's bytes do not depend on the order of its values.
   const float lo = static_cast<float>(__builtin_elementwise_minimum(lo2[0], lo2[1])) + 0.f;
-  const float span = static_cast<float>(__builtin_elementwise_maximum(hi2[0], hi2[1])) - lo;
+  const float span = static_cast<float>(__builtin_elementwise_maximum(hi2[0], hi2[1])) - lo + 0.f;  // (-0 of a row of -0 alone)
   uint32_t step_bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(span * (1.0f / 15.0f)));
   // 15 s is exact in fp32 (4 and 11 bits).
   if (static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(step_bits))) * 15.0f < span) ++step_bits;

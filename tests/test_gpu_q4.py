@@ -231,6 +231,20 @@ def test_rows_of_every_kind(device):
     assert (got == expected).all()
 
 
+@pytest.mark.parametrize("tokens", [3, 1200])
+def test_rows_of_zeros_have_the_bytes_of_zero(device, tokens):
+    """Rows of -0 alone, of both zeros, of +0: all of them a minimum and a step of +0. (-0 less +0 is -0, which must not become the step.)"""
+    x = np.zeros((4, tokens, 4, 64), dtype=np.float16)
+    x[:, ::3] = -0.0
+    x[:, 1::3, :, ::2] = -0.0
+    slots = torch.arange(tokens, device=device)
+    pool = torch.full((22, tokens // 16 + 1, 4, ref.UNIT), 255, dtype=torch.uint8, device=device)
+    expected = pool.cpu().numpy()
+    ref.write(expected, 2, x, x, range(tokens))
+    _hip.kv_append_q4(pool, 2, _up(x, device), _up(x, device), slots)
+    assert torch.equal(pool.cpu(), torch.from_numpy(expected))
+
+
 def _attend(device, pool, layer, query, tables, lengths, new=None, out=None, workspace=None):
     batch = len(lengths)
     lens, tabs = np.asarray(lengths, dtype=np.int32), np.asarray(tables, dtype=np.int32)
