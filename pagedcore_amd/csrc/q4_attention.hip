@@ -8,9 +8,11 @@
 // so scales and minima enter once per token and head, and the products run on the levels themselves:
 //   * q . n on the fp16 instruction, n taken as the fp16 whose bits are n or 16 n (the subnormals n 2^-24 and n 2^-20:
 //     exact, and one mask and at most one shift for two of them; the query's elements make up for the factor);
-//   * (p s') n' on the bf16 instruction, n' as 128 + n' (bf16 bits 0x4300 | n'), p s' as bf16 and the bf16 of its
+//   * (p s') n' on the bf16 instruction, n' as 16 + n' (bf16 bits 0x4180 | n' << 3, exact), p s' as bf16 and the bf16 of its
 //     remainder in the two halves of the columns (16 bits of it; bf16 because p s' spans fp32's range), and
-//     128 sum(p s') of the same rounded weights, from one more product with ones, is taken off at the end.
+//     16 sum(p s') of the same rounded weights, from one more product with ones, is taken off at the end. 16 is the least
+//     offset that needs no conversion: the sums hold three times what is wanted, 1.5 bits of their 24 (128 + n', a shift less
+//     in eight, would hold eighteen times it).
 //
 // One or two waves of a workgroup take a kv head of its bin, four blocks (64 tokens) a step. The row of a product's tile is
 // chosen so that no data crosses lanes: tile i's row 4b + e is token 4i + e of the step's block b, which leaves lane
@@ -165,11 +167,12 @@ __device__ __forceinline__ half8_t key_levels(uint32_t w) {
   return __builtin_bit_cast(half8_t, r);
 }
 
-// Levels of two words (tokens 0-3 and 4-7; shift 4: the byte's upper half) as bf16 128 + n. `bias` is 0x43004300 in a vector
-// register: an and-or takes one constant from the scalar ones.
-__device__ __forceinline__ bf16x8_t value_levels(uint32_t a, uint32_t b, int shift, uint32_t bias) {
-  uint4_t r = {(a >> shift & 0x000F000Fu) | bias, (a >> (8 + shift) & 0x000F000Fu) | bias, (b >> shift & 0x000F000Fu) | bias,
-               (b >> (8 + shift) & 0x000F000Fu) | bias};
+// Levels of two words (tokens 0-3 and 4-7; upper: the byte's upper half) as bf16 16 + n, n in bits 3-6 of each half. `bias` is
+// 0x41804180 in a vector register: an and-or takes one constant from the scalar ones.
+__device__ __forceinline__ bf16x8_t value_levels(uint32_t a, uint32_t b, bool upper, uint32_t bias) {
+  constexpr uint32_t kLevels = 0x00780078u;
+  uint4_t r = {((upper ? a >> 1 : a << 3) & kLevels) | bias, ((upper ? a >> 9 : a >> 5) & kLevels) | bias,
+               ((upper ? b >> 1 : b << 3) & kLevels) | bias, ((upper ? b >> 9 : b >> 5) & kLevels) | bias};
   return __builtin_bit_cast(bf16x8_t, r);
 }
 
@@ -389,7 +392,7 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
   }
 
   uint32_t bias;
-  asm("v_mov_b32 %0, 0x43004300" : "=v"(bias));
+  asm("v_mov_b32 %0, 0x41804180" : "=v"(bias));
   // A zero that the compiler does not see through: p s + 0 is one instruction on the pair's half, p s a conversion and a product.
   float none;
   asm("s_mov_b32 %0, 0" : "=s"(none));
@@ -514,7 +517,7 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
         for (int a = 0; a < 2; ++a) {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(d.v[a][t >> 1], d.v[a][2 + (t >> 1)], 4 * (t & 1), bias), weights[a], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_levels(d.v[a][t >> 1], d.v[a][2 + (t >> 1)], (t & 1) != 0, bias), weights[a], acc[t], 0, 0, 0);
           }
           const uint4_t one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
           wacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), weights[a], wacc, 0, 0, 0);
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
       Part p;
       p.m = m * to_log2;
       p.l = add_halves(sum_over_groups(lsum));
-      const float shift = fmaf(-128.f, add_halves(wacc[0]), add_halves(sum_over_groups(usum)));
+      const float shift = fmaf(-16.f, add_halves(wacc[0]), add_halves(sum_over_groups(usum)));
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
