@@ -482,9 +482,9 @@ int pc_kv_read_q4(void* key, int64_t key_layer_stride, int64_t key_token_stride,
 /*
  * Paged decode attention of one layer over the 4-bit pool: pc_paged_decode_attn with the same plan, workspace, faults and
  * rules, over the values lo + s n that the rows stand for (not rounded to fp16). Scores, softmax and sums are fp32, the
- * weights that multiply V's levels are held in 16 bits of significand, the output is rounded once. Slots past a sequence's
- * length never reach the output, whatever their bytes are. Without sequences or plan rows the call does nothing and their pointers
- * may be null.
+ * weights that multiply V's levels are held in 16 bits of significand, the output is rounded once (65504 where it passes that,
+ * as pc_kv_read_q4's values may). Slots past a sequence's length never reach the output, whatever their bytes are. Without
+ * sequences or plan rows the call does nothing and their pointers may be null.
  */
 int pc_paged_decode_attn_q4(void* out, const void* query, const void* pool, int64_t num_blocks, int32_t layer,
                             const int32_t* context_lens, int32_t batch, int32_t max_blocks, const int32_t* plan,

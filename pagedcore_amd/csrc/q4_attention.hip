@@ -85,6 +85,8 @@ __device__ __forceinline__ void fold_part(Part& acc, const Part& p) {
   acc.m = mn;
 }
 
+// A row's values may pass 65504 by half a step (row_values in q4_device.h), and so may their mean: it is 65504 then, by a minimum
+// that hands a NaN on.
 __device__ __forceinline__ void store_output(_Float16* rows, int lane, const Part& p) {
   const int c = lane & 15, g = lane >> 4;
   _Float16* at = rows + (c & 7) * kHeadDim + 32 * (c >> 3) + 4 * g;
@@ -94,7 +96,8 @@ __device__ __forceinline__ void store_output(_Float16* rows, int lane, const Par
     half4_t x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = static_cast<_Float16>(p.o[4 * k + e] * inverse);
-    *reinterpret_cast<half4_t*>(at + 16 * k) = x;
+    const _Float16 most = static_cast<_Float16>(65504.f);
+    *reinterpret_cast<half4_t*>(at + 16 * k) = __builtin_elementwise_minimum(x, half4_t{most, most, most, most});
   }
 }
 

@@ -1,0 +1,60 @@
+"""Decode attention over the 4-bit pool at the edges of fp16's range."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import q4_reference as ref
+from pagedcore_amd import _hip
+from tests.support import flags_clear
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(device, pool, layer, query, tables, lengths, new=(None, None), pad=False):
+    lens, tabs = np.asarray(lengths, dtype=np.int32), np.asarray(tables, dtype=np.int32)
+    plan = _hip.decode_plan(lens, tabs)
+    if pad:
+        full = np.zeros((_hip.plan_capacity(len(lens), tabs.shape[1]), plan.shape[1]), dtype=np.int32)
+        full[: plan.shape[0]] = plan
+        plan = full
+    workspace = torch.zeros(_hip.workspace_bytes(len(lens), tabs.shape[1]), dtype=torch.uint8, device=device)
+    out = torch.full((len(lens), 32, 64), 3.0, dtype=torch.float16, device=device)
+    up = lambda x: torch.from_numpy(np.ascontiguousarray(x)).to(device)  # noqa: E731
+    _hip.planned_decode_attention_q4(out, query, pool, layer, up(lens), up(plan), tabs.shape[1], workspace, new_key=new[0], new_value=new[1])
+    torch.cuda.synchronize()
+    _hip.check_attention_faults(workspace, "test")
+    assert flags_clear(workspace)
+    return out
+
+
+@pytest.mark.parametrize("length", [1, 15, 700])
+@pytest.mark.parametrize("low", [0.0, -65504.0])
+@pytest.mark.parametrize("fused", [False, True])
+def test_steps_rounded_up_past_the_largest_value(device, length, low, fused):
+    """Rows from `low` to 65504 have a step whose fifteenth multiple passes 65504 (65520 and 65536 in all). They are read as 65504,
+    and tokens that all hold such a row attend to 65504 as well: no infinity comes of finite rows. A row of NaN stays NaN."""
+    rng = np.random.default_rng(length)
+    blocks = -(-length // 16)
+    row = np.where(rng.integers(0, 2, (4, 64)) == 1, np.float16(65504), np.float16(low)).astype(np.float16)
+    row[:, 0], row[:, 1] = low, 65504
+    value = torch.from_numpy(row).to(device).expand(1, length, 4, 64).contiguous()
+    key = torch.randn(1, length, 4, 64, dtype=torch.float16, device=device)
+    pool = torch.zeros((22, blocks, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    slots = torch.arange(length, device=device)
+    written = length - 1 if fused else length
+    _hip.kv_append_q4(pool, 2, key[:, :written], value[:, :written], slots[:written])
+    query = torch.randn(1, 32, 64, dtype=torch.float16, device=device)
+    new = (key[0, -1:], value[0, -1:]) if fused else (None, None)
+    tables = np.arange(blocks)[None]
+    out = _attend(device, pool, 2, query, tables, [length], new)
+    assert torch.equal(out[0].cpu(), torch.from_numpy(np.repeat(row, 8, axis=0)))
+    back = torch.zeros_like(value)
+    _hip.kv_read_q4(torch.zeros_like(key), back, pool, 2, slots)
+    assert torch.equal(back, value)
+    value[0, 0, 1, 3] = float("nan")
+    _hip.kv_append_q4(pool, 2, key[:, :1], value[:, :1], slots[:1])
+    out = _attend(device, pool, 2, query, tables, [length])
+    assert torch.isnan(out[0, 8:16]).all() and torch.isfinite(out[0, :8]).all() and torch.isfinite(out[0, 16:]).all()
