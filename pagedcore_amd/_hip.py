@@ -895,6 +895,19 @@ def _refuse_overlapping_rows(layers: int, tokens: int, *strides: Tuple[int, ...]
             raise HipExtensionError("the rows of key and value must not overlap")
 
 
+def _rows_meet(distance: int, ks: Tuple[int, ...], vs: Tuple[int, ...], layers: int, tokens: int) -> bool:
+    """Whether a row of key and a row of value, whose first rows lie `distance` elements apart, have an element in common."""
+    layer, token = np.arange(layers, dtype=np.int64), np.arange(tokens, dtype=np.int64)
+    if ks[:2] == vs[:2]:  # then their places differ by whole strides: for each step in layers the nearest two in tokens
+        apart = distance + np.arange(1 - layers, layers, dtype=np.int64) * ks[0]
+        near = np.clip(-apart // max(ks[1], 1), 1 - tokens, tokens - 1)
+        return bool((np.minimum(abs(apart + near * ks[1]), abs(apart + np.minimum(near + 1, tokens - 1) * ks[1])) < 256).any())
+    key = np.sort((layer[:, None] * ks[0] + token * ks[1]).reshape(-1))
+    value = (layer[:, None] * vs[0] + token * vs[1]).reshape(-1) + distance
+    after = np.minimum(np.searchsorted(key, value), key.size - 1)
+    return bool((np.minimum(abs(key[after] - value), abs(key[np.maximum(after - 1, 0)] - value)) < 256).any())
+
+
 def kv_append_q4(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
     """kv_append into a 4-bit pool (uint8 [22, blocks, 4, 1152]): each row [64] of key/value[l, t] quantised to 16 levels
     between its smallest and its largest value and written to slot slot_mapping[t] of layer layer_begin + l.
@@ -923,8 +936,8 @@ def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_
     """key/value[l, t] = the values of slot slot_mapping[t] in layer layer_begin + l of a 4-bit pool, rounded to float16.
 
     key/value: float16 [layers, tokens, 4, 64] to write, each [4, 64] row contiguous, layer and token strides free but for rows
-    that overlap; the rows of a slot outside the pool are left as they are. slot_mapping: int64 [tokens]. On the current stream
-    of the pool's device."""
+    that overlap, of one of them or of both (a single row given for both is value's); the rows of a slot outside the pool are left
+    as they are. slot_mapping: int64 [tokens]. On the current stream of the pool's device."""
     if not _q4_rows_fit(pool, layer_begin, key, value, slot_mapping):
         _refuse_q4_rows(pool, layer_begin, key, value, slot_mapping)
     ks, vs = key.stride(), value.stride()
@@ -933,6 +946,14 @@ def kv_read_q4(key: Tensor, value: Tensor, pool: Tensor, layer_begin: int, slot_
     layers, tokens = key.shape[0], key.shape[1]
     if ks[1] < 256 or vs[1] < 256 or ks[0] < ks[1] * tokens or vs[0] < vs[1] * tokens:  # not layer behind layer
         _refuse_overlapping_rows(layers, tokens, ks, vs)
+    apart = value.data_ptr() - key.data_ptr()
+    if (
+        apart < 2 * (ks[0] * (layers - 1) + ks[1] * (tokens - 1) + 256) and -apart < 2 * (vs[0] * (layers - 1) + vs[1] * (tokens - 1) + 256)
+        and tokens and _rows_meet(apart // 2, ks, vs, layers, tokens)
+    ):
+        if apart or layers * tokens > 1:
+            raise HipExtensionError("the rows of key and value must not overlap")
+        key = key.clone()
     lib = load()
     args = (key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], pool.data_ptr(), pool.shape[1], layer_begin, layers,
             slot_mapping.data_ptr(), tokens)

@@ -58,3 +58,30 @@ def test_steps_rounded_up_past_the_largest_value(device, length, low, fused):
     _hip.kv_append_q4(pool, 2, key[:, :1], value[:, :1], slots[:1])
     out = _attend(device, pool, 2, query, tables, [length])
     assert torch.isnan(out[0, 8:16]).all() and torch.isfinite(out[0, :8]).all() and torch.isfinite(out[0, 16:]).all()
+
+
+def test_a_row_given_for_both_is_the_values(device):
+    key, value = (torch.randn(1, 1, 4, 64, dtype=torch.float16, device=device) for _ in range(2))
+    pool = torch.zeros((22, 2, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    slots = torch.full((1,), 21, dtype=torch.int64, device=device)
+    _hip.kv_append_q4(pool, 9, key, value, slots)
+    both, rows = torch.zeros_like(key), [torch.zeros_like(key) for _ in range(2)]
+    _hip.kv_read_q4(both, both, pool, 9, slots)
+    _hip.kv_read_q4(*rows, pool, 9, slots)
+    assert torch.equal(both, rows[1]) and not torch.equal(rows[0], rows[1])
+
+
+def test_key_and_value_read_side_by_side(device):
+    """K and V of a token next to each other, each a view of one buffer; one tensor for both is refused."""
+    layers, tokens = 3, 40
+    key, value = (torch.randn(layers, tokens, 4, 64, dtype=torch.float16, device=device) for _ in range(2))
+    pool = torch.zeros((22, 3, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    slots = torch.arange(tokens, device=device)
+    _hip.kv_append_q4(pool, 1, key, value, slots)
+    apart = [torch.zeros_like(key) for _ in range(2)]
+    _hip.kv_read_q4(*apart, pool, 1, slots)
+    beside = torch.zeros((layers, tokens, 2, 4, 64), dtype=torch.float16, device=device)
+    _hip.kv_read_q4(beside[:, :, 0], beside[:, :, 1], pool, 1, slots)
+    assert torch.equal(beside, torch.stack(apart, dim=2))
+    with pytest.raises(_hip.HipExtensionError, match="overlap"):
+        _hip.kv_read_q4(key, key, pool, 1, slots)

@@ -1,0 +1,86 @@
+"""What the binding of the 4-bit KV pool's calls takes and refuses, without a GPU."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from pagedcore_amd import _hip
+from tests.test_fp8_devices import OnGpu, calls  # noqa: F401  (the fixture)
+
+
+def _pool():
+    return OnGpu(torch.zeros((22, 3, 4, 1152), dtype=torch.uint8), 0)
+
+
+def _view(base, offset, layers, tokens, layer_stride, token_stride):
+    return OnGpu(base.as_strided((layers, tokens, 4, 64), (layer_stride, token_stride, 64, 1), offset), 0)
+
+
+# (offset, layer stride, token stride) of K and of V, in elements of one buffer; layers, tokens; whether a row meets another
+SHARED = [
+    ((0, 1280, 256), (0, 1280, 256), 2, 5, True),  # one tensor for both
+    ((0, 1280, 256), (255, 1280, 256), 2, 5, True),
+    ((0, 1280, 256), (2 * 1280 - 1, 1280, 256), 2, 5, True),  # the last row's last element
+    ((0, 1280, 256), (2 * 1280, 1280, 256), 2, 5, False),  # one behind the other
+    ((2560, 1280, 256), (0, 1280, 256), 2, 5, False),
+    ((0, 2560, 512), (256, 2560, 512), 2, 5, False),  # K and V of a token side by side
+    ((0, 2560, 512), (255, 2560, 512), 2, 5, True),
+    ((0, 2560, 512), (257, 2560, 512), 2, 5, True),
+    ((256, 2560, 512), (0, 2560, 512), 2, 5, False),
+    ((0, 2560, 256), (1280, 2560, 256), 2, 5, False),  # of a layer
+    ((0, 2560, 256), (1279, 2560, 256), 2, 5, True),
+    ((0, 2560, 256), (1281, 2560, 256), 2, 5, True),
+    ((0, 256, 512), (5120, 256, 512), 2, 5, False),  # tokens outside, layers inside
+    ((0, 256, 1024), (512, 256, 1024), 2, 5, False),
+    ((0, 256, 1024), (256, 256, 1024), 2, 5, True),  # K's second layer is V's first
+    ((0, 1280, 256), (2560, 2048, 512), 2, 4, False),  # strides of their own
+    ((0, 2048, 512), (256, 4096, 1024), 2, 4, False),
+    ((0, 2048, 512), (256, 4096, 1025), 2, 4, True),
+    ((0, 0, 512), (256, 0, 512), 1, 7, False),  # one layer: its stride is of no account
+    ((0, 0, 512), (512, 0, 512), 1, 7, True),
+    ((0, 512, 0), (256, 512, 0), 3, 1, False),
+    ((0, 512, 0), (512, 512, 0), 3, 1, True),
+    ((0, 0, 0), (256, 0, 0), 1, 1, False),
+    ((0, 0, 0), (255, 0, 0), 1, 1, True),
+    ((0, 0, 0), (0, 0, 0), 1, 0, False),  # no rows at all
+]
+
+
+@pytest.mark.parametrize("key,value,layers,tokens,meet", SHARED)
+def test_key_and_value_must_not_share_rows(calls, key, value, layers, tokens, meet):  # noqa: F811
+    base = torch.zeros(20000, dtype=torch.float16)
+    elements = lambda at: {at[0] + layer * at[1] + t * at[2] + i for layer in range(layers) for t in range(tokens) for i in range(256)}  # noqa: E731
+    assert bool(elements(key) & elements(value)) == meet
+    rows = [_view(base, offset, layers, tokens, *strides) for offset, *strides in (key, value)]
+    slots = OnGpu(torch.zeros(tokens, dtype=torch.int64), 0)
+    if meet:
+        with pytest.raises(_hip.HipExtensionError, match="overlap"):
+            _hip.kv_read_q4(*rows, _pool(), 0, slots)
+        assert calls == []
+    else:
+        _hip.kv_read_q4(*rows, _pool(), 0, slots)
+        assert [name for name, *_ in calls] == ["pc_kv_read_q4"]
+    _hip.kv_append_q4(_pool(), 0, *rows, slots)  # what is only read may overlap
+    assert calls[-1][0] == "pc_kv_append_q4"
+
+
+def test_rows_that_meet_against_every_element():
+    rng = np.random.default_rng(0)
+    seen = [0, 0]
+    for _ in range(4000):
+        layers, tokens = (int(n) for n in rng.integers(1, 5, 2))
+        places = []
+        for _ in range(2):
+            inner = int(rng.integers(256, 900))
+            strides = (inner, 256 + inner * (layers - 1)) if rng.random() < 0.3 else (256 + inner * (tokens - 1) + int(rng.integers(0, 700)), inner)
+            places.append(strides)
+        if rng.random() < 0.5:
+            places[1] = places[0]
+        distance = int(rng.integers(-3000, 3000))
+        at = [np.add.outer(np.arange(layers) * s[0], np.arange(tokens) * s[1]).reshape(-1) for s in places]
+        meet = bool((abs(at[0][:, None] - (at[1] + distance)) < 256).any())
+        seen[meet] += 1
+        assert _hip._rows_meet(distance, places[0], places[1], layers, tokens) == meet
+    assert min(seen) > 500
