@@ -989,6 +989,12 @@ def paged_decode_attention_q4(
 _PLAN_INTS = 296  # pc_attn_plan_record_ints()
 
 
+def _holds_heads(rows: Tensor, batch: int, heads: int) -> bool:
+    """Whether `rows` is [batch, heads, 64], or that with dimensions of 1 between."""
+    shape = rows.shape
+    return shape == (batch, heads, 64) or shape == (batch, heads, 1, 64) or (shape[:1] == (batch,) and tuple(n for n in shape[1:] if n != 1) == (heads, 64))
+
+
 def _refuse_q4_attention(out, query, pool, context_lens, plan, max_blocks, workspace, nbytes, new_key, new_value) -> None:
     device = _check_q4_pool(pool)
     if context_lens.dtype is not _I32 or context_lens.dim() != 1 or not context_lens.is_contiguous() or context_lens.get_device() != device:
@@ -1001,7 +1007,7 @@ def _refuse_q4_attention(out, query, pool, context_lens, plan, max_blocks, works
             if new_key is not None or new_value is not None:
                 raise HipExtensionError("new_key and new_value are given together")
             continue
-        if rows.dtype is not _F16 or rows.dim() < 2 or rows.shape[0] != batch or rows.numel() != batch * heads * 64 or not rows.is_contiguous() or rows.get_device() != device:
+        if rows.dtype is not _F16 or not _holds_heads(rows, batch, heads) or not rows.is_contiguous() or rows.get_device() != device:
             raise HipExtensionError(f"{name} must be contiguous float16 [{batch}, {heads}, 64] on GPU {device}")
     if plan.dtype is not _I32 or plan.dim() != 2 or plan.shape[1] != _PLAN_INTS or not plan.is_contiguous() or plan.get_device() != device:
         raise HipExtensionError(f"plan must be a contiguous int32 decode_plan() array on GPU {device}")
@@ -1013,7 +1019,7 @@ def planned_decode_attention_q4(
     workspace: Tensor, *, new_key: Optional[Tensor] = None, new_value: Optional[Tensor] = None,
 ) -> None:
     """planned_decode_attention over a 4-bit pool (uint8 [22, blocks, 4, 1152]): out/query float16 [batch, 32, 64] contiguous
-    (a dimension of 1 more between is taken), the plan, lengths and workspace as there. With new_key and new_value (float16
+    (dimensions of 1 more between are taken), the plan, lengths and workspace as there. With new_key and new_value (float16
     [batch, 4, 64]) each sequence's newest token is quantised and written in the same launch, with the results of
     kv_append_q4 followed by attention."""
     lib = load()
@@ -1023,19 +1029,17 @@ def planned_decode_attention_q4(
     if not (
         device >= 0 and is_q4_pool(pool) and nbytes > 0
         and context_lens.dtype is _I32 and context_lens.is_contiguous() and context_lens.get_device() == device
-        and out.dtype is _F16 and out.numel() == batch * 2048 and out.shape[0] == batch and out.is_contiguous() and out.get_device() == device
-        and query.dtype is _F16 and query.numel() == batch * 2048 and query.shape[0] == batch and query.is_contiguous()
-        and query.get_device() == device
+        and out.dtype is _F16 and _holds_heads(out, batch, 32) and out.is_contiguous() and out.get_device() == device
+        and query.dtype is _F16 and _holds_heads(query, batch, 32) and query.is_contiguous() and query.get_device() == device
         and plan.dtype is _I32 and len(plan_shape) == 2 and plan_shape[1] == _PLAN_INTS and plan.is_contiguous() and plan.get_device() == device
         and workspace.nbytes >= nbytes and workspace.is_contiguous() and workspace.get_device() == device
         and (
             (new_key is None and new_value is None)
             or (
                 new_key is not None and new_value is not None
-                and new_key.dtype is _F16 and new_key.numel() == batch * 256 and new_key.shape[0] == batch
-                and new_key.is_contiguous() and new_key.get_device() == device
-                and new_value.dtype is _F16 and new_value.numel() == batch * 256 and new_value.shape[0] == batch
-                and new_value.is_contiguous() and new_value.get_device() == device
+                and new_key.dtype is _F16 and _holds_heads(new_key, batch, 4) and new_key.is_contiguous() and new_key.get_device() == device
+                and new_value.dtype is _F16 and _holds_heads(new_value, batch, 4) and new_value.is_contiguous()
+                and new_value.get_device() == device
             )
         )
     ):

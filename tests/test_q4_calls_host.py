@@ -84,3 +84,29 @@ def test_rows_that_meet_against_every_element():
         seen[meet] += 1
         assert _hip._rows_meet(distance, places[0], places[1], layers, tokens) == meet
     assert min(seen) > 500
+
+
+def test_attention_rows_are_told_by_their_whole_shape(calls, monkeypatch):  # noqa: F811
+    """Rows of as many elements in another order are refused, not read as [batch, heads, 64]; dimensions of 1 between are taken."""
+    on = lambda shape, dtype=torch.float16: OnGpu(torch.zeros(shape, dtype=dtype), 0)  # noqa: E731
+    stand_in = _hip.load()
+
+    class Library:
+        def __getattr__(self, name):
+            return (lambda *args: 1 << 20) if name == "pc_attn_workspace_bytes" else getattr(stand_in, name)
+
+    monkeypatch.setattr(_hip, "load", lambda: Library())
+    good = {
+        "out": on((3, 32, 64)), "query": on((3, 32, 64)), "pool": _pool(), "layer": 0, "context_lens": on((3,), torch.int32),
+        "plan": on((8, 296), torch.int32), "max_blocks": 2, "workspace": on((1 << 20,), torch.uint8), "new_key": on((3, 4, 64)),
+        "new_value": on((3, 4, 64)),
+    }
+    for name, heads in (("out", 32), ("query", 32), ("new_key", 4), ("new_value", 4)):
+        for shape in ((3, 64, heads), (3, heads * 64), (3, heads // 2, 128), (3, 2, heads // 2, 64), (3 * heads, 64), (heads, 3, 64), (3, 64, heads, 1), (3 * heads * 64,)):
+            with pytest.raises(_hip.HipExtensionError, match=name):
+                _hip.planned_decode_attention_q4(**{**good, name: on(shape)})
+    assert calls == []
+    for name, heads in (("out", 32), ("query", 32), ("new_key", 4), ("new_value", 4)):
+        for shape in ((3, heads, 1, 64), (3, 1, heads, 64), (3, 1, heads, 1, 64)):
+            _hip.planned_decode_attention_q4(**{**good, name: on(shape)})
+    assert [name for name, *_ in calls] == ["pc_kv_append_paged_decode_attn_q4"] * 12
