@@ -255,7 +255,7 @@ def kv_append(pool: Tensor, layer_begin: int, key: Tensor, value: Tensor, slot_m
 
 
 def _check_fp16_pool(pool: Optional[Tensor]) -> None:
-    if pool is not None and pool.dtype is _U8:
+    if pool is not None and pool.dtype is _U8 and pool.shape[2:] == (4, Q4_UNIT_BYTES):
         raise HipExtensionError("pool must be float16 [22, 2, blocks, 16, 4, 64] (the _q4 calls take a 4-bit pool)")
 
 

@@ -110,3 +110,12 @@ def test_attention_rows_are_told_by_their_whole_shape(calls, monkeypatch):  # no
         for shape in ((3, heads, 1, 64), (3, 1, heads, 64), (3, 1, heads, 1, 64)):
             _hip.planned_decode_attention_q4(**{**good, name: on(shape)})
     assert [name for name, *_ in calls] == ["pc_kv_append_paged_decode_attn_q4"] * 12
+
+
+def test_the_fp16_calls_take_a_pool_as_bytes(calls):  # noqa: F811
+    """The fp16 pool as uint8 [22, 2, blocks, 16, 4, 128] went through its calls before there were 4-bit pools, and does now."""
+    pool = torch.zeros((22, 2, 3, 16, 4, 64), dtype=torch.float16).view(torch.uint8)
+    rows, slots = torch.zeros((1, 2, 4, 64), dtype=torch.float16), torch.zeros(2, dtype=torch.int64)
+    _hip.kv_append(pool, 0, rows, rows, slots)
+    _hip.rope_kv_append(rows, torch.zeros((2, 2560), dtype=torch.float16), slots, rows, pool=pool, slot_mapping=slots)
+    assert [name for name, *_ in calls] == ["pc_kv_append", "pc_rope_kv_append"]
