@@ -31,6 +31,7 @@ struct RowArgs {
   char* pool;
   int64_t num_blocks;
   uint32_t tokens, rows;  // rows = layers * tokens * 2 kinds * 4 heads
+  uint32_t begin;         // the launch's first row (eight lanes a row: a launch has less than 2^32 threads)
   int32_t layer_begin;
 };
 
@@ -58,7 +59,7 @@ __device__ __forceinline__ Row row_of(const RowArgs& args, uint32_t row) {
 // VEC: the rows are 16-byte aligned; else they are read and written a value at a time.
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv_append_q4_kernel(RowArgs args) {
-  const uint32_t row = blockIdx.x * kRowsPerGroup + threadIdx.x / kRowLanes;
+  const uint32_t row = args.begin + blockIdx.x * kRowsPerGroup + threadIdx.x / kRowLanes;
   if (row >= args.rows) return;
   const int a = threadIdx.x % kRowLanes;
   const Row r = row_of(args, row);
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_q4_kernel(RowArgs args) {
 
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(RowArgs args) {
-  const uint32_t row = blockIdx.x * kRowsPerGroup + threadIdx.x / kRowLanes;
+  const uint32_t row = args.begin + blockIdx.x * kRowsPerGroup + threadIdx.x / kRowLanes;
   if (row >= args.rows) return;
   const int a = threadIdx.x % kRowLanes;
   const Row r = row_of(args, row);
@@ -320,6 +321,7 @@ int row_args(RowArgs& args, const void* pool, int64_t num_blocks, int32_t layer_
   args.num_blocks = num_blocks;
   args.tokens = static_cast<uint32_t>(num_tokens);
   args.rows = static_cast<uint32_t>(num_tokens * num_layers * 2 * kKVHeads);
+  args.begin = 0;
   args.layer_begin = layer_begin;
   return PC_OK;
 }
@@ -329,7 +331,15 @@ bool rows_aligned(const RowArgs& args) {
          args.value_layer % 16 == 0 && args.value_token % 16 == 0;
 }
 
-unsigned grid_of(const RowArgs& args) { return (args.rows + kRowsPerGroup - 1) / kRowsPerGroup; }
+// Rows of one launch of the kernels that take a wave a token, and the launches that all rows take: one, but for more than 2^25
+// tokens of a layer, or of several together, that are not 16-byte aligned.
+constexpr uint32_t kLaunchRows = 1u << 28;
+void launch_rows(void (*kernel)(RowArgs), RowArgs args, void* stream) {
+  for (; args.begin < args.rows; args.begin += kLaunchRows) {
+    const uint32_t rows = args.rows - args.begin < kLaunchRows ? args.rows - args.begin : kLaunchRows;
+    hipLaunchKernelGGL(kernel, dim3((rows + kRowsPerGroup - 1) / kRowsPerGroup), dim3(kThreads), 0, static_cast<hipStream_t>(stream), args);
+  }
+}
 
 // A wave a token and layer where there are few, for a short way to the end; eight tokens a wave above.
 bool in_groups(const RowArgs& args) { return rows_aligned(args) && args.rows > kGroupRows; }
@@ -356,8 +366,7 @@ int pc_kv_append_q4(void* pool, int64_t num_blocks, int32_t layer_begin, int32_t
     hipLaunchKernelGGL(kv_append_q4_groups_kernel, dim3(groups_grid_of(args)), dim3(64 * kGroupWaves), 0, static_cast<hipStream_t>(stream), args);
     return check_launch("kv_append_q4");
   }
-  hipLaunchKernelGGL(rows_aligned(args) ? kv_append_q4_kernel<true> : kv_append_q4_kernel<false>, dim3(grid_of(args)), dim3(kThreads),
-                     0, static_cast<hipStream_t>(stream), args);
+  launch_rows(rows_aligned(args) ? kv_append_q4_kernel<true> : kv_append_q4_kernel<false>, args, stream);
   return check_launch("kv_append_q4");
 }
 
@@ -375,8 +384,7 @@ int pc_kv_read_q4(void* key, int64_t key_layer_stride, int64_t key_token_stride,
     hipLaunchKernelGGL(kv_read_q4_groups_kernel, dim3(groups_grid_of(args)), dim3(64 * kGroupWaves), 0, static_cast<hipStream_t>(stream), args);
     return check_launch("kv_read_q4");
   }
-  hipLaunchKernelGGL(rows_aligned(args) ? kv_read_q4_kernel<true> : kv_read_q4_kernel<false>, dim3(grid_of(args)), dim3(kThreads), 0,
-                     static_cast<hipStream_t>(stream), args);
+  launch_rows(rows_aligned(args) ? kv_read_q4_kernel<true> : kv_read_q4_kernel<false>, args, stream);
   return check_launch("kv_read_q4");
 }
 

@@ -85,3 +85,23 @@ def test_key_and_value_read_side_by_side(device):
     assert torch.equal(beside, torch.stack(apart, dim=2))
     with pytest.raises(_hip.HipExtensionError, match="overlap"):
         _hip.kv_read_q4(key, key, pool, 1, slots)
+
+
+def test_more_rows_than_a_launch_has_threads_for(device):
+    """2^26 tokens and some, a row of 128 bytes at an odd address given for all of them (a token stride of 0): the first, the last and
+    those around the middle are written, the others' slots lie outside the pool."""
+    tokens, blocks = (1 << 26) + 37, 4
+    rng = np.random.default_rng(2)
+    rows = rng.standard_normal((2, 1, 1, 4, 64)).astype(np.float16)
+    wide = torch.zeros(2, 257, dtype=torch.float16, device=device)
+    wide[:, 1:] = torch.from_numpy(rows.reshape(2, 256)).to(device)
+    key, value = (row[1:].view(1, 1, 4, 64).expand(1, tokens, 4, 64) for row in wide)
+    slots = torch.full((tokens,), -1, dtype=torch.int64, device=device)
+    at = [0, 1, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, tokens - 2, tokens - 1]
+    places = [3, 17, 18, 40, 41, 42, 60, 63]
+    slots[torch.tensor(at, device=device)] = torch.tensor(places, device=device)
+    pool = torch.full((22, blocks, 4, ref.UNIT), 255, dtype=torch.uint8, device=device)
+    expected = pool.cpu().numpy()
+    _hip.kv_append_q4(pool, 6, key, value, slots)
+    ref.write(expected, 6, *(np.repeat(x, len(at), axis=1) for x in rows), places)
+    assert torch.equal(pool.cpu(), torch.from_numpy(expected))
