@@ -76,6 +76,7 @@ int pc_kv_append(void* pool, int64_t num_blocks, int32_t layer_begin, int32_t nu
  *   plan         num_records rows of pc_attn_plan_record_ints() int32 from pc_attn_plan()
  *                for the same lengths and block tables (device copy), optionally followed
  *                by all-zero padding rows; one plan serves every layer of a decode step
+ *                (at most 2^24 - 8 rows in all, of the 4-bit pool's calls 2^23 - 8: a launch's)
  *   out[b][h] = softmax(q[b][h] . K[b][:len]^T / 8) . V[b][:len], computed in fp32 and
  *   rounded once to fp16. Slots past len are never multiplied, so poisoned (NaN) tail
  *   slots do not reach the output. A block id outside [0, num_blocks) is never

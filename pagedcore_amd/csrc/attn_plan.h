@@ -95,6 +95,17 @@ inline int64_t plan_rows_bound(int32_t batch, int32_t max_blocks) {
   return static_cast<int64_t>(kGroups) * group_bins_bound(batch, max_blocks);
 }
 
+// `threads`: of a workgroup, which takes a row. A launch of 2^32 threads or more would be done modulo 2^32, without an error.
+inline int check_plan_rows(int32_t num_records, int32_t batch, int32_t max_blocks, int threads) {
+  using pc_internal::set_error;
+  if (num_records < 0 || num_records > plan_rows_bound(batch, max_blocks)) {
+    return set_error(PC_ERR_ARGUMENT, "num_records %d outside [0, pc_attn_plan_capacity]", num_records);
+  }
+  const int64_t most = ((int64_t{1} << 32) - 1) / threads / kGroups * kGroups;
+  if (num_records > most) return set_error(PC_ERR_ARGUMENT, "num_records %d above %lld, a launch's", num_records, static_cast<long long>(most));
+  return PC_OK;
+}
+
 // Partial slots that always suffice: one per bin at most (a bin ends at most one cut part
 // that is not a sequence's last). The bins over all groups number at most the target plus
 // one per kMaxUnits blocks plus rounding (kGroups x 1.5), plus the early closes.

@@ -852,9 +852,7 @@ int launch_decode_attn(void* out, const void* query, void* pool, int64_t num_blo
       !aligned(plan, 16) || !aligned(context_lens, 4)) {
     return set_error(PC_ERR_ARGUMENT, "query/out/pool/plan must be 16-byte, workspace 256-byte aligned");
   }
-  if (num_records < 0 || num_records > plan_rows_bound(batch, max_blocks)) {
-    return set_error(PC_ERR_ARGUMENT, "num_records %d outside [0, pc_attn_plan_capacity]", num_records);
-  }
+  if (int rc = check_plan_rows(num_records, batch, max_blocks, kBinThreads)) return rc;
   const int64_t nslots = slots_bound(batch, max_blocks);
   if (batch == 0 || num_records == 0) return ok();
   hipStream_t s = static_cast<hipStream_t>(stream);

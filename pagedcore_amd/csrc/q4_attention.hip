@@ -636,9 +636,7 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
       !aligned(context_lens, 4) || !aligned(new_key, 16) || !aligned(new_value, 16)) {
     return set_error(PC_ERR_ARGUMENT, "query/out/plan/new rows must be 16-byte, pool 128-byte, workspace 256-byte aligned");
   }
-  if (num_records < 0 || num_records > plan_rows_bound(batch, max_blocks)) {
-    return set_error(PC_ERR_ARGUMENT, "num_records %d outside [0, pc_attn_plan_capacity]", num_records);
-  }
+  if (int rc = check_plan_rows(num_records, batch, max_blocks, 2 * 64 * kKVHeads)) return rc;
   if (batch == 0 || num_records == 0) return ok();
   // Fewer bins a group, or of a sequence, and each of an XCD's CUs has at most two of them.
   const bool spread = num_records > kGroups * kSpreadBins && max_blocks > kMinBinBlocks * kSpreadBins;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -119,3 +121,17 @@ def test_the_fp16_calls_take_a_pool_as_bytes(calls):  # noqa: F811
     _hip.kv_append(pool, 0, rows, rows, slots)
     _hip.rope_kv_append(rows, torch.zeros((2, 2560), dtype=torch.float16), slots, rows, pool=pool, slot_mapping=slots)
     assert [name for name, *_ in calls] == ["pc_kv_append", "pc_rope_kv_append"]
+
+
+def test_plans_of_more_rows_than_a_launch_has_threads_for():
+    """A plan padded to a capacity of 2^23 rows and more (of 512 threads each; 2^24 of the fp16 kernel's 256) is refused."""
+    lib = _hip.load()
+    buffer = ctypes.create_string_buffer(1 << 12)
+    at = (ctypes.addressof(buffer) + 255) // 256 * 256
+    assert _hip.plan_capacity(1 << 20, 1 << 16) > 1 << 30
+    shape = (at, at, at, 3, 0, at, 1 << 20, 1 << 16, at)
+    for rows in (1 << 23, (1 << 23) + 1, 1 << 29):
+        assert lib.pc_paged_decode_attn_q4(*shape, rows, at, None) == 1 and b"8388600" in lib.pc_last_error()
+        assert lib.pc_kv_append_paged_decode_attn_q4(*shape, rows, at, at, at, None) == 1 and b"8388600" in lib.pc_last_error()
+        assert lib.pc_paged_decode_attn(*shape, 2 * rows, at, None) == 1 and b"16777208" in lib.pc_last_error()
+        assert lib.pc_kv_append_paged_decode_attn(*shape, 2 * rows, at, at, at, None) == 1 and b"16777208" in lib.pc_last_error()
