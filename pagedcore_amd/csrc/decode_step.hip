@@ -26,6 +26,7 @@ namespace {
 using namespace rope_device;
 using pc_internal::aligned;
 using pc_internal::check_launch;
+using pc_internal::check_threads;
 using pc_internal::ok;
 using pc_internal::set_error;
 
@@ -351,6 +352,7 @@ int rope_kv_append(void* query_out, void* key_out, void* value_out, const void* 
   if (!aligned(query_out, 16) || !aligned(qkv, 16) || !aligned(qkv_parts, 16) || !aligned(rope_table, 16) ||
       !aligned(pool, 16) || !aligned(key_out, 16) || !aligned(value_out, 16))
     return set_error(PC_ERR_ARGUMENT, "buffers must be 16-byte aligned");
+  if (int rc = check_threads(num_tokens, kRopeThreads, "rope_kv_append")) return rc;
   const int64_t kind_elems = pool ? num_blocks * kSlots * kRowElems : 0;
   _Float16* layer_pool = pool ? static_cast<_Float16*>(pool) + static_cast<int64_t>(layer) * 2 * kind_elems : nullptr;
   with_splits(qkv_parts == nullptr, splits, [&](auto instance) {
@@ -375,6 +377,7 @@ int add_rms_norm(void* out, void* hidden, const void* delta, const float* delta_
   if (!aligned(out, 16) || !aligned(hidden, 16) || !aligned(delta, 16) || !aligned(delta_parts, 16) ||
       !aligned(weight, 16))
     return set_error(PC_ERR_ARGUMENT, "buffers must be 16-byte aligned");
+  if (int rc = check_threads(rows, kNormThreads, "add_rms_norm")) return rc;
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows)), dim3(kNormThreads), 0, static_cast<hipStream_t>(stream),
                        static_cast<_Float16*>(hidden), delta_parts ? static_cast<const void*>(delta_parts) : delta,
@@ -453,7 +456,7 @@ int pc_silu_mul(void* out, const void* gate_up, int64_t rows, int32_t width, voi
   if (!aligned(out, 16) || !aligned(gate_up, 16)) return set_error(PC_ERR_ARGUMENT, "buffers must be 16-byte aligned");
   const int64_t chunks = rows * (width / 8);
   const int64_t blocks = (chunks + kSiluThreads - 1) / kSiluThreads;
-  if (blocks > INT32_MAX) return set_error(PC_ERR_ARGUMENT, "silu_mul too large");
+  if (int rc = check_threads(blocks, kSiluThreads, "silu_mul")) return rc;
   hipLaunchKernelGGL(silu_mul_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kSiluThreads), 0,
                      static_cast<hipStream_t>(stream), static_cast<_Float16*>(out),
                      static_cast<const _Float16*>(gate_up), rows, width);

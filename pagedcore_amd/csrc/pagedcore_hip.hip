@@ -150,9 +150,9 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_word_kernel(
     uint16_t* __restrict__ pool, int64_t num_blocks, int layer_begin, uint32_t num_tokens,
     uint64_t total_words, const char* __restrict__ key, int64_t key_layer_bytes,
     int64_t key_token_bytes, const char* __restrict__ value, int64_t value_layer_bytes,
-    int64_t value_token_bytes, const int64_t* __restrict__ slot_mapping) {
+    int64_t value_token_bytes, const int64_t* __restrict__ slot_mapping, uint64_t first_word) {
   const int64_t slot_limit = num_blocks * kSlots;
-  const uint64_t w = static_cast<uint64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
+  const uint64_t w = first_word + static_cast<uint64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
   if (w >= total_words) return;
   const uint32_t e = w % kRowElems;
   const uint64_t row = w / kRowElems;
@@ -1078,11 +1078,14 @@ int pc_kv_append(void* pool, int64_t num_blocks, int32_t layer_begin, int32_t nu
   } else {
     if (!aligned(key, 2) || !aligned(value, 2)) return set_error(PC_ERR_ARGUMENT, "K/V must be 2-byte aligned");
     const uint64_t words = rows * kRowElems;
-    const unsigned grid = static_cast<unsigned>((words + kAppendThreads - 1) / kAppendThreads);
-    hipLaunchKernelGGL(kv_append_word_kernel, dim3(grid), dim3(kAppendThreads), 0, s,
-                       static_cast<uint16_t*>(pool), num_blocks, layer_begin,
-                       static_cast<uint32_t>(num_tokens), words, static_cast<const char*>(key), kl, kt,
-                       static_cast<const char*>(value), vl, vt, slot_mapping);
+    constexpr uint64_t kLaunchWords = uint64_t{1} << 31;  // a launch has less than 2^32 threads
+    for (uint64_t first = 0; first < words; first += kLaunchWords) {
+      const unsigned grid = static_cast<unsigned>((std::min(words - first, kLaunchWords) + kAppendThreads - 1) / kAppendThreads);
+      hipLaunchKernelGGL(kv_append_word_kernel, dim3(grid), dim3(kAppendThreads), 0, s,
+                         static_cast<uint16_t*>(pool), num_blocks, layer_begin,
+                         static_cast<uint32_t>(num_tokens), words, static_cast<const char*>(key), kl, kt,
+                         static_cast<const char*>(value), vl, vt, slot_mapping, first);
+    }
   }
   return check_launch("kv_append");
 }

@@ -22,6 +22,12 @@ int check_launch(const char* what);
 // The calling thread's error text.
 const char* last_error();
 
+// Refuses a launch of 2^32 threads or more, which would be done modulo 2^32 without an error.
+inline int check_threads(int64_t groups, int threads, const char* what) {
+  if (groups > static_cast<int64_t>(UINT32_MAX) / threads) return set_error(PC_ERR_ARGUMENT, "%s too large for a launch", what);
+  return PC_OK;
+}
+
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
 }  // namespace pc_internal
