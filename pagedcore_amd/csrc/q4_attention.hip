@@ -595,10 +595,12 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
       }
       last = kidx == nspan - 1;
       // A tree: at every level the last part of 2^bits (and the span's last part) folds the others', by now of 2^bits times as
-      // many parts each. A level costs a flag's way and one trip for every kMergeParts partials: spread, four at a time are
-      // best (32763 tokens, 256 parts: 12.9 us; eight 14.5, sixteen 15.6); on one XCD eight (4096 tokens, 32 parts: 8.9 us;
-      // four 9.2, sixteen 9.6), and up to sixteen at once (8 ragged sequences: 7.85 us; four 8.2, eight 8.8).
-      const int bits = SPREAD ? 2 : (nspan <= 16 ? 4 : 3), others = (1 << bits) - 1;
+      // many parts each. A level costs a flag's way and one trip for every kMergeParts partials: of many parts, which are
+      // spread, four at a time are best (32763 tokens, 256 parts: 12.9 us; eight 14.5, sixteen 15.6); of up to 32 eight (4096
+      // tokens, 32 parts on one XCD: 8.9 us; four 9.2, sixteen 9.6), and up to sixteen at once (8 ragged sequences: 7.85 us;
+      // four 8.2, eight 8.8). By the parts alone: SPREAD goes by the plan's rows, padding among them, and the order of the
+      // sums, so the output's bits, must not.
+      const int bits = nspan > kSpreadBins ? 2 : (nspan > 16 ? 3 : 4), others = (1 << bits) - 1;
 #pragma nounroll
       for (int shift = 0, at = kidx, spins = kMaxSpins; at > 0 && (last || (at & others) == others); shift += bits, at >>= bits, spins = min(2 * spins, 16 * kMaxSpins)) {
         const Waited waited = {(((at & ~others) + 1) << shift) - 1, 1 << shift, at & others, spins};
@@ -638,7 +640,8 @@ int launch(void* out, const void* query, void* pool, int64_t num_blocks, int32_t
   }
   if (int rc = check_plan_rows(num_records, batch, max_blocks, 2 * 64 * kKVHeads)) return rc;
   if (batch == 0 || num_records == 0) return ok();
-  // Fewer bins a group, or of a sequence, and each of an XCD's CUs has at most two of them.
+  // Fewer bins a group, or of a sequence, and each of an XCD's CUs has at most two of them. Rows of a padded plan count, so that
+  // behind a wide table short sequences are spread too, which costs time (13.1 us for 10.4 above) and changes no bit.
   const bool spread = num_records > kGroups * kSpreadBins && max_blocks > kMinBinBlocks * kSpreadBins;
   // Bins of one segment and, at their least, two steps.
   const bool single = batch <= kGroups && static_cast<int64_t>(batch) * max_blocks <= kTargetBins * kMinBinBlocks;

@@ -105,3 +105,22 @@ def test_more_rows_than_a_launch_has_threads_for(device):
     _hip.kv_append_q4(pool, 6, key, value, slots)
     ref.write(expected, 6, *(np.repeat(x, len(at), axis=1) for x in rows), places)
     assert torch.equal(pool.cpu(), torch.from_numpy(expected))
+
+
+@pytest.mark.parametrize("lengths", [[2000, 9, 700, 1500, 40], [4000], [1 + 97 * i % 2048 for i in range(30)], [5000, 300, 9000]])
+@pytest.mark.parametrize("fused", [False, True])
+def test_padding_a_plan_changes_no_bit(device, lengths, fused):
+    """The same sequences behind the same tables, with the plan as it is and padded to its capacity with empty rows."""
+    rng = np.random.default_rng(sum(lengths))
+    need = -(-np.asarray(lengths) // 16)
+    blocks = int(need.sum())
+    tables, ids = np.zeros((len(lengths), max(300, int(need.max()))), dtype=np.int32), rng.permutation(blocks)
+    for b, n in enumerate(need):
+        tables[b, :n], ids = ids[:n], ids[n:]
+    pool = torch.zeros((22, blocks, 4, ref.UNIT), dtype=torch.uint8, device=device)
+    rows = [torch.randn(1, blocks * 16, 4, 64, dtype=torch.float16, device=device) for _ in range(2)]
+    _hip.kv_append_q4(pool, 8, *rows, torch.arange(blocks * 16, device=device))
+    query = torch.randn(len(lengths), 32, 64, dtype=torch.float16, device=device)
+    new = tuple(torch.randn(len(lengths), 4, 64, dtype=torch.float16, device=device) for _ in range(2)) if fused else (None, None)
+    plain, padded = (_attend(device, pool, 8, query, tables, lengths, new, pad) for pad in (False, True))
+    assert torch.equal(plain.view(torch.int16), padded.view(torch.int16)), (plain != padded).flatten(1).any(1).nonzero().flatten().tolist()
