@@ -5,9 +5,10 @@ depends on register allocation or occupancy. The prompt attention kernel and the
 decode attention kernel issue loads and LDS reads as inline assembly that the compiler does
 not track, with hand-counted `vmcnt` waits: that is only correct while no register targeted
 by an outstanding load is copied, spilled or reused. The decode attention kernel also relies
-on two of its workgroups fitting one CU (empty plan rows then run beside the real ones). A
-spill (scratch use) or a register budget below the occupancy a kernel was laid out for fails
-the build instead of producing a library whose outputs or speed could silently change.
+on two of its workgroups fitting one CU (empty plan rows then run beside the real ones), as
+does that of the 4-bit pool. A spill (scratch use) or a register budget below the occupancy a
+kernel was laid out for fails the build instead of producing a library whose outputs or speed
+could silently change.
 """
 
 from __future__ import annotations
@@ -72,6 +73,8 @@ GUARDED_KERNELS: Dict[str, int] = {
     "fp8_stream_kernelILi4ELi2ELi4ELi1E": 3,  # three (52 KB)
     "fp8_stream_kernelILi1ELi2ELi4ELi2ELb0E": 3,  # three of four waves (52 KB)
     "fp8_tile_kernel": 2,  # a workgroup of eight waves
+    "paged_decode_q4_kernel": 4,  # two workgroups of eight waves, four of four
+    "kv_append_q4_groups_kernel": 8,  # the 22 groups of a long prompt that a CU has at once
 }
 
 _NOISE = "packed-fp32-ops' is not a recognized feature"

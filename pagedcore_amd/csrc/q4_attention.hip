@@ -300,11 +300,13 @@ struct Blocks {
 //   Two waves a head have more loads in flight and halve a bin's chain of steps: 256 sequences of 2048 tokens 30.1 us (one wave
 // 37.2, four 31.0), 64 ragged ones 10.5 (11.1, 12.6), 256 of at most 64 tokens 8.6 (10.3, 8.0). One wave needs no barrier and no
 // fold: 128 tokens 3.9 us (two 4.6), eight ragged sequences 7.8 (8.1), one of 8192 tokens 10.4 (10.9).
-//   126 registers leave two workgroups of eight waves on a CU, which a plan of more bins than CUs needs.
+//   126 vector registers and no spills, of scalar ones neither, leave two workgroups of eight waves on a CU, which a plan of more
+// bins than CUs needs (the build checks it).
 template <bool APPEND, bool SPREAD, int PARTS>
 __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kernel(
     const int32_t* __restrict__ plan, const _Float16* query, char* pool, uint32_t num_blocks, int layer, int rows, int batch, int nslots,
     _Float16* out, char* workspace, const _Float16* new_key, const _Float16* new_value) {
+  static_assert(PARTS == 1 || PARTS == 2, "a segment that goes on past a wave ends in the next");
   constexpr int kWaves = PARTS * kKVHeads;
   __shared__ uint32_t shared_lines[kWaves * kMaxUnits];
   __shared__ __attribute__((aligned(16))) char shared_parts[kWaves * 2 * kPartBytes];
@@ -533,7 +535,11 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
       // A block id outside the pool among the segment's blocks here.
       bool bad = false;
       if (any_outside) {
-        for (int u = kStepBlocks * from + lane; u < min(kStepBlocks * to, nblk); u += 64) bad |= static_cast<uint32_t>(row[kRecordInts + seg_begin + u]) >= num_blocks;
+#pragma unroll  // (a loop's stride and end would be held in scalar registers through the loops around, and spill others)
+        for (int k = 0; k < kMaxUnits / 64; ++k) {
+          const int u = kStepBlocks * from + lane + 64 * k;
+          if (u < min(kStepBlocks * to, nblk)) bad |= static_cast<uint32_t>(row[kRecordInts + seg_begin + u]) >= num_blocks;
+        }
         bad = __builtin_amdgcn_ballot_w64(bad) != 0;
       }
       Part p;
@@ -579,13 +585,8 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
     const int sb = again[0], kidx = again[5], nspan = again[6], slot0 = again[7], k00 = again[4];
     const int seg_end = r ? last_end : first_end;
     Part total = take_part(areas + r * kPartBytes, tail_lane);
-    // The waves behind this one whose first segment this is.
-    for (int p = part + 1; p < PARTS && p * steps / PARTS < seg_end; ++p) {
-      if ((p + 1) * steps / PARTS > p * steps / PARTS) {
-        const char* area = shared_parts + (p * kKVHeads + h) * 2 * kPartBytes;
-        fold_part(total, take_part(area, tail_lane));
-      }
-    }
+    // The wave behind this one, if this is its first segment.
+    if (part + 1 < PARTS && end < seg_end) fold_part(total, take_part(areas + kKVHeads * 2 * kPartBytes, tail_lane));
     bool last = true;
     if (nspan != 1) {
       // The span's slots [slot0, slot0 + parts - 1) lie in the workspace, and the part in the span.
