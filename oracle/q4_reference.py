@@ -113,3 +113,57 @@ def attention(query: np.ndarray, units: np.ndarray, table: Sequence[int], length
         spread = min(2 * size, span)
         bound[head] = 2.0**-11 * np.abs(out[head]) + 2.0**-25 + 2 * (weight * spread + 2.0**-17 * row_span + add + (length / 8 + 80) * 2.0**-24 * np.abs(out[head]))
     return out, bound
+
+
+def close_attention(query: np.ndarray, units: np.ndarray, table: Sequence[int], length: int) -> Tuple[np.ndarray, np.ndarray]:
+    """attention() with a bound that goes by each token's own error and weight, [32, 64].
+
+    With u = 2^-24 and the formula y = s (q . n) + lo sum(q), before the division by 8: the two sums are 64 exact products each,
+    added in any order (64 u of their terms' magnitudes); the running maximum m, at most the largest |y|, is taken off within
+    the second product and again wherever it is raised (by 8 binary orders or more) or two parts meet. A head with an element of
+    thousands (squares of its sixteenths past 65500) has half of its elements divided by 16, to within 2^-21 of an element. These
+    make token t's exponent off by e_t, and with the roundings of the base-2 exponential and its argument its weight by
+    d_t = exp(e_t + ...) - 1, which moves the output by p_t d_t |v_t - out|, and by no more than the values spread. Weights
+    times steps keep 17 bits of the levels' product; levels enter it as 16 + n, and n / 32 products and 56 joins are rounded, of the
+    minima's and the weights' sums length / 8 and 16 additions a lane. Then the rounding to fp16."""
+    u = 2.0**-24
+    slots = np.array([table[p // SLOTS] * SLOTS + p % SLOTS for p in range(length)])
+    block, t = np.divmod(slots, SLOTS)
+    out, bound = np.empty((32, DIM)), np.empty((32, DIM))
+    q = query.astype(np.float64)
+    halved = np.isin(np.arange(DIM) % 8, (2, 3, 6, 7))
+    for kv in range(HEADS):
+        fields = []
+        for kind in range(2):
+            taken = units[block, kv]  # [tokens, 1152]
+            places = _PLACES[kind][t]
+            n = np.take_along_axis(taken, places[..., 0], axis=-1) >> places[..., 1] & 15
+            pair = np.take_along_axis(taken, (1024 + 64 * kind + 4 * t)[:, None] + np.arange(4), axis=-1).copy().view(np.float16).astype(np.float64)
+            fields.append((n.astype(np.float64), pair[:, :1], pair[:, 1:]))
+        (kn, klo, ks), (vn, vlo, vs) = fields
+        v = vlo + vs * vn
+        for head in range(8 * kv, 8 * kv + 8):
+            size = np.abs(q[head]).sum()
+            y = (klo + ks * kn) @ q[head]
+            most = np.abs(y).max()
+            span = (y.max() - y.min()) / 8.0
+            raises = 1 + min(span / np.log(2.0) / 8.0, length / 64)
+            error = 64 * u * (ks[:, 0] * (kn @ np.abs(q[head])) + np.abs(klo[:, 0]) * size) + u * (np.abs(klo[:, 0] * q[head].sum()) + (4 + 2 * raises + 8) * most)
+            if ((q[head] / 16) ** 2).sum() > 65400:
+                error = error + 2.0**-21 * ks[:, 0] * kn[:, halved].sum(1)
+            z = (y - y.max()) / 8.0
+            p = np.exp(z)
+            p /= p.sum()
+            with np.errstate(over="ignore"):
+                d = np.expm1(error / 8.0 + 3 * u * np.minimum(-z, 100.0) + (3 + raises) * 2.0**-22 + 16 * 2.0**-23)
+            out[head] = p @ v
+            apart = np.abs(v - out[head])
+            moved = np.minimum((p * np.minimum(d, 1e300)) @ apart, np.abs(v.max(0) - v.min(0)))
+            steps = p @ vs
+            levels = (p[:, None] * vs * (16 + vn)).sum(0) + 16 * steps
+            lane = length / 8 + 16
+            bound[head] = (
+                2.0**-11 * np.abs(out[head]) + 2.0**-25 + 1.01 * moved + 2.0**-17 * (p[:, None] * vs * vn).sum(0)
+                + u * ((length / 32 + 56) * levels + lane * (p @ np.abs(vlo)) + lane * np.abs(out[head]))
+            )
+    return out, bound
