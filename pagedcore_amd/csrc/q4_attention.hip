@@ -184,6 +184,11 @@ __device__ __forceinline__ half8_t scaled_query(half8_t q, _Float16 even, _Float
   return q * half8_t{even, even, odd, odd, even, even, odd, odd};
 }
 
+__device__ __forceinline__ half8_t sixteenth_squared(half8_t q) {
+  q *= static_cast<_Float16>(0.0625f);
+  return q * q;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   bf16x2_t v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, v);
@@ -429,19 +434,19 @@ __global__ __launch_bounds__(64 * PARTS * kKVHeads, 4) void paged_decode_q4_kern
       for (int t = 0; t < 4; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
       // (Set here, while the loads are on their way, and not behind the wait for them.)
       asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(wacc));
-      // sum(q) of every head, by a product with ones, and the heads' products with each other, which tell if any of them may
-      // have an element of 4095 or more (none is larger than a head's own, and that is at least its largest element's square).
+      // sum(q) of the lane's head, by a product with ones, and by another the sum of (q / 16)^2, which tells if the head may have
+      // an element of 4096 or more (its square is past fp16's range; 4094, the next smaller one, gives 65472).
       // The products give 2^-20 (q . n) with 16 q at the places of n 2^-24; where 16 q might pass fp16's range 2^-24 (q . n) with
-      // q / 16 at the others (what that rounds off is at most 2^-25). `to_log2`: a score in this unit as a base-2 exponent,
-      // log2(e) / 8 over the unit.
+      // q / 16 at the others: what that rounds off, 2^-21 of an element of a head whose largest are thousands, is below the
+      // sums' own roundings. `to_log2`: a score in this unit as a base-2 exponent, log2(e) / 8 over the unit.
       const _Float16 o = static_cast<_Float16>(1.f);
       const half8_t ones = {o, o, o, o, o, o, o, o};
       const float4_t zero = {0.f, 0.f, 0.f, 0.f};
       float4_t sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qa, zero, 0, 0, 0);
-      float4_t gram = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa, qa, zero, 0, 0, 0);
+      float4_t squares = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, sixteenth_squared(qa), zero, 0, 0, 0);
       sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qb, sums, 0, 0, 0);
-      gram = __builtin_amdgcn_mfma_f32_16x16x32_f16(qb, qb, gram, 0, 0, 0);
-      const bool large = __builtin_amdgcn_ballot_w64(!(fmaxf(fmaxf(gram[0], gram[1]), fmaxf(gram[2], gram[3])) < 4094.f * 4094.f)) != 0;
+      squares = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, sixteenth_squared(qb), squares, 0, 0, 0);
+      const bool large = !(squares[0] < 65500.f);
       const float qsum = sums[0] * (large ? 1.f / 16777216.f : 1.f / 1048576.f);
       const float to_log2 = large ? 16777216.f * kScoreToLog2 : 1048576.f * kScoreToLog2;
       const _Float16 even = static_cast<_Float16>(large ? 1.f : 16.f), odd = static_cast<_Float16>(large ? 0.0625f : 1.f);

@@ -34,6 +34,14 @@ def _large(elements):
     return make
 
 
+def _large_and_small_heads(rng, lengths, tokens):
+    """Head 0 of each group has an element of 4096 to 65504; the others' are of 2^-15, over keys to 32768."""
+    query, _, value = _ordinary(rng, lengths, tokens)
+    query = (query.astype(np.float64) * 2.0**-15).astype(np.float16)
+    query[:, 0::8, 10] = np.array([4096, 65504, -65504, 8192], dtype=np.float16)
+    return query, _on_levels(rng, tokens, 4096.0, [10]), value
+
+
 def _one_wins(rng, lengths, tokens):
     """Queries to 60000 in every element along one token's key: its value, and no other's, is what comes out."""
     key = _on_levels(rng, tokens, 2.0**-3)
@@ -53,6 +61,7 @@ CASES = {
     "large elements": (_large({d: [4094, 4096, 65504, -65504, 5000, -4098] for d in (0, 2, 13, 31, 32, 38, 55, 61)}), [90, 33]),
     "one large element": (_large({3: [65504, -65504]}), [64, 200]),
     "border": (_large({4: [4094, -4094], 6: [4092]}), [64, 200]),
+    "large and small heads": (_large_and_small_heads, [50, 300]),
     "one wins": (_one_wins, [70, 260]),
     "rising": (_rising, [512, 300]),
 }
