@@ -91,8 +91,8 @@ def attention(query: np.ndarray, units: np.ndarray, table: Sequence[int], length
 
     The bound, to first order and doubled: a score is 64 products and a few roundings of 2^-24 of its terms' magnitudes, so
     each weight is off by that over 8, by the exponential's own 2^-21 and by the rounding of its argument; the weights that
-    multiply the levels keep 16 bits; sums run over length / 32 (matrix instruction, levels up to 15 beside an offset of
-    128) or length / 8 (a lane's) additions and 80 at the joins."""
+    multiply the levels keep 16 bits; sums run over length / 32 (matrix instruction, levels up to 15 beside an offset, for
+    which 128 is allowed) or length / 8 (a lane's) additions and 80 at the joins."""
     slots = np.array([table[p // SLOTS] * SLOTS + p % SLOTS for p in range(length)])
     k, v = rows(units, 0, slots), rows(units, 1, slots)
     q = query.astype(np.float64)

@@ -1,8 +1,9 @@
 // Rows of the 4-bit KV pool: quantised as they are written (pc_kv_append_q4), and read back as fp16
 // (pc_kv_read_q4). The format and its bytes are in q4_device.h. Both are bound by HBM, with vector instructions close behind
 // (970 a wave of 64 rows in the append, 700 in the read, which took 12.7 us below and not 10.7 with 960): 1024 bytes of fp16 and
-// 288 of the pool per token and layer: 2048 tokens of 22 layers (59 MB) are appended in 14.5 us and read back in 10.7
-// with the launch, 16384 in 88 and 69 (5.4 and 6.8 TB/s; a large fill reaches 6.9, a large copy 4.9).
+// 288 of the pool per token and layer. In a graph, with the launch, 2048 tokens of 22 layers (59 MB) are appended in 16.2 us and
+// read back in 13.5 where every call has other data, 16384 in 88 and 81 (5.4 and 5.8 TB/s; a large fill reaches 6.9, a large
+// copy 4.9). One call repeated finds its source in the last-level cache: 14.5 and 10.7, 88 and 69. The figures below are such.
 
 #include <hip/hip_runtime.h>
 
