@@ -85,7 +85,7 @@ def build(name, lengths=None, seed=0):
         for b, n in enumerate(lengths):
             winner = key[0, slots[b][n // 3]].astype(np.float64)  # [4, 64]
             scale = np.resize([60000.0, 30000.0, 4096.0, 512.0], 8)[None, :, None]
-            query[b] = (np.sign(winner)[:, None, :] * np.abs(winner[:, None, :]) * scale).reshape(32, 64).astype(np.float16)
+            query[b] = (winner[:, None, :] * scale).reshape(32, 64).astype(np.float16)
     if name == "rising":
         # A third of every key along the first query of its group's sum, ever longer.
         for b, n in enumerate(lengths):

@@ -96,3 +96,26 @@ def test_fused_append_of_a_serving_batch(device, lengths):
     out, _ = _attend(device, pool, 7, query, tables, lengths, new)
     assert torch.equal(out.view(torch.int16), expected.view(torch.int16))
     assert torch.equal(pool[7], pair[7])
+
+
+@pytest.mark.parametrize("lengths", [SERVING, [2041] * 600], ids=["12 ragged", "600 x 2041"])
+def test_block_ids_outside_the_pool_of_a_serving_batch(device, lengths):
+    """Whichever wave and whichever of its blocks they belong to: their sequence is NaN, the others keep their bits."""
+    pool, query, tables = _batch(device, lengths, 2, 9)
+    clean, _ = _attend(device, pool, 2, query, tables, lengths)
+    lens = np.asarray(lengths, dtype=np.int32)
+    broken, hit = tables.copy(), []
+    for b in range(1, len(lengths), 5):
+        blocks = -(-lengths[b] // 16)
+        broken[b, (0, blocks - 1, blocks // 2, 63, 64, 65, 100)[b // 5 % 7] % blocks] = (pool.shape[1], -1, 1 << 30)[b // 5 % 3]
+        hit.append(b)
+    plan = torch.from_numpy(_hip.decode_plan(lens, broken)).to(device)
+    workspace = torch.zeros(_hip.workspace_bytes(len(lens), tables.shape[1]), dtype=torch.uint8, device=device)
+    out = torch.zeros_like(query)
+    _hip.planned_decode_attention_q4(out, query, pool, 2, torch.from_numpy(lens).to(device), plan, tables.shape[1], workspace)
+    torch.cuda.synchronize()
+    with pytest.raises(_hip.AttentionFaultError, match="block id"):
+        _hip.check_attention_faults(workspace, "test")
+    others = [b for b in range(len(lengths)) if b not in hit]
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[others].view(torch.int16), clean[others].view(torch.int16))
