@@ -9,6 +9,7 @@ fails to load, every entry point raises HipExtensionError.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import threading
 from typing import Dict, Optional, Tuple
@@ -897,6 +898,9 @@ def _refuse_overlapping_rows(layers: int, tokens: int, *strides: Tuple[int, ...]
 
 def _rows_meet(distance: int, ks: Tuple[int, ...], vs: Tuple[int, ...], layers: int, tokens: int) -> bool:
     """Whether a row of key and a row of value, whose first rows lie `distance` elements apart, have an element in common."""
+    common = math.gcd(*((ks[0], vs[0]) if layers > 1 else ()), *((ks[1], vs[1]) if tokens > 1 else ()))
+    if 256 <= distance % max(common, 1) <= common - 256:  # all of them lie as the first ones do (K and V of a token side by side)
+        return False
     layer, token = np.arange(layers, dtype=np.int64), np.arange(tokens, dtype=np.int64)
     if ks[:2] == vs[:2]:  # then their places differ by whole strides: for each step in layers the nearest two in tokens
         apart = distance + np.arange(1 - layers, layers, dtype=np.int64) * ks[0]
